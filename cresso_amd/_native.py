@@ -85,6 +85,24 @@ class SpectralUnit(ctypes.Structure):
                 ("lane", ctypes.c_int32), ("pad", ctypes.c_int32)]
 
 
+class ResidualNormDesc(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in (
+        "residual", "update", "gate", "post", "pre", "scale_vec", "out", "normed", "stats", "d_out", "d_normed",
+        "d_residual", "d_update", "d_gate", "d_post", "d_pre", "d_scale")] + [(k, ctypes.c_int64) for k in (
+            "residual_stride", "update_stride", "gate_stride", "d_out_stride", "d_normed_stride", "rows", "width",
+            "rows_per_gate")] + [("scale", ctypes.c_float), ("eps", ctypes.c_float)] + [(k, ctypes.c_int32) for k in (
+                "dtype", "gate_dtype", "post_dtype", "pre_dtype", "scale_dtype", "act")]
+
+
+class DistillDesc(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in (
+        "logits", "index", "teacher", "labels", "weights", "loss", "total", "stats", "d_loss", "grad")] + [
+            (k, ctypes.c_int64) for k in ("logits_stride", "index_stride", "teacher_stride", "grad_stride",
+                                          "d_loss_stride", "rows", "vocab", "ignore_index")] + [
+                (k, ctypes.c_float) for k in ("temperature", "mix", "weight")] + [(k, ctypes.c_int32) for k in (
+                    "top", "dtype", "teacher_dtype", "index_bytes", "label_bytes")]
+
+
 def hyper_from_group(group: dict) -> Hyper:
     return Hyper(*[float(group[n]) for n in HYPER_DOUBLES], int(group["warmup_steps"]), 1 if bool(group["maximize"]) else 0)
 
@@ -193,6 +211,29 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.cresso_spectral_workspace_basis.restype = c.c_int32
     lib.cresso_spectral_workspace_basis.argtypes = [c.c_void_p, c.c_void_p, c.c_size_t, c.c_int32, c.c_void_p,
                                                     c.c_void_p, c.c_void_p]
+    size = c.c_size_t
+    lib.cresso_embedding_forward.restype = i32
+    lib.cresso_embedding_forward.argtypes = [vp, i32, i64, vp, i64, i64, i64, i32, f64, vp, vp]
+    lib.cresso_embedding_backward_workspace_bytes.restype = size
+    lib.cresso_embedding_backward_workspace_bytes.argtypes = [i64, i64, i32]
+    lib.cresso_embedding_backward.restype = i32
+    lib.cresso_embedding_backward.argtypes = [vp, i32, i64, vp, i64, i64, i64, i32, f64, vp, vp, size, vp]
+    norm_desc, distill_desc = c.POINTER(ResidualNormDesc), c.POINTER(DistillDesc)
+    lib.cresso_residual_norm_forward.restype = i32
+    lib.cresso_residual_norm_forward.argtypes = [norm_desc, vp]
+    lib.cresso_residual_norm_backward_workspace_bytes.restype = size
+    lib.cresso_residual_norm_backward_workspace_bytes.argtypes = [norm_desc]
+    lib.cresso_residual_norm_backward.restype = i32
+    lib.cresso_residual_norm_backward.argtypes = [norm_desc, vp, size, vp]
+    for distill in (lib.cresso_distill_loss, lib.cresso_distill_backward):
+        distill.restype = i32
+        distill.argtypes = [distill_desc, vp]
+    lib.cresso_block_product_workspace_bytes.restype = size
+    lib.cresso_block_product_workspace_bytes.argtypes = [i64, i64, i64, vp, i64, i32]
+    lib.cresso_block_product.restype = i32
+    lib.cresso_block_product.argtypes = [vp, i64, i32, i64, i64, i64, vp, i64, vp, i64, i32, vp, vp, size, vp]
+    lib.cresso_block_quantize.restype = i32
+    lib.cresso_block_quantize.argtypes = [vp, i64, i32, i64, i64, vp, vp, vp]
 
 
 def load() -> ctypes.CDLL:
@@ -251,3 +292,57 @@ def check(rc: int, what: str) -> None:
 
 def stream_handle(device: torch.device) -> int:
     return int(torch.cuda.current_stream(device).cuda_stream)
+
+
+# ---------------------------------------------------------------------------
+# what the operators' front ends share
+# ---------------------------------------------------------------------------
+ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def require(ok: bool, what: str, why: str) -> None:
+    if not ok:
+        raise ValueError(f"{what}: {why}")
+
+
+def require_gpu(what: str, **tensors) -> torch.device:
+    """Every tensor given is on the same GPU; -> its device.  There is no CPU path."""
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not torch.is_tensor(t):
+            raise ValueError(f"{what}: {name} must be a tensor, not {type(t).__name__}")
+        if not t.is_cuda:
+            raise RuntimeError(f"{what}: {name} is on {t.device}; the operators run on the GPU only")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise RuntimeError(f"{what}: {name} is on {t.device}, others on {device}")
+    return device
+
+
+def rows_of(t: torch.Tensor) -> tuple:
+    """t seen as rows of its last dimension -> (tensor, row stride in elements).
+    Rows at one stride are taken where they lie; anything else is copied."""
+    if t.ndim == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t, t.stride(0)
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t, t.shape[-1] if t.ndim else 1
+
+
+def call(fn, what: str, device: torch.device, *args) -> None:
+    """One library call on the device's current stream (the call's last argument)."""
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != 0:
+        check(rc, what)
+
+
+def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Scratch of one call, from torch's allocator on the current stream."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)

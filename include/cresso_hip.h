@@ -418,6 +418,91 @@ int32_t cresso_drive_update(void* param, int32_t param_dtype, const float* tange
                             float* drive_energy, int64_t numel, int32_t step, int32_t hard, const cresso_hyper* hyper,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Operators of a training step around the optimizer (no reference
+ * counterpart): embedding, the seam between blocks, products with an 8-bit
+ * frozen weight, the distillation loss.  Rows are `width` consecutive elements
+ * (f32, bf16 or f16) at a row stride given in elements; nothing needs more
+ * alignment than its element.
+ * ------------------------------------------------------------------------- */
+
+/* out[t] = scale * table[ids[t]], rows of zeros for ids outside [0, rows).
+ * ids: int32 or int64 (id_bytes 4 or 8), contiguous; out: contiguous. */
+int32_t cresso_embedding_forward(const void* ids, int32_t id_bytes, int64_t tokens, const void* table, int64_t rows,
+                                 int64_t width, int64_t row_stride, int32_t dtype, double scale, void* out, void* stream);
+
+/* grad_table[v] = scale * sum of grad[t] over ids[t] == v in the order of t
+ * (fp32), zeros for rows that no id names; contiguous, written whole. */
+size_t cresso_embedding_backward_workspace_bytes(int64_t tokens, int64_t width, int32_t dtype);
+int32_t cresso_embedding_backward(const void* ids, int32_t id_bytes, int64_t tokens, const void* grad,
+                                  int64_t grad_stride, int64_t rows, int64_t width, int32_t dtype, double scale,
+                                  void* grad_table, void* workspace, size_t workspace_bytes, void* stream);
+
+#define CRESSO_GATE_NONE 0
+#define CRESSO_GATE_SIGMOID 1
+#define CRESSO_GATE_TANH 2
+
+/* The seam between two blocks:
+ *   H = s*residual + act(gate) * (update*rms(update)*post),  normed = H*rms(H)*pre,  rms(x) = 1/sqrt(mean(x^2) + eps).
+ * NULL leaves a part out: update (then gate and post too), gate (1), post (the
+ * update is not normalized), pre (no `normed`), scale_vec (s = scale for every
+ * channel).  gate: [rows / rows_per_gate][width], a row of it for each run of
+ * rows_per_gate rows.  Vectors are f32 or of the rows' dtype, each by its own
+ * code.  out, normed and the d_* of rows are contiguous.  Width <= 16384. */
+typedef struct cresso_residual_norm_desc {
+    const void *residual, *update, *gate, *post, *pre, *scale_vec;
+    void *out, *normed;
+    float* stats;                       /* [rows][2], written forward when not NULL, read backward */
+    const void *d_out, *d_normed;       /* gradients that arrive; NULL: zero */
+    void *d_residual, *d_update, *d_gate, *d_post, *d_pre, *d_scale;   /* gradients wanted, NULL: not; of the inputs' dtypes */
+    int64_t residual_stride, update_stride, gate_stride, d_out_stride, d_normed_stride;
+    int64_t rows, width, rows_per_gate;
+    float scale, eps;
+    int32_t dtype, gate_dtype, post_dtype, pre_dtype, scale_dtype, act;
+} cresso_residual_norm_desc;
+int32_t cresso_residual_norm_forward(const cresso_residual_norm_desc* desc, void* stream);
+size_t cresso_residual_norm_backward_workspace_bytes(const cresso_residual_norm_desc* desc);
+int32_t cresso_residual_norm_backward(const cresso_residual_norm_desc* desc, void* workspace, size_t workspace_bytes,
+                                      void* stream);
+
+/* Distillation from a teacher's top logits.  Per row:
+ *   loss = w * (mix*t^2 * KL(softmax(teacher/t) || softmax(logits/t)) + (1-mix) * CE(logits, label)).
+ * index [rows][top] (int32 or int64): outside [0, vocab) is absent.  labels
+ * may be NULL; ignore_index and labels outside the vocabulary give no term.
+ * weights may be NULL (then `weight` for every row); a row of weight 0, or
+ * without teacher and label, gives 0 whatever it holds.  top <= 1024. */
+typedef struct cresso_distill_desc {
+    const void *logits, *index, *teacher, *labels;
+    const float* weights;
+    float *loss, *total;                /* [rows]; total may be NULL: their sum */
+    float* stats;                       /* [rows][3], written with the loss when not NULL, read by the gradient */
+    const float* d_loss;                /* gradient: d_loss[d_loss_stride * row] */
+    void* grad;                         /* with the loss: NULL or the gradient for d_loss = 1; may be the logits */
+    int64_t logits_stride, index_stride, teacher_stride, grad_stride, d_loss_stride;
+    int64_t rows, vocab, ignore_index;
+    float temperature, mix, weight;
+    int32_t top, dtype, teacher_dtype, index_bytes, label_bytes;
+} cresso_distill_desc;
+int32_t cresso_distill_loss(const cresso_distill_desc* desc, void* stream);
+int32_t cresso_distill_backward(const cresso_distill_desc* desc, void* stream);
+
+/* out[rows][cols] = x[rows][depth] times an e4m3 weight with one fp32 scale
+ * for each 128 x 128 block.  turned 0: w is [cols][depth], out = x w^T;
+ * turned 1: w is [depth][cols], out = x w (the gradient of the other).
+ * scales: [ceil(w rows / 128)][scale_stride >= ceil(w cols / 128)].  x is
+ * rounded to e4m3 with a power of two per row and 128 elements (the smallest
+ * 2^e with max <= 448 * 2^e, e >= -117); what is not finite becomes NaN, and
+ * what would round to 2^128 becomes 15/16 of it.  out: contiguous,
+ * of x's dtype.  Sums are fp32. */
+size_t cresso_block_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, const void* w, int64_t w_stride,
+                                            int32_t turned);
+int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int64_t depth,
+                             const void* w, int64_t w_stride, const float* scales, int64_t scale_stride, int32_t turned,
+                             void* out, void* workspace, size_t workspace_bytes, void* stream);
+/* A weight [rows][cols] to e4m3 values and scales (max/448 of each block). */
+int32_t cresso_block_quantize(const void* w, int64_t w_stride, int32_t dtype, int64_t rows, int64_t cols, void* values,
+                              float* scales, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
