@@ -295,54 +295,32 @@ def stream_handle(device: torch.device) -> int:
 
 
 # ---------------------------------------------------------------------------
-# what the operators' front ends share
+# the operators' host side (csrc/operators.cpp)
 # ---------------------------------------------------------------------------
-ROW_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_OPS = None
+OPERATOR_SYMBOLS = (
+    "cresso_hip_last_error", "cresso_embedding_forward", "cresso_embedding_backward_workspace_bytes",
+    "cresso_embedding_backward", "cresso_residual_norm_forward", "cresso_residual_norm_backward_workspace_bytes",
+    "cresso_residual_norm_backward", "cresso_distill_loss", "cresso_distill_backward",
+    "cresso_block_product_workspace_bytes", "cresso_block_product", "cresso_block_quantize")
 
 
-def require(ok: bool, what: str, why: str) -> None:
-    if not ok:
-        raise ValueError(f"{what}: {why}")
+def operators():
+    """The operators' C++ host side, bound to the loaded library; RuntimeError if either is missing."""
+    global _OPS
+    if _OPS is None:
+        lib = load()
+        try:
+            from . import _operators as ops  # type: ignore[attr-defined]
+        except ImportError as exc:
+            raise RuntimeError(f"CRESSO5 CUDA ops failed to load: {exc}; build them with `python -m cresso_amd.build`") from exc
+        ops.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in OPERATOR_SYMBOLS})
+        _OPS = ops
+    return _OPS
 
 
-def require_gpu(what: str, **tensors) -> torch.device:
-    """Every tensor given is on the same GPU; -> its device.  There is no CPU path."""
-    device = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not torch.is_tensor(t):
+def check_tensors(what: str, **given) -> None:
+    """ValueError for the first of `given` that is neither a tensor nor None (the C++ side has refused the call's types)."""
+    for name, t in given.items():
+        if t is not None and not torch.is_tensor(t):
             raise ValueError(f"{what}: {name} must be a tensor, not {type(t).__name__}")
-        if not t.is_cuda:
-            raise RuntimeError(f"{what}: {name} is on {t.device}; the operators run on the GPU only")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise RuntimeError(f"{what}: {name} is on {t.device}, others on {device}")
-    return device
-
-
-def rows_of(t: torch.Tensor) -> tuple:
-    """t seen as rows of its last dimension -> (tensor, row stride in elements).
-    Rows at one stride are taken where they lie; anything else is copied."""
-    if t.ndim == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
-        return t, t.stride(0)
-    if not t.is_contiguous():
-        t = t.contiguous()
-    return t, t.shape[-1] if t.ndim else 1
-
-
-def call(fn, what: str, device: torch.device, *args) -> None:
-    """One library call on the device's current stream (the call's last argument)."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    if rc != 0:
-        check(rc, what)
-
-
-def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
-    """Scratch of one call, from torch's allocator on the current stream."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)

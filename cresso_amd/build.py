@@ -31,37 +31,42 @@ def sources():
     return sorted(CSRC.glob("*.hip"))
 
 
-HOST_SRC = CSRC / "host_batch.cpp"
+# torch C++ extensions of the host side: source -> module
+HOST_EXTENSIONS = {"host_batch.cpp": "_hostbatch", "operators.cpp": "_operators"}
 
 
-def host_ext_path() -> Path:
+def host_ext_path(module: str) -> Path:
     import sysconfig
 
-    return HERE / ("_hostbatch" + sysconfig.get_config_var("EXT_SUFFIX"))
+    return HERE / (module + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
-def host_cmd() -> list:
-    """g++ line of the host bookkeeping extension (a torch C++ extension, CPU only)."""
+def host_cmd(source: str, module: str) -> list:
+    """g++ line of a host extension (no device code)."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension as ce
 
-    inc = [f"-I{d}" for d in ce.include_paths()] + [f"-I{sysconfig.get_paths()['include']}"]
+    rocm = Path(hipcc()).resolve().parents[1]
+    inc = [f"-I{d}" for d in ce.include_paths()] + [f"-I{sysconfig.get_paths()['include']}", f"-I{rocm / 'include'}"]
     libdir = ce.library_paths()[0]
     abi = int(bool(torch._C._GLIBCXX_USE_CXX11_ABI))
-    tmp = host_ext_path().with_suffix(".tmp")
-    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", str(HOST_SRC), "-o", str(tmp), *inc,
-            "-DTORCH_EXTENSION_NAME=_hostbatch", "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-            f"-L{libdir}", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{libdir}"]
+    tmp = host_ext_path(module).with_suffix(".tmp")
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", str(CSRC / source), "-o", str(tmp), *inc,
+            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-DTORCH_EXTENSION_NAME={module}",
+            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", f"-L{libdir}", "-lc10", "-lc10_hip",
+            "-ltorch", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{libdir}"]
 
 
 def build(verbose: bool = False, jobs: int = 8) -> Path:
-    # the host extension (slowest compile: torch headers) starts first, in parallel
-    hcmd = host_cmd()
-    if verbose:
-        print(" ".join(hcmd), flush=True)
-    hproc = subprocess.Popen(hcmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    # the host extensions (slowest compiles: torch headers) start first, in parallel
+    hprocs = []
+    for source, module in HOST_EXTENSIONS.items():
+        hcmd = host_cmd(source, module)
+        if verbose:
+            print(" ".join(hcmd), flush=True)
+        hprocs.append((source, module, subprocess.Popen(hcmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     srcs = sources()
     objdir = HERE / "_build"
     objdir.mkdir(exist_ok=True)
@@ -89,10 +94,11 @@ def build(verbose: bool = False, jobs: int = 8) -> Path:
     if out.returncode != 0:
         raise RuntimeError("link failed:\n" + out.stdout.decode(errors="replace"))
     os.replace(tmp, LIB)
-    hout, _ = hproc.communicate()
-    if hproc.returncode != 0:
-        raise RuntimeError("g++ failed on host_batch.cpp:\n" + hout.decode(errors="replace"))
-    os.replace(host_ext_path().with_suffix(".tmp"), host_ext_path())
+    for source, module, hproc in hprocs:
+        hout, _ = hproc.communicate()
+        if hproc.returncode != 0:
+            raise RuntimeError(f"g++ failed on {source}:\n" + hout.decode(errors="replace"))
+        os.replace(host_ext_path(module).with_suffix(".tmp"), host_ext_path(module))
     return LIB
 
 

@@ -124,6 +124,14 @@ def test_infinities_stay_in_their_rows():
     assert torch.isinf(g[4]).all() and torch.isfinite(g[[0, 1, 2, 3, 5, 6, 7, 8]]).all()
 
 
+def test_no_second_derivative():
+    ids, table = torch.tensor([1, 2, 2]).cuda(), rand((5, 4)).requires_grad_(True)
+    by = rand((3, 4)).requires_grad_(True)
+    g, = torch.autograd.grad(cresso_amd.embedding(ids, table), table, by, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated twice"):
+        g.sum().backward()
+
+
 def test_another_stream():
     ids, table, grad = make_ids(5000, 300, "skewed").cuda(), rand((300, 256)), rand((5000, 256), seed=6)
     want_out, want = cresso_amd.embedding(ids, table), cresso_amd.embedding_grad(ids, grad, 300)
