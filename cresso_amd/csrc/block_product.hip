@@ -13,8 +13,13 @@
 // products of a group before they add them and keep 13 bits below the largest
 // (2^16 + 2^2 - 2^16 gives 0), which is 1.4e-5 of the result for normally
 // distributed numbers against 6e-9, and more where products differ in size.
-// A block's partial sum is multiplied by its fp32 scale when it is added to
-// the fp32 accumulator.
+//
+// A block's scale is split into a power of two, which the conversion of w to
+// bf16 applies exactly, and a factor f of magnitude 1 to 2.  The fp32
+// accumulators are kept in units of the current block's f and multiplied by
+// f_before / f_now where a block begins: one multiplication per accumulator
+// and block, and no second set of accumulators for a block's own sum, which
+// is what lets a wave hold 128 x 64 outputs.
 #include "row_ops.hpp"
 
 #include <algorithm>
@@ -26,7 +31,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int BP = 128;            // block of a scale
 constexpr int BP_NT = 256;
-constexpr int BP_TM = 128, BP_TN = 128;
 constexpr int BP_MIN_EXP = -117;   // the smallest step, 2^-9 * 2^-117, is a normal number
 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
@@ -87,7 +91,7 @@ __global__ __launch_bounds__(BP_NT) void round_rows_kernel(const T* x, int64_t r
 
 // ---------------------------------------------------------------------------
 // The weight's other layout: along n for the gradient (TURN), or only with
-// rows padded to whole 16-byte pieces.  64 x 64 bytes a block.
+// rows padded to whole blocks and 16-byte pieces.  64 x 64 bytes a block.
 // ---------------------------------------------------------------------------
 template <bool TURN>
 __global__ __launch_bounds__(BP_NT) void lay_out_kernel(const uint8_t* w, int64_t rows, int64_t cols, int64_t stride,
@@ -118,107 +122,170 @@ struct ProductArgs {
     const uint8_t* w;
     const float* scales;
     void* out;
-    int64_t rows, cols, depth;          // m, n, k
+    int64_t rows, cols, depth;          // m, n, k: depth is whole blocks
     int64_t r_stride, w_stride, out_stride;
     int64_t scale_n, scale_k;           // strides of the scales along n's and k's blocks
+    uint32_t tiles_m, tiles_n;
 };
 
-// Byte offsets in the tiles, whose rows are one block of k: 256 bytes of r,
-// 128 of w.  The 16-byte pieces of a row change places by the row's number, so
-// that 16 rows' pieces of one column lie in different banks.
-__device__ __forceinline__ int r_at(int row, int piece) { return row * 256 + ((piece ^ (row & 15)) * 16); }
-__device__ __forceinline__ int w_at(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) * 16); }
+// Byte offsets in the tiles of a stage, whose rows are 64 of k: 128 bytes of
+// r, 64 of w.  The 16-byte pieces of a row change places by the row's number,
+// so that the 16 rows that a wave reads at once lie in different banks.
+constexpr int BK = 64;
+__device__ __forceinline__ int r_at(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) * 16); }
+__device__ __forceinline__ int w_at(int row, int piece) { return row * 64 + ((piece ^ ((row >> 4) & 3)) * 16); }
 
-// eight e4m3 values as bf16
-__device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+// eight e4m3 values times a power of two as bf16
+__device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, float unit) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, unit, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, unit, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, unit, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, unit, true);
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-template <typename T>
-__global__ __launch_bounds__(BP_NT) void product_kernel(ProductArgs a) {
-    __shared__ __align__(16) uint8_t rt[BP_TM * 256], wt[BP_TN * 128];
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const int64_t m0 = (int64_t)blockIdx.y * BP_TM, n0 = (int64_t)blockIdx.x * BP_TN;
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+// s = unit * f: a power of two between 2^-100 and 2^100, and the rest (1 to 2
+// in magnitude unless s is beyond those).  A scale of 0 keeps f = 1 and is
+// told by `zero`: its block counts as zeros.
+struct SplitScale {
+    float unit, f;
+    bool zero;
+};
+__device__ __forceinline__ SplitScale split_scale(float s) {
+    SplitScale r{1.0f, 1.0f, s == 0.0f};
+    if (!r.zero) {
+        int e;
+        frexpf(s, &e);
+        e = min(max(e - 1, -100), 100);
+        r.unit = ldexpf(1.0f, e);
+        r.f = ldexpf(s, -e);
+    }
+    return r;
+}
+
+// Tile of a workgroup.  Workgroups go to the 8 XCDs in turn; each XCD takes a
+// run of tiles, in columns of 8 tiles of m, so that the tiles that run
+// together on one XCD share rows of both operands in its L2.
+__device__ __forceinline__ void tile_of(const ProductArgs& a, uint32_t& tm, uint32_t& tn) {
+    const uint32_t total = a.tiles_m * a.tiles_n, per = total / 8, rest = total % 8;
+    const uint32_t xcd = blockIdx.x % 8, i = blockIdx.x / 8;
+    uint32_t t = xcd * per + min(xcd, rest) + i;
+    const uint32_t group = 8 * a.tiles_n, g = t / group, in = t - g * group;
+    const uint32_t height = min(8u, a.tiles_m - g * 8);
+    tm = g * 8 + in % height;
+    tn = in / height;
+}
+
+// 16 bytes a lane from global memory to LDS: lane i's go to lds + 16 * i.
+__device__ __forceinline__ void load_lds(const char* from, uint8_t* lds) {
+    __builtin_amdgcn_global_load_lds((const CRESSO_GLOBAL uint32_t*)from, (__attribute__((address_space(3))) uint32_t*)lds, 16, 0, 0);
+}
+// Waits until at most N of the wave's loads are on their way and all its LDS
+// reads have ended (the stage they read is filled anew), then for the other waves.
+template <int N> __device__ __forceinline__ void stage_ready() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// WM x WN waves of FM x FN fragments of 16 x 16 each.  Three stages of LDS:
+// while one is multiplied, the next two are on their way from memory.
+template <typename T, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) {
+    constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16;
+    constexpr int RL = TM * 8 / NT, WL = TN * 4 / NT;   // 16-byte pieces a thread loads per stage
+    static_assert(RL * NT == TM * 8 && WL * NT == TN * 4 && FN == 4, "tile");
+    constexpr int STAGE = TM * 128 + TN * 64;
+    __shared__ __align__(16) uint8_t lds[3 * STAGE];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    uint32_t tm, tn;
+    tile_of(a, tm, tn);
+    const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
+    const int wm = (wave % WM) * (FM * 16), wn = (wave / WM) * (FN * 16);
     const int l16 = lane & 15, quad = lane >> 4;
-    f32x4 acc[4][4];   // [n][m]
+    f32x4 acc[FN][FM] = {};
+    // A thread's piece of the tile is the one whose place in LDS it fills.
+    // Rows beyond the end load the last row's numbers; what they give is not stored.
+    const char* const rbase = (const char*)(a.r + m0 * a.r_stride);
+    const char* const wbase = (const char*)(a.w + n0 * a.w_stride);
+    uint32_t ro[RL], wo[WL];   // byte offsets: a tile spans less than 2^32
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    const int64_t blocks = (a.depth + BP - 1) / BP;
-    for (int64_t b = 0; b < blocks; ++b) {
-        u32x4 gr[8], gw[4];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int piece = tid + i * BP_NT, row = piece >> 4, col = piece & 15;
-            gr[i] = u32x4{0, 0, 0, 0};
-            if (m0 + row < a.rows) gr[i] = *(const u32x4*)(a.r + (m0 + row) * a.r_stride + b * BP + col * 8);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int piece = tid + i * BP_NT, row = piece >> 3, col = piece & 7;
-            const int64_t k = b * BP + col * 16;
-            gw[i] = u32x4{0, 0, 0, 0};
-            if (n0 + row < a.cols && k < a.depth) gw[i] = *(const u32x4*)(a.w + (n0 + row) * a.w_stride + k);
-        }
-        const float sc = a.scales[n0 / BP * a.scale_n + b * a.scale_k];
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int piece = tid + i * BP_NT;
-            *(u32x4*)(rt + r_at(piece >> 4, piece & 15)) = gr[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int piece = tid + i * BP_NT;
-            *(u32x4*)(wt + w_at(piece >> 3, piece & 7)) = gw[i];
-        }
-        __syncthreads();
-        f32x4 p[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[i][j] = f32x4{0, 0, 0, 0};
-        // a lane's k: 32 of its quarter of the block, 8 for each of four steps
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            u32x4 fw[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) fw[i] = *(const u32x4*)(wt + w_at(wn + i * 16 + l16, quad * 2 + h));
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                bf16x8 fr[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) fr[j] = *(const bf16x8*)(rt + r_at(wm + j * 16 + l16, quad * 4 + h * 2 + s));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bf16x8 f = widen8(fw[i][2 * s], fw[i][2 * s + 1]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) p[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, fr[j], p[i][j], 0, 0, 0);
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] += p[i][j][e] * sc;
+    for (int i = 0; i < RL; ++i) {
+        const int place = tid + i * NT, row = place >> 3, piece = (place & 7) ^ ((row >> 1) & 7);
+        ro[i] = (uint32_t)min((int64_t)row, a.rows - 1 - m0) * (uint32_t)(a.r_stride * 2) + piece * 16;
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int i = 0; i < WL; ++i) {
+        const int place = tid + i * NT, row = place >> 2, piece = (place & 3) ^ ((row >> 4) & 3);
+        wo[i] = (uint32_t)min((int64_t)row, a.cols - 1 - n0) * (uint32_t)a.w_stride + piece * 16;
+    }
+    typedef const __attribute__((address_space(4))) float* scalar_floats;   // read once, by scalar loads
+    const scalar_floats sp = (scalar_floats)(uintptr_t)(a.scales + min(n0 + wn, a.cols - 1) / BP * a.scale_n);
+    const int stages = (int)(a.depth / BK);   // an even number
+    const auto fetch = [&](int k) {
+        uint8_t* to = lds + k % 3 * STAGE + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < RL; ++i) load_lds(rbase + (int64_t)k * (BK * 2) + ro[i], to + i * (NT * 16));
+#pragma unroll
+        for (int i = 0; i < WL; ++i) load_lds(wbase + (int64_t)k * BK + wo[i], to + TM * 128 + i * (NT * 16));
+    };
+    SplitScale now{1.0f, 1.0f, true};
+    if (stages) {
+        fetch(0);
+        fetch(1);
+    }
+    for (int k = 0; k < stages; ++k) {
+        if (k + 1 < stages) stage_ready<RL + WL>();
+        else stage_ready<0>();
+        if (k + 2 < stages) fetch(k + 2);
+        if (!(k & 1)) {   // a block begins
+            const SplitScale s = split_scale(sp[k / 2 * a.scale_k]);
+            const float by = now.f / s.f;
+            if (k) {
+#pragma unroll
+                for (int i = 0; i < FN; ++i)
+#pragma unroll
+                    for (int j = 0; j < FM; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] *= by;
+            }
+            now = s;
+        }
+        // a lane's k: 16 of its quarter of the stage, 8 for each of two steps;
+        // a fragment's row r of w is column 16*(r/4) + 4*i + r%4, so that a
+        // lane ends with 16 consecutive columns of a row of the result
+        const uint8_t* rt = lds + k % 3 * STAGE;
+        const uint8_t* wt = rt + TM * 128;
+        u32x4 fw[FN];
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            fw[i] = *(const u32x4*)(wt + w_at(wn + (l16 >> 2) * 16 + i * 4 + (l16 & 3), quad));
+            if (now.zero) fw[i] = u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            bf16x8 fr[FM];
+#pragma unroll
+            for (int j = 0; j < FM; ++j) fr[j] = *(const bf16x8*)(rt + r_at(wm + j * 16 + l16, quad * 2 + s));
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                const bf16x8 f = widen8(fw[i][2 * s], fw[i][2 * s + 1], now.unit);
+#pragma unroll
+                for (int j = 0; j < FM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, fr[j], acc[i][j], 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
         const int64_t m = m0 + wm + j * 16 + l16;
         if (m >= a.rows) continue;
+        constexpr int E = Unit<T>::n;
+        T* to = (T*)a.out + m * a.out_stride;
+        const int64_t n = n0 + wn + quad * 16;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t n = n0 + wn + i * 16 + quad * 4;
-            T* to = (T*)a.out + m * a.out_stride + n;
+        for (int u = 0; u < 16 / E; ++u) {
+            float v[E];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < a.cols) to[e] = from_w<T>(acc[i][j][e]);
+            for (int e = 0; e < E; ++e) v[e] = acc[(u * E + e) / 4][j][(u * E + e) % 4] * now.f;
+            store_unit(to, (n + u * E) / E, a.cols, narrow<T>(v));
         }
     }
 }
@@ -283,7 +350,7 @@ ProductLayout product_layout(int64_t rows, int64_t cols, int64_t depth, bool cop
     const auto take = [&](int64_t b) { const int64_t at = off; off = up(off + b, 256); return at; };
     o.r_stride = up(depth, BP);
     o.r = take(rows * o.r_stride * 2);
-    o.w_stride = up(depth, 16);
+    o.w_stride = up(depth, BP);
     if (copy) o.w = take(cols * o.w_stride);
     o.total = std::max<int64_t>(off, 256);
     return o;
@@ -298,7 +365,7 @@ int32_t check_product(const char* what, int64_t rows, int64_t cols, int64_t dept
     return CRESSO_OK;
 }
 bool needs_copy(const void* w, int64_t w_stride, int64_t depth, int32_t turned) {
-    return turned || depth % 16 || w_stride % 16 || ((uintptr_t)w & 15);
+    return turned || depth % BP || w_stride % 16 || ((uintptr_t)w & 15);
 }
 
 }  // namespace
@@ -342,7 +409,8 @@ extern "C" int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t
     if (depth > 0) {
         if (copy) {
             const int64_t r = turned ? depth : cols, c = turned ? cols : depth;   // the weight as it is held
-            const dim3 grid((uint32_t)(up(c, 64) / 64), (uint32_t)(up(r, 64) / 64));
+            // the laid-out rows' ends are written too
+            const dim3 grid((uint32_t)((turned ? up(c, 64) : o.w_stride) / 64), (uint32_t)((turned ? o.w_stride : up(r, 64)) / 64));
             if (turned)
                 hipLaunchKernelGGL(lay_out_kernel<true>, grid, dim3(BP_NT), 0, st, (const uint8_t*)w, r, c, w_stride,
                                    (uint8_t*)ws + o.w, o.w_stride);
@@ -358,8 +426,16 @@ extern "C" int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t
         });
     }
     with_row_dtype(dtype, [&](auto t) {
-        const dim3 grid((uint32_t)((cols + BP_TN - 1) / BP_TN), (uint32_t)((rows + BP_TM - 1) / BP_TM));
-        hipLaunchKernelGGL(product_kernel<decltype(t)>, grid, dim3(BP_NT), 0, st, a);
+        using T = decltype(t);
+        const auto go = [&](auto kernel, int tm, int tn, int threads) {
+            a.tiles_m = (uint32_t)((rows + tm - 1) / tm);
+            a.tiles_n = (uint32_t)((cols + tn - 1) / tn);
+            hipLaunchKernelGGL(kernel, dim3(a.tiles_m * a.tiles_n), dim3(threads), 0, st, a);
+        };
+        if (((rows + 255) / 256) * ((cols + 255) / 256) >= 256)
+            go(product_kernel<T, 2, 4, 8, 4>, 256, 256, 512);
+        else
+            go(product_kernel<T, 2, 2, 4, 4>, 128, 128, 256);
     });
     return launched("block product");
 }
