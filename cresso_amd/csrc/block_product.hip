@@ -128,12 +128,13 @@ struct ProductArgs {
     uint32_t tiles_m, tiles_n;
 };
 
-// Byte offsets in the tiles of a stage, whose rows are 64 of k: 128 bytes of
-// r, 64 of w.  The 16-byte pieces of a row change places by the row's number,
-// so that the 16 rows that a wave reads at once lie in different banks.
+// The tiles of a stage have rows of 64 of k: 128 bytes of r, 64 of w.  The
+// 16-byte pieces of a row change places by the row's number, so that 16 lanes
+// that read 16 bytes each in one cycle (0-3, 12-15, 20-23 and 24-27, and
+// likewise on) find them in different banks.
 constexpr int BK = 64;
-__device__ __forceinline__ int r_at(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) * 16); }
-__device__ __forceinline__ int w_at(int row, int piece) { return row * 64 + ((piece ^ ((row >> 4) & 3)) * 16); }
+__device__ __forceinline__ int r_turn(int row) { return ((row >> 1) & 7) ^ (row & 4); }
+__device__ __forceinline__ int w_turn(int row) { return ((row >> 4) & 1) * 2 + ((row >> 1) & 1); }
 
 // eight e4m3 values times a power of two as bf16
 __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, float unit) {
@@ -187,10 +188,13 @@ template <int N> __device__ __forceinline__ void stage_ready() {
 }
 
 // WM x WN waves of FM x FN fragments of 16 x 16 each.  Three stages of LDS:
-// while one is multiplied, the next two are on their way from memory.
+// while one is multiplied, the next two are on their way from memory.  A
+// stage is multiplied in four groups (two steps of k, two halves of the rows),
+// and each group's fragments are read from LDS while the group before is
+// multiplied, also across the barrier between two stages.
 template <typename T, int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) {
-    constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16;
+    constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16, H = FM / 2;
     constexpr int RL = TM * 8 / NT, WL = TN * 4 / NT;   // 16-byte pieces a thread loads per stage
     static_assert(RL * NT == TM * 8 && WL * NT == TN * 4 && FN == 4, "tile");
     constexpr int STAGE = TM * 128 + TN * 64;
@@ -204,74 +208,113 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
     f32x4 acc[FN][FM] = {};
     // A thread's piece of the tile is the one whose place in LDS it fills.
     // Rows beyond the end load the last row's numbers; what they give is not stored.
-    const char* const rbase = (const char*)(a.r + m0 * a.r_stride);
-    const char* const wbase = (const char*)(a.w + n0 * a.w_stride);
+    const char* rbase = (const char*)(a.r + m0 * a.r_stride);
+    const char* wbase = (const char*)(a.w + n0 * a.w_stride);
     uint32_t ro[RL], wo[WL];   // byte offsets: a tile spans less than 2^32
 #pragma unroll
     for (int i = 0; i < RL; ++i) {
-        const int place = tid + i * NT, row = place >> 3, piece = (place & 7) ^ ((row >> 1) & 7);
+        const int place = tid + i * NT, row = place >> 3, piece = (place & 7) ^ r_turn(row);
         ro[i] = (uint32_t)min((int64_t)row, a.rows - 1 - m0) * (uint32_t)(a.r_stride * 2) + piece * 16;
     }
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
-        const int place = tid + i * NT, row = place >> 2, piece = (place & 3) ^ ((row >> 4) & 3);
+        const int place = tid + i * NT, row = place >> 2, piece = (place & 3) ^ w_turn(row);
         wo[i] = (uint32_t)min((int64_t)row, a.cols - 1 - n0) * (uint32_t)a.w_stride + piece * 16;
     }
     typedef const __attribute__((address_space(4))) float* scalar_floats;   // read once, by scalar loads
     const scalar_floats sp = (scalar_floats)(uintptr_t)(a.scales + min(n0 + wn, a.cols - 1) / BP * a.scale_n);
-    const int stages = (int)(a.depth / BK);   // an even number
-    const auto fetch = [&](int k) {
-        uint8_t* to = lds + k % 3 * STAGE + wave * 1024;
+    const int blocks = (int)(a.depth / BP), stages = 2 * blocks;
+    int to = wave * 1024;   // where the next stage goes
+    int left = stages;      // that are not yet on their way; past the last one it is loaded again, and not used
+    const auto fetch = [&] {
 #pragma unroll
-        for (int i = 0; i < RL; ++i) load_lds(rbase + (int64_t)k * (BK * 2) + ro[i], to + i * (NT * 16));
+        for (int i = 0; i < RL; ++i) load_lds(rbase + ro[i], lds + to + i * (NT * 16));
 #pragma unroll
-        for (int i = 0; i < WL; ++i) load_lds(wbase + (int64_t)k * BK + wo[i], to + TM * 128 + i * (NT * 16));
+        for (int i = 0; i < WL; ++i) load_lds(wbase + wo[i], lds + to + TM * 128 + i * (NT * 16));
+        --left;
+        rbase += left > 0 ? BK * 2 : 0;
+        wbase += left > 0 ? BK : 0;
+        to = to >= 2 * STAGE ? to - 2 * STAGE : to + STAGE;
+    };
+    // a lane's k: 16 of its quarter of the stage, 8 for each of two steps; a
+    // fragment's row r of w is column 16*(r/4) + 4*i + r%4, so that a lane ends
+    // with 16 consecutive columns of a row of the result (i leaves w_turn as it is)
+    const int wrow = wn + (l16 >> 2) * 16 + (l16 & 3), wat = TM * 128 + wrow * 64 + ((quad ^ w_turn(wrow)) * 16);
+    const int rrow = wm + l16, rat[2] = {rrow * 128 + (((quad * 2) ^ r_turn(rrow)) * 16), rrow * 128 + (((quad * 2 + 1) ^ r_turn(rrow)) * 16)};
+    int from = 0;           // the stage that is read
+    u32x4 fw[FN];
+    bf16x8 fr[2][H];
+    const auto read_w = [&] {
+#pragma unroll
+        for (int i = 0; i < FN; ++i) fw[i] = *(const u32x4*)(lds + from + wat + i * 256);
+    };
+    const auto read_r = [&](int set, int s, int h) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) fr[set][j] = *(const bf16x8*)(lds + from + rat[s] + (h * H + j) * 2048);
+    };
+    bf16x8 f[FN];
+    const auto widen = [&](int s, const SplitScale& by) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i) f[i] = widen8(by.zero ? 0 : fw[i][2 * s], by.zero ? 0 : fw[i][2 * s + 1], by.unit);
+    };
+    const auto multiply = [&](int set, int h) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+                acc[i][h * H + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[i], fr[set][j], acc[i][h * H + j], 0, 0, 0);
+    };
+    const auto rescale = [&](int h, float by) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][h * H + j][e] *= by;
+    };
+    // Multiplies a stage and reads the first fragments of the next.  Where a
+    // block begins, the second half's accumulators are multiplied by `by` on
+    // the way; where it ends, the first half's, for the next block.
+    const auto stage = [&](const SplitScale& now, bool begins, float by) {
+        read_r(1, 0, 1);
+        if (begins) rescale(1, by);
+        widen(0, now);
+        multiply(0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        read_r(0, 1, 0);
+        multiply(1, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        read_r(1, 1, 1);
+        widen(1, now);
+        multiply(0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        stage_ready<RL + WL>();
+        fetch();
+        from = from >= 2 * STAGE ? 0 : from + STAGE;
+        read_w();
+        read_r(0, 0, 0);
+        if (!begins) rescale(0, by);
+        multiply(1, 1);
+        __builtin_amdgcn_sched_barrier(0);
     };
     SplitScale now{1.0f, 1.0f, true};
-    if (stages) {
-        fetch(0);
-        fetch(1);
-    }
-    for (int k = 0; k < stages; ++k) {
-        if (k + 1 < stages) stage_ready<RL + WL>();
-        else stage_ready<0>();
-        if (k + 2 < stages) fetch(k + 2);
-        if (!(k & 1)) {   // a block begins
-            const SplitScale s = split_scale(sp[k / 2 * a.scale_k]);
-            const float by = now.f / s.f;
-            if (k) {
-#pragma unroll
-                for (int i = 0; i < FN; ++i)
-#pragma unroll
-                    for (int j = 0; j < FM; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][j][e] *= by;
-            }
-            now = s;
+    if (blocks) {
+        fetch();
+        fetch();
+        fetch();
+        now = split_scale(sp[0]);
+        stage_ready<2 * (RL + WL)>();
+        read_w();
+        read_r(0, 0, 0);
+        float by = 1.0f;
+        for (int b = 0; b < blocks; ++b) {
+            const SplitScale next = split_scale(sp[min(b + 1, blocks - 1) * a.scale_k]);
+            stage(now, true, by);
+            by = now.f / next.f;
+            stage(now, false, by);
+            now = next;
         }
-        // a lane's k: 16 of its quarter of the stage, 8 for each of two steps;
-        // a fragment's row r of w is column 16*(r/4) + 4*i + r%4, so that a
-        // lane ends with 16 consecutive columns of a row of the result
-        const uint8_t* rt = lds + k % 3 * STAGE;
-        const uint8_t* wt = rt + TM * 128;
-        u32x4 fw[FN];
-#pragma unroll
-        for (int i = 0; i < FN; ++i) {
-            fw[i] = *(const u32x4*)(wt + w_at(wn + (l16 >> 2) * 16 + i * 4 + (l16 & 3), quad));
-            if (now.zero) fw[i] = u32x4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            bf16x8 fr[FM];
-#pragma unroll
-            for (int j = 0; j < FM; ++j) fr[j] = *(const bf16x8*)(rt + r_at(wm + j * 16 + l16, quad * 2 + s));
-#pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                const bf16x8 f = widen8(fw[i][2 * s], fw[i][2 * s + 1], now.unit);
-#pragma unroll
-                for (int j = 0; j < FM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, fr[j], acc[i][j], 0, 0, 0);
-            }
-        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way to LDS when the workgroup ends
     }
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
