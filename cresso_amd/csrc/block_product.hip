@@ -143,24 +143,38 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, float unit) {
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// s = unit * f: a power of two between 2^-100 and 2^100, and the rest (1 to 2
-// in magnitude unless s is beyond those).  A scale of 0 keeps f = 1 and is
-// told by `zero`: its block counts as zeros.
-struct SplitScale {
-    float unit, f;
-    bool zero;
+// The scales of a wave's columns, one block of k after another: lane i holds
+// that of block i of a run of 64.  s = unit * f: a power of two between 2^-100
+// and 2^100, and the rest (1 to 2 in magnitude unless s is beyond those); by is
+// the f before over this one.  A scale of 0 keeps f = 1 and is told by `zero`:
+// its block counts as zeros.
+struct BlockScale {
+    float unit, f, by;
+    uint32_t keep;   // 0 for a scale of 0, else all ones
 };
-__device__ __forceinline__ SplitScale split_scale(float s) {
-    SplitScale r{1.0f, 1.0f, s == 0.0f};
-    if (!r.zero) {
-        int e;
-        frexpf(s, &e);
-        e = min(max(e - 1, -100), 100);
-        r.unit = ldexpf(1.0f, e);
-        r.f = ldexpf(s, -e);
+struct BlockScales {
+    float unit, f, by;
+    uint32_t keep;
+    __device__ __forceinline__ void load(const float* s, int64_t stride, int first, int blocks, float f_before) {
+        const int lane = threadIdx.x & (kWave - 1);
+        const float v = s[(int64_t)min(first + lane, blocks - 1) * stride];
+        unit = f = 1.0f;
+        keep = v == 0.0f ? 0u : ~0u;
+        if (keep) {
+            int e;
+            frexpf(v, &e);
+            e = min(max(e - 1, -100), 100);
+            unit = ldexpf(1.0f, e);
+            f = ldexpf(v, -e);
+        }
+        const float before = __shfl_up(f, 1, kWave);
+        by = (lane ? before : first ? f_before : f) / f;
     }
-    return r;
-}
+    __device__ __forceinline__ BlockScale at(int b) const {
+        const auto lane = [&](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), b & 63)); };
+        return {lane(unit), lane(f), lane(by), (uint32_t)__builtin_amdgcn_readlane((int)keep, b & 63)};
+    }
+};
 
 // Tile of a workgroup.  Workgroups go to the 8 XCDs in turn; each XCD takes a
 // run of tiles, in columns of 8 tiles of m, so that the tiles that run
@@ -175,9 +189,9 @@ __device__ __forceinline__ void tile_of(const ProductArgs& a, uint32_t& tm, uint
     tn = in / height;
 }
 
-// 16 bytes a lane from global memory to LDS: lane i's go to lds + 16 * i.
-__device__ __forceinline__ void load_lds(const char* from, uint8_t* lds) {
-    __builtin_amdgcn_global_load_lds((const CRESSO_GLOBAL uint32_t*)from, (__attribute__((address_space(3))) uint32_t*)lds, 16, 0, 0);
+// 16 bytes a lane from a buffer to LDS: lane i's go to lds + 16 * i.
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, uint32_t lane_at, uint32_t at, uint8_t* lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)lds, 16, lane_at, at, 0, 0);
 }
 // Waits until at most N of the wave's loads are on their way and all its LDS
 // reads have ended (the stage they read is filled anew), then for the other waves.
@@ -185,6 +199,13 @@ template <int N> __device__ __forceinline__ void stage_ready() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+}
+
+// A group begins with its reads from LDS, whose data the next group needs.
+template <int READS> __device__ __forceinline__ void group_order() {
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // WM x WN waves of FM x FN fragments of 16 x 16 each.  Three stages of LDS:
@@ -208,32 +229,30 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
     f32x4 acc[FN][FM] = {};
     // A thread's piece of the tile is the one whose place in LDS it fills.
     // Rows beyond the end load the last row's numbers; what they give is not stored.
-    const char* rbase = (const char*)(a.r + m0 * a.r_stride);
-    const char* wbase = (const char*)(a.w + n0 * a.w_stride);
+    const int64_t rrows = min((int64_t)TM, a.rows - m0), wrows = min((int64_t)TN, a.cols - n0);
+    const __amdgpu_buffer_rsrc_t rbuf = make_rsrc(a.r + m0 * a.r_stride, (uint32_t)(rrows * a.r_stride * 2));
+    const __amdgpu_buffer_rsrc_t wbuf = make_rsrc(a.w + n0 * a.w_stride, (uint32_t)((wrows - 1) * a.w_stride + a.depth));
     uint32_t ro[RL], wo[WL];   // byte offsets: a tile spans less than 2^32
 #pragma unroll
     for (int i = 0; i < RL; ++i) {
         const int place = tid + i * NT, row = place >> 3, piece = (place & 7) ^ r_turn(row);
-        ro[i] = (uint32_t)min((int64_t)row, a.rows - 1 - m0) * (uint32_t)(a.r_stride * 2) + piece * 16;
+        ro[i] = (uint32_t)min((int64_t)row, rrows - 1) * (uint32_t)(a.r_stride * 2) + piece * 16;
     }
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
         const int place = tid + i * NT, row = place >> 2, piece = (place & 3) ^ w_turn(row);
-        wo[i] = (uint32_t)min((int64_t)row, a.cols - 1 - n0) * (uint32_t)a.w_stride + piece * 16;
+        wo[i] = (uint32_t)min((int64_t)row, wrows - 1) * (uint32_t)a.w_stride + piece * 16;
     }
-    typedef const __attribute__((address_space(4))) float* scalar_floats;   // read once, by scalar loads
-    const scalar_floats sp = (scalar_floats)(uintptr_t)(a.scales + min(n0 + wn, a.cols - 1) / BP * a.scale_n);
+    const float* const sp = a.scales + min(n0 + wn, a.cols - 1) / BP * a.scale_n;
     const int blocks = (int)(a.depth / BP), stages = 2 * blocks;
     int to = wave * 1024;   // where the next stage goes
-    int left = stages;      // that are not yet on their way; past the last one it is loaded again, and not used
+    int next = 0;           // the stage to load; past the last one that is loaded again, and not used
     const auto fetch = [&] {
 #pragma unroll
-        for (int i = 0; i < RL; ++i) load_lds(rbase + ro[i], lds + to + i * (NT * 16));
+        for (int i = 0; i < RL; ++i) load_lds(rbuf, ro[i], next * (BK * 2), lds + to + i * (NT * 16));
 #pragma unroll
-        for (int i = 0; i < WL; ++i) load_lds(wbase + wo[i], lds + to + TM * 128 + i * (NT * 16));
-        --left;
-        rbase += left > 0 ? BK * 2 : 0;
-        wbase += left > 0 ? BK : 0;
+        for (int i = 0; i < WL; ++i) load_lds(wbuf, wo[i], next * BK, lds + to + TM * 128 + i * (NT * 16));
+        next = min(next + 1, stages - 1);
         to = to >= 2 * STAGE ? to - 2 * STAGE : to + STAGE;
     };
     // a lane's k: 16 of its quarter of the stage, 8 for each of two steps; a
@@ -253,9 +272,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
         for (int j = 0; j < H; ++j) fr[set][j] = *(const bf16x8*)(lds + from + rat[s] + (h * H + j) * 2048);
     };
     bf16x8 f[FN];
-    const auto widen = [&](int s, const SplitScale& by) {
+    const auto widen = [&](int s, const BlockScale& by) {
 #pragma unroll
-        for (int i = 0; i < FN; ++i) f[i] = widen8(by.zero ? 0 : fw[i][2 * s], by.zero ? 0 : fw[i][2 * s + 1], by.unit);
+        for (int i = 0; i < FN; ++i) f[i] = widen8(fw[i][2 * s] & by.keep, fw[i][2 * s + 1] & by.keep, by.unit);
     };
     const auto multiply = [&](int set, int h) {
 #pragma unroll
@@ -275,19 +294,19 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
     // Multiplies a stage and reads the first fragments of the next.  Where a
     // block begins, the second half's accumulators are multiplied by `by` on
     // the way; where it ends, the first half's, for the next block.
-    const auto stage = [&](const SplitScale& now, bool begins, float by) {
+    const auto stage = [&](const BlockScale& now, bool begins, float by) {
         read_r(1, 0, 1);
         if (begins) rescale(1, by);
         widen(0, now);
         multiply(0, 0);
-        __builtin_amdgcn_sched_barrier(0);
+        group_order<H>();
         read_r(0, 1, 0);
         multiply(1, 1);
-        __builtin_amdgcn_sched_barrier(0);
+        group_order<H>();
         read_r(1, 1, 1);
         widen(1, now);
         multiply(0, 0);
-        __builtin_amdgcn_sched_barrier(0);
+        group_order<H>();
         stage_ready<RL + WL>();
         fetch();
         from = from >= 2 * STAGE ? 0 : from + STAGE;
@@ -295,23 +314,26 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
         read_r(0, 0, 0);
         if (!begins) rescale(0, by);
         multiply(1, 1);
-        __builtin_amdgcn_sched_barrier(0);
+        group_order<FN + H>();
     };
-    SplitScale now{1.0f, 1.0f, true};
+    BlockScale now{1.0f, 1.0f, 1.0f, 0u};
     if (blocks) {
+        BlockScales scales;
+        scales.load(sp, a.scale_k, 0, blocks, 1.0f);
+        now = scales.at(0);
         fetch();
         fetch();
         fetch();
-        now = split_scale(sp[0]);
         stage_ready<2 * (RL + WL)>();
         read_w();
         read_r(0, 0, 0);
-        float by = 1.0f;
         for (int b = 0; b < blocks; ++b) {
-            const SplitScale next = split_scale(sp[min(b + 1, blocks - 1) * a.scale_k]);
-            stage(now, true, by);
-            by = now.f / next.f;
-            stage(now, false, by);
+            if (((b + 1) & 63) == 0) scales.load(sp, a.scale_k, b + 1, blocks, now.f);
+            BlockScale next = now;
+            next.by = 1.0f;
+            if (b + 1 < blocks) next = scales.at(b + 1);
+            stage(now, true, now.by);
+            stage(now, false, next.by);
             now = next;
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way to LDS when the workgroup ends
@@ -408,7 +430,8 @@ int32_t check_product(const char* what, int64_t rows, int64_t cols, int64_t dept
     return CRESSO_OK;
 }
 bool needs_copy(const void* w, int64_t w_stride, int64_t depth, int32_t turned) {
-    return turned || depth % BP || w_stride % 16 || ((uintptr_t)w & 15);
+    // the kernel takes whole blocks of k, aligned 16-byte pieces, and 32-bit places in a tile's rows
+    return turned || depth % BP || w_stride % 16 || ((uintptr_t)w & 15) || w_stride >= (int64_t)1 << 23;
 }
 
 }  // namespace
