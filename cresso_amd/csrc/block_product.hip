@@ -36,80 +36,115 @@ constexpr int BP_MIN_EXP = -117;   // the smallest step, 2^-9 * 2^-117, is a nor
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 // ---------------------------------------------------------------------------
-// x rounded to e4m3 times a power of two, as bf16: 16 lanes hold one row's 128
-// elements
+// x rounded to e4m3 times a power of two, as bf16
 // ---------------------------------------------------------------------------
+constexpr uint32_t BP_INF = 0x7f800000u;
+__device__ __forceinline__ float float_of(uint32_t b) { return __builtin_bit_cast(float, b); }
+__device__ __forceinline__ uint32_t bits_of(float v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ __forceinline__ uint32_t raw_of(bf16x2 v) { return __builtin_bit_cast(uint32_t, v); }
+
+// N values of a row's block, the rest of which other lanes hold; join(u) is
+// the largest u among those lanes.  All lanes of the wave take part.
+template <int N, typename Join>
+__device__ __forceinline__ void round_block(float (&v)[N], uint32_t (&out)[N / 2], Join&& join) {
+    uint32_t top = 0;   // largest magnitude, as bits: they order as the numbers do
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = max(top, bits_of(v[i]) & 0x7fffffffu);
+    top = join(top);
+    const bool odd = top >= BP_INF;
+    if (__any(odd)) {   // of the finite ones
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t u = bits_of(v[i]) & 0x7fffffffu;
+            top = max(top, u < BP_INF ? u : 0u);
+        }
+        top = join(top);
+    }
+    // top = 1.m * 2^(E-127) <= 448 * 2^e = 1.75 * 2^(e+8)
+    const int e = max(BP_MIN_EXP, (int)(top >> 23) - 135 + ((top & 0x7fffffu) > 0x600000u));
+    const float down = float_of((uint32_t)(127 - e) << 23), up = float_of((uint32_t)(127 + e) << 23);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] *= down;
+    if (__any(odd || e == 120)) {   // no infinities in the format; 256 * 2^120 is beyond fp32
+        const float most = e == 120 ? 240.0f : 448.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = fabsf(v[i]) < INFINITY ? fminf(fmaxf(v[i], -most), most) : __builtin_nanf("");
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+        out[i] = raw_of(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2 * i], v[2 * i + 1], 0, false), up, false));
+}
+
+// N values from column `at` of a row of `width` (0 beyond it); N is whole units
+template <typename T, int N> __device__ __forceinline__ void load_values(const T* row, int64_t at, int64_t width, float (&v)[N]) {
+    constexpr int E = Unit<T>::n;
+#pragma unroll
+    for (int u = 0; u < N / E; ++u) {
+        float t[E];
+        widen<T>(load_unit(row, at / E + u, width), t);
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[u * E + i] = t[i];
+    }
+}
+
+// 16 lanes hold one row's 128 elements.
 template <typename T>
 __global__ __launch_bounds__(BP_NT) void round_rows_kernel(const T* x, int64_t rows, int64_t width, int64_t stride,
                                                            uint16_t* q, int64_t q_stride) {
     const int64_t blocks = q_stride / BP;
     const int64_t job = ((int64_t)blockIdx.x * BP_NT + threadIdx.x) / 16;
-    const int part = threadIdx.x & 15;
-    if (job >= rows * blocks) return;
-    const int64_t row = job / blocks, b = job - row * blocks, at = b * BP + part * 8;
+    const bool on = job < rows * blocks;
+    const int64_t row = on ? job / blocks : 0, at = on ? (job - row * blocks) * BP + (threadIdx.x & 15) * 8 : width;
     float v[8];
-    const T* p = x + row * stride;
-    if constexpr (sizeof(T) == 4) {
-        float lo[4], hi[4];
-        widen<T>(load_unit(p, at / 4, width), lo);
-        widen<T>(load_unit(p, at / 4 + 1, width), hi);
+    load_values(x + row * stride, at, width, v);
+    uint32_t r[4];
+    round_block(v, r, [](uint32_t u) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = lo[i];
-            v[4 + i] = hi[i];
-        }
-    } else {
-        widen<T>(load_unit(p, at / 8, width), v);
-    }
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.0f);
-#pragma unroll
-    for (int m = 8; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, kWave));
-    int e = 0;
-    if (top > 0.0f) {
-        const float f = frexpf(top, &e);   // top = f * 2^e, 0.5 <= f < 1; 448 = 0.875 * 2^9
-        e = max(BP_MIN_EXP, e - 9 + (f > 0.875f));
-    }
-    const float unit = ldexpf(1.0f, e);
-    const float most = e == 120 ? 240.0f : 448.0f;   // 256 * 2^120 is beyond fp32
-    u32x4 r;
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-        float t[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            t[i] = ldexpf(v[2 * h + i], -e);
-            // the format has no infinities
-            t[i] = fabsf(t[i]) < INFINITY ? fminf(fmaxf(t[i], -most), most) : __builtin_nanf("");
-        }
-        const uint32_t pair = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t[0], t[1], 0, false);
-        r[h] = narrow2<__hip_bfloat16>(__builtin_amdgcn_cvt_f32_fp8(pair, 0) * unit, __builtin_amdgcn_cvt_f32_fp8(pair, 1) * unit);
-    }
-    *(u32x4*)(q + row * q_stride + at) = r;
+        for (int m = 8; m >= 1; m >>= 1) u = max(u, (uint32_t)__shfl_xor((int)u, m, kWave));
+        return u;
+    });
+    if (on) *(u32x4*)(q + row * q_stride + at) = u32x4{r[0], r[1], r[2], r[3]};
 }
 
 // ---------------------------------------------------------------------------
 // The weight's other layout: along n for the gradient (TURN), or only with
-// rows padded to whole blocks and 16-byte pieces.  64 x 64 bytes a block.
+// rows padded to whole blocks and 16-byte pieces.  64 x 64 bytes a workgroup,
+// 16 a lane in and out; turned, a lane gathers 16 bytes of a column from LDS,
+// whose rows are 17 words apart, so that a wave's four runs of 16 rows lie 16
+// banks from one another.
 // ---------------------------------------------------------------------------
+__device__ __forceinline__ u32x4 load_bytes(const uint8_t* p, int64_t left) {
+    if (left >= 16) return ((const CRESSO_GLOBAL Raw16h*)p)->v;
+    u32x4 r = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 15; ++i)
+        if (i < left) r[i / 4] |= (uint32_t)((const CRESSO_GLOBAL uint8_t*)p)[i] << (8 * (i & 3));
+    return r;
+}
 template <bool TURN>
 __global__ __launch_bounds__(BP_NT) void lay_out_kernel(const uint8_t* w, int64_t rows, int64_t cols, int64_t stride,
                                                         uint8_t* out, int64_t out_stride) {
-    __shared__ uint8_t tile[64][68];
+    const int a = threadIdx.x >> 2, b = (threadIdx.x & 3) * 16;
     const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
-    for (int i = threadIdx.x; i < 64 * 64; i += BP_NT) {
-        const int r = i / 64, c = i & 63;
-        tile[r][c] = r0 + r < rows && c0 + c < cols ? w[(r0 + r) * stride + c0 + c] : 0;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 64; i += BP_NT) {
-        const int a = i / 64, b = i & 63;
-        if constexpr (TURN) {
-            if (c0 + a < cols && r0 + b < out_stride) out[(c0 + a) * out_stride + r0 + b] = tile[b][a];
-        } else {
-            if (r0 + a < rows && c0 + b < out_stride) out[(r0 + a) * out_stride + c0 + b] = tile[a][b];
+    u32x4 v = {0, 0, 0, 0};
+    if (r0 + a < rows) v = load_bytes(w + (r0 + a) * stride + c0 + b, cols - c0 - b);
+    if constexpr (TURN) {
+        __shared__ uint32_t tile[64][17];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tile[a][b / 4 + i] = v[i];
+        __syncthreads();
+        if (c0 + a >= cols) return;
+        const uint8_t* from = (const uint8_t*)tile + a;   // column a, rows b on
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i] |= (uint32_t)from[(b + 4 * i + k) * 68] << (8 * k);
         }
+        *(u32x4*)(out + (c0 + a) * out_stride + r0 + b) = v;
+    } else {
+        if (r0 + a < rows) *(u32x4*)(out + (r0 + a) * out_stride + c0 + b) = v;
     }
 }
 
@@ -134,7 +169,13 @@ struct ProductArgs {
 // likewise on) find them in different banks.
 constexpr int BK = 64;
 __device__ __forceinline__ int r_turn(int row) { return ((row >> 1) & 7) ^ (row & 4); }
-__device__ __forceinline__ int w_turn(int row) { return ((row >> 4) & 1) * 2 + ((row >> 1) & 1); }
+// r of the 16 columns of a fragment of w: row of the tile of w
+template <int FN> __device__ __forceinline__ int w_row(int r) { return (r >> 2) * (4 * FN) + (r & 3); }
+template <int FN> __device__ __forceinline__ int w_turn(int row) {
+    if constexpr (FN == 4) return ((row >> 4) & 1) * 2 + ((row >> 1) & 1);
+    const int a = row / (4 * FN);
+    return ((a ^ (a >> 1)) & 1) * 2 + ((a >> 1) & 1);
+}
 
 // eight e4m3 values times a power of two as bf16
 __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, float unit) {
@@ -143,11 +184,18 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, float unit) {
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// s = unit * f: a power of two between 2^-100 and 2^100, and the rest (1 to 2
+// in magnitude unless s is 0 or beyond those).  With the power of two in w no
+// sum of products overflows that does not in the result.
+__device__ __forceinline__ void split_scale(float s, float& unit, float& f) {
+    const int e = min(max((int)((bits_of(s) >> 23) & 255) - 127, -100), 100);
+    unit = float_of((uint32_t)(127 + e) << 23);
+    f = s * float_of((uint32_t)(127 - e) << 23);
+}
+
 // The scales of a wave's columns, one block of k after another: lane i holds
-// that of block i of a run of 64.  s = unit * f: a power of two between 2^-100
-// and 2^100, and the rest (1 to 2 in magnitude unless s is beyond those); by is
-// the f before over this one.  A scale of 0 keeps f = 1 and is told by `zero`:
-// its block counts as zeros.
+// that of block i of a run of 64; by is the f before over this one.  A scale of
+// 0 has f = 1, and `keep` makes its block count as zeros.
 struct BlockScale {
     float unit, f, by;
     uint32_t keep;   // 0 for a scale of 0, else all ones
@@ -158,15 +206,9 @@ struct BlockScales {
     __device__ __forceinline__ void load(const float* s, int64_t stride, int first, int blocks, float f_before) {
         const int lane = threadIdx.x & (kWave - 1);
         const float v = s[(int64_t)min(first + lane, blocks - 1) * stride];
-        unit = f = 1.0f;
+        split_scale(v, unit, f);
         keep = v == 0.0f ? 0u : ~0u;
-        if (keep) {
-            int e;
-            frexpf(v, &e);
-            e = min(max(e - 1, -100), 100);
-            unit = ldexpf(1.0f, e);
-            f = ldexpf(v, -e);
-        }
+        if (!keep) f = 1.0f;
         const float before = __shfl_up(f, 1, kWave);
         by = (lane ? before : first ? f_before : f) / f;
     }
@@ -209,15 +251,19 @@ template <int READS> __device__ __forceinline__ void group_order() {
 }
 
 // WM x WN waves of FM x FN fragments of 16 x 16 each.  Three stages of LDS:
-// while one is multiplied, the next two are on their way from memory.  A
-// stage is multiplied in four groups (two steps of k, two halves of the rows),
-// and each group's fragments are read from LDS while the group before is
-// multiplied, also across the barrier between two stages.
+// while one is multiplied, the next two are on their way from memory.
+// Fragments are read from LDS a group of matrix instructions before they are
+// needed, also across the barrier between two stages.  A group is a quarter of
+// a stage where a wave has many rows (FM = 8: one of two steps of k, one half of
+// the rows), since there are no registers for more; a whole stage otherwise,
+// as fewer instructions do not cover the latency of LDS.
 template <typename T, int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) {
-    constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16, H = FM / 2;
+    constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16;
+    constexpr bool QUARTERS = FM > 4;
+    constexpr int H = QUARTERS ? FM / 2 : FM, SETS = QUARTERS ? 1 : 2;
     constexpr int RL = TM * 8 / NT, WL = TN * 4 / NT;   // 16-byte pieces a thread loads per stage
-    static_assert(RL * NT == TM * 8 && WL * NT == TN * 4 && FN == 4, "tile");
+    static_assert(RL * NT == TM * 8 && WL * NT == TN * 4, "tile");
     constexpr int STAGE = TM * 128 + TN * 64;
     __shared__ __align__(16) uint8_t lds[3 * STAGE];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -240,7 +286,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
     }
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
-        const int place = tid + i * NT, row = place >> 2, piece = (place & 3) ^ w_turn(row);
+        const int place = tid + i * NT, row = place >> 2, piece = (place & 3) ^ w_turn<FN>(row);
         wo[i] = (uint32_t)min((int64_t)row, wrows - 1) * (uint32_t)a.w_stride + piece * 16;
     }
     const float* const sp = a.scales + min(n0 + wn, a.cols - 1) / BP * a.scale_n;
@@ -256,25 +302,24 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
         to = to >= 2 * STAGE ? to - 2 * STAGE : to + STAGE;
     };
     // a lane's k: 16 of its quarter of the stage, 8 for each of two steps; a
-    // fragment's row r of w is column 16*(r/4) + 4*i + r%4, so that a lane ends
-    // with 16 consecutive columns of a row of the result (i leaves w_turn as it is)
-    const int wrow = wn + (l16 >> 2) * 16 + (l16 & 3), wat = TM * 128 + wrow * 64 + ((quad ^ w_turn(wrow)) * 16);
+    // fragment's row r of w is column 4*FN*(r/4) + 4*i + r%4, so that a lane ends
+    // with 4*FN consecutive columns of a row of the result (i leaves w_turn as it is)
+    const int wrow = wn + w_row<FN>(l16), wat = TM * 128 + wrow * 64 + ((quad ^ w_turn<FN>(wrow)) * 16);
     const int rrow = wm + l16, rat[2] = {rrow * 128 + (((quad * 2) ^ r_turn(rrow)) * 16), rrow * 128 + (((quad * 2 + 1) ^ r_turn(rrow)) * 16)};
     int from = 0;           // the stage that is read
-    u32x4 fw[FN];
-    bf16x8 fr[2][H];
-    const auto read_w = [&] {
+    u32x4 fw[SETS][FN];
+    bf16x8 fr[2 * SETS][H], f[FN];
+    const auto read_w = [&](int set) {
 #pragma unroll
-        for (int i = 0; i < FN; ++i) fw[i] = *(const u32x4*)(lds + from + wat + i * 256);
+        for (int i = 0; i < FN; ++i) fw[set][i] = *(const u32x4*)(lds + from + wat + i * 256);
     };
     const auto read_r = [&](int set, int s, int h) {
 #pragma unroll
         for (int j = 0; j < H; ++j) fr[set][j] = *(const bf16x8*)(lds + from + rat[s] + (h * H + j) * 2048);
     };
-    bf16x8 f[FN];
-    const auto widen = [&](int s, const BlockScale& by) {
+    const auto widen = [&](int set, int s, const BlockScale& by) {
 #pragma unroll
-        for (int i = 0; i < FN; ++i) f[i] = widen8(fw[i][2 * s] & by.keep, fw[i][2 * s + 1] & by.keep, by.unit);
+        for (int i = 0; i < FN; ++i) f[i] = widen8(fw[set][i][2 * s] & by.keep, fw[set][i][2 * s + 1] & by.keep, by.unit);
     };
     const auto multiply = [&](int set, int h) {
 #pragma unroll
@@ -291,30 +336,47 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[i][h * H + j][e] *= by;
     };
-    // Multiplies a stage and reads the first fragments of the next.  Where a
-    // block begins, the second half's accumulators are multiplied by `by` on
-    // the way; where it ends, the first half's, for the next block.
-    const auto stage = [&](const BlockScale& now, bool begins, float by) {
-        read_r(1, 0, 1);
-        if (begins) rescale(1, by);
-        widen(0, now);
-        multiply(0, 0);
-        group_order<H>();
-        read_r(0, 1, 0);
-        multiply(1, 1);
-        group_order<H>();
-        read_r(1, 1, 1);
-        widen(1, now);
-        multiply(0, 0);
-        group_order<H>();
+    const auto turn = [&] {   // to the next stage
         stage_ready<RL + WL>();
         fetch();
         from = from >= 2 * STAGE ? 0 : from + STAGE;
-        read_w();
-        read_r(0, 0, 0);
-        if (!begins) rescale(0, by);
-        multiply(1, 1);
-        group_order<FN + H>();
+    };
+    // Multiplies a stage, the first or second of its block, and reads the first
+    // fragments of the next.  The accumulators are multiplied by the block's
+    // `by` on the way; in quarters the second half's where the block begins
+    // and the first half's where the one before it ends.
+    const auto stage = [&](const BlockScale& now, const BlockScale& next, int second) {
+        if constexpr (QUARTERS) {
+            read_r(1, 0, 1);
+            if (!second) rescale(1, now.by);
+            widen(0, 0, now);
+            multiply(0, 0);
+            group_order<H>();
+            read_r(0, 1, 0);
+            multiply(1, 1);
+            group_order<H>();
+            read_r(1, 1, 1);
+            widen(0, 1, now);
+            multiply(0, 0);
+            group_order<H>();
+            turn();
+            read_w(0);
+            read_r(0, 0, 0);
+            if (second) rescale(0, next.by);
+            multiply(1, 1);
+            group_order<FN + H>();
+        } else {
+            turn();
+            read_w(second ^ 1);
+            read_r((second ^ 1) * 2, 0, 0);
+            read_r((second ^ 1) * 2 + 1, 1, 0);
+            if (!second) rescale(0, now.by);
+            widen(second, 0, now);
+            multiply(second * 2, 0);
+            widen(second, 1, now);
+            multiply(second * 2 + 1, 0);
+            group_order<FN + 2 * H>();
+        }
     };
     BlockScale now{1.0f, 1.0f, 1.0f, 0u};
     if (blocks) {
@@ -325,15 +387,16 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
         fetch();
         fetch();
         stage_ready<2 * (RL + WL)>();
-        read_w();
+        read_w(0);
         read_r(0, 0, 0);
+        if constexpr (!QUARTERS) read_r(1, 1, 0);
         for (int b = 0; b < blocks; ++b) {
             if (((b + 1) & 63) == 0) scales.load(sp, a.scale_k, b + 1, blocks, now.f);
             BlockScale next = now;
             next.by = 1.0f;
             if (b + 1 < blocks) next = scales.at(b + 1);
-            stage(now, true, now.by);
-            stage(now, false, next.by);
+            stage(now, next, 0);
+            stage(now, next, 1);
             now = next;
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way to LDS when the workgroup ends
@@ -342,16 +405,100 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
     for (int j = 0; j < FM; ++j) {
         const int64_t m = m0 + wm + j * 16 + l16;
         if (m >= a.rows) continue;
-        constexpr int E = Unit<T>::n;
         T* to = (T*)a.out + m * a.out_stride;
-        const int64_t n = n0 + wn + quad * 16;
+        const int64_t n = n0 + wn + quad * (4 * FN);
+        constexpr int E = Unit<T>::n;
+        if constexpr (4 * FN < E) {   // half a unit
+            const uint32_t lo = narrow2<T>(acc[0][j][0] * now.f, acc[0][j][1] * now.f), hi = narrow2<T>(acc[0][j][2] * now.f, acc[0][j][3] * now.f);
+            if (n + 4 <= a.cols) store8(to + n, u32x2{lo, hi});
+            else if (n < a.cols) store_part(to + n, u32x4{lo, hi, 0, 0}, (int)(a.cols - n));
+        } else {
 #pragma unroll
-        for (int u = 0; u < 16 / E; ++u) {
-            float v[E];
+            for (int u = 0; u < 4 * FN / E; ++u) {
+                float v[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = acc[(u * E + e) / 4][j][(u * E + e) % 4] * now.f;
-            store_unit(to, (n + u * E) / E, a.cols, narrow<T>(v));
+                for (int e = 0; e < E; ++e) v[e] = acc[(u * E + e) / 4][j][(u * E + e) % 4] * now.f;
+                store_unit(to, (n + u * E) / E, a.cols, narrow<T>(v));
+            }
         }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// At most 16 rows: bound by the weight's bytes, and below some megabytes by
+// latency.
+//
+// A workgroup takes 16 FN columns and all of k, its eight waves every eighth
+// block of 128 each; the waves' sums are added in LDS in their order.  The
+// weight goes from memory to registers, as it lies (any alignment); a lane's
+// 32 bytes of a row's block are the operand of four matrix instructions.  Each
+// wave rounds its part of the rows itself, in that same layout: repeated for
+// every workgroup, but the whole product is one launch.  The rounding is most
+// of the arithmetic, so wide weights take FN = 2 or 4, as long as that leaves a
+// workgroup for each CU.
+// ---------------------------------------------------------------------------
+constexpr int FEW_WAVES = 8;
+constexpr int FEW_ROWS = 16;
+
+template <typename T, int FN>
+__global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(ProductArgs a, const T* x, int64_t x_stride) {
+    __shared__ f32x4 sums[FEW_WAVES][FN][kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int l16 = lane & 15, quad = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * FN);
+    const int blocks = (int)((a.depth + BP - 1) / BP);
+    const uint8_t* wp[FN];
+#pragma unroll
+    for (int i = 0; i < FN; ++i) wp[i] = a.w + min(n0 + i * 16 + l16, a.cols - 1) * a.w_stride;
+    const float* sp = a.scales + n0 / BP * a.scale_n;   // 16 FN divides 128
+    const T* xp = x + min((int64_t)l16, a.rows - 1) * x_stride;
+    f32x4 acc[FN] = {};
+    for (int b = wave; b < blocks; b += FEW_WAVES) {
+        const int64_t k = (int64_t)b * BP + quad * 32;
+        u32x4 w[FN][2];
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[i][h] = load_bytes(wp[i] + k + h * 16, a.depth - k - h * 16);
+        const float scale = sp[b * a.scale_k];
+        float v[32];
+        load_values(xp, k, a.depth, v);
+        uint32_t u[16];
+        round_block(v, u, [](uint32_t t) {
+            t = max(t, (uint32_t)__shfl_xor((int)t, 16, kWave));
+            return max(t, (uint32_t)__shfl_xor((int)t, 32, kWave));
+        });
+        float unit, f;
+        split_scale(scale, unit, f);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            f32x4 p = {0, 0, 0, 0};
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    widen8(w[i][s / 2][2 * (s & 1)], w[i][s / 2][2 * (s & 1) + 1], unit),
+                    __builtin_bit_cast(bf16x8, u32x4{u[4 * s], u[4 * s + 1], u[4 * s + 2], u[4 * s + 3]}), p, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][e] += p[e] * f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < FN; ++i) sums[wave][i][lane] = acc[i];
+    __syncthreads();
+    if (wave >= FN) return;   // a wave for each fragment
+    f32x4 v = sums[0][wave][lane];
+#pragma unroll
+    for (int k = 1; k < FEW_WAVES; ++k) {
+        const f32x4 o = sums[k][wave][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += o[e];
+    }
+    const int64_t n = n0 + wave * 16 + quad * 4;
+    if (l16 < a.rows) {
+        T* to = (T*)a.out + l16 * a.out_stride + n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < a.cols) to[e] = from_w<T>(v[e]);
     }
 }
 
@@ -405,18 +552,39 @@ __global__ __launch_bounds__(BP_NT) void quantize_blocks_kernel(const T* w, int6
     }
 }
 
-struct ProductLayout {
+// How a product is computed: up to 16 rows in one launch (tile 0), more of them
+// rounded first and then multiplied in tiles.
+//
+// 256 x 256 tiles run one to a CU and 128 x 128 two, in rounds of 256 and 512;
+// a round of the first takes 1.6 to 1.9 times as long as one of the second
+// (16384 x 2048 x 5632 372 us in 6 rounds, 416 in 11; 4096 x 4096 x 4096 114 in
+// one, 122 in two; but 4352 x 2048 x 4352, 289 tiles of 256 or 1156 of 128, 111
+// us against 81).  Smaller tiles take over where
+// too few would be left for all CUs: 64 x 64 below 192 tiles of 128 (512 x 2048
+// x 5632 25.5 us against 26.9, but 1024 x 4096 x 4096 58 against 47), 32 x 64
+// below 256 tiles of 64 (200 x 2048 x 2048 13.0 us against 15.1, but 333 x
+// 4096 x 5632 38.7 against 36.9).
+struct ProductPlan {
+    int tile;
+    bool copy;   // the weight is laid out anew
     int64_t r, w, total, r_stride, w_stride;
 };
-// rows x cols outputs of depth `depth`; copy: the weight is laid out anew
-ProductLayout product_layout(int64_t rows, int64_t cols, int64_t depth, bool copy) {
-    ProductLayout o{};
+ProductPlan product_plan(int64_t rows, int64_t cols, int64_t depth, const void* weight, int64_t w_stride, int32_t turned) {
+    ProductPlan o{};
+    if (rows > FEW_ROWS) {
+        const auto tiles = [&](int64_t t) { return ((rows + t - 1) / t) * ((cols + t - 1) / t); };
+        const int64_t rounds256 = (tiles(256) + 255) / 256, rounds128 = (tiles(128) + 511) / 512;
+        if (50 * rounds256 <= 29 * rounds128) o.tile = 256;
+        else o.tile = tiles(128) >= 192 ? 128 : tiles(64) >= 256 ? 64 : 32;
+    }
+    // tiles take whole blocks of k, aligned 16-byte pieces, and 32-bit places in a tile's rows
+    o.copy = turned || (o.tile && (depth % BP || w_stride % 16 || ((uintptr_t)weight & 15) || w_stride >= (int64_t)1 << 23));
     int64_t off = 0;
     const auto take = [&](int64_t b) { const int64_t at = off; off = up(off + b, 256); return at; };
     o.r_stride = up(depth, BP);
-    o.r = take(rows * o.r_stride * 2);
+    if (o.tile) o.r = take(rows * o.r_stride * 2);
     o.w_stride = up(depth, BP);
-    if (copy) o.w = take(cols * o.w_stride);
+    if (o.copy) o.w = take(cols * o.w_stride);
     o.total = std::max<int64_t>(off, 256);
     return o;
 }
@@ -429,11 +597,6 @@ int32_t check_product(const char* what, int64_t rows, int64_t cols, int64_t dept
                     (long long)cols, (long long)depth);
     return CRESSO_OK;
 }
-bool needs_copy(const void* w, int64_t w_stride, int64_t depth, int32_t turned) {
-    // the kernel takes whole blocks of k, aligned 16-byte pieces, and 32-bit places in a tile's rows
-    return turned || depth % BP || w_stride % 16 || ((uintptr_t)w & 15) || w_stride >= (int64_t)1 << 23;
-}
-
 }  // namespace
 }  // namespace cresso
 
@@ -442,7 +605,7 @@ using namespace cresso;
 extern "C" size_t cresso_block_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, const void* w,
                                                        int64_t w_stride, int32_t turned) {
     if (check_product("block product", rows, cols, depth, CRESSO_F32) != CRESSO_OK) return 0;
-    return (size_t)product_layout(rows, cols, depth, needs_copy(w, w_stride, depth, turned)).total;
+    return (size_t)product_plan(rows, cols, depth, w, w_stride, turned).total;
 }
 
 extern "C" int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols,
@@ -453,8 +616,7 @@ extern "C" int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t
     if (rc != CRESSO_OK) return rc;
     if (rows == 0 || cols == 0) return CRESSO_OK;
     if (!out || (depth > 0 && (!x || !w || !scales))) return fail(CRESSO_E_INVALID, "block product: null argument");
-    const bool copy = needs_copy(w, w_stride, depth, turned);
-    const ProductLayout o = product_layout(rows, cols, depth, copy);
+    const ProductPlan o = product_plan(rows, cols, depth, w, w_stride, turned);
     if (!workspace || workspace_bytes < (size_t)o.total)
         return fail(CRESSO_E_INVALID, "block product: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)o.total);
     hipStream_t st = (hipStream_t)stream;
@@ -462,8 +624,8 @@ extern "C" int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t
     ProductArgs a{};
     a.r = (const uint16_t*)(ws + o.r);
     a.r_stride = o.r_stride;
-    a.w = copy ? (uint8_t*)ws + o.w : (const uint8_t*)w;
-    a.w_stride = copy ? o.w_stride : w_stride;
+    a.w = o.copy ? (uint8_t*)ws + o.w : (const uint8_t*)w;
+    a.w_stride = o.copy ? o.w_stride : w_stride;
     a.scales = scales;
     a.scale_n = turned ? 1 : scale_stride;
     a.scale_k = turned ? scale_stride : 1;
@@ -471,37 +633,44 @@ extern "C" int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t
     a.out_stride = cols;
     a.rows = rows;
     a.cols = cols;
-    a.depth = copy ? o.w_stride : depth;
-    if (depth > 0) {
-        if (copy) {
-            const int64_t r = turned ? depth : cols, c = turned ? cols : depth;   // the weight as it is held
-            // the laid-out rows' ends are written too
-            const dim3 grid((uint32_t)((turned ? up(c, 64) : o.w_stride) / 64), (uint32_t)((turned ? o.w_stride : up(r, 64)) / 64));
-            if (turned)
-                hipLaunchKernelGGL(lay_out_kernel<true>, grid, dim3(BP_NT), 0, st, (const uint8_t*)w, r, c, w_stride,
-                                   (uint8_t*)ws + o.w, o.w_stride);
-            else
-                hipLaunchKernelGGL(lay_out_kernel<false>, grid, dim3(BP_NT), 0, st, (const uint8_t*)w, r, c, w_stride,
-                                   (uint8_t*)ws + o.w, o.w_stride);
-        }
-        const int64_t jobs = rows * (o.r_stride / BP);
-        with_row_dtype(dtype, [&](auto t) {
-            using T = decltype(t);
-            hipLaunchKernelGGL(round_rows_kernel<T>, dim3((uint32_t)((jobs * 16 + BP_NT - 1) / BP_NT)), dim3(BP_NT), 0, st,
-                               (const T*)x, rows, depth, x_stride, (uint16_t*)(ws + o.r), o.r_stride);
-        });
+    a.depth = o.copy ? o.w_stride : depth;
+    if (o.copy && depth > 0) {
+        const int64_t r = turned ? depth : cols, c = turned ? cols : depth;   // the weight as it is held
+        // the laid-out rows' ends are written too
+        const dim3 grid((uint32_t)((turned ? up(c, 64) : o.w_stride) / 64), (uint32_t)((turned ? o.w_stride : up(r, 64)) / 64));
+        if (turned)
+            hipLaunchKernelGGL(lay_out_kernel<true>, grid, dim3(BP_NT), 0, st, (const uint8_t*)w, r, c, w_stride,
+                               (uint8_t*)ws + o.w, o.w_stride);
+        else
+            hipLaunchKernelGGL(lay_out_kernel<false>, grid, dim3(BP_NT), 0, st, (const uint8_t*)w, r, c, w_stride,
+                               (uint8_t*)ws + o.w, o.w_stride);
     }
     with_row_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const auto go = [&](auto kernel, int tm, int tn, int threads) {
+        if (!o.tile) {
+            a.depth = depth;   // x itself is not padded
+            const auto few = [&](auto kernel, int fn) {
+                hipLaunchKernelGGL(kernel, dim3((uint32_t)((cols + 16 * fn - 1) / (16 * fn))), dim3(FEW_WAVES * 64), 0, st, a, (const T*)x,
+                                   x_stride);
+            };
+            if (cols <= 4096) few(few_rows_kernel<T, 1>, 1);
+            else if (cols <= 8192) few(few_rows_kernel<T, 2>, 2);
+            else few(few_rows_kernel<T, 4>, 4);
+            return;
+        }
+        const auto tiles = [&](auto kernel, int tm, int tn, int threads) {
             a.tiles_m = (uint32_t)((rows + tm - 1) / tm);
             a.tiles_n = (uint32_t)((cols + tn - 1) / tn);
             hipLaunchKernelGGL(kernel, dim3(a.tiles_m * a.tiles_n), dim3(threads), 0, st, a);
         };
-        if (((rows + 255) / 256) * ((cols + 255) / 256) >= 256)
-            go(product_kernel<T, 2, 4, 8, 4>, 256, 256, 512);
-        else
-            go(product_kernel<T, 2, 2, 4, 4>, 128, 128, 256);
+        const int64_t jobs = rows * (o.r_stride / BP);
+        if (jobs > 0)
+            hipLaunchKernelGGL(round_rows_kernel<T>, dim3((uint32_t)((jobs * 16 + BP_NT - 1) / BP_NT)), dim3(BP_NT), 0, st,
+                               (const T*)x, rows, depth, x_stride, (uint16_t*)(ws + o.r), o.r_stride);
+        if (o.tile == 256) tiles(product_kernel<T, 2, 4, 8, 4>, 256, 256, 512);
+        else if (o.tile == 128) tiles(product_kernel<T, 1, 4, 8, 2>, 128, 128, 256);
+        else if (o.tile == 64) tiles(product_kernel<T, 1, 4, 4, 1>, 64, 64, 256);
+        else tiles(product_kernel<T, 1, 4, 2, 1>, 32, 64, 256);
     });
     return launched("block product");
 }

@@ -20,6 +20,7 @@ template <typename T> struct Unit { static constexpr int n = 16 / (int)sizeof(T)
 // 16 bytes at an address that is aligned to its element alone
 struct __attribute__((packed, aligned(2), may_alias)) Raw16h { u32x4 v; };
 struct __attribute__((packed, aligned(4), may_alias)) Raw16w { u32x4 v; };
+struct __attribute__((packed, aligned(2), may_alias)) Raw8h { u32x2 v; };
 typedef uint16_t __attribute__((may_alias)) raw16_t;
 typedef uint32_t __attribute__((may_alias)) raw32_t;
 
@@ -30,6 +31,11 @@ template <typename T> __device__ __forceinline__ u32x4 load16(const T* p) {
 template <typename T> __device__ __forceinline__ void store16(T* p, u32x4 v) {
     if constexpr (sizeof(T) == 4) ((CRESSO_GLOBAL Raw16w*)p)->v = v;
     else ((CRESSO_GLOBAL Raw16h*)p)->v = v;
+}
+// four 16-bit elements
+template <typename T> __device__ __forceinline__ void store8(T* p, u32x2 v) {
+    static_assert(sizeof(T) == 2, "16-bit elements");
+    ((CRESSO_GLOBAL Raw8h*)p)->v = v;
 }
 
 // two 16-bit elements of a word as floats
