@@ -88,25 +88,6 @@ template <typename T, int N> __device__ __forceinline__ void load_values(const T
     }
 }
 
-// 16 lanes hold one row's 128 elements.
-template <typename T>
-__global__ __launch_bounds__(BP_NT) void round_rows_kernel(const T* x, int64_t rows, int64_t width, int64_t stride,
-                                                           uint16_t* q, int64_t q_stride) {
-    const int64_t blocks = q_stride / BP;
-    const int64_t job = ((int64_t)blockIdx.x * BP_NT + threadIdx.x) / 16;
-    const bool on = job < rows * blocks;
-    const int64_t row = on ? job / blocks : 0, at = on ? (job - row * blocks) * BP + (threadIdx.x & 15) * 8 : width;
-    float v[8];
-    load_values(x + row * stride, at, width, v);
-    uint32_t r[4];
-    round_block(v, r, [](uint32_t u) {
-#pragma unroll
-        for (int m = 8; m >= 1; m >>= 1) u = max(u, (uint32_t)__shfl_xor((int)u, m, kWave));
-        return u;
-    });
-    if (on) *(u32x4*)(q + row * q_stride + at) = u32x4{r[0], r[1], r[2], r[3]};
-}
-
 // ---------------------------------------------------------------------------
 // The weight's other layout: along n for the gradient (TURN), or only with
 // rows padded to whole blocks and 16-byte pieces.  64 x 64 bytes a workgroup,
@@ -122,30 +103,62 @@ __device__ __forceinline__ u32x4 load_bytes(const uint8_t* p, int64_t left) {
         if (i < left) r[i / 4] |= (uint32_t)((const CRESSO_GLOBAL uint8_t*)p)[i] << (8 * (i & 3));
     return r;
 }
-template <bool TURN>
-__global__ __launch_bounds__(BP_NT) void lay_out_kernel(const uint8_t* w, int64_t rows, int64_t cols, int64_t stride,
-                                                        uint8_t* out, int64_t out_stride) {
+struct LayOut {
+    const uint8_t* w;
+    int64_t rows, cols, stride;   // as the weight is held
+    uint8_t* out;
+    int64_t out_stride;
+    uint32_t wide, high;          // workgroups; 0: the weight is taken as it is
+    int32_t turn;
+};
+__device__ __forceinline__ void lay_out(const LayOut& l, uint32_t block) {
+    __shared__ uint32_t tile[64][17];
     const int a = threadIdx.x >> 2, b = (threadIdx.x & 3) * 16;
-    const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
+    const int64_t r0 = (int64_t)(block / l.wide) * 64, c0 = (int64_t)(block % l.wide) * 64;
     u32x4 v = {0, 0, 0, 0};
-    if (r0 + a < rows) v = load_bytes(w + (r0 + a) * stride + c0 + b, cols - c0 - b);
-    if constexpr (TURN) {
-        __shared__ uint32_t tile[64][17];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tile[a][b / 4 + i] = v[i];
-        __syncthreads();
-        if (c0 + a >= cols) return;
-        const uint8_t* from = (const uint8_t*)tile + a;   // column a, rows b on
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[i] |= (uint32_t)from[(b + 4 * i + k) * 68] << (8 * k);
-        }
-        *(u32x4*)(out + (c0 + a) * out_stride + r0 + b) = v;
-    } else {
-        if (r0 + a < rows) *(u32x4*)(out + (r0 + a) * out_stride + c0 + b) = v;
+    if (r0 + a < l.rows) v = load_bytes(l.w + (r0 + a) * l.stride + c0 + b, l.cols - c0 - b);
+    if (!l.turn) {
+        if (r0 + a < l.rows) *(u32x4*)(l.out + (r0 + a) * l.out_stride + c0 + b) = v;
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tile[a][b / 4 + i] = v[i];
+    __syncthreads();
+    if (c0 + a >= l.cols) return;
+    const uint8_t* from = (const uint8_t*)tile + a;   // column a, rows b on
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i] |= (uint32_t)from[(b + 4 * i + k) * 68] << (8 * k);
+    }
+    *(u32x4*)(l.out + (c0 + a) * l.out_stride + r0 + b) = v;
+}
+
+// What comes before a product, in one launch: the first workgroups lay the
+// weight out, where that is wanted, the others round the rows: 16 lanes hold
+// one row's 128 elements.
+template <typename T>
+__global__ __launch_bounds__(BP_NT) void prepare_kernel(LayOut l, const T* x, int64_t rows, int64_t width, int64_t stride, uint16_t* q,
+                                                        int64_t q_stride) {
+    const uint32_t laying = l.wide * l.high;
+    if (blockIdx.x < laying) {
+        lay_out(l, blockIdx.x);
+        return;
+    }
+    const int64_t blocks = q_stride / BP;
+    const int64_t job = ((int64_t)(blockIdx.x - laying) * BP_NT + threadIdx.x) / 16;
+    const bool on = job < rows * blocks;
+    const int64_t row = on ? job / blocks : 0, at = on ? (job - row * blocks) * BP + (threadIdx.x & 15) * 8 : width;
+    float v[8];
+    load_values(x + row * stride, at, width, v);
+    uint32_t r[4];
+    round_block(v, r, [](uint32_t u) {
+#pragma unroll
+        for (int m = 8; m >= 1; m >>= 1) u = max(u, (uint32_t)__shfl_xor((int)u, m, kWave));
+        return u;
+    });
+    if (on) *(u32x4*)(q + row * q_stride + at) = u32x4{r[0], r[1], r[2], r[3]};
 }
 
 // ---------------------------------------------------------------------------
@@ -634,19 +647,21 @@ extern "C" int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t
     a.rows = rows;
     a.cols = cols;
     a.depth = o.copy ? o.w_stride : depth;
+    LayOut l{};
     if (o.copy && depth > 0) {
-        const int64_t r = turned ? depth : cols, c = turned ? cols : depth;   // the weight as it is held
+        l = {(const uint8_t*)w, turned ? depth : cols, turned ? cols : depth, w_stride, (uint8_t*)ws + o.w, o.w_stride, 0, 0, turned};
         // the laid-out rows' ends are written too
-        const dim3 grid((uint32_t)((turned ? up(c, 64) : o.w_stride) / 64), (uint32_t)((turned ? o.w_stride : up(r, 64)) / 64));
-        if (turned)
-            hipLaunchKernelGGL(lay_out_kernel<true>, grid, dim3(BP_NT), 0, st, (const uint8_t*)w, r, c, w_stride,
-                               (uint8_t*)ws + o.w, o.w_stride);
-        else
-            hipLaunchKernelGGL(lay_out_kernel<false>, grid, dim3(BP_NT), 0, st, (const uint8_t*)w, r, c, w_stride,
-                               (uint8_t*)ws + o.w, o.w_stride);
+        l.wide = (uint32_t)((turned ? up(cols, 64) : o.w_stride) / 64);
+        l.high = (uint32_t)((turned ? o.w_stride : up(cols, 64)) / 64);
     }
     with_row_dtype(dtype, [&](auto t) {
         using T = decltype(t);
+        // 16 rows and fewer are rounded by the product itself
+        const int64_t jobs = o.tile ? rows * (o.r_stride / BP) : 0;
+        const uint32_t groups = l.wide * l.high + (uint32_t)((jobs * 16 + BP_NT - 1) / BP_NT);
+        if (groups)
+            hipLaunchKernelGGL(prepare_kernel<T>, dim3(groups), dim3(BP_NT), 0, st, l, (const T*)x, jobs ? rows : 0, depth, x_stride,
+                               (uint16_t*)(ws + o.r), o.r_stride);
         if (!o.tile) {
             a.depth = depth;   // x itself is not padded
             const auto few = [&](auto kernel, int fn) {
@@ -663,10 +678,6 @@ extern "C" int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t
             a.tiles_n = (uint32_t)((cols + tn - 1) / tn);
             hipLaunchKernelGGL(kernel, dim3(a.tiles_m * a.tiles_n), dim3(threads), 0, st, a);
         };
-        const int64_t jobs = rows * (o.r_stride / BP);
-        if (jobs > 0)
-            hipLaunchKernelGGL(round_rows_kernel<T>, dim3((uint32_t)((jobs * 16 + BP_NT - 1) / BP_NT)), dim3(BP_NT), 0, st,
-                               (const T*)x, rows, depth, x_stride, (uint16_t*)(ws + o.r), o.r_stride);
         if (o.tile == 256) tiles(product_kernel<T, 2, 4, 8, 4>, 256, 256, 512);
         else if (o.tile == 128) tiles(product_kernel<T, 1, 4, 8, 2>, 128, 128, 256);
         else if (o.tile == 64) tiles(product_kernel<T, 1, 4, 4, 1>, 64, 64, 256);

@@ -8,11 +8,16 @@
 //
 // The row's maximum m and the sums of exp((z-m)/t) and exp(z-m) come from one
 // pass over the row (a running maximum, sums rescaled when it grows), so the
-// loss reads each logit once.  The gradient is written by a second pass over
-// the row as if there were no teacher and no label; their few places are
-// written again afterwards from logits that were read before, so it may take
-// the logits' own memory.  Bound by HBM and, where both exponentials of each
-// logit are needed in both passes, by the transcendental rate.
+// loss reads each logit once.  The gradient is written as if there were no
+// teacher and no label; their few places are written again afterwards from
+// logits that were read before, so it may take the logits' own memory.
+//
+// Exponents are kept in base 2: z*c - C with c = log2(e)/t and C = c*m rounded
+// once, one fused operation per logit.  The rounding of C is the same for the
+// whole row and drops out, since the sum is taken against the same C.  Where t
+// is 1 or 2, exp(z-m) is exp((z-m)/t) or its square: one transcendental
+// operation per logit instead of two, which is what bounds the passes next to
+// HBM.
 //
 // A row without weight, or without any teacher entry and label, is not read:
 // its loss and gradient are 0 whatever it holds.  Entries with an index
@@ -24,16 +29,16 @@
 namespace cresso {
 namespace {
 
-constexpr int DI_NT = 512;
-constexpr int DI_WAVES = DI_NT / kWave;
+constexpr int DI_MAX_WAVES = 8;
 constexpr int DI_MAX_TOP = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
 
 enum { DI_LOSS, DI_BOTH, DI_GRAD };
 
 struct DistillLds {
-    float red[DI_WAVES][3];
-    float row[8];                   // m, log sums, has teacher
+    float red[DI_MAX_WAVES][3];
+    float soft;                     // 1: the row has a teacher
     int32_t index[DI_MAX_TOP + 1];  // the teacher's entries, then the label; -1: absent
     float p[DI_MAX_TOP + 1];
     float z[DI_MAX_TOP + 1];
@@ -55,167 +60,271 @@ __device__ __forceinline__ float wave_max(float v) {
 // a maximum to subtract: 0 for a row whose every entry is -inf
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 
-template <typename T, int MODE>
-__global__ __launch_bounds__(DI_NT) void distill_kernel(cresso_distill_desc d) {
-    constexpr int E = Unit<T>::n;
-    __shared__ DistillLds s;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const int64_t row = blockIdx.x, vocab = d.vocab, units = (vocab + E - 1) / E;
-    const T* z = (const T*)d.logits + row * d.logits_stride;
-    T* out = (T*)d.grad + row * d.grad_stride;
-    const float w = d.weights ? d.weights[row] : d.weight;
-    const bool two = d.labels != nullptr;   // the batch has labels: both sums are kept
+// The exponentials of a row against its maximum.  P: how exp(z-m) comes
+// about.  0: it is not wanted; 1, 2: that power of exp((z-m)/t); -1: neither.
+template <int P> struct RowExp {
+    float c;      // log2(e) / t
+    float C, C1;  // c*m, log2(e)*m
+    __device__ __forceinline__ void set(float m) {
+        C = c * m;
+        C1 = LOG2E * m;
+    }
+    __device__ __forceinline__ float soft2(float v) const { return fmaf(v, c, -C); }
+    __device__ __forceinline__ float hard2(float v) const { return P > 0 ? (float)P * soft2(v) : fmaf(v, LOG2E, -C1); }
+    // log2 of what a sum of exp(z-m) against `from` is multiplied by
+    __device__ __forceinline__ float hard_by(const RowExp& from) const { return P > 0 ? (float)P * (from.C - C) : from.C1 - C1; }
+    // exp(z-m), given exp((z-m)/t)
+    __device__ __forceinline__ float hard(float v, float t) const {
+        return P == 1 ? t : P == 2 ? t * t : fexp2(fmaf(v, LOG2E, -C1));
+    }
+};
+template <int P> __device__ __forceinline__ RowExp<P> row_exp(const cresso_distill_desc& d) { return {LOG2E / d.temperature, 0.0f, 0.0f}; }
 
-    // the teacher's entries and the label
+// A sum against another maximum; one that holds nothing yet has none.
+__device__ __forceinline__ float moved(float sum, float by2) { return sum == 0.0f ? 0.0f : sum * fexp2(by2); }
+
+// A thread's running maximum and sums; x is set to the maximum.
+template <int P> struct RowSums {
+    float top = -INFINITY, st = 0.0f, s1 = 0.0f;
+    template <int E> __device__ __forceinline__ void add(const float (&v)[E], RowExp<P>& x) {
+        float um = v[0];
+#pragma unroll
+        for (int e = 1; e < E; ++e) um = fmaxf(um, v[e]);
+        if (um > top) {
+            const RowExp<P> before = x;
+            top = um;
+            x.set(um);
+            st = moved(st, before.C - x.C);
+            if (P) s1 = moved(s1, x.hard_by(before));
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float t = fexp2(x.soft2(v[e]));
+            st += t;
+            if (P) s1 += x.hard(v[e], t);
+        }
+    }
+};
+// Joins the threads' sums: x is set to the row's maximum m; l_t, l_1: log2 of
+// the sums against it.  One barrier.
+template <int P>
+__device__ __forceinline__ void join_sums(DistillLds& s, RowSums<P> r, RowExp<P>& x, float& m, float& l_t, float& l_1) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+    const float wm = wave_max(r.top);
+    RowExp<P> b = x;
+    b.set(base_of(wm));
+    r.st = wave_sum(moved(r.st, x.C - b.C));
+    r.s1 = P ? wave_sum(moved(r.s1, b.hard_by(x))) : 0.0f;
+    if (lane == 0) {
+        s.red[wave][0] = wm;
+        s.red[wave][1] = r.st;
+        s.red[wave][2] = r.s1;
+    }
+    __syncthreads();
+    m = s.red[0][0];
+#pragma unroll 1
+    for (int k = 1; k < waves; ++k) m = fmaxf(m, s.red[k][0]);
+    m = base_of(m);
+    x.set(m);
+    float st = 0.0f, s1 = 0.0f;
+#pragma unroll 1
+    for (int k = 0; k < waves; ++k) {
+        b.set(base_of(s.red[k][0]));
+        st += moved(s.red[k][1], b.C - x.C);
+        if (P) s1 += moved(s.red[k][2], x.hard_by(b));
+    }
+    l_t = log2f(st);
+    l_1 = P ? log2f(s1) : 0.0f;
+}
+
+// The row's weight; its teacher's entries and label, and the logits at their
+// places, go to LDS.  -> whether the row gives anything.  One barrier.
+template <typename T>
+__device__ __forceinline__ bool row_begins(const cresso_distill_desc& d, DistillLds& s, const T* z, int64_t row, float& w, int32_t& label) {
+    w = d.weights ? d.weights[row] : d.weight;
     bool some = false;
-    for (int j = tid; j < d.top; j += DI_NT) {
+#pragma unroll 1
+    for (int j = threadIdx.x; j < d.top; j += blockDim.x) {
         const int64_t v = load_int(d.index, d.index_bytes, row * d.index_stride + j);
-        const bool on = v >= 0 && v < vocab;
+        const bool on = v >= 0 && v < d.vocab;
         s.index[j] = on ? (int32_t)v : -1;
+        s.p[j] = on ? load_any(d.teacher, d.teacher_dtype, row * d.teacher_stride + j) : -INFINITY;
+        s.z[j] = on ? to_f(z[v]) : 0.0f;
         some |= on;
     }
-    int64_t label = -1;
-    if (two) {
-        label = load_int(d.labels, d.label_bytes, row);
-        if (label == d.ignore_index || label < 0 || label >= vocab) label = -1;
+    label = -1;
+    if (d.labels) {
+        const int64_t l = load_int(d.labels, d.label_bytes, row);
+        if (l != d.ignore_index && l >= 0 && l < d.vocab) label = (int32_t)l;
     }
-    if (tid == 0) s.index[d.top] = (int32_t)label;
-    const bool teacher = __syncthreads_or(some);
-    if (w == 0.0f || (!teacher && label < 0)) {
-        if (MODE != DI_GRAD && tid == 0) {
-            d.loss[row] = 0.0f;
-            if (d.stats) d.stats[3 * row] = d.stats[3 * row + 1] = d.stats[3 * row + 2] = 0.0f;
-        }
-        if (MODE != DI_LOSS)
-            for (int64_t u = tid; u < units; u += DI_NT) store_unit(out, u, vocab, u32x4{0, 0, 0, 0});
-        return;
+    if (threadIdx.x == 0) {
+        s.index[d.top] = label;
+        s.p[d.top] = 0.0f;
+        s.z[d.top] = label >= 0 ? to_f(z[label]) : 0.0f;
     }
-    const float ct = LOG2E / d.temperature;
+    some = __syncthreads_or(some);
+    return w != 0.0f && (some || label >= 0);
+}
 
-    float m, log_t, log_1;   // maximum; log of the sums of exp((z-m)/t) and exp(z-m)
-    if (MODE == DI_GRAD) {
-        m = d.stats[3 * row];
-        log_t = d.stats[3 * row + 1];
-        log_1 = d.stats[3 * row + 2];
-    } else {
-        float top = -INFINITY, st = 0.0f, s1 = 0.0f;
-        for (int64_t u = tid; u < units; u += DI_NT) {
-            float v[E];
-            widen<T>(load_unit(z, u, vocab), v);
-            if (u == units - 1) {
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (u * E + e >= vocab) v[e] = -INFINITY;
-            }
-            float um = v[0];
-#pragma unroll
-            for (int e = 1; e < E; ++e) um = fmaxf(um, v[e]);
-            if (um > top) {
-                st *= fexp2((top - um) * ct);
-                s1 *= fexp2((top - um) * LOG2E);
-                top = um;
-            }
-            const float b = base_of(top);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                st += fexp2((v[e] - b) * ct);
-                if (two) s1 += fexp2((v[e] - b) * LOG2E);
-            }
-        }
-        const float wm = wave_max(top), wb = base_of(wm);
-        st = wave_sum(st * fexp2((top - wb) * ct));
-        s1 = wave_sum(s1 * fexp2((top - wb) * LOG2E));
-        if (lane == 0) {
-            s.red[wave][0] = wm;
-            s.red[wave][1] = st;
-            s.red[wave][2] = s1;
-        }
-        __syncthreads();
-        m = s.red[0][0];
-        for (int k = 1; k < DI_WAVES; ++k) m = fmaxf(m, s.red[k][0]);
-        m = base_of(m);
-        st = s1 = 0.0f;
-        for (int k = 0; k < DI_WAVES; ++k) {
-            st += s.red[k][1] * fexp2((s.red[k][0] - m) * ct);
-            s1 += s.red[k][2] * fexp2((s.red[k][0] - m) * LOG2E);
-        }
-        log_t = logf(st);
-        log_1 = two ? logf(s1) : 0.0f;
+// The first wave: the teacher's distribution in its logits' place, and, if
+// `loss`, the row's loss.
+template <int P>
+__device__ __forceinline__ void teacher_of(const cresso_distill_desc& d, DistillLds& s, int64_t row, float w, int32_t label, const RowExp<P>& x,
+                                           float l_t, float l_1, bool loss) {
+    const int lane = threadIdx.x & (kWave - 1);
+    float top = -INFINITY, total = 0.0f, kl = 0.0f;
+#pragma unroll 1
+    for (int j = lane; j < d.top; j += kWave) {
+        top = fmaxf(top, s.p[j]);
     }
+    const float A = x.c * base_of(wave_max(top));
+#pragma unroll 1
+    for (int j = lane; j < d.top; j += kWave) total += fexp2(fmaf(s.p[j], x.c, -A));
+    total = wave_sum(total);
+    const bool any = !(total == 0.0f);   // entries that all are -inf are no teacher
+    const float l_total = log2f(total);
+#pragma unroll 1
+    for (int j = lane; j < d.top; j += kWave) {
+        const float a2 = fmaf(s.p[j], x.c, -A), v = s.z[j];
+        const float p = any && s.index[j] >= 0 ? fexp2(a2) / total : 0.0f;
+        if (!(p == 0.0f)) kl += p * ((a2 - l_total) - (x.soft2(v) - l_t));
+        s.p[j] = p;
+    }
+    kl = wave_sum(kl);
+    if (lane == 0) {
+        s.soft = any ? 1.0f : 0.0f;
+        const float hard = label >= 0 ? l_1 - x.hard2(s.z[d.top]) : 0.0f;
+        if (loss) d.loss[row] = w * LN2 * (d.mix * d.temperature * d.temperature * kl + (1.0f - d.mix) * hard);
+    }
+}
 
-    if (wave == 0) {   // the teacher's distribution; the loss
-        float a_top = -INFINITY, total = 0.0f, kl = 0.0f;
-        for (int j = lane; j < d.top; j += kWave) {
-            const float a = s.index[j] >= 0 ? load_any(d.teacher, d.teacher_dtype, row * d.teacher_stride + j) : -INFINITY;
-            s.p[j] = a;
-            a_top = fmaxf(a_top, a);
-        }
-        a_top = base_of(wave_max(a_top));
-        for (int j = lane; j < d.top; j += kWave) total += fexp2((s.p[j] - a_top) * ct);
-        total = wave_sum(total);
-        // entries that all are -inf: no teacher
-        const bool any = !(total == 0.0f);
-        const float log_total = logf(total);
-        for (int j = lane; j < d.top; j += kWave) {
-            const float a = s.p[j];
-            const float p = any && s.index[j] >= 0 ? fexp2((a - a_top) * ct) / total : 0.0f;
-            const float v = s.index[j] >= 0 ? to_f(z[s.index[j]]) : 0.0f;
-            if (!(p == 0.0f)) kl += p * (((a - a_top) - (v - m)) / d.temperature - log_total + log_t);
-            s.p[j] = p;
-            s.z[j] = v;
-        }
-        kl = wave_sum(kl);
-        if (lane == 0) {
-            float hard = 0.0f;
-            s.p[d.top] = 0.0f;
-            if (label >= 0) {
-                const float v = to_f(z[label]);
-                s.z[d.top] = v;
-                hard = log_1 - (v - m);
-            }
-            s.row[0] = any ? 1.0f : 0.0f;
-            if (MODE != DI_GRAD) {
-                d.loss[row] = w * (d.mix * d.temperature * d.temperature * kl + (1.0f - d.mix) * hard);
-                if (d.stats) {
-                    d.stats[3 * row] = m;
-                    d.stats[3 * row + 1] = log_t;
-                    d.stats[3 * row + 2] = log_1;
-                }
-            }
-        }
+// The gradient without the teacher's and the label's own terms.
+template <int P> struct RowGrad {
+    RowExp<P> x;
+    float kt, k1;   // factors of exp((z-m)/t) and exp(z-m)
+    __device__ __forceinline__ float of(float v) const {
+        const float t = fexp2(x.soft2(v));
+        return P ? fmaf(k1, x.hard(v, t), kt * t) : kt * t;
     }
-    if (MODE == DI_LOSS) return;
-    __syncthreads();
-    const float g = MODE == DI_GRAD ? w * d.d_loss[d.d_loss_stride * row] : w;
-    const bool soft = s.row[0] != 0.0f, hard = label >= 0;
+};
+template <int P>
+__device__ __forceinline__ RowGrad<P> row_grad(const cresso_distill_desc& d, const RowExp<P>& x, float g, bool soft, bool hard, float l_t,
+                                               float l_1) {
+    return {x, soft ? g * d.mix * d.temperature * fexp2(-l_t) : 0.0f, hard ? g * (1.0f - d.mix) * fexp2(-l_1) : 0.0f};
+}
+// The places of the teacher and the label, after the others are written (a barrier before).
+template <typename T, int P>
+__device__ __forceinline__ void patch_row(const cresso_distill_desc& d, const DistillLds& s, T* out, const RowGrad<P>& r, float g,
+                                          int32_t label) {
     const float kt = g * d.mix * d.temperature, k1 = g * (1.0f - d.mix);
-    const float bt = log_t * LOG2E, b1 = log_1 * LOG2E;
-    const auto grad_of = [&](float v) {
-        float r = 0.0f;
-        if (soft) r = kt * fexp2((v - m) * ct - bt);
-        if (hard) r += k1 * fexp2((v - m) * LOG2E - b1);
-        return r;
-    };
-    for (int64_t u = tid; u < units; u += DI_NT) {
-        float v[E];
-        widen<T>(load_unit(z, u, vocab), v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = grad_of(v[e]);
-        store_unit(out, u, vocab, narrow<T>(v));
-    }
-    __syncthreads();   // the places below were written above
-    for (int j = tid; j <= d.top; j += DI_NT) {
+#pragma unroll 1
+    for (int j = threadIdx.x; j <= d.top; j += blockDim.x) {
         const int32_t v = s.index[j];
         if (v < 0) continue;
         float p = 0.0f;
         bool first = true;
+#pragma unroll 1
         for (int k = 0; k < d.top; ++k)
             if (s.index[k] == v) {
                 first &= k >= j;
                 p += s.p[k];
             }
-        if (first) out[v] = from_w<T>(grad_of(s.z[j]) - kt * p - (v == label ? k1 : 0.0f));
+        if (!first) continue;
+        out[v] = from_w<T>(r.of(s.z[j]) - kt * p - (v == label ? k1 : 0.0f));
     }
+}
+// The units of a row, NT threads side by side: fn(unit, raw) for each of a
+// thread's, with the loads of four of them on their way at a time.  The units
+// that all threads have whole lie at addresses of a common base and a 32-bit
+// place of the thread's own.  BACK: from the row's end, where a pass before
+// has read last and the caches still hold it.
+constexpr int DI_AHEAD = 4;
+template <typename T, int NT, bool BACK, typename F> __device__ __forceinline__ void for_units(const T* z, int64_t vocab, F&& fn) {
+    constexpr int E = Unit<T>::n, PIECE = NT * E;
+    const int fours = (int)(vocab / (PIECE * DI_AHEAD)), tid = threadIdx.x;
+    const uint32_t place = (uint32_t)tid * E;
+    const auto rest = [&] {
+        for (int64_t u = (int64_t)fours * DI_AHEAD * NT + tid; u * E < vocab; u += NT) fn(u, load_unit(z, u, vocab));
+    };
+    if (BACK) rest();
+    for (int f = 0; f < fours; ++f) {
+        const int i = (BACK ? fours - 1 - f : f) * DI_AHEAD;
+        const T* p = z + (int64_t)i * PIECE;
+        u32x4 raw[DI_AHEAD];
+#pragma unroll
+        for (int k = 0; k < DI_AHEAD; ++k) raw[k] = load16(p + k * PIECE + place);
+#pragma unroll
+        for (int k = 0; k < DI_AHEAD; ++k) fn((int64_t)(i + k) * NT + tid, raw[k]);
+    }
+    if (!BACK) rest();
+}
+// a unit's logits; beyond the row's end -inf, which adds nothing
+template <typename T> __device__ __forceinline__ void logits_of(u32x4 r, int64_t u, int64_t vocab, float (&v)[Unit<T>::n]) {
+    constexpr int E = Unit<T>::n;
+    widen<T>(r, v);
+    if ((u + 1) * E > vocab) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (u * E + e >= vocab) v[e] = -INFINITY;
+    }
+}
+__device__ __forceinline__ void put_stats(const cresso_distill_desc& d, int64_t row, float m, float l_t, float l_1) {
+    if (!d.stats || threadIdx.x) return;
+    d.stats[3 * row] = m;
+    d.stats[3 * row + 1] = l_t;
+    d.stats[3 * row + 2] = l_1;
+}
+
+// A workgroup per row: the loss, or the gradient from the loss's maximum and sums.
+template <typename T, int MODE, int P, int NT>
+__global__ __launch_bounds__(NT) void distill_kernel(cresso_distill_desc d) {
+    constexpr int E = Unit<T>::n;
+    __shared__ DistillLds s;
+    const int64_t row = blockIdx.x, vocab = d.vocab, units = (vocab + E - 1) / E;
+    const T* z = (const T*)d.logits + row * d.logits_stride;
+    T* out = (T*)d.grad + row * d.grad_stride;
+    float w, m, l_t, l_1;
+    int32_t label;
+    if (!row_begins(d, s, z, row, w, label)) {
+        if (MODE != DI_GRAD) {
+            if (threadIdx.x == 0) d.loss[row] = 0.0f;
+            put_stats(d, row, 0.0f, 0.0f, 0.0f);
+        }
+        if (MODE != DI_LOSS) {
+            for (int64_t u = threadIdx.x; u < units; u += NT) store_unit(out, u, vocab, u32x4{0, 0, 0, 0});
+        }
+        return;
+    }
+    RowExp<P> x = row_exp<P>(d);
+    if (MODE == DI_GRAD) {
+        m = d.stats[3 * row];
+        l_t = d.stats[3 * row + 1];
+        l_1 = d.stats[3 * row + 2];
+        x.set(m);
+    } else {
+        RowSums<P> sums;
+        for_units<T, NT, false>(z, vocab, [&](int64_t u, u32x4 raw) {
+            float v[E];
+            logits_of<T>(raw, u, vocab, v);
+            sums.add(v, x);
+        });
+        join_sums(s, sums, x, m, l_t, l_1);
+        put_stats(d, row, m, l_t, l_1);
+    }
+    if (threadIdx.x < kWave) teacher_of(d, s, row, w, label, x, l_t, l_1, MODE != DI_GRAD);
+    if (MODE == DI_LOSS) return;
+    __syncthreads();
+    const float g = MODE == DI_GRAD ? w * d.d_loss[d.d_loss_stride * row] : w;
+    const RowGrad<P> r = row_grad(d, x, g, s.soft != 0.0f, label >= 0, l_t, l_1);
+    for_units<T, NT, MODE == DI_BOTH>(z, vocab, [&](int64_t u, u32x4 raw) {
+        float v[E];
+        widen<T>(raw, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = r.of(v[e]);
+        store_unit_past(out, u, vocab, narrow<T>(v));
+    });
+    __syncthreads();
+    patch_row(d, s, out, r, g, label);
 }
 
 // The sum of the rows' losses, in a fixed order in fp64.
@@ -244,12 +353,33 @@ int32_t check_distill(const char* what, const cresso_distill_desc* d) {
     return CRESSO_OK;
 }
 
-template <int MODE> void launch_distill(const cresso_distill_desc& d, hipStream_t st) {
+// Calls fn(T, P) for the logits' type and the way to exp(z-m).
+template <typename F> void with_exp(const cresso_distill_desc& d, F&& fn) {
+    using std::integral_constant;
     with_row_dtype(d.dtype, [&](auto t) {
-        hipLaunchKernelGGL((distill_kernel<decltype(t), MODE>), dim3((uint32_t)d.rows), dim3(DI_NT), 0, st, d);
+        if (!d.labels) fn(t, integral_constant<int, 0>{});
+        else if (d.temperature == 1.0f) fn(t, integral_constant<int, 1>{});
+        else if (d.temperature == 2.0f) fn(t, integral_constant<int, 2>{});
+        else fn(t, integral_constant<int, -1>{});
     });
 }
-
+template <int MODE> void launch_distill(const cresso_distill_desc& d, hipStream_t st) {
+    with_exp(d, [&](auto t, auto p) {
+        using T = decltype(t);
+        constexpr int P = decltype(p)::value;
+        const auto go = [&](auto kernel, int threads) {
+            hipLaunchKernelGGL(kernel, dim3((uint32_t)d.rows), dim3(threads), 0, st, d);
+        };
+        const int64_t units = (d.vocab + Unit<T>::n - 1) / Unit<T>::n;
+        // Long rows take 512 threads (4096 x 131072 bf16: 494 us, 550 with 256, 569
+        // with 1024); where there are rows enough for more workgroups at once,
+        // shorter ones fewer (4096 x 32000: 140 us with 256, 147 with 512; 8192 x
+        // 1000: 35 us with 64, 46 with 256).
+        if (units <= 256) go(distill_kernel<T, MODE, P, 64>, 64);
+        else if (units <= 6144 && d.rows > 512) go(distill_kernel<T, MODE, P, 256>, 256);
+        else go(distill_kernel<T, MODE, P, 512>, 512);
+    });
+}
 }  // namespace
 }  // namespace cresso
 
@@ -259,7 +389,7 @@ extern "C" int32_t cresso_distill_loss(const cresso_distill_desc* desc, void* st
     const int32_t rc = check_distill("distillation loss", desc);
     if (rc != CRESSO_OK) return rc;
     if (!desc->total && desc->rows == 0) return CRESSO_OK;
-    if (desc->rows > 0 && !desc->loss) return fail(CRESSO_E_INVALID, "distillation loss: null argument");
+    if (desc->rows > 0 && (!desc->loss || (desc->grad && !desc->stats))) return fail(CRESSO_E_INVALID, "distillation loss: null argument");
     hipStream_t st = (hipStream_t)stream;
     if (desc->rows > 0) {
         if (desc->grad) launch_distill<DI_BOTH>(*desc, st);

@@ -527,7 +527,8 @@ std::tuple<Tensor, Tensor> distill_loss_and_grad(const Tensor& logits, const Ten
     } else {
         grad = at::empty(logits.sizes(), logits.options().requires_grad(false));
     }
-    return {std::get<1>(distill_run(c, true, Tensor(), grad)), grad};
+    const Tensor stats = at::empty({logits.size(0), 3}, logits.options().dtype(at::kFloat).requires_grad(false));
+    return {std::get<1>(distill_run(c, true, stats, grad)), grad};
 }
 
 // ---------------------------------------------------------------------------

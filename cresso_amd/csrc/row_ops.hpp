@@ -127,6 +127,18 @@ template <typename T> __device__ __forceinline__ void store_unit(T* row, int64_t
     else if (left > 0) store_part(row + at, v, (int)left);
 }
 
+// The same past the caches, for what is not read again soon.
+template <typename T> __device__ __forceinline__ void store_unit_past(T* row, int64_t u, int64_t width, u32x4 v) {
+    constexpr int E = Unit<T>::n;
+    const int64_t at = u * E, left = width - at;
+    if (left >= E) {
+        if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(v, &((CRESSO_GLOBAL Raw16w*)(row + at))->v);
+        else __builtin_nontemporal_store(v, &((CRESSO_GLOBAL Raw16h*)(row + at))->v);
+    } else if (left > 0) {
+        store_part(row + at, v, (int)left);
+    }
+}
+
 inline int32_t launched(const char* what) {
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? CRESSO_OK : hip_fail(e, what);

@@ -475,7 +475,8 @@ typedef struct cresso_distill_desc {
     const void *logits, *index, *teacher, *labels;
     const float* weights;
     float *loss, *total;                /* [rows]; total may be NULL: their sum */
-    float* stats;                       /* [rows][3], written with the loss when not NULL, read by the gradient */
+    float* stats;                       /* [rows][3], written with the loss when not NULL, read by the gradient; with
+                                         * the loss and `grad` it must be there */
     const float* d_loss;                /* gradient: d_loss[d_loss_stride * row] */
     void* grad;                         /* with the loss: NULL or the gradient for d_loss = 1; may be the logits */
     int64_t logits_stride, index_stride, teacher_stride, grad_stride, d_loss_stride;
