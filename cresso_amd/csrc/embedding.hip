@@ -28,8 +28,9 @@ constexpr int SO_NT = 1024;        // threads of the sort: 16 waves
 constexpr int SO_WAVES = SO_NT / kWave;
 constexpr int SO_BITS = 9;         // digit
 constexpr int SO_DIGITS = 1 << SO_BITS;
-constexpr int SO_ROUNDS = 16;      // keys per thread
+constexpr int SO_ROUNDS = 4;       // keys per thread of the counting sort
 constexpr int SO_TILE = SO_NT * SO_ROUNDS;
+constexpr int SO_MERGE = 32;       // tiles of SO_NT keys that are merged in one step
 
 template <typename I> __device__ __forceinline__ int64_t id_at(const void* ids, int64_t t) {
     return (int64_t)((const CRESSO_GLOBAL I*)ids)[t];
@@ -38,40 +39,58 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int32_t id_bytes, in
     return id_bytes == 8 ? id_at<int64_t>(ids, t) : id_at<int32_t>(ids, t);
 }
 
-template <typename T>
+// K units a thread: their ids, then their rows' units are on their way together.
+template <typename T, int K>
 __global__ __launch_bounds__(EM_NT) void embed_forward_kernel(const void* ids, int32_t id_bytes, int64_t tokens,
                                                               const T* table, int64_t rows, int64_t row_stride,
-                                                              int64_t width, uint32_t units, uint32_t tokens_per_block,
-                                                              float scale, T* out) {
-    for (int64_t t0 = (int64_t)blockIdx.x * tokens_per_block; t0 < tokens; t0 += (int64_t)gridDim.x * tokens_per_block) {
-        const uint32_t here = (uint32_t)min((int64_t)tokens_per_block, tokens - t0);
-        for (uint32_t i = threadIdx.x; i < here * units; i += EM_NT) {
-            const uint32_t k = i / units, u = i - k * units;
-            const int64_t t = t0 + k, id = load_id(ids, id_bytes, t);
-            u32x4 r = {0, 0, 0, 0};
-            if (id >= 0 && id < rows) {
-                r = load_unit(table + id * row_stride, u, width);
-                float v[Unit<T>::n];
-                widen<T>(r, v);
+                                                              int64_t width, uint32_t units, float scale, T* out) {
+    const uint64_t total = (uint64_t)tokens * units;
+    for (uint64_t i0 = (uint64_t)blockIdx.x * (EM_NT * K); i0 < total; i0 += (uint64_t)gridDim.x * (EM_NT * K)) {
+        const uint64_t t0 = i0 / units;   // the first token; the others by 32-bit steps from it
+        const uint32_t u0 = (uint32_t)(i0 - t0 * units) + threadIdx.x;
+        int64_t t[K], id[K];
+        uint32_t u[K];
+        u32x4 r[K];
 #pragma unroll
-                for (int e = 0; e < Unit<T>::n; ++e) v[e] *= scale;
-                r = narrow<T>(v);
-            }
-            store_unit(out + t * width, u, width, r);
+        for (int k = 0; k < K; ++k) {
+            const uint32_t at = u0 + k * EM_NT, step = at / units;
+            t[k] = (int64_t)(t0 + step);
+            u[k] = at - step * units;
+            id[k] = t[k] < tokens ? load_id(ids, id_bytes, t[k]) : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            r[k] = u32x4{0, 0, 0, 0};
+            if (id[k] >= 0 && id[k] < rows) r[k] = load_unit(table + id[k] * row_stride, u[k], width);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (t[k] >= tokens) continue;
+            const bool there = id[k] >= 0 && id[k] < rows;
+            float v[Unit<T>::n];
+            widen<T>(r[k], v);
+#pragma unroll
+            for (int e = 0; e < Unit<T>::n; ++e) v[e] = there ? v[e] * scale : 0.0f;   // a scale may be infinite
+            store_unit(out + t[k] * width, u[k], width, narrow<T>(v));
         }
     }
 }
 
 // ---------------------------------------------------------------------------
-// Stable sort of (id, token) by id, least significant digit first.
+// Stable sort of (id, token) by id.
 //
-// A tile of up to 16384 keys is ranked by one workgroup: each wave takes a
-// contiguous part, 64 keys a round, finds the lanes with its key's digit by
-// one ballot per digit bit, and keeps a running count per digit in LDS.
+// A tile of 1024 R keys is ranked by one workgroup, least significant digit
+// first: each wave takes a contiguous part, 64 keys a round, finds the lanes
+// with its key's digit by one ballot per digit bit, and keeps a running count
+// per digit in LDS.  Up to 32 tiles of 1024 are sorted side by side and then
+// merged in one step: a key's place is its own in its tile plus, for each other
+// tile, the number of keys there that go before it, by binary search in LDS.
+// More tokens go through one counting sort per digit, in tiles of 4096.  (All
+// of 16384 in one workgroup took 34 us, tiles and merge take 10.)
 // ---------------------------------------------------------------------------
-struct SortTile {
-    uint32_t key[SO_TILE];
-    uint16_t from[SO_TILE];
+template <int R> struct SortTile {
+    uint32_t key[SO_NT * R];
+    uint16_t from[SO_NT * R];
     uint32_t count[SO_WAVES][SO_DIGITS];   // per wave and digit; then the first place of each
     uint32_t scan[SO_DIGITS / kWave];
 };
@@ -80,14 +99,14 @@ __device__ __forceinline__ uint32_t digit_of(uint32_t key, int shift) { return (
 
 // Ranks the keys of a wave's part among the wave's keys of the same digit.
 // Thread-held: key[r], rank[r] for round r; `mine` keys in this wave's part.
-__device__ __forceinline__ void rank_wave(SortTile& s, const uint32_t (&key)[SO_ROUNDS], uint32_t (&rank)[SO_ROUNDS],
-                                          int mine, int shift) {
+template <int R>
+__device__ __forceinline__ void rank_wave(SortTile<R>& s, const uint32_t (&key)[R], uint32_t (&rank)[R], int mine, int shift) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     for (int d = lane; d < SO_DIGITS; d += kWave) s.count[wave][d] = 0;
     __builtin_amdgcn_wave_barrier();
     const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
-    for (int r = 0; r < SO_ROUNDS; ++r) {
+    for (int r = 0; r < R; ++r) {
         if (r * kWave < mine) {
             const bool on = r * kWave + lane < mine;
             const uint32_t d = digit_of(key[r], shift);
@@ -109,7 +128,7 @@ __device__ __forceinline__ void rank_wave(SortTile& s, const uint32_t (&key)[SO_
 }
 
 // Exclusive prefix of count[][] in digit order, then wave order.  All threads.
-__device__ __forceinline__ void scan_counts(SortTile& s) {
+template <int R> __device__ __forceinline__ void scan_counts(SortTile<R>& s) {
     const int t = threadIdx.x, lane = t & (kWave - 1);
     uint32_t total = 0;
     if (t < SO_DIGITS)
@@ -146,52 +165,60 @@ __device__ __forceinline__ uint32_t key_of(const void* ids, int32_t id_bytes, in
     return (uint32_t)(id >= 0 && id < rows ? id : rows);   // ids outside the table go last
 }
 
-// The whole sort of up to SO_TILE tokens in one workgroup.
+// Sorts each SO_NT tokens.  The last tile is filled up with the largest number.
 __global__ __launch_bounds__(SO_NT) void embed_sort_tile_kernel(const void* ids, int32_t id_bytes, int32_t tokens,
                                                                 int64_t rows, int32_t bits, uint32_t* sorted_ids,
                                                                 uint32_t* sorted_tokens) {
-    extern __shared__ __align__(16) char lds[];
-    SortTile& s = *reinterpret_cast<SortTile*>(lds);
-    const int lane = threadIdx.x & (kWave - 1);
+    __shared__ SortTile<1> s;
+    const int t0 = blockIdx.x * SO_NT, n = min(SO_NT, tokens - t0);
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     int first, mine;
-    wave_part(tokens, threadIdx.x / kWave, first, mine);
-    uint32_t key[SO_ROUNDS], rank[SO_ROUNDS], from[SO_ROUNDS];
-#pragma unroll
-    for (int r = 0; r < SO_ROUNDS; ++r) {
-        const int i = r * kWave + lane;
-        key[r] = i < mine ? key_of(ids, id_bytes, first + i, rows) : 0;
-        from[r] = (uint32_t)(first + i);
-        rank[r] = 0;
-    }
+    wave_part(n, wave, first, mine);
+    const bool on = lane < mine;
+    uint32_t key[1] = {on ? key_of(ids, id_bytes, t0 + first + lane, rows) : 0}, rank[1] = {0}, from = first + lane;
     for (int shift = 0; shift < bits; shift += SO_BITS) {
         rank_wave(s, key, rank, mine, shift);
         __syncthreads();
         scan_counts(s);
-#pragma unroll
-        for (int r = 0; r < SO_ROUNDS; ++r)
-            if (r * kWave + lane < mine) {
-                const uint32_t at = s.count[threadIdx.x / kWave][digit_of(key[r], shift)] + rank[r];
-                s.key[at] = key[r];
-                s.from[at] = (uint16_t)from[r];
-            }
+        if (on) {
+            const uint32_t at = s.count[wave][digit_of(key[0], shift)] + rank[0];
+            s.key[at] = key[0];
+            s.from[at] = (uint16_t)from;
+        }
         __syncthreads();
-#pragma unroll
-        for (int r = 0; r < SO_ROUNDS; ++r) {
-            const int i = r * kWave + lane;
-            if (i < mine) {
-                key[r] = s.key[first + i];
-                from[r] = s.from[first + i];
-            }
+        if (on) {
+            key[0] = s.key[first + lane];
+            from = s.from[first + lane];
         }
     }
+    // one wave's part after another, filled up behind the last key
+    const int i = threadIdx.x;
+    sorted_ids[t0 + i] = i < n ? s.key[i] : ~0u;
+    sorted_tokens[t0 + i] = i < n ? (uint32_t)t0 + s.from[i] : 0u;
+}
+// The place of each key of a sorted tile among all tiles.
+__global__ __launch_bounds__(SO_NT) void embed_merge_kernel(const uint32_t* ids, const uint32_t* from, int32_t tokens, int32_t tiles,
+                                                            uint32_t* sorted_ids, uint32_t* sorted_tokens) {
+    extern __shared__ __align__(16) uint32_t keys[];   // [tiles][SO_NT]
+    const int mine = blockIdx.x, i = threadIdx.x, t = mine * SO_NT + i;
+    for (int c = 0; c < tiles; ++c) keys[c * SO_NT + i] = ids[c * SO_NT + i];
+    __syncthreads();
+    if (t >= tokens) return;
+    const uint32_t key = keys[t], token = from[t];
+    uint32_t place = i;
+#pragma unroll 4
+    for (int c = 0; c < tiles; ++c) {
+        // of the tiles before, equal keys go before, too: keys < key + 1
+        const uint32_t bound = c < mine ? key + 1 : key;
+        const uint32_t* k = keys + c * SO_NT;
+        uint32_t n = 0;
 #pragma unroll
-    for (int r = 0; r < SO_ROUNDS; ++r) {
-        const int i = r * kWave + lane;
-        if (i < mine) {
-            sorted_ids[first + i] = key[r];
-            sorted_tokens[first + i] = from[r];
-        }
+        for (int step = SO_NT / 2; step >= 1; step /= 2) n += k[n + step - 1] < bound ? step : 0;
+        n += k[n] < bound;
+        place += c == mine ? 0 : n;
     }
+    sorted_ids[place] = key;
+    sorted_tokens[place] = token;
 }
 
 // One digit of the sort of more tokens: counts of each tile, their places, the move.
@@ -244,8 +271,7 @@ __global__ __launch_bounds__(SO_NT) void embed_sort_scan_kernel(uint32_t* places
     }
 }
 __global__ __launch_bounds__(SO_NT) void embed_sort_move_kernel(SortPass p) {
-    extern __shared__ __align__(16) char lds[];
-    SortTile& s = *reinterpret_cast<SortTile*>(lds);
+    __shared__ SortTile<SO_ROUNDS> s;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int64_t t0 = (int64_t)blockIdx.x * SO_TILE;
     const int n = (int)min((int64_t)SO_TILE, p.tokens - t0);
@@ -425,23 +451,29 @@ int64_t al256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 
 struct EmbedLayout {
     int64_t ids, tokens, ids2, tokens2, places, partial, total;
-    uint32_t chunks, tiles, sort_tiles;
+    uint32_t chunks, tiles;
+    uint32_t merge_tiles, count_tiles;   // of the sort: tiles of SO_NT, or of SO_TILE if there are too many of those
 };
 EmbedLayout embed_layout(int64_t tokens, int64_t width, int32_t dtype) {
     EmbedLayout o{};
     const int64_t e = dtype == CRESSO_F32 ? 4 : 8;
     o.chunks = (uint32_t)((tokens + EM_CHUNK - 1) / EM_CHUNK);
     o.tiles = (uint32_t)((width + kWave * e - 1) / (kWave * e));
-    o.sort_tiles = (uint32_t)((tokens + SO_TILE - 1) / SO_TILE);
+    o.merge_tiles = (uint32_t)((tokens + SO_NT - 1) / SO_NT);
+    if (o.merge_tiles > SO_MERGE) {
+        o.merge_tiles = 0;
+        o.count_tiles = (uint32_t)((tokens + SO_TILE - 1) / SO_TILE);
+    }
     int64_t off = 0;
     auto take = [&](int64_t b) { const int64_t at = off; off = al256(off + b); return at; };
-    o.ids = take(tokens * 4);
-    o.tokens = take(tokens * 4);
-    if (o.sort_tiles > 1) {
-        o.ids2 = take(tokens * 4);
-        o.tokens2 = take(tokens * 4);
-        o.places = take((int64_t)SO_DIGITS * o.sort_tiles * 4);
+    const int64_t held = std::max<int64_t>(tokens, (int64_t)o.merge_tiles * SO_NT);   // tiles are filled up
+    o.ids = take(held * 4);
+    o.tokens = take(held * 4);
+    if (o.merge_tiles != 1 && tokens > 0) {
+        o.ids2 = take(held * 4);
+        o.tokens2 = take(held * 4);
     }
+    if (o.count_tiles) o.places = take((int64_t)SO_DIGITS * o.count_tiles * 4);
     if (o.chunks > 1) o.partial = take((int64_t)o.chunks * 2 * o.tiles * kWave * e * 4);
     o.total = std::max<int64_t>(off, 256);
     return o;
@@ -477,11 +509,15 @@ extern "C" int32_t cresso_embedding_forward(const void* ids, int32_t id_bytes, i
     with_row_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const uint32_t units = (uint32_t)((width + Unit<T>::n - 1) / Unit<T>::n);
-        const uint32_t per = std::max<uint32_t>(1, EM_NT / units);
-        const int64_t blocks = std::min<int64_t>((tokens + per - 1) / per, EM_MAX_BLOCKS);
-        hipLaunchKernelGGL(embed_forward_kernel<T>, dim3((uint32_t)blocks), dim3(EM_NT), 0, (hipStream_t)stream,
-                           ids, id_bytes, tokens, (const T*)table, rows, row_stride, width, units, per, (float)scale,
-                           (T*)out);
+        // four units a thread once that leaves enough workgroups for all CUs
+        const int64_t total = tokens * units;
+        const auto go = [&](auto kernel, int k) {
+            const int64_t blocks = std::min<int64_t>((total + EM_NT * k - 1) / (EM_NT * k), EM_MAX_BLOCKS);
+            hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(EM_NT), 0, (hipStream_t)stream, ids, id_bytes, tokens, (const T*)table,
+                               rows, row_stride, width, units, (float)scale, (T*)out);
+        };
+        if (total >= (int64_t)EM_NT * 4 * 1024) go(embed_forward_kernel<T, 4>, 4);
+        else go(embed_forward_kernel<T, 1>, 1);
     });
     return launched("embedding");
 }
@@ -508,17 +544,23 @@ extern "C" int32_t cresso_embedding_backward(const void* ids, int32_t id_bytes, 
     uint32_t *sid = (uint32_t*)(ws + o.ids), *sfrom = (uint32_t*)(ws + o.tokens);
     int bits = 1;   // of the largest key, `rows`
     while (((int64_t)1 << bits) <= rows) ++bits;
-    if (o.sort_tiles == 1) {
-        hipLaunchKernelGGL(embed_sort_tile_kernel, dim3(1), dim3(SO_NT), sizeof(SortTile), st, ids, id_bytes,
-                           (int32_t)tokens, rows, bits, sid, sfrom);
-    } else if (o.sort_tiles > 1) {
-        uint32_t *a_ids = sid, *a_tok = sfrom, *b_ids = (uint32_t*)(ws + o.ids2), *b_tok = (uint32_t*)(ws + o.tokens2);
+    uint32_t *a_ids = sid, *a_tok = sfrom, *b_ids = (uint32_t*)(ws + o.ids2), *b_tok = (uint32_t*)(ws + o.tokens2);
+    if (o.merge_tiles) {
+        hipLaunchKernelGGL(embed_sort_tile_kernel, dim3(o.merge_tiles), dim3(SO_NT), 0, st, ids, id_bytes, (int32_t)tokens, rows, bits,
+                           a_ids, a_tok);
+        if (o.merge_tiles > 1) {
+            hipLaunchKernelGGL(embed_merge_kernel, dim3(o.merge_tiles), dim3(SO_NT), o.merge_tiles * SO_NT * 4, st, a_ids, a_tok,
+                               (int32_t)tokens, (int32_t)o.merge_tiles, b_ids, b_tok);
+            sid = b_ids;
+            sfrom = b_tok;
+        }
+    } else if (o.count_tiles) {
         SortPass p{};
         p.ids = ids;
         p.places = (uint32_t*)(ws + o.places);
         p.tokens = tokens;
         p.rows = rows;
-        p.tiles = o.sort_tiles;
+        p.tiles = o.count_tiles;
         p.id_bytes = id_bytes;
         for (p.shift = 0; p.shift < bits; p.shift += SO_BITS) {
             p.first_pass = p.shift == 0;
@@ -526,10 +568,9 @@ extern "C" int32_t cresso_embedding_backward(const void* ids, int32_t id_bytes, 
             p.in_tokens = a_tok;
             p.out_ids = b_ids;
             p.out_tokens = b_tok;
-            hipLaunchKernelGGL(embed_sort_count_kernel, dim3(o.sort_tiles), dim3(SO_NT), 0, st, p);
-            hipLaunchKernelGGL(embed_sort_scan_kernel, dim3(1), dim3(SO_NT), 0, st, p.places,
-                               (size_t)SO_DIGITS * o.sort_tiles);
-            hipLaunchKernelGGL(embed_sort_move_kernel, dim3(o.sort_tiles), dim3(SO_NT), sizeof(SortTile), st, p);
+            hipLaunchKernelGGL(embed_sort_count_kernel, dim3(o.count_tiles), dim3(SO_NT), 0, st, p);
+            hipLaunchKernelGGL(embed_sort_scan_kernel, dim3(1), dim3(SO_NT), 0, st, p.places, (size_t)SO_DIGITS * o.count_tiles);
+            hipLaunchKernelGGL(embed_sort_move_kernel, dim3(o.count_tiles), dim3(SO_NT), 0, st, p);
             std::swap(a_ids, b_ids);
             std::swap(a_tok, b_tok);
         }

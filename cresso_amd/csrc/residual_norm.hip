@@ -30,7 +30,7 @@ namespace {
 
 constexpr int RN_MIN_NT = 256;
 constexpr int RN_MAX_WIDTH = 16384;
-constexpr int RN_WORKERS = 512;     // of the gradient, about
+constexpr int RN_WIDE = 4096;       // above, the gradient holds no row in registers
 constexpr int RN_FWD_BLOCKS = 2048;
 
 struct SeamArgs {
@@ -257,34 +257,47 @@ __global__ __launch_bounds__(WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64) void s
     }
     int64_t gate = -1;
     int turn = 0;
-    for (int64_t k = 0; k < a.worker_rows; ++k) {   // the same count for every slot: the row sums hold a barrier
-        const int64_t row = first + k;
+    u32x4 hr[NU], yr[NU], ar[NU], nr[NU];   // the row, and the next one's on their way
+    u32x4 hn[NU], yn_[NU], an[NU], nn[NU];
+    float ry = 1.0f, rh = 0.0f, ry_n = 1.0f, rh_n = 0.0f;
+    const auto fetch = [&](int64_t row) {
         const bool on = row < last;
-        u32x4 hr[NU], yr[NU], ar[NU], nr[NU];
-        float ry = 1.0f, rh = 0.0f;
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
             const int64_t u = tid + i * (WPR * 64);
-            hr[i] = yr[i] = ar[i] = nr[i] = u32x4{0, 0, 0, 0};
+            hn[i] = yn_[i] = an[i] = nn[i] = u32x4{0, 0, 0, 0};
             if (on) {
-                hr[i] = load_unit((const T*)d.residual + row * d.residual_stride, u, width);
-                if (d.update) yr[i] = load_unit((const T*)d.update + row * d.update_stride, u, width);
-                if (d.d_out) ar[i] = load_unit((const T*)d.d_out + row * d.d_out_stride, u, width);
-                if (d.d_normed) nr[i] = load_unit((const T*)d.d_normed + row * d.d_normed_stride, u, width);
+                hn[i] = load_unit((const T*)d.residual + row * d.residual_stride, u, width);
+                if (d.update) yn_[i] = load_unit((const T*)d.update + row * d.update_stride, u, width);
+                if (d.d_out) an[i] = load_unit((const T*)d.d_out + row * d.d_out_stride, u, width);
+                if (d.d_normed) nn[i] = load_unit((const T*)d.d_normed + row * d.d_normed_stride, u, width);
             }
         }
-        if (on) {
-            if (d.post) ry = d.stats[2 * row];
-            if (d.d_normed) rh = d.stats[2 * row + 1];
-            if (d.gate && row / d.rows_per_gate != gate) {
-                gate = row / d.rows_per_gate;
-                const char* g = gate_row(d, row, vec_bytes<T>(d.gate_dtype));
+        if (on && d.post) ry_n = d.stats[2 * row];
+        if (on && d.d_normed) rh_n = d.stats[2 * row + 1];
+    };
+    fetch(first);
+    for (int64_t k = 0; k < a.worker_rows; ++k) {   // the same count for every slot: the row sums hold a barrier
+        const int64_t row = first + k;
+        const bool on = row < last;
 #pragma unroll
-                for (int i = 0; i < NU; ++i) {
-                    load_vec<T>(g, d.gate_dtype, tid + i * (WPR * 64), width, ga[i]);
+        for (int i = 0; i < NU; ++i) {
+            hr[i] = hn[i];
+            yr[i] = yn_[i];
+            ar[i] = an[i];
+            nr[i] = nn[i];
+        }
+        ry = ry_n;
+        rh = rh_n;
+        fetch(row + 1);
+        if (on && d.gate && row / d.rows_per_gate != gate) {
+            gate = row / d.rows_per_gate;
+            const char* g = gate_row(d, row, vec_bytes<T>(d.gate_dtype));
 #pragma unroll
-                    for (int e = 0; e < E; ++e) ga[i][e] = act_of(d.act, ga[i][e]);
-                }
+            for (int i = 0; i < NU; ++i) {
+                load_vec<T>(g, d.gate_dtype, tid + i * (WPR * 64), width, ga[i]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) ga[i][e] = act_of(d.act, ga[i][e]);
             }
         }
         float ss[3] = {0.0f, 0.0f, 0.0f};
@@ -361,6 +374,121 @@ __global__ __launch_bounds__(WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64) void s
     }
 }
 
+// The same for rows of more than 4096 elements (512 threads, NU units each),
+// whose registers would not hold a row, its parameters and the shared sums: only
+// the sums stay in registers.  A row is read twice, the second time from L2, and
+// its parameters with it.  (Above 8192 elements the sums alone pass what is
+// left beside a unit's numbers, and some of them lie in scratch memory.)
+template <typename T, int NU>
+__global__ __launch_bounds__(512) void seam_backward_wide_kernel(SeamArgs a) {
+    constexpr int E = Unit<T>::n, WPR = 8, NT = 512;
+    __shared__ float lds[2 * 16 * 3];
+    const cresso_residual_norm_desc& d = a.d;
+    const int tid = threadIdx.x;
+    const int64_t width = d.width, worker = blockIdx.x;
+    const float inv = 1.0f / (float)width;
+    int64_t first, last;
+    if (a.workers_per_gate == 1) {
+        first = worker * a.worker_rows;
+        last = min(d.rows, first + a.worker_rows);
+    } else {
+        const int64_t g = worker / a.workers_per_gate, j = worker - g * a.workers_per_gate;
+        first = g * d.rows_per_gate + j * a.worker_rows;
+        last = min((g + 1) * d.rows_per_gate, first + a.worker_rows);
+    }
+    float d1[NU][E] = {}, d2[NU][E] = {}, ds[NU][E] = {}, dg[NU][E] = {};
+    struct Part {
+        float h[E], y[E], t[E], dn[E], w1[E], w2[E], sc[E], ga[E];
+    };
+    const auto load = [&](int64_t row, int64_t u) {
+        Part p;
+        u32x4 r[4] = {};
+        r[0] = load_unit((const T*)d.residual + row * d.residual_stride, u, width);
+        if (d.update) r[1] = load_unit((const T*)d.update + row * d.update_stride, u, width);
+        if (d.d_out) r[2] = load_unit((const T*)d.d_out + row * d.d_out_stride, u, width);
+        if (d.d_normed) r[3] = load_unit((const T*)d.d_normed + row * d.d_normed_stride, u, width);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            p.w1[e] = p.w2[e] = p.ga[e] = 1.0f;
+            p.sc[e] = d.scale;
+        }
+        if (d.post) load_vec<T>(d.post, d.post_dtype, u, width, p.w1);
+        if (d.pre) load_vec<T>(d.pre, d.pre_dtype, u, width, p.w2);
+        if (d.scale_vec) load_vec<T>(d.scale_vec, d.scale_dtype, u, width, p.sc);
+        if (d.gate) {
+            load_vec<T>(gate_row(d, row, vec_bytes<T>(d.gate_dtype)), d.gate_dtype, u, width, p.ga);
+#pragma unroll
+            for (int e = 0; e < E; ++e) p.ga[e] = act_of(d.act, p.ga[e]);
+        }
+        widen<T>(r[0], p.h);
+        widen<T>(r[1], p.y);
+        widen<T>(r[2], p.t);
+        widen<T>(r[3], p.dn);
+        return p;
+    };
+    int turn = 0;
+    for (int64_t row = first; row < last; ++row) {
+        const float ry = d.post ? d.stats[2 * row] : 1.0f, rh = d.d_normed ? d.stats[2 * row + 1] : 0.0f;
+        float ss[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+        for (int i = 0; i < NU; ++i) {
+            const Part p = load(row, tid + i * NT);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float q = d.update ? p.ga[e] * p.w1[e] * (p.y[e] * ry) : 0.0f;
+                const float Hn = (p.sc[e] * p.h[e] + q) * rh, en = p.dn[e] * p.w2[e];
+                ss[0] += en * Hn;
+                ss[1] += q * (p.t[e] + rh * en);
+                ss[2] += q * Hn;
+            }
+        }
+        row_sum<WPR>(ss, lds, turn++);
+        const float c1 = rh * ss[0] * inv;
+        const float c2 = d.post ? (ss[1] - c1 * ss[2]) * inv : 0.0f;
+        const bool gate_ends = d.d_gate && a.workers_per_gate == 1 && (row + 1) % d.rows_per_gate == 0;
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int64_t u = tid + i * NT;
+            const Part p = load(row, u);
+            float dh[E], dy[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float yn = d.update ? p.y[e] * ry : 0.0f;
+                const float Hn = (p.sc[e] * p.h[e] + p.ga[e] * p.w1[e] * yn) * rh;
+                const float D = p.t[e] + rh * (p.dn[e] * p.w2[e]) - Hn * c1;
+                dh[e] = p.sc[e] * D;
+                ds[i][e] += D * p.h[e];
+                d2[i][e] += p.dn[e] * Hn;
+                const float da = D * p.ga[e];
+                d1[i][e] += da * yn;
+                dg[i][e] += D * (yn * p.w1[e]);
+                dy[e] = ry * (da * p.w1[e] - yn * c2);
+            }
+            if (d.d_residual) store_unit((T*)d.d_residual + row * width, u, width, narrow<T>(dh));
+            if (d.d_update) store_unit((T*)d.d_update + row * width, u, width, narrow<T>(dy));
+            if (gate_ends) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) dg[i][e] *= act_slope(d.act, p.ga[e]);
+                store_vec<T>((char*)d.d_gate + row / d.rows_per_gate * width * vec_bytes<T>(d.gate_dtype), d.gate_dtype, u, width, dg[i]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) dg[i][e] = 0.0f;
+            }
+            __builtin_amdgcn_sched_barrier(0);   // one unit's numbers at a time
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        const int64_t u = tid + i * NT;
+        const auto put = [&](int which, const float (&v)[E]) {
+            store_vec<T>(a.partial + ((int64_t)which * a.workers + worker) * a.padded, CRESSO_F32, u, width, v);
+        };
+        if (d.d_post) put(G_POST, d1[i]);
+        if (d.d_pre) put(G_PRE, d2[i]);
+        if (d.d_scale) put(G_SCALE, ds[i]);
+        if (d.d_gate && a.workers_per_gate > 1) put(G_GATE, dg[i]);
+    }
+}
+
 // Adds the workers' partial sums, 64 columns and one vector a block: the
 // waves take equal runs of workers in order and their sums are added in order.
 template <typename T>
@@ -416,13 +544,17 @@ template <typename F> void with_shape(int32_t dtype, int64_t width, F&& fn) {
 }
 int slots_of(int wpr) { return wpr * 64 < RN_MIN_NT ? RN_MIN_NT / (wpr * 64) : 1; }
 
-// Workers of the gradient: about RN_WORKERS, each with whole gates' rows or a part of one gate's.
+// Workers of the gradient, each with whole gates' rows or a part of one gate's.
+// As many as are resident at once (8 waves to a CU, by the registers of a row,
+// its gradients and what is summed): more would only write more partial sums.
 SeamArgs plan_of(const cresso_residual_norm_desc& d) {
     SeamArgs a{};
     a.d = d;
     a.padded = (d.width + 63) / 64 * 64;
     const int64_t rpg = d.gate ? d.rows_per_gate : d.rows, gates = d.rows / rpg;
-    const int64_t want = std::max<int64_t>(1, (d.rows + RN_WORKERS - 1) / RN_WORKERS);
+    int64_t resident = 256;
+    if (d.width <= RN_WIDE) with_shape(d.dtype, d.width, [&](auto, auto wpr, auto) { resident = 256 * std::max(1, 8 / (int)decltype(wpr)::value); });
+    const int64_t want = std::max<int64_t>(1, (d.rows + resident - 1) / resident);
     if (rpg > want) {
         a.worker_rows = want;
         a.workers_per_gate = (rpg + want - 1) / want;
@@ -508,13 +640,27 @@ extern "C" int32_t cresso_residual_norm_backward(const cresso_residual_norm_desc
         return fail(CRESSO_E_INVALID, "residual norm gradient: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     const int64_t gates = a.d.gate && a.workers_per_gate > 1 ? a.d.rows / a.d.rows_per_gate : 0;
     a.partial = (float*)workspace;
-    with_shape(desc->dtype, desc->width, [&](auto t, auto wpr, auto nu) {
-        constexpr int WPR = decltype(wpr)::value, NU = decltype(nu)::value;
-        const int slots = slots_of(WPR);
-        const int64_t blocks = (a.workers + slots - 1) / slots;
-        hipLaunchKernelGGL((seam_backward_kernel<decltype(t), WPR, NU>), dim3((uint32_t)blocks), dim3(WPR * 64 * slots), 0,
-                           (hipStream_t)stream, a);
-    });
+    if (desc->width > RN_WIDE) {
+        with_row_dtype(desc->dtype, [&](auto t) {
+            using T = decltype(t);
+            const auto go = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3((uint32_t)a.workers), dim3(512), 0, (hipStream_t)stream, a);
+            };
+            constexpr int PER = 512 * Unit<T>::n;
+            if (desc->width <= 8192) go(seam_backward_wide_kernel<T, 8192 / PER>);
+            else go(seam_backward_wide_kernel<T, 16384 / PER>);
+        });
+    } else {
+        with_shape(desc->dtype, desc->width, [&](auto t, auto wpr, auto nu) {
+            constexpr int WPR = decltype(wpr)::value, NU = decltype(nu)::value;
+            if constexpr (WPR * NU * 64 * Unit<decltype(t)>::n <= RN_WIDE) {
+                const int slots = slots_of(WPR);
+                const int64_t blocks = (a.workers + slots - 1) / slots;
+                hipLaunchKernelGGL((seam_backward_kernel<decltype(t), WPR, NU>), dim3((uint32_t)blocks), dim3(WPR * 64 * slots), 0,
+                                   (hipStream_t)stream, a);
+            }
+        });
+    }
     if (a.d.d_post || a.d.d_pre || a.d.d_scale || (a.d.d_gate && gates > 0)) {
         with_row_dtype(desc->dtype, [&](auto t) {
             hipLaunchKernelGGL(seam_reduce_kernel<decltype(t)>, dim3((uint32_t)(a.padded / 64), (uint32_t)(3 + gates)),
