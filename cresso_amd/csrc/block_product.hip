@@ -605,7 +605,9 @@ ProductPlan product_plan(int64_t rows, int64_t cols, int64_t depth, const void* 
 int32_t check_product(const char* what, int64_t rows, int64_t cols, int64_t depth, int32_t dtype) {
     if (!row_dtype(dtype)) return fail(CRESSO_E_UNSUPPORTED, "%s: dtype %d not supported (f32, bf16, f16)", what, dtype);
     if (rows < 0 || cols < 0 || depth < 0) return fail(CRESSO_E_INVALID, "%s: negative size", what);
-    if (rows >= (int64_t)1 << 22 || cols >= (int64_t)1 << 21 || depth >= (int64_t)1 << 21 || rows * (depth / BP + 1) >= (int64_t)1 << 28)
+    // grids of up to 2^32 threads, 32-bit places in a tile's rows
+    if (rows >= (int64_t)1 << 22 || cols >= (int64_t)1 << 21 || depth >= (int64_t)1 << 21 || rows * (depth / BP + 1) >= (int64_t)1 << 27 ||
+        cols * depth >= (int64_t)1 << 34 || rows * cols >= (int64_t)1 << 38)
         return fail(CRESSO_E_UNSUPPORTED, "%s: %lld x %lld x %lld is more than one call takes", what, (long long)rows,
                     (long long)cols, (long long)depth);
     return CRESSO_OK;
@@ -630,8 +632,9 @@ extern "C" int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t
     if (rows == 0 || cols == 0) return CRESSO_OK;
     if (!out || (depth > 0 && (!x || !w || !scales))) return fail(CRESSO_E_INVALID, "block product: null argument");
     const ProductPlan o = product_plan(rows, cols, depth, w, w_stride, turned);
-    if (!workspace || workspace_bytes < (size_t)o.total)
-        return fail(CRESSO_E_INVALID, "block product: workspace of %zu bytes, %lld needed", workspace_bytes, (long long)o.total);
+    if (!workspace || workspace_bytes < (size_t)o.total || ((uintptr_t)workspace & 15))
+        return fail(CRESSO_E_INVALID, "block product: workspace of %zu bytes at %p, %lld at a multiple of 16 needed", workspace_bytes, workspace,
+                    (long long)o.total);
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     ProductArgs a{};

@@ -22,6 +22,7 @@ namespace {
 
 constexpr int EM_NT = 256;
 constexpr int EM_CHUNK = 32;       // sorted tokens per wave (at most a wave's lanes)
+constexpr uint32_t EM_AHEAD = 8;   // of them whose loads are on their way together
 constexpr int EM_MAX_BLOCKS = 1 << 20;   // of the lookup; more tokens are looped over
 constexpr int EM_ZROWS = 8;        // table rows per wave of the fill
 constexpr int SO_NT = 1024;        // threads of the sort: 16 waves
@@ -377,26 +378,37 @@ __global__ __launch_bounds__(EM_NT) void embed_sum_kernel(EmbedSum a, const T* g
     float s[E] = {};
     uint32_t current = __builtin_amdgcn_readfirstlane(my_id);
     bool head = from_before;   // the current segment began in an earlier chunk
-    for (uint32_t i = 0; i < n; ++i) {
-        const uint32_t v = __builtin_amdgcn_readlane(my_id, i);
-        if (v != current) {
-            if (head) {
-                float* q = partial_at<T>(a, chunk, 0, tile);
+    for (uint32_t i0 = 0; i0 < n; i0 += EM_AHEAD) {
+        u32x4 raw[EM_AHEAD];
 #pragma unroll
-                for (int e = 0; e < E; ++e) q[e] = s[e];
-            } else {
-                write_row(a, out, current, unit, s);
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) s[e] = 0.0f;
-            head = false;
-            current = v;
+        for (uint32_t k = 0; k < EM_AHEAD; ++k) {
+            raw[k] = u32x4{0, 0, 0, 0};
+            if (i0 + k < n && (uint32_t)__builtin_amdgcn_readlane(my_id, i0 + k) < a.rows)
+                raw[k] = load_unit(grad + (int64_t)__builtin_amdgcn_readlane(my_from, i0 + k) * a.grad_stride, unit, a.width);
         }
-        if (v < a.rows) {
-            float g[E];
-            widen<T>(load_unit(grad + (int64_t)__builtin_amdgcn_readlane(my_from, i) * a.grad_stride, unit, a.width), g);
 #pragma unroll
-            for (int e = 0; e < E; ++e) s[e] += g[e];
+        for (uint32_t k = 0; k < EM_AHEAD; ++k) {
+            if (i0 + k >= n) break;
+            const uint32_t v = __builtin_amdgcn_readlane(my_id, i0 + k);
+            if (v != current) {
+                if (head) {
+                    float* q = partial_at<T>(a, chunk, 0, tile);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) q[e] = s[e];
+                } else {
+                    write_row(a, out, current, unit, s);
+                }
+#pragma unroll
+                for (int e = 0; e < E; ++e) s[e] = 0.0f;
+                head = false;
+                current = v;
+            }
+            if (v < a.rows) {
+                float g[E];
+                widen<T>(raw[k], g);
+#pragma unroll
+                for (int e = 0; e < E; ++e) s[e] += g[e];
+            }
         }
     }
     if (head || goes_on) {
@@ -536,9 +548,9 @@ extern "C" int32_t cresso_embedding_backward(const void* ids, int32_t id_bytes, 
     if (!grad_table || (tokens > 0 && !grad)) return fail(CRESSO_E_INVALID, "embedding gradient: null argument");
     if (tokens > 1 && grad_stride < 0) return fail(CRESSO_E_INVALID, "embedding gradient: negative row stride");
     const EmbedLayout o = embed_layout(tokens, width, dtype);
-    if (!workspace || workspace_bytes < (size_t)o.total)
-        return fail(CRESSO_E_INVALID, "embedding gradient: workspace of %zu bytes, %lld needed", workspace_bytes,
-                    (long long)o.total);
+    if (!workspace || workspace_bytes < (size_t)o.total || ((uintptr_t)workspace & 15))
+        return fail(CRESSO_E_INVALID, "embedding gradient: workspace of %zu bytes at %p, %lld at a multiple of 16 needed", workspace_bytes,
+                    workspace, (long long)o.total);
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)workspace;
     uint32_t *sid = (uint32_t*)(ws + o.ids), *sfrom = (uint32_t*)(ws + o.tokens);

@@ -528,7 +528,10 @@ std::tuple<Tensor, Tensor> distill_loss_and_grad(const Tensor& logits, const Ten
         grad = at::empty(logits.sizes(), logits.options().requires_grad(false));
     }
     const Tensor stats = at::empty({logits.size(0), 3}, logits.options().dtype(at::kFloat).requires_grad(false));
-    return {std::get<1>(distill_run(c, true, stats, grad)), grad};
+    Tensor total = std::get<1>(distill_run(c, true, stats, grad));
+    // written behind torch's back: what has saved it for its own gradient has to notice
+    if (out.has_value()) grad.unsafeGetTensorImpl()->bump_version();
+    return {total, grad};
 }
 
 // ---------------------------------------------------------------------------

@@ -636,8 +636,9 @@ extern "C" int32_t cresso_residual_norm_backward(const cresso_residual_norm_desc
     SeamArgs a = plan_of(*desc);
     if (!a.d.gate) a.d.rows_per_gate = a.d.rows;
     const size_t need = (size_t)4 * a.workers * a.padded * sizeof(float);
-    if (!workspace || workspace_bytes < need)
-        return fail(CRESSO_E_INVALID, "residual norm gradient: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
+        return fail(CRESSO_E_INVALID, "residual norm gradient: workspace of %zu bytes at %p, %zu at a multiple of 16 needed", workspace_bytes,
+                    workspace, need);
     const int64_t gates = a.d.gate && a.workers_per_gate > 1 ? a.d.rows / a.d.rows_per_gate : 0;
     a.partial = (float*)workspace;
     if (desc->width > RN_WIDE) {

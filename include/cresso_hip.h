@@ -423,7 +423,8 @@ int32_t cresso_drive_update(void* param, int32_t param_dtype, const float* tange
  * counterpart): embedding, the seam between blocks, products with an 8-bit
  * frozen weight, the distillation loss.  Rows are `width` consecutive elements
  * (f32, bf16 or f16) at a row stride given in elements; nothing needs more
- * alignment than its element.
+ * alignment than its element, but a workspace 16 bytes.  Workspaces hold
+ * nothing between calls.
  * ------------------------------------------------------------------------- */
 
 /* out[t] = scale * table[ids[t]], rows of zeros for ids outside [0, rows).

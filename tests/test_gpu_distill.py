@@ -232,6 +232,15 @@ def test_gradient_against_differences():
     assert abs(got - slope) <= 2e-5 * float((g.double().cpu() * direction).abs().sum())
 
 
+def test_logits_that_were_overwritten_are_noticed():
+    z = rand((4, 30), seed=17).requires_grad_(True)
+    y = torch.sigmoid(z)   # keeps its output for its own gradient
+    index, a = torch.zeros(4, 1, dtype=torch.int64).cuda(), torch.zeros(4, 1).cuda()
+    _, g = cresso_amd.distill_loss_and_grad(y, index, a, out=y.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(g)
+
+
 def test_without_rows():
     z, index, a = torch.zeros(0, 10).cuda(), torch.zeros(0, 3, dtype=torch.int64).cuda(), torch.zeros(0, 3).cuda()
     assert cresso_amd.distill_loss(z, index, a).item() == 0.0
