@@ -175,6 +175,7 @@ def test_strides_and_shapes(rows):
     check(rand((rows, 2, 333), torch.float16, 3), values, scales)
     check(rand((333,), torch.float32, 3), values, scales)
     assert torch.equal(cresso_amd.block_product(x, values, scales.t().contiguous().t()), want)
+    assert torch.equal(cresso_amd.block_product(x, values.t().contiguous().t(), scales), want)
 
 
 def test_weights_whose_rows_end_inside_a_block():
