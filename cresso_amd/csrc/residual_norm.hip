@@ -21,6 +21,11 @@
 // from its load to its store; the gradients of what is shared by rows are kept
 // in registers over a worker's rows, written once per worker as fp32 and added
 // by a second kernel in worker order.  All sums are fp32.
+//
+// 16384 x 4096 bf16, a gate and a scale per channel: forward 99 us (537 MB, 5.4
+// TB/s), gradient 170 us (805 MB, 4.7 TB/s) and 6.2 us for the sums of 256
+// workers.  8 x 2048 bf16 forward: 4.4 us, latency of the loads and of two
+// sums over four waves.  1533 x 1001 fp32: 8.9, 13.7 and 8.9 us.
 #include "row_ops.hpp"
 
 #include <algorithm>
@@ -120,7 +125,9 @@ __device__ __forceinline__ void row_sum(float (&x)[V], float* lds, int turn) {
     }
 }
 
-// waves per row WPR, units per thread NU
+// waves per row WPR, units per thread NU: a unit a thread as long as a workgroup
+// has room, so that a row's loads are one instruction a wave and its sums few
+// steps.  What all rows share is read once and kept in registers.
 template <typename T, int WPR, int NU>
 __global__ __launch_bounds__(WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64) void seam_forward_kernel(SeamArgs a) {
     constexpr int E = Unit<T>::n, NT = WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64, SLOTS = NT / (WPR * 64);
@@ -377,7 +384,8 @@ __global__ __launch_bounds__(WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64) void s
 // The same for rows of more than 4096 elements (512 threads, NU units each),
 // whose registers would not hold a row, its parameters and the shared sums: only
 // the sums stay in registers.  A row is read twice, the second time from L2, and
-// its parameters with it.  (Above 8192 elements the sums alone pass what is
+// its parameters with it: 8192 x 8192 bf16 346 us with the sums, 1361 as
+// above with the row's registers spilled.  (Above 8192 elements the sums alone pass what is
 // left beside a unit's numbers, and some of them lie in scratch memory.)
 template <typename T, int NU>
 __global__ __launch_bounds__(512) void seam_backward_wide_kernel(SeamArgs a) {
@@ -546,7 +554,9 @@ int slots_of(int wpr) { return wpr * 64 < RN_MIN_NT ? RN_MIN_NT / (wpr * 64) : 1
 
 // Workers of the gradient, each with whole gates' rows or a part of one gate's.
 // As many as are resident at once (8 waves to a CU, by the registers of a row,
-// its gradients and what is summed): more would only write more partial sums.
+// its gradients and what is summed): more would only write more partial sums
+// (16384 x 4096 bf16: 176 us with the sums; 206 with more workers and without the
+// next row's loads ahead).
 SeamArgs plan_of(const cresso_residual_norm_desc& d) {
     SeamArgs a{};
     a.d = d;

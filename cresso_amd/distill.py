@@ -29,7 +29,8 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_logi
     reduction: "sum" (fp32 scalar) or "none" (fp32 [rows], weighted).
 
     The gradient goes to the logits alone.  Where the loss is the end of the
-    program, :func:`distill_loss_and_grad` gives both in one pass.
+    program, :func:`distill_loss_and_grad` gives both in one call,
+    without keeping anything for a backward pass.
     """
     if reduction not in ("sum", "none"):
         raise ValueError(f"distill_loss: reduction must be 'sum' or 'none', not {reduction!r}")
