@@ -6,7 +6,7 @@
 // Forward: one read and one write of each token's row, 16 bytes per lane;
 // bound by HBM (16384 x 4096 bf16 of 32000 rows: 43 to 48 us, 134 MB written and
 // 110 read, 5.1 to 5.7 TB/s) or, for a few tokens, by the launch and the two
-// loads that wait for one another (8 x 2048: 3.0 us).
+// loads that wait for one another (8 x 2048: 2.7 us).
 //
 // Gradient: the tokens are sorted by id (stable, so a row's terms keep the
 // order of the tokens and the result does not depend on timing), then the
