@@ -471,7 +471,8 @@ int32_t cresso_residual_norm_backward(const cresso_residual_norm_desc* desc, voi
  * index [rows][top] (int32 or int64): outside [0, vocab) is absent.  labels
  * may be NULL; ignore_index and labels outside the vocabulary give no term.
  * weights may be NULL (then `weight` for every row); a row of weight 0, or
- * without teacher and label, gives 0 whatever it holds.  top <= 1024. */
+ * without teacher and label, gives 0 whatever it holds; so does a term whose
+ * factor is 0 (mix 1 or 0).  top <= 1024. */
 typedef struct cresso_distill_desc {
     const void *logits, *index, *teacher, *labels;
     const float* weights;

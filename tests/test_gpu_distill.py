@@ -283,3 +283,28 @@ def test_refusals():
         cresso_amd.distill_loss_and_grad(z, index, a, out=torch.zeros(30, 4).cuda().t())
     with pytest.raises(RuntimeError, match="GPU only"):
         cresso_amd.distill_loss(z, index.cpu(), a)
+
+
+@pytest.mark.parametrize("mix", [0.0, 1.0])
+def test_a_factor_of_zero_leaves_its_term_out(mix):
+    """An infinite term must not come through a factor of 0 as NaN: as if what makes the term were not given."""
+    z, index, a, _ = make(6, 700, 5, seed=11, labels=False)
+    index[index == 0] = 699
+    lab = torch.zeros(6, dtype=torch.int64, device="cuda")
+    lab[4] = -100
+    gone = lab.clamp(min=0) if mix == 1.0 else index[:, 1]
+    z[torch.arange(6, device="cuda"), gone] = -math.inf
+    kw = dict(temperature=1.5, mix=mix)
+    want = cresso_amd.distill_loss_and_grad(z, index if mix == 1.0 else torch.full_like(index, -1), a,
+                                            labels=None if mix == 1.0 else lab, **kw)
+    got = cresso_amd.distill_loss_and_grad(z, index, a, labels=lab, **kw)
+    assert torch.isfinite(got[0]) and torch.isfinite(got[1]).all()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    zr = z.clone().requires_grad_(True)
+    loss = cresso_amd.distill_loss(zr, index, a, labels=lab, **kw)
+    (grad,) = torch.autograd.grad(loss, zr)
+    assert torch.equal(loss.detach(), want[0]) and torch.isfinite(grad).all()
+    assert torch.equal(got[1] == 0, grad == 0)
+    if mix == 1.0:   # a row with nothing but a label has no term left
+        alone = cresso_amd.distill_loss(z, torch.full_like(index, -1), a, labels=lab, reduction="none", **kw)
+        assert torch.equal(alone, torch.zeros_like(alone))
