@@ -23,9 +23,9 @@
 // by a second kernel in worker order.  All sums are fp32.
 //
 // 16384 x 4096 bf16, a gate and a scale per channel: forward 99 us (537 MB, 5.4
-// TB/s), gradient 170 us (805 MB, 4.7 TB/s) and 6.2 us for the sums of 256
+// TB/s), gradient 170 us (805 MB, 4.7 TB/s) and 5.2 us for the sums of 256
 // workers.  8 x 2048 bf16 forward: 4.4 us, latency of the loads and of two
-// sums over four waves.  1533 x 1001 fp32: 8.9, 13.7 and 8.9 us.
+// sums over four waves.  1533 x 1001 fp32: 8.6, 13.7 and 5.4 us.
 #include "row_ops.hpp"
 
 #include <algorithm>
@@ -34,6 +34,7 @@ namespace cresso {
 namespace {
 
 constexpr int RN_MIN_NT = 256;
+constexpr int RN_SUM_NT = 1024;
 constexpr int RN_MAX_WIDTH = 16384;
 constexpr int RN_WIDE = 4096;       // above, the gradient holds no row in registers
 constexpr int RN_FWD_BLOCKS = 2048;
@@ -499,9 +500,11 @@ __global__ __launch_bounds__(512) void seam_backward_wide_kernel(SeamArgs a) {
 
 // Adds the workers' partial sums, 64 columns and one vector a block: the
 // waves take equal runs of workers in order and their sums are added in order.
+// Latency of a run's loads bounds it, so there are as many waves as a block
+// has (512 workers x 1001: 5.4 us, with four waves 8.9).
 template <typename T>
-__global__ __launch_bounds__(RN_MIN_NT) void seam_reduce_kernel(SeamArgs a) {
-    constexpr int W = RN_MIN_NT / kWave;
+__global__ __launch_bounds__(RN_SUM_NT) void seam_reduce_kernel(SeamArgs a) {
+    constexpr int W = RN_SUM_NT / kWave;
     __shared__ float part[W][kWave];
     const cresso_residual_norm_desc& d = a.d;
     const int which = blockIdx.y < 3 ? (int)blockIdx.y : (int)G_GATE;
@@ -555,7 +558,7 @@ int slots_of(int wpr) { return wpr * 64 < RN_MIN_NT ? RN_MIN_NT / (wpr * 64) : 1
 // Workers of the gradient, each with whole gates' rows or a part of one gate's.
 // As many as are resident at once (8 waves to a CU, by the registers of a row,
 // its gradients and what is summed): more would only write more partial sums
-// (16384 x 4096 bf16: 176 us with the sums; 206 with more workers and without the
+// (16384 x 4096 bf16: 175 us with the sums; 206 with more workers and without the
 // next row's loads ahead).
 SeamArgs plan_of(const cresso_residual_norm_desc& d) {
     SeamArgs a{};
@@ -675,7 +678,7 @@ extern "C" int32_t cresso_residual_norm_backward(const cresso_residual_norm_desc
     if (a.d.d_post || a.d.d_pre || a.d.d_scale || (a.d.d_gate && gates > 0)) {
         with_row_dtype(desc->dtype, [&](auto t) {
             hipLaunchKernelGGL(seam_reduce_kernel<decltype(t)>, dim3((uint32_t)(a.padded / 64), (uint32_t)(3 + gates)),
-                               dim3(RN_MIN_NT), 0, (hipStream_t)stream, a);
+                               dim3(RN_SUM_NT), 0, (hipStream_t)stream, a);
         });
     }
     return launched("residual norm gradient");
