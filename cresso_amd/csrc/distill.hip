@@ -14,12 +14,13 @@
 // teacher and no label; their few places are written again afterwards from
 // logits that were read before, so it may take the logits' own memory.
 //
-// Exponents are kept in base 2: z*c - C with c = log2(e)/t and C = c*m rounded
-// once, one fused operation per logit.  The rounding of C is the same for the
-// whole row and drops out, since the sum is taken against the same C.  Where t
-// is 1 or 2, exp(z-m) is exp((z-m)/t) or its square: one transcendental
-// operation per logit instead of two, which is what bounds the passes next to
-// HBM.
+// Exponents are kept in base 2: (z-m)*c with c = log2(e)/t.  The difference
+// comes first, so that the largest logit's exponent is 0 at any size and the
+// others are off by 2^-24 of themselves: z*c - m*c, though one operation less,
+// is off by 2^-24 of m*c, which from 2^31 on (a row, or a thread's part of
+// one, that holds only mask values) is more than fp32 has exponents.  Where t is 1
+// or 2, exp(z-m) is exp((z-m)/t) or its square: one transcendental operation
+// per logit instead of two, which is what bounds the passes next to HBM.
 //
 // A row without weight, or without any teacher entry and label, is not read:
 // its loss and gradient are 0 whatever it holds.  Entries with an index
@@ -74,22 +75,14 @@ __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f
 // The exponentials of a row against its maximum.  P: how exp(z-m) comes
 // about.  0: it is not wanted; 1, 2: that power of exp((z-m)/t); -1: neither.
 template <int P> struct RowExp {
-    float c;      // log2(e) / t
-    float C, C1;  // c*m, log2(e)*m
-    __device__ __forceinline__ void set(float m) {
-        C = c * m;
-        C1 = LOG2E * m;
-    }
-    __device__ __forceinline__ float soft2(float v) const { return fmaf(v, c, -C); }
-    __device__ __forceinline__ float hard2(float v) const { return P > 0 ? (float)P * soft2(v) : fmaf(v, LOG2E, -C1); }
-    // log2 of what a sum of exp(z-m) against `from` is multiplied by
-    __device__ __forceinline__ float hard_by(const RowExp& from) const { return P > 0 ? (float)P * (from.C - C) : from.C1 - C1; }
+    float c;   // log2(e) / t
+    float m;   // finite, or a logit's own infinity
+    __device__ __forceinline__ float soft2(float v) const { return (v - m) * c; }
+    __device__ __forceinline__ float hard2(float v) const { return P > 0 ? (float)P * soft2(v) : (v - m) * LOG2E; }
     // exp(z-m), given exp((z-m)/t)
-    __device__ __forceinline__ float hard(float v, float t) const {
-        return P == 1 ? t : P == 2 ? t * t : fexp2(fmaf(v, LOG2E, -C1));
-    }
+    __device__ __forceinline__ float hard(float v, float t) const { return P == 1 ? t : P == 2 ? t * t : fexp2(hard2(v)); }
 };
-template <int P> __device__ __forceinline__ RowExp<P> row_exp(const cresso_distill_desc& d) { return {LOG2E / d.temperature, 0.0f, 0.0f}; }
+template <int P> __device__ __forceinline__ RowExp<P> row_exp(const cresso_distill_desc& d) { return {LOG2E / d.temperature, 0.0f}; }
 
 // A sum against another maximum; one that holds nothing yet has none.
 __device__ __forceinline__ float moved(float sum, float by2) { return sum == 0.0f ? 0.0f : sum * fexp2(by2); }
@@ -102,11 +95,11 @@ template <int P> struct RowSums {
 #pragma unroll
         for (int e = 1; e < E; ++e) um = fmaxf(um, v[e]);
         if (um > top) {
-            const RowExp<P> before = x;
+            const float before = x.m;
             top = um;
-            x.set(um);
-            st = moved(st, before.C - x.C);
-            if (P) s1 = moved(s1, x.hard_by(before));
+            x.m = um;
+            st = moved(st, x.soft2(before));
+            if (P) s1 = moved(s1, x.hard2(before));
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -122,10 +115,10 @@ template <int P>
 __device__ __forceinline__ void join_sums(DistillLds& s, RowSums<P> r, RowExp<P>& x, float& m, float& l_t, float& l_1) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
     const float wm = wave_max(r.top);
-    RowExp<P> b = x;
-    b.set(base_of(wm));
-    r.st = wave_sum(moved(r.st, x.C - b.C));
-    r.s1 = P ? wave_sum(moved(r.s1, b.hard_by(x))) : 0.0f;
+    const float own = x.m;
+    x.m = base_of(wm);
+    r.st = wave_sum(moved(r.st, x.soft2(own)));
+    r.s1 = P ? wave_sum(moved(r.s1, x.hard2(own))) : 0.0f;
     if (lane == 0) {
         s.red[wave][0] = wm;
         s.red[wave][1] = r.st;
@@ -136,13 +129,13 @@ __device__ __forceinline__ void join_sums(DistillLds& s, RowSums<P> r, RowExp<P>
 #pragma unroll 1
     for (int k = 1; k < waves; ++k) m = fmaxf(m, s.red[k][0]);
     m = base_of(m);
-    x.set(m);
+    x.m = m;
     float st = 0.0f, s1 = 0.0f;
 #pragma unroll 1
     for (int k = 0; k < waves; ++k) {
-        b.set(base_of(s.red[k][0]));
-        st += moved(s.red[k][1], b.C - x.C);
-        if (P) s1 += moved(s.red[k][2], x.hard_by(b));
+        const float of = base_of(s.red[k][0]);
+        st += moved(s.red[k][1], x.soft2(of));
+        if (P) s1 += moved(s.red[k][2], x.hard2(of));
     }
     l_t = log2f(st);
     l_1 = P ? log2f(s1) : 0.0f;
@@ -188,15 +181,15 @@ __device__ __forceinline__ void teacher_of(const cresso_distill_desc& d, Distill
     for (int j = lane; j < d.top; j += kWave) {
         top = fmaxf(top, s.p[j]);
     }
-    const float A = x.c * base_of(wave_max(top));
+    const RowExp<0> a{x.c, base_of(wave_max(top))};
 #pragma unroll 1
-    for (int j = lane; j < d.top; j += kWave) total += fexp2(fmaf(s.p[j], x.c, -A));
+    for (int j = lane; j < d.top; j += kWave) total += fexp2(a.soft2(s.p[j]));
     total = wave_sum(total);
     const bool any = !(total == 0.0f);   // entries that all are -inf are no teacher
     const float l_total = log2f(total);
 #pragma unroll 1
     for (int j = lane; j < d.top; j += kWave) {
-        const float a2 = fmaf(s.p[j], x.c, -A), v = s.z[j];
+        const float a2 = a.soft2(s.p[j]), v = s.z[j];
         const float p = any && s.index[j] >= 0 ? fexp2(a2) / total : 0.0f;
         if (!(p == 0.0f)) kl += p * ((a2 - l_total) - (x.soft2(v) - l_t));
         s.p[j] = p;
@@ -311,7 +304,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(cresso_distill_desc d) {
         m = d.stats[3 * row];
         l_t = d.stats[3 * row + 1];
         l_1 = d.stats[3 * row + 2];
-        x.set(m);
+        x.m = m;
     } else {
         RowSums<P> sums;
         for_units<T, NT, false>(z, vocab, [&](int64_t u, u32x4 raw) {
