@@ -12,7 +12,9 @@
 // element and reads the row again, from its end, where the caches still hold
 // it; it is written as if there were no
 // teacher and no label; their few places are written again afterwards from
-// logits that were read before, so it may take the logits' own memory.
+// logits that were read before, so it may take the logits' own memory: the
+// same rows at the same stride.  Any other share in what is read is refused,
+// since a workgroup would overwrite what another has yet to read.
 //
 // Exponents are kept in base 2: (z-m)*c with c = log2(e)/t.  The difference
 // comes first, so that the largest logit's exponent is 0 at any size and the
@@ -34,6 +36,7 @@
 // of the row spilled, and nothing on its way while it computes.  The loss of
 // 512 x 32000 bf16: 11 us (33 MB in one round of workgroups, most of it start
 // and end); of 301 x 50257 fp32: 20 us, and the gradient 24 us (4.9 TB/s).
+#include "overlap.hpp"
 #include "row_ops.hpp"
 
 #include <algorithm>
@@ -354,6 +357,10 @@ int32_t check_distill(const char* what, const cresso_distill_desc* d) {
         return fail(CRESSO_E_INVALID, "%s: temperature must be positive and mix within 0..1", what);
     if (d->rows > 0 && (!d->logits || (d->top > 0 && (!d->index || !d->teacher))))
         return fail(CRESSO_E_INVALID, "%s: null argument", what);
+    if (d->grad) {
+        const char* with = distill_overlap(*d);
+        if (with) return fail(CRESSO_E_INVALID, "%s: the gradient's memory overlaps the %s", what, with);
+    }
     return CRESSO_OK;
 }
 

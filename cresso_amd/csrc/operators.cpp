@@ -17,6 +17,7 @@
 #include <string>
 
 #include "../../include/cresso_hip.h"
+#include "overlap.hpp"
 
 namespace {
 
@@ -459,6 +460,9 @@ std::tuple<Tensor, Tensor> distill_run(const Distill& c, bool sum, const Tensor&
     if (grad.defined()) {
         d.grad = grad.mutable_data_ptr();
         d.grad_stride = grad.stride(0);
+        const char* with = cresso::distill_overlap(d);
+        TORCH_CHECK_VALUE(!with, "distill_loss: out shares memory with the ", with ? with : "",
+                          " (it may take the logits' place: the same rows at the same stride)");
     }
     const c10::DeviceGuard guard(c.logits.device());
     done(g_api.distill_loss(&d, stream_of(c.logits)), "distill_loss");

@@ -50,7 +50,8 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_index: torch.Tensor, tea
     """-> (summed loss, its gradient with respect to the logits) of
     :func:`distill_loss`, for programs that drive the backward pass from the
     logits themselves (``logits.backward(grad)``).  `out`: where the gradient
-    goes, rows at any stride; it may be `logits` itself."""
+    goes, rows at any stride; it may be `logits` itself (the same rows at the
+    same stride), but share no other memory with the inputs."""
     try:
         return _native.operators().distill_loss_and_grad(logits, teacher_index, teacher_logits, labels, row_weights,
                                                          temperature, mix, ignore_index, out)

@@ -424,7 +424,8 @@ int32_t cresso_drive_update(void* param, int32_t param_dtype, const float* tange
  * frozen weight, the distillation loss.  Rows are `width` consecutive elements
  * (f32, bf16 or f16) at a row stride given in elements; nothing needs more
  * alignment than its element, but a workspace 16 bytes.  Workspaces hold
- * nothing between calls.
+ * nothing between calls.  Outputs share no memory with what a call reads,
+ * unless it is said below.
  * ------------------------------------------------------------------------- */
 
 /* out[t] = scale * table[ids[t]], rows of zeros for ids outside [0, rows).
@@ -480,7 +481,8 @@ typedef struct cresso_distill_desc {
     float* stats;                       /* [rows][3], written with the loss when not NULL, read by the gradient; with
                                          * the loss and `grad` it must be there */
     const float* d_loss;                /* gradient: d_loss[d_loss_stride * row] */
-    void* grad;                         /* with the loss: NULL or the gradient for d_loss = 1; may be the logits */
+    void* grad;                         /* with the loss: NULL or the gradient for d_loss = 1.  May be the logits (the same
+                                         * address and stride); any other share in what is read is refused */
     int64_t logits_stride, index_stride, teacher_stride, grad_stride, d_loss_stride;
     int64_t rows, vocab, ignore_index;
     float temperature, mix, weight;
