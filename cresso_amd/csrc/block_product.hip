@@ -641,6 +641,12 @@ extern "C" int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t
     if (rc != CRESSO_OK) return rc;
     if (rows == 0 || cols == 0) return CRESSO_OK;
     if (!out || (depth > 0 && (!x || !w || !scales))) return fail(CRESSO_E_INVALID, "block product: null argument");
+    const int64_t w_rows = turned ? depth : cols, w_cols = turned ? cols : depth;
+    if (!row_stride_ok(x, rows, depth, x_stride)) return fail(CRESSO_E_INVALID, "block product: row stride %lld of x below the depth", (long long)x_stride);
+    if (w_rows > 1 && w_stride < w_cols)
+        return fail(CRESSO_E_INVALID, "block product: row stride %lld of a weight of %lld columns", (long long)w_stride, (long long)w_cols);
+    if (w_rows > BP && scale_stride < up(w_cols, BP) / BP)
+        return fail(CRESSO_E_INVALID, "block product: row stride %lld of the scales of %lld columns", (long long)scale_stride, (long long)w_cols);
     const ProductPlan o = product_plan(rows, cols, depth, w, w_stride, turned);
     if (!workspace || workspace_bytes < (size_t)o.total || ((uintptr_t)workspace & 15))
         return fail(CRESSO_E_INVALID, "block product: workspace of %zu bytes at %p, %lld at a multiple of 16 needed", workspace_bytes, workspace,
@@ -705,6 +711,7 @@ extern "C" int32_t cresso_block_quantize(const void* w, int64_t w_stride, int32_
     if (rc != CRESSO_OK) return rc;
     if (rows == 0 || cols == 0) return CRESSO_OK;
     if (!w || !values || !scales) return fail(CRESSO_E_INVALID, "block quantization: null argument");
+    if (!row_stride_ok(w, rows, cols, w_stride)) return fail(CRESSO_E_INVALID, "block quantization: row stride %lld below the width", (long long)w_stride);
     with_row_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const dim3 grid((uint32_t)(up(cols, BP) / BP), (uint32_t)(up(rows, BP) / BP));

@@ -357,6 +357,14 @@ int32_t check_distill(const char* what, const cresso_distill_desc* d) {
         return fail(CRESSO_E_INVALID, "%s: temperature must be positive and mix within 0..1", what);
     if (d->rows > 0 && (!d->logits || (d->top > 0 && (!d->index || !d->teacher))))
         return fail(CRESSO_E_INVALID, "%s: null argument", what);
+    const struct { const void* p; int64_t width, stride; const char* name; } spans[] = {
+        {d->logits, d->vocab, d->logits_stride, "logits"}, {d->index, d->top, d->index_stride, "teacher's indexes"},
+        {d->teacher, d->top, d->teacher_stride, "teacher's logits"}, {d->d_loss, 1, d->d_loss_stride, "gradient that arrives"}};
+    for (const auto& v : spans)
+        if (!row_stride_ok(v.p, d->rows, v.width, v.stride))
+            return fail(CRESSO_E_INVALID, "%s: row stride %lld of the %s below the width", what, (long long)v.stride, v.name);
+    if (d->grad && d->rows > 1 && d->grad_stride < d->vocab)
+        return fail(CRESSO_E_INVALID, "%s: row stride %lld of the gradient below the width", what, (long long)d->grad_stride);
     if (d->grad) {
         const char* with = distill_overlap(*d);
         if (with) return fail(CRESSO_E_INVALID, "%s: the gradient's memory overlaps the %s", what, with);

@@ -560,7 +560,7 @@ extern "C" int32_t cresso_embedding_backward(const void* ids, int32_t id_bytes, 
     if (rc != CRESSO_OK) return rc;
     if (rows == 0 || width == 0) return CRESSO_OK;
     if (!grad_table || (tokens > 0 && !grad)) return fail(CRESSO_E_INVALID, "embedding gradient: null argument");
-    if (tokens > 1 && grad_stride < 0) return fail(CRESSO_E_INVALID, "embedding gradient: negative row stride");
+    if (!row_stride_ok(grad, tokens, width, grad_stride)) return fail(CRESSO_E_INVALID, "embedding gradient: row stride below the width");
     const EmbedLayout o = embed_layout(tokens, width, dtype);
     if (!workspace || workspace_bytes < (size_t)o.total || ((uintptr_t)workspace & 15))
         return fail(CRESSO_E_INVALID, "embedding gradient: workspace of %zu bytes at %p, %lld at a multiple of 16 needed", workspace_bytes,

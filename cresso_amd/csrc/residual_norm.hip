@@ -605,6 +605,13 @@ int32_t check_seam(const char* what, const cresso_residual_norm_desc* d) {
             return fail(CRESSO_E_INVALID, "%s: %lld rows are no multiple of %lld rows per gate", what, (long long)d->rows,
                         (long long)d->rows_per_gate);
     }
+    const struct { const void* p; int64_t stride, rows; const char* name; } spans[] = {
+        {d->residual, d->residual_stride, d->rows, "residual"}, {d->update, d->update_stride, d->rows, "update"},
+        {d->gate, d->gate_stride, d->gate ? d->rows / d->rows_per_gate : 0, "gate"},
+        {d->d_out, d->d_out_stride, d->rows, "gradient of out"}, {d->d_normed, d->d_normed_stride, d->rows, "gradient of normed"}};
+    for (const auto& v : spans)
+        if (!row_stride_ok(v.p, v.rows, d->width, v.stride))
+            return fail(CRESSO_E_INVALID, "%s: row stride %lld of the %s below the width", what, (long long)v.stride, v.name);
     return CRESSO_OK;
 }
 

@@ -146,6 +146,12 @@ inline int32_t launched(const char* what) {
 // row-element dtypes of these operators
 inline bool row_dtype(int32_t c) { return c == CRESSO_F32 || c == CRESSO_BF16 || c == CRESSO_F16; }
 
+// Rows of `width` elements that are read: at a stride that leaves each its own
+// elements, or all of them at one place (stride 0).
+inline bool row_stride_ok(const void* p, int64_t rows, int64_t width, int64_t stride) {
+    return !p || rows < 2 || stride == 0 || stride >= width;
+}
+
 // Runs fn(T{}) for the element type of `code` (checked by row_dtype before).
 template <typename F> inline void with_row_dtype(int32_t code, F&& fn) {
     if (code == CRESSO_F32) fn(float{});

@@ -422,7 +422,8 @@ int32_t cresso_drive_update(void* param, int32_t param_dtype, const float* tange
  * Operators of a training step around the optimizer (no reference
  * counterpart): embedding, the seam between blocks, products with an 8-bit
  * frozen weight, the distillation loss.  Rows are `width` consecutive elements
- * (f32, bf16 or f16) at a row stride given in elements; nothing needs more
+ * (f32, bf16 or f16) at a row stride given in elements, at least the width (or
+ * 0 for rows that are read: one row for all); nothing needs more
  * alignment than its element, but a workspace 16 bytes.  Workspaces hold
  * nothing between calls.  Outputs share no memory with what a call reads,
  * unless it is said below.
