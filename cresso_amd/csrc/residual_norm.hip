@@ -14,7 +14,9 @@
 //
 // d is linear in mean(e*Hn), so with t = dH + rh*e and q = a*w1*yn
 //   mean(d*q) = mean(t*q) - rh*mean(e*Hn)*mean(Hn*q)
-// and one round of three sums per row serves both norms.
+// and one round of three sums per row serves both norms.  Where nothing arrives
+// at n, or there is no norm after the block, its terms are left out: a factor
+// of 0 would make an infinite element the whole row's NaN.
 //
 // Both directions are bound by HBM: 4 rows of traffic forward (h, y in; H, n
 // out), 6 backward (h, y, dH, dn in; dh, dy out).  A row stays in registers
@@ -230,7 +232,10 @@ __global__ __launch_bounds__(WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64) void s
 // which of the four shared gradients, in `partial` and in the reduction
 enum { G_POST, G_PRE, G_SCALE, G_GATE };
 
-template <typename T, int WPR, int NU>
+// FULL: something arrives at n, and there is a norm after the block.  The other
+// forms ask for either on the way (in one kernel for all of them 16384 x 2048
+// fp32 takes 183 us, 176 as it is).
+template <typename T, int WPR, int NU, bool FULL>
 __global__ __launch_bounds__(WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64) void seam_backward_kernel(SeamArgs a) {
     constexpr int E = Unit<T>::n, NT = WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64, SLOTS = NT / (WPR * 64);
     __shared__ float lds[2 * 16 * 3];
@@ -238,6 +243,7 @@ __global__ __launch_bounds__(WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64) void s
     const int slot = threadIdx.x / (WPR * 64), tid = threadIdx.x % (WPR * 64);
     const int64_t width = d.width, worker = (int64_t)blockIdx.x * SLOTS + slot;
     const float inv = 1.0f / (float)width;
+    const bool normed = FULL || d.d_normed, post = FULL || d.post;
     // the worker's rows: whole gates' rows, or a part of one gate's
     int64_t first, last;
     if (a.workers_per_gate == 1) {
@@ -319,15 +325,19 @@ __global__ __launch_bounds__(WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64) void s
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float q = d.update ? ga[i][e] * w1[i][e] * (y[e] * ry) : 0.0f;
-                const float Hn = (sc[i][e] * h[e] + q) * rh, en = dn[e] * w2[i][e];
-                ss[0] += en * Hn;
-                ss[1] += q * (t[e] + rh * en);
-                ss[2] += q * Hn;
+                if (normed) {
+                    const float Hn = (sc[i][e] * h[e] + q) * rh, en = dn[e] * w2[i][e];
+                    ss[0] += en * Hn;
+                    ss[1] += q * (t[e] + rh * en);
+                    ss[2] += q * Hn;
+                } else {
+                    ss[1] += q * t[e];
+                }
             }
         }
         row_sum<WPR>(ss, lds, turn++);
-        const float c1 = rh * ss[0] * inv;                          // rh * mean(e*Hn)
-        const float c2 = d.post ? (ss[1] - c1 * ss[2]) * inv : 0.0f;   // mean(d*q)
+        const float c1 = rh * ss[0] * inv;            // rh * mean(e*Hn)
+        const float c2 = (normed ? ss[1] - c1 * ss[2] : ss[1]) * inv;   // mean(d*q)
         if (on) {
 #pragma unroll
             for (int i = 0; i < NU; ++i) {
@@ -340,15 +350,19 @@ __global__ __launch_bounds__(WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64) void s
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float yn = d.update ? y[e] * ry : 0.0f;
-                    const float Hn = (sc[i][e] * h[e] + ga[i][e] * w1[i][e] * yn) * rh;
-                    const float D = t[e] + rh * (dn[e] * w2[i][e]) - Hn * c1;
+                    float D = t[e];
+                    if (normed) {
+                        const float Hn = (sc[i][e] * h[e] + ga[i][e] * w1[i][e] * yn) * rh;
+                        D = t[e] + rh * (dn[e] * w2[i][e]) - Hn * c1;
+                        d2[i][e] += dn[e] * Hn;
+                    }
                     dh[e] = sc[i][e] * D;
                     ds[i][e] += D * h[e];
-                    d2[i][e] += dn[e] * Hn;
                     const float da = D * ga[i][e];
                     d1[i][e] += da * yn;
                     dg[i][e] += D * (yn * w1[i][e]);
-                    dy[e] = ry * (da * w1[i][e] - yn * c2);
+                    dy[e] = da * w1[i][e];
+                    if (post) dy[e] = ry * (dy[e] - yn * c2);
                 }
                 if (d.d_residual) store_unit((T*)d.d_residual + row * width, u, width, narrow<T>(dh));
                 if (d.d_update) store_unit((T*)d.d_update + row * width, u, width, narrow<T>(dy));
@@ -388,7 +402,7 @@ __global__ __launch_bounds__(WPR * 64 < RN_MIN_NT ? RN_MIN_NT : WPR * 64) void s
 // its parameters with it: 8192 x 8192 bf16 346 us with the sums, 1361 as
 // above with the row's registers spilled.  (Above 8192 elements the sums alone pass what is
 // left beside a unit's numbers, and some of them lie in scratch memory.)
-template <typename T, int NU>
+template <typename T, int NU, bool FULL>
 __global__ __launch_bounds__(512) void seam_backward_wide_kernel(SeamArgs a) {
     constexpr int E = Unit<T>::n, WPR = 8, NT = 512;
     __shared__ float lds[2 * 16 * 3];
@@ -396,6 +410,7 @@ __global__ __launch_bounds__(512) void seam_backward_wide_kernel(SeamArgs a) {
     const int tid = threadIdx.x;
     const int64_t width = d.width, worker = blockIdx.x;
     const float inv = 1.0f / (float)width;
+    const bool normed = FULL || d.d_normed, post = FULL || d.post;
     int64_t first, last;
     if (a.workers_per_gate == 1) {
         first = worker * a.worker_rows;
@@ -445,15 +460,19 @@ __global__ __launch_bounds__(512) void seam_backward_wide_kernel(SeamArgs a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float q = d.update ? p.ga[e] * p.w1[e] * (p.y[e] * ry) : 0.0f;
-                const float Hn = (p.sc[e] * p.h[e] + q) * rh, en = p.dn[e] * p.w2[e];
-                ss[0] += en * Hn;
-                ss[1] += q * (p.t[e] + rh * en);
-                ss[2] += q * Hn;
+                if (normed) {
+                    const float Hn = (p.sc[e] * p.h[e] + q) * rh, en = p.dn[e] * p.w2[e];
+                    ss[0] += en * Hn;
+                    ss[1] += q * (p.t[e] + rh * en);
+                    ss[2] += q * Hn;
+                } else {
+                    ss[1] += q * p.t[e];
+                }
             }
         }
         row_sum<WPR>(ss, lds, turn++);
         const float c1 = rh * ss[0] * inv;
-        const float c2 = d.post ? (ss[1] - c1 * ss[2]) * inv : 0.0f;
+        const float c2 = (normed ? ss[1] - c1 * ss[2] : ss[1]) * inv;
         const bool gate_ends = d.d_gate && a.workers_per_gate == 1 && (row + 1) % d.rows_per_gate == 0;
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
@@ -463,15 +482,19 @@ __global__ __launch_bounds__(512) void seam_backward_wide_kernel(SeamArgs a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float yn = d.update ? p.y[e] * ry : 0.0f;
-                const float Hn = (p.sc[e] * p.h[e] + p.ga[e] * p.w1[e] * yn) * rh;
-                const float D = p.t[e] + rh * (p.dn[e] * p.w2[e]) - Hn * c1;
+                float D = p.t[e];
+                if (normed) {
+                    const float Hn = (p.sc[e] * p.h[e] + p.ga[e] * p.w1[e] * yn) * rh;
+                    D = p.t[e] + rh * (p.dn[e] * p.w2[e]) - Hn * c1;
+                    d2[i][e] += p.dn[e] * Hn;
+                }
                 dh[e] = p.sc[e] * D;
                 ds[i][e] += D * p.h[e];
-                d2[i][e] += p.dn[e] * Hn;
                 const float da = D * p.ga[e];
                 d1[i][e] += da * yn;
                 dg[i][e] += D * (yn * p.w1[e]);
-                dy[e] = ry * (da * p.w1[e] - yn * c2);
+                dy[e] = da * p.w1[e];
+                if (post) dy[e] = ry * (dy[e] - yn * c2);
             }
             if (d.d_residual) store_unit((T*)d.d_residual + row * width, u, width, narrow<T>(dh));
             if (d.d_update) store_unit((T*)d.d_update + row * width, u, width, narrow<T>(dy));
@@ -661,6 +684,7 @@ extern "C" int32_t cresso_residual_norm_backward(const cresso_residual_norm_desc
                     workspace, need);
     const int64_t gates = a.d.gate && a.workers_per_gate > 1 ? a.d.rows / a.d.rows_per_gate : 0;
     a.partial = (float*)workspace;
+    const bool full = desc->d_normed && desc->post;
     if (desc->width > RN_WIDE) {
         with_row_dtype(desc->dtype, [&](auto t) {
             using T = decltype(t);
@@ -668,8 +692,8 @@ extern "C" int32_t cresso_residual_norm_backward(const cresso_residual_norm_desc
                 hipLaunchKernelGGL(kernel, dim3((uint32_t)a.workers), dim3(512), 0, (hipStream_t)stream, a);
             };
             constexpr int PER = 512 * Unit<T>::n;
-            if (desc->width <= 8192) go(seam_backward_wide_kernel<T, 8192 / PER>);
-            else go(seam_backward_wide_kernel<T, 16384 / PER>);
+            if (desc->width <= 8192) full ? go(seam_backward_wide_kernel<T, 8192 / PER, true>) : go(seam_backward_wide_kernel<T, 8192 / PER, false>);
+            else go(seam_backward_wide_kernel<T, 16384 / PER, false>);   // less of it in scratch: 4096 x 16384 bf16 695 us, 887 with true
         });
     } else {
         with_shape(desc->dtype, desc->width, [&](auto t, auto wpr, auto nu) {
@@ -677,8 +701,10 @@ extern "C" int32_t cresso_residual_norm_backward(const cresso_residual_norm_desc
             if constexpr (WPR * NU * 64 * Unit<decltype(t)>::n <= RN_WIDE) {
                 const int slots = slots_of(WPR);
                 const int64_t blocks = (a.workers + slots - 1) / slots;
-                hipLaunchKernelGGL((seam_backward_kernel<decltype(t), WPR, NU>), dim3((uint32_t)blocks), dim3(WPR * 64 * slots), 0,
-                                   (hipStream_t)stream, a);
+                const auto go = [&](auto kernel) {
+                    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(WPR * 64 * slots), 0, (hipStream_t)stream, a);
+                };
+                full ? go(seam_backward_kernel<decltype(t), WPR, NU, true>) : go(seam_backward_kernel<decltype(t), WPR, NU, false>);
             }
         });
     }
