@@ -81,13 +81,16 @@ const char* name_of(at::ScalarType t) { return c10::toString(t); }
 void check_row_type(const char* what, const char* name, const Tensor& t) {
     TORCH_CHECK_VALUE(row_type(t.scalar_type()), what, ": ", name, " must be fp32, bf16 or fp16, not ", name_of(t.scalar_type()));
 }
-// Every tensor given lies on one GPU; there is no CPU path.
+// Every tensor given lies on one GPU; there is no CPU path.  None is a dual
+// tensor: the operators have no forward-mode derivatives, and an output without
+// a tangent would say that its derivative is zero.
 struct OneGpu {
     const char* what;
     const Tensor* first = nullptr;
     void add(const char* name, const Tensor& t) {
         if (!t.defined()) return;
         TORCH_CHECK(t.is_cuda(), what, ": ", name, " is on ", t.device(), "; the operators run on the GPU only");
+        TORCH_CHECK(!t._fw_grad(0).defined(), what, ": ", name, " has a forward-mode derivative, the operators have reverse mode only");
         if (!first) first = &t;
         TORCH_CHECK(t.device() == first->device(), what, ": ", name, " is on ", t.device(), ", others on ", first->device());
     }
@@ -517,6 +520,7 @@ std::tuple<Tensor, Tensor> distill_loss_and_grad(const Tensor& logits, const Ten
                                                  double mix, int64_t ignore, const optional<Tensor>& out) {
     const char* what = "distill_loss";
     const at::NoGradGuard no_grad;
+    OneGpu{what}.add("logits", logits);   // detach() drops a tangent
     const Distill c{logits.detach(), index, teacher, or_none(labels), or_none(weights), temperature, mix, ignore};
     check_distill(c);
     Tensor grad = or_none(out);
