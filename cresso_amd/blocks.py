@@ -19,8 +19,9 @@ def block_product(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor) -
     x (fp32, bf16, fp16) is rounded to e4m3 in the call, with one power of two
     for each row and 128 of its elements: the smallest 2^e with max|x| <= 448 *
     2^e (e >= -117), taken over the finite ones.  An infinity or NaN makes its
-    row's outputs NaN; what would round to 2^128 becomes 15/16 of it.  Sums are
-    fp32, rounded once.
+    row's outputs NaN; what would round to 2^128 becomes 15/16 of it.  A block
+    whose scale is 0 counts as zeros whatever its values are.  Sums are fp32,
+    rounded once.
 
     The weight is frozen: the gradient goes to x alone, as the product of the
     incoming gradient, rounded in the same manner, with the weight.

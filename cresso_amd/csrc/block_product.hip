@@ -21,6 +21,9 @@
 // and block, and no second set of accumulators for a block's own sum, which
 // is what lets a wave hold 128 x 64 outputs.
 //
+// A block whose scale is 0 counts as zeros, whatever its values: who divides a
+// block of zeros by its largest magnitude is left with that scale and NaN.
+//
 // 16384 x 2048 x 5632 bf16: 372 us, 1015 TFLOP/s, after 23 us for the rounding
 // (a plain bf16 product of the library: 354 to 374 us); its gradient 325 us,
 // 1163 TFLOP/s, after 62 us (the library: 246).  The matrix instructions are
@@ -493,6 +496,10 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void few_rows_kernel(ProductArgs a,
         });
         float unit, f;
         split_scale(scale, unit, f);
+        if (scale == 0.0f) {   // the block counts as zeros, as in the tiles
+#pragma unroll
+            for (int i = 0; i < FN; ++i) w[i][0] = w[i][1] = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int i = 0; i < FN; ++i) {
             f32x4 p = {0, 0, 0, 0};

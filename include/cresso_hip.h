@@ -498,7 +498,8 @@ int32_t cresso_distill_backward(const cresso_distill_desc* desc, void* stream);
  * scales: [ceil(w rows / 128)][scale_stride >= ceil(w cols / 128)].  x is
  * rounded to e4m3 with a power of two per row and 128 elements (the smallest
  * 2^e with max <= 448 * 2^e, e >= -117); what is not finite becomes NaN, and
- * what would round to 2^128 becomes 15/16 of it.  out: contiguous,
+ * what would round to 2^128 becomes 15/16 of it.  A block of scale 0 counts as
+ * zeros whatever its values are.  out: contiguous,
  * of x's dtype.  Sums are fp32. */
 size_t cresso_block_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, const void* w, int64_t w_stride,
                                             int32_t turned);
