@@ -98,15 +98,24 @@ struct OneGpu {
 Tensor or_none(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 optional<Tensor> or_null(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : optional<Tensor>(); }
 
-// t seen as rows of its last dimension: rows at one stride are taken where
-// they lie, anything else is copied.
+// t seen as rows of its last dimension: rows at one stride of at least their
+// width, whatever dimensions they are counted by, are taken where they lie,
+// anything else is copied.
 Tensor rows_of(const Tensor& t, int64_t& stride) {
-    if (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= t.size(1)) {
-        stride = t.stride(0);
-        return t;
+    const int64_t n = t.dim() - 1, width = n >= 0 ? t.size(n) : 1;
+    int64_t at = 0, rows = 1;   // the rows' stride, 0 before a dimension has given it; rows counted so far
+    bool taken = n >= 0 && (width < 2 || t.stride(n) == 1);
+    for (int64_t i = n - 1; taken && i >= 0; --i) {
+        if (t.size(i) == 1) continue;
+        if (!at) {
+            at = t.stride(i);
+            taken = at >= width;
+        }
+        taken = taken && t.stride(i) == at * rows;
+        rows *= t.size(i);
     }
-    stride = t.dim() ? t.size(-1) : 1;
-    return t.contiguous();
+    stride = taken && at ? at : width;
+    return taken ? t : t.contiguous();
 }
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 void done(int32_t rc, const char* what) {
