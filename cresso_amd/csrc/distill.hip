@@ -393,10 +393,13 @@ template <int MODE> void launch_distill(const cresso_distill_desc& d, hipStream_
         // Long rows take 512 threads (4096 x 131072 bf16: 494 us, 550 with 256, 569
         // with 1024); where there are rows enough for more workgroups at once,
         // shorter ones fewer (4096 x 32000: 140 us with 256, 147 with 512; 8192 x
-        // 1000: 35 us with 64, 46 with 256; the loss of 512 x 32000: 10.9 us with
-        // 256, 11.4 with 512, of 256 x 32000 10.5 and 9.8).
+        // 1000: 35 us with 64, 46 with 256).  Rows enough are more than two to a CU:
+        // loss and gradient of 384, 512, 576, 768 and 1024 rows x 16000 take 18.4, 19.0,
+        // 20.7, 21.7 and 24.3 us with 256, 17.8, 18.1, 20.6, 21.5 and 27.7 with 512; of
+        // 32000 24.5, 25.9, 28.5, 31.1, 40.7 and 23.2, 24.2, 28.3, 31.1, 44.3; the loss
+        // alone of 32000 11.3, 11.8, 13.1, 13.8, 16.5 and 11.3, 11.7, 13.7, 14.5, 19.7.
         if (units <= 256) go(distill_kernel<T, MODE, P, 64>, 64);
-        else if (units <= 6144 && d.rows >= 512) go(distill_kernel<T, MODE, P, 256>, 256);
+        else if (units <= 6144 && d.rows > 512) go(distill_kernel<T, MODE, P, 256>, 256);
         else go(distill_kernel<T, MODE, P, 512>, 512);
     });
 }
