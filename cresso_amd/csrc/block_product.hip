@@ -27,9 +27,10 @@
 // 16384 x 2048 x 5632 bf16: 372 us, 1015 TFLOP/s, after 23 us for the rounding
 // (a plain bf16 product of the library: 354 to 374 us); its gradient 325 us,
 // 1163 TFLOP/s, after 62 us (the library: 246).  The matrix instructions are
-// busy for 47 and 54 % of the time, without a conflict in LDS; the rest is the
-// conversion of w beside them (two vector instructions to each) and the ends
-// of the rounds.  8 x 2048 x 5632: 6 to 7 us, 1.8 TB/s, latency; 333 x 1024 x
+// busy for 47 and 54 % of the time, without a conflict in LDS; beside each of 16
+// cycles stand 2.1 other vector instructions of 4 (conversion, rescaling), the
+// last of the rounds is half empty (8 %), and all waves of a workgroup pass a
+// barrier a stage, so the two of a SIMD read and convert at the same time.  8 x 2048 x 5632: 6 to 7 us, 1.8 TB/s, latency; 333 x 1024 x
 // 1536 5.4 + 7.7 us.
 #include "row_ops.hpp"
 
@@ -461,7 +462,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void product_kernel(ProductArgs a) 
 // of the arithmetic, so wide weights take FN = 2 or 4, as long as that leaves a
 // workgroup for about each CU (8 x 2048 x 2048: 5.4 us with 1, 6.5 with 2; x 5632: 8.6
 // with 1, 7.3 with 2, 8.5 with 4; 8 x 4096 x 8192: 13.2, 11.6 and 13.4; x 11008:
-// 18.9, 17.6 and 14.3).  16 x 2048 x 5632 takes 7.3 us, in tiles 4.8 + 8.9.
+// 18.9, 17.6 and 14.3).  The depth does not move the edges: of 45 products from 512
+// x 1024 to 16384 x 32000 the columns alone chose the fastest but once (512 x 32000
+// 8.4 with 4, 8.2 with 2); 512 x 4096 3.5 with 1 and 3.8 with 2, x 5632 4.0 and 3.8,
+// 16384 x 4096 26.9 and 29.9, x 5632 39.6 and 34.2.  16 x 2048 x 5632 takes 7.3
+// us, in tiles 4.8 + 8.9.
 // ---------------------------------------------------------------------------
 constexpr int FEW_WAVES = 8;
 constexpr int FEW_ROWS = 16;
@@ -593,7 +598,7 @@ __global__ __launch_bounds__(BP_NT) void quantize_blocks_kernel(const T* w, int6
 // too few would be left for all CUs: 64 x 64 below 192 tiles of 128 (512 x 2048
 // x 5632 25.5 us against 26.9, but 1024 x 4096 x 4096 58 against 47), 32 x 64
 // below 256 tiles of 64 (200 x 2048 x 2048 13.0 us against 15.1, but 333 x
-// 4096 x 5632 38.7 against 36.9).
+// 4096 x 5632 38.7 against 36.9; all of these with the rounding before them).
 struct ProductPlan {
     int tile;
     bool copy;   // the weight is laid out anew

@@ -26,7 +26,8 @@ def distill_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher_logi
     that is ignore_index or outside the vocabulary, and no labels at all, leave
     the cross entropy out.  row_weights: fp32 [rows], 1/rows each where not
     given; a row of weight 0 gives no loss and no gradient whatever it holds,
-    and a term whose factor is 0 (mix 1 or 0) nothing either.
+    and a term whose factor is 0 (mix 1 or 0) nothing either.  Masked logits
+    may be any finite number or -inf.
     reduction: "sum" (fp32 scalar) or "none" (fp32 [rows], weighted).
 
     The gradient goes to the logits alone.  Where the loss is the end of the
