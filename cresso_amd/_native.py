@@ -103,6 +103,21 @@ class DistillDesc(ctypes.Structure):
                     "top", "dtype", "teacher_dtype", "index_bytes", "label_bytes")]
 
 
+class GradDesc(ctypes.Structure):
+    _fields_ = [("grad", ctypes.c_void_p), ("out", ctypes.c_void_p), ("numel", ctypes.c_int64), ("dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32)]
+
+
+class RouteDesc(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_void_p) for k in ("logits", "bias", "weights", "experts", "order", "places", "offsets")] + [
+        ("logits_stride", ctypes.c_int64), ("tokens", ctypes.c_int64)] + [(k, ctypes.c_int32) for k in (
+            "num_experts", "top", "dtype", "score", "normalize")] + [("scale", ctypes.c_float)]
+
+
+NORM_2, NORM_MAX = 2, 0
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+
+
 def hyper_from_group(group: dict) -> Hyper:
     return Hyper(*[float(group[n]) for n in HYPER_DOUBLES], int(group["warmup_steps"]), 1 if bool(group["maximize"]) else 0)
 
@@ -234,6 +249,22 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.cresso_block_product.argtypes = [vp, i64, i32, i64, i64, i64, vp, i64, vp, i64, i32, vp, vp, size, vp]
     lib.cresso_block_quantize.restype = i32
     lib.cresso_block_quantize.argtypes = [vp, i64, i32, i64, i64, vp, vp, vp]
+    grad_desc, route_desc = c.POINTER(GradDesc), c.POINTER(RouteDesc)
+    for bytes_of, args in ((lib.cresso_clip_workspace_bytes, [grad_desc, i32]), (lib.cresso_route_workspace_bytes, [route_desc]),
+                           (lib.cresso_expert_product_workspace_bytes, [i64, i64, i64, i32, i32]),
+                           (lib.cresso_expert_product_weight_workspace_bytes, [i64, i64, i64, i32, i32])):
+        bytes_of.restype = size
+        bytes_of.argtypes = args
+    for fn, args in ((lib.cresso_clip_gradients, [grad_desc, i32, i32, f64, f64, vp, vp, size, vp]),
+                     (lib.cresso_route_forward, [route_desc, vp, size, vp]),
+                     (lib.cresso_route_backward, [route_desc, vp, vp, vp]),
+                     (lib.cresso_dispatch_rows, [vp, i64, i32, i64, i32, i64, vp, vp, vp, vp]),
+                     (lib.cresso_combine_rows, [vp, i64, i32, i64, i32, i64, vp, vp, vp, vp, vp]),
+                     (lib.cresso_combine_backward, [vp, i64, vp, i64, i32, i64, i32, i64, vp, vp, vp, vp, vp, vp]),
+                     (lib.cresso_expert_product, [vp, i64, i32, i64, i64, i64, vp, i64, i64, i32, i32, vp, vp, vp, size, vp]),
+                     (lib.cresso_expert_product_weight, [vp, i64, i64, vp, i64, i64, i32, i64, i32, vp, vp, vp, size, vp])):
+        fn.restype = i32
+        fn.argtypes = args
 
 
 def load() -> ctypes.CDLL:
@@ -302,7 +333,10 @@ OPERATOR_SYMBOLS = (
     "cresso_hip_last_error", "cresso_embedding_forward", "cresso_embedding_backward_workspace_bytes",
     "cresso_embedding_backward", "cresso_residual_norm_forward", "cresso_residual_norm_backward_workspace_bytes",
     "cresso_residual_norm_backward", "cresso_distill_loss", "cresso_distill_backward",
-    "cresso_block_product_workspace_bytes", "cresso_block_product", "cresso_block_quantize")
+    "cresso_block_product_workspace_bytes", "cresso_block_product", "cresso_block_quantize", "cresso_clip_workspace_bytes",
+    "cresso_clip_gradients", "cresso_route_workspace_bytes", "cresso_route_forward", "cresso_route_backward", "cresso_dispatch_rows",
+    "cresso_combine_rows", "cresso_combine_backward", "cresso_expert_product_workspace_bytes", "cresso_expert_product",
+    "cresso_expert_product_weight_workspace_bytes", "cresso_expert_product_weight")
 
 
 def operators():

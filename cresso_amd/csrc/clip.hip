@@ -1,0 +1,366 @@
+// The norm over a set of gradients, and the set clipped by it.
+//
+//   n = s * (sum over all elements of g^2)^(1/2)   or   s * max |g|
+//   out = g * s * c,   c = max_norm / n where n is finite and above max_norm, else 1
+//
+// Two passes over the data, each one launch over all tensors: the elements are
+// cut into chunks of 32 KB, and each workgroup takes an equal run of chunks,
+// whatever tensors they belong to.  The second pass begins where the first one
+// ended, with what the last cache still holds, and where c * s is 1 and the
+// tensors are clipped in place it reads nothing but the norm.
+//
+// Squares and their sums are fp64: gradients of 1e-30 and of 1e30 count as they
+// are, and no order of the tensors changes more than the last bits.  A thread's
+// sum, the waves' and the workgroups' are joined in a fixed order.
+#include "row_ops.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace cresso {
+namespace {
+
+constexpr int CL_NT = 256;
+constexpr int CL_UNITS = 8;                           // 16-byte units a thread holds of a chunk
+constexpr int CL_CHUNK = CL_NT * CL_UNITS * 16;       // bytes
+constexpr int CL_MAX_BLOCKS = 1024;                   // partial sums: each workgroup of the second pass adds them all up
+constexpr int CL_FILL = 160;                          // entries of one fill launch: its arguments stay below 4 KB
+
+// What a tensor is to the kernels: elements of `in` (and `out`) from chunk
+// `first` on, `tail` of them in its last chunk.
+struct ClipEntry {
+    const void* in;
+    void* out;
+    uint32_t first;
+    uint32_t tail_types;   // tail << 4 | in << 2 | out, types as CRESSO_*
+};
+static_assert(sizeof(ClipEntry) == 24 && (CL_CHUNK / 2) < (1 << 28), "entry");
+struct ClipFill {
+    ClipEntry e[CL_FILL];
+};
+struct ClipArgs {
+    ClipEntry* table;
+    double* partials;
+    float* norm;
+    uint32_t count, chunks, blocks;
+    int32_t kind;
+    double max_norm, scale;
+    int32_t write, in_place;   // write: there are outputs; in_place: every one is its input
+};
+
+int64_t element_bytes(int32_t code) { return code == CRESSO_F64 ? 8 : code == CRESSO_F32 ? 4 : 2; }
+
+// The table, from the arguments of the launch to memory: thread i copies entry i.
+__global__ __launch_bounds__(CL_FILL) void clip_fill_kernel(ClipFill f, ClipEntry* to, uint32_t count) {
+    // the arguments' own memory, so that the lane's index needs no copy of them
+    const auto* from = (const __attribute__((address_space(4))) ClipEntry*)__builtin_amdgcn_kernarg_segment_ptr();
+    if (threadIdx.x < count) {
+        const ClipEntry e = {from[threadIdx.x].in, from[threadIdx.x].out, from[threadIdx.x].first, from[threadIdx.x].tail_types};
+        to[threadIdx.x] = e;
+    }
+}
+
+// Index of the entry that holds `chunk`: how many begin at or before it, less one.
+__device__ __forceinline__ uint32_t entry_of(const ClipArgs& a, uint32_t chunk) {
+    __shared__ uint32_t found[CL_NT / kWave];
+    uint32_t n = 0;
+    for (uint32_t i = threadIdx.x; i < a.count; i += CL_NT) n += a.table[i].first <= chunk ? 1u : 0u;
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) n += __shfl_xor(n, m, kWave);
+    if ((threadIdx.x & (kWave - 1)) == 0) found[threadIdx.x / kWave] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < CL_NT / kWave; ++w) n += found[w];
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)n) - 1;
+}
+
+// ---------------------------------------------------------------------------
+// units of 16 bytes as doubles
+// ---------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ u32x4 clip_load(const T* p) {
+    if constexpr (sizeof(T) == 8) return load16((const float*)p);
+    else return load16(p);
+}
+template <typename T> __device__ __forceinline__ double clip_value(u32x4 r, int i);
+template <> __device__ __forceinline__ double clip_value<float>(u32x4 r, int i) {
+    const uint32_t w = r[i];
+    return (double)__builtin_bit_cast(float, w);
+}
+template <> __device__ __forceinline__ double clip_value<double>(u32x4 r, int i) {
+    const uint64_t w = (uint64_t)r[2 * i] | (uint64_t)r[2 * i + 1] << 32;
+    return __builtin_bit_cast(double, w);
+}
+template <> __device__ __forceinline__ double clip_value<__hip_bfloat16>(u32x4 r, int i) {
+    const uint32_t w = i & 1 ? r[i / 2] & 0xffff0000u : r[i / 2] << 16;
+    return (double)__builtin_bit_cast(float, w);
+}
+template <> __device__ __forceinline__ double clip_value<__half>(u32x4 r, int i) {
+    const uint32_t w = r[i / 2];
+    const f16x2 h = __builtin_bit_cast(f16x2, w);
+    return (double)(float)h[i & 1];
+}
+
+// Sums of squares are doubles; a maximum is the largest pattern of |g| as a
+// double: patterns order as the magnitudes do, NaN above infinity.
+template <bool MAX> struct ClipSum {
+    double v = 0.0;
+    __device__ __forceinline__ void add(double g) {
+        if constexpr (MAX) join(fabs(g));
+        else v = fma(g, g, v);
+    }
+    __device__ __forceinline__ void join(double o) {
+        if constexpr (MAX) {
+            const uint64_t x = (uint64_t)__double_as_longlong(v), y = (uint64_t)__double_as_longlong(o);
+            v = __longlong_as_double((long long)(x > y ? x : y));
+        } else {
+            v += o;
+        }
+    }
+};
+
+template <typename T, bool MAX> __device__ __forceinline__ void clip_sum(const T* at, uint32_t left, ClipSum<MAX> (&sum)[2]) {
+    constexpr int E = 16 / (int)sizeof(T);
+    constexpr uint32_t whole = CL_CHUNK / sizeof(T);
+    if (left == whole) {
+        u32x4 r[CL_UNITS];
+#pragma unroll
+        for (int u = 0; u < CL_UNITS; ++u) r[u] = clip_load(at + (uint32_t)(u * CL_NT + threadIdx.x) * E);
+#pragma unroll
+        for (int u = 0; u < CL_UNITS; ++u)
+#pragma unroll
+            for (int i = 0; i < E; ++i) sum[i & 1].add(clip_value<T>(r[u], i));
+        return;
+    }
+    for (uint32_t u = threadIdx.x * E; u < left; u += CL_NT * E) {
+        if (u + E <= left) {
+            const u32x4 r = clip_load(at + u);
+#pragma unroll
+            for (int i = 0; i < E; ++i) sum[i & 1].add(clip_value<T>(r, i));
+        } else {
+            for (uint32_t i = u; i < left; ++i) {
+                if constexpr (sizeof(T) == 8) sum[0].add(at[i]);
+                else sum[0].add((double)to_f(at[i]));
+            }
+        }
+    }
+}
+
+// Everybody's sums joined: lanes, then waves, in their order.
+template <bool MAX> __device__ __forceinline__ double clip_join(double v, double* lds) {
+    ClipSum<MAX> s;
+    s.v = v;
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) s.join(__shfl_xor(s.v, m, kWave));
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = s.v;
+    __syncthreads();
+    s.v = lds[0];
+#pragma unroll
+    for (int w = 1; w < CL_NT / kWave; ++w) s.join(lds[w]);
+    return s.v;
+}
+
+__device__ __forceinline__ void clip_run(const ClipArgs& a, uint32_t& lo, uint32_t& hi) {
+    lo = (uint32_t)((uint64_t)blockIdx.x * a.chunks / a.blocks);
+    hi = (uint32_t)((uint64_t)(blockIdx.x + 1) * a.chunks / a.blocks);
+}
+
+template <bool MAX> __global__ __launch_bounds__(CL_NT) void clip_norm_kernel(ClipArgs a) {
+    __shared__ double lds[CL_NT / kWave];
+    uint32_t lo, hi;
+    clip_run(a, lo, hi);
+    uint32_t e = entry_of(a, lo);
+    ClipSum<MAX> sum[2];
+    ClipEntry t = a.table[e];
+    uint32_t end = e + 1 < a.count ? a.table[e + 1].first : a.chunks;
+    for (uint32_t c = lo; c < hi; ++c) {
+        if (c == end) {
+            t = a.table[++e];
+            end = e + 1 < a.count ? a.table[e + 1].first : a.chunks;
+        }
+        const char* at = (const char*)t.in + (uint64_t)(c - t.first) * CL_CHUNK;
+        const uint32_t tail = t.tail_types >> 4, type = (t.tail_types >> 2) & 3;
+        const bool last = c + 1 == end;
+        if (type == CRESSO_F32) clip_sum<float>((const float*)at, last ? tail : CL_CHUNK / 4, sum);
+        else if (type == CRESSO_BF16) clip_sum<__hip_bfloat16>((const __hip_bfloat16*)at, last ? tail : CL_CHUNK / 2, sum);
+        else if (type == CRESSO_F16) clip_sum<__half>((const __half*)at, last ? tail : CL_CHUNK / 2, sum);
+        else clip_sum<double>((const double*)at, last ? tail : CL_CHUNK / 8, sum);
+    }
+    sum[0].join(sum[1].v);
+    const double v = clip_join<MAX>(sum[0].v, lds);
+    if (threadIdx.x == 0) a.partials[blockIdx.x] = v;
+}
+
+// E elements from `in` times f, rounded once, to `out`.
+template <typename T, typename O> __device__ __forceinline__ void clip_scale_unit(const T* in, O* out, double f) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const u32x4 r = clip_load(in);
+    if constexpr (sizeof(O) == 8) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint64_t v = (uint64_t)__double_as_longlong(clip_value<T>(r, i) * f);
+            w[2 * i] = (uint32_t)v;
+            w[2 * i + 1] = (uint32_t)(v >> 32);
+        }
+        store16((float*)out, w);
+    } else {
+        constexpr int EO = Unit<O>::n;   // a unit of 16 bytes in is one or two of fp32 out
+#pragma unroll
+        for (int h = 0; h < E / EO; ++h) {
+            float v[EO];
+#pragma unroll
+            for (int i = 0; i < EO; ++i) v[i] = (float)(clip_value<T>(r, h * EO + i) * f);
+            store16(out + h * EO, narrow<O>(v));
+        }
+    }
+}
+template <typename T, typename O> __device__ __forceinline__ void clip_scale(const T* in, O* out, uint32_t left, double f) {
+    constexpr int E = 16 / (int)sizeof(T);
+    if (left == CL_CHUNK / sizeof(T)) {
+#pragma unroll
+        for (int u = 0; u < CL_UNITS; ++u) {
+            const uint32_t at = (uint32_t)(u * CL_NT + threadIdx.x) * E;
+            clip_scale_unit(in + at, out + at, f);
+        }
+        return;
+    }
+    for (uint32_t u = threadIdx.x * E; u < left; u += CL_NT * E) {
+        if (u + E <= left) {
+            clip_scale_unit(in + u, out + u, f);
+        } else {
+            for (uint32_t i = u; i < left; ++i) {
+                if constexpr (sizeof(T) == 8) out[i] = in[i] * f;
+                else out[i] = from_w<O>((float)((double)to_f(in[i]) * f));
+            }
+        }
+    }
+}
+
+template <bool MAX> __global__ __launch_bounds__(CL_NT) void clip_scale_kernel(ClipArgs a) {
+    __shared__ double lds[CL_NT / kWave];
+    ClipSum<MAX> sum;
+#pragma unroll
+    for (int i = 0; i < CL_MAX_BLOCKS / CL_NT; ++i) {
+        const uint32_t at = i * CL_NT + threadIdx.x;
+        if (at < a.blocks) sum.join(a.partials[at]);
+    }
+    const double total = clip_join<MAX>(sum.v, lds);
+    const double norm = (MAX ? total : sqrt(total)) * fabs(a.scale);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.norm = (float)norm;
+    if (!a.write) return;
+    double f = a.scale;
+    if (norm > a.max_norm && norm < INFINITY) f *= a.max_norm / norm;
+    if (a.in_place && f == 1.0) return;
+    uint32_t lo, hi;
+    clip_run(a, lo, hi);
+    uint32_t e = entry_of(a, hi - 1);
+    ClipEntry t = a.table[e];
+    uint32_t end = e + 1 < a.count ? a.table[e + 1].first : a.chunks;
+    for (uint32_t c = hi; c-- > lo;) {   // backwards: what was read last is still in a cache
+        if (c < t.first) {
+            end = t.first;
+            t = a.table[--e];
+        }
+        if (!t.out || (t.out == t.in && f == 1.0)) continue;
+        const uint32_t tail = t.tail_types >> 4, types = t.tail_types & 15, type = types >> 2;
+        const uint32_t size = type == CRESSO_F64 ? 8 : type == CRESSO_F32 ? 4 : 2, out_size = (types & 3) == CRESSO_F64 ? 8 : (types & 3) == CRESSO_F32 ? 4 : 2;
+        const uint64_t first = (uint64_t)(c - t.first) * (CL_CHUNK / size);
+        const char* in = (const char*)t.in + first * size;
+        char* out = (char*)t.out + first * out_size;
+        const uint32_t left = c + 1 == end ? tail : CL_CHUNK / size;
+        if (types == (CRESSO_F32 << 2 | CRESSO_F32)) clip_scale((const float*)in, (float*)out, left, f);
+        else if (types == (CRESSO_BF16 << 2 | CRESSO_BF16)) clip_scale((const __hip_bfloat16*)in, (__hip_bfloat16*)out, left, f);
+        else if (types == (CRESSO_BF16 << 2 | CRESSO_F32)) clip_scale((const __hip_bfloat16*)in, (float*)out, left, f);
+        else if (types == (CRESSO_F16 << 2 | CRESSO_F16)) clip_scale((const __half*)in, (__half*)out, left, f);
+        else if (types == (CRESSO_F16 << 2 | CRESSO_F32)) clip_scale((const __half*)in, (float*)out, left, f);
+        else clip_scale((const double*)in, (double*)out, left, f);
+    }
+}
+
+bool clip_dtype(int32_t c) { return c >= CRESSO_F32 && c <= CRESSO_BF16; }
+
+int32_t check_clip(const cresso_grad_desc* g, int32_t count, uint32_t& entries, uint32_t& chunks) {
+    if (count < 0 || (count > 0 && !g)) return fail(CRESSO_E_INVALID, "gradient norm: null argument or negative count");
+    int64_t total = 0;
+    entries = 0;
+    for (int32_t i = 0; i < count; ++i) {
+        if (!clip_dtype(g[i].dtype)) return fail(CRESSO_E_UNSUPPORTED, "gradient norm: dtype %d not supported (f32, f64, f16, bf16)", g[i].dtype);
+        if (g[i].numel < 0) return fail(CRESSO_E_INVALID, "gradient norm: tensor %d has a negative size", i);
+        if (g[i].numel > 0 && !g[i].grad) return fail(CRESSO_E_INVALID, "gradient norm: tensor %d is null", i);
+        if (g[i].out && g[i].out_dtype != g[i].dtype && (g[i].out_dtype != CRESSO_F32 || g[i].dtype == CRESSO_F64))
+            return fail(CRESSO_E_UNSUPPORTED, "gradient norm: tensor %d of dtype %d to dtype %d (its own or, of 16 bits, f32)", i, g[i].dtype,
+                        g[i].out_dtype);
+        const int64_t per = CL_CHUNK / element_bytes(g[i].dtype);
+        total += g[i].numel / per + (g[i].numel % per ? 1 : 0);
+        if (total >= (int64_t)1 << 31) return fail(CRESSO_E_UNSUPPORTED, "gradient norm: more elements than one call takes");
+        entries += g[i].numel > 0;
+    }
+    chunks = (uint32_t)total;
+    return CRESSO_OK;
+}
+size_t table_bytes(uint32_t entries) { return ((size_t)entries * sizeof(ClipEntry) + 15) / 16 * 16; }
+}  // namespace
+}  // namespace cresso
+
+using namespace cresso;
+
+extern "C" size_t cresso_clip_workspace_bytes(const cresso_grad_desc* grads, int32_t count) {
+    uint32_t entries, chunks;
+    if (check_clip(grads, count, entries, chunks) != CRESSO_OK) return 0;
+    return CL_MAX_BLOCKS * sizeof(double) + table_bytes(entries);
+}
+
+extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t count, int32_t norm_kind, double max_norm,
+                                         double grad_scale, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+    uint32_t entries, chunks;
+    const int32_t rc = check_clip(grads, count, entries, chunks);
+    if (rc != CRESSO_OK) return rc;
+    if (norm_kind != CRESSO_NORM_2 && norm_kind != CRESSO_NORM_MAX)
+        return fail(CRESSO_E_INVALID, "gradient norm: unknown norm %d", norm_kind);
+    if (!(max_norm >= 0.0)) return fail(CRESSO_E_INVALID, "gradient norm: max_norm must not be negative");
+    if (!std::isfinite(grad_scale)) return fail(CRESSO_E_INVALID, "gradient norm: grad_scale must be finite");
+    if (!norm) return fail(CRESSO_E_INVALID, "gradient norm: null norm");
+    const size_t need = CL_MAX_BLOCKS * sizeof(double) + table_bytes(entries);
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
+        return fail(CRESSO_E_INVALID, "gradient norm: workspace of %zu bytes at %p, %zu at a multiple of 16 needed", workspace_bytes, workspace, need);
+    hipStream_t st = (hipStream_t)stream;
+    ClipArgs a{};
+    a.partials = (double*)workspace;
+    a.table = (ClipEntry*)((char*)workspace + CL_MAX_BLOCKS * sizeof(double));
+    a.norm = norm;
+    a.count = entries;
+    a.chunks = chunks;
+    a.blocks = std::min<uint32_t>(chunks, CL_MAX_BLOCKS);
+    a.kind = norm_kind;
+    a.max_norm = max_norm;
+    a.scale = grad_scale;
+    a.in_place = 1;
+    ClipFill f;
+    uint32_t held = 0, sent = 0, first = 0;
+    const auto flush = [&] {
+        if (held) hipLaunchKernelGGL(clip_fill_kernel, dim3(1), dim3(CL_FILL), 0, st, f, a.table + sent, held);
+        sent += held;
+        held = 0;
+    };
+    for (int32_t i = 0; i < count; ++i) {
+        const cresso_grad_desc& g = grads[i];
+        if (!g.numel) continue;
+        const int64_t per = CL_CHUNK / element_bytes(g.dtype);
+        const uint32_t n = (uint32_t)((g.numel + per - 1) / per), tail = (uint32_t)(g.numel - (int64_t)(n - 1) * per);
+        f.e[held++] = {g.grad, g.out, first, tail << 4 | (uint32_t)g.dtype << 2 | (uint32_t)(g.out ? g.out_dtype : 0)};
+        first += n;
+        if (g.out) a.write = 1;
+        if (g.out && g.out != g.grad) a.in_place = 0;
+        if (held == CL_FILL) flush();
+    }
+    flush();
+    const auto run = [&](auto norm_kernel, auto scale_kernel) {
+        if (a.blocks) hipLaunchKernelGGL(norm_kernel, dim3(a.blocks), dim3(CL_NT), 0, st, a);
+        hipLaunchKernelGGL(scale_kernel, dim3(a.write ? std::max(1u, a.blocks) : 1), dim3(CL_NT), 0, st, a);
+    };
+    if (norm_kind == CRESSO_NORM_2) run(clip_norm_kernel<false>, clip_scale_kernel<false>);
+    else run(clip_norm_kernel<true>, clip_scale_kernel<true>);
+    return launched("gradient norm");
+}

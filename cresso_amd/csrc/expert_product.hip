@@ -1,0 +1,98 @@
+// Grouped products: checks of the arguments and the choice of a kernel
+// (expert_product.hpp has the kernels, one source file a dtype compiles them).
+#include "expert_product.hpp"
+
+#include <algorithm>
+
+namespace cresso {
+template <> void group_launch<float>(GroupArgs, bool, bool, int, hipStream_t);
+template <> void group_launch<__half>(GroupArgs, bool, bool, int, hipStream_t);
+template <> void group_launch<__hip_bfloat16>(GroupArgs, bool, bool, int, hipStream_t);
+
+namespace {
+int32_t check_group(const char* what, int32_t dtype, int64_t rows, int64_t a, int64_t b, int32_t experts) {
+    if (!row_dtype(dtype)) return fail(CRESSO_E_UNSUPPORTED, "%s: dtype %d not supported (f32, bf16, f16)", what, dtype);
+    if (rows < 0 || a < 0 || b < 0 || experts < 0) return fail(CRESSO_E_INVALID, "%s: negative size", what);
+    // offsets of 32 bits; grids of up to 2^31 workgroups of the smallest tiles
+    const int64_t tiles = (rows / 32 + experts) * ((std::max(a, b) + 63) / 64);
+    if (rows >= (int64_t)1 << 31 || a >= (int64_t)1 << 22 || b >= (int64_t)1 << 22 || experts > 1 << 16 || tiles >= (int64_t)1 << 30 ||
+        (int64_t)experts * ((a + 31) / 32) * ((b + 63) / 64) >= (int64_t)1 << 30)
+        return fail(CRESSO_E_UNSUPPORTED, "%s: %lld rows, %d matrices of %lld x %lld are more than one call takes", what, (long long)rows,
+                    experts, (long long)a, (long long)b);
+    return CRESSO_OK;
+}
+}  // namespace
+}  // namespace cresso
+
+using namespace cresso;
+
+extern "C" size_t cresso_expert_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype) {
+    return check_group("expert product", dtype, rows, cols, depth, experts) == CRESSO_OK ? 16 : 0;
+}
+extern "C" size_t cresso_expert_product_weight_workspace_bytes(int64_t rows, int64_t p_width, int64_t q_width, int32_t experts,
+                                                               int32_t dtype) {
+    return check_group("expert product gradient", dtype, rows, p_width, q_width, experts) == CRESSO_OK ? 16 : 0;
+}
+
+extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int64_t depth,
+                                         const void* w, int64_t w_expert_stride, int64_t w_stride, int32_t turned, int32_t experts,
+                                         const int32_t* offsets, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "expert product";
+    const int32_t rc = check_group(what, dtype, rows, cols, depth, experts);
+    if (rc != CRESSO_OK) return rc;
+    if (rows == 0 || cols == 0) return CRESSO_OK;
+    if (!out || !offsets || (depth > 0 && (!x || (experts > 0 && !w)))) return fail(CRESSO_E_INVALID, "%s: null argument", what);
+    if (!row_stride_ok(x, rows, depth, x_stride)) return fail(CRESSO_E_INVALID, "%s: row stride %lld of x below the depth", what, (long long)x_stride);
+    const int64_t w_rows = turned ? depth : cols, w_cols = turned ? cols : depth;
+    if (w_rows > 1 && w_stride < w_cols)
+        return fail(CRESSO_E_INVALID, "%s: row stride %lld of a weight of %lld columns", what, (long long)w_stride, (long long)w_cols);
+    if (w_expert_stride < 0) return fail(CRESSO_E_INVALID, "%s: negative stride between experts", what);
+    if (!workspace || workspace_bytes < cresso_expert_product_workspace_bytes(rows, cols, depth, experts, dtype) || ((uintptr_t)workspace & 15))
+        return fail(CRESSO_E_INVALID, "%s: workspace of %zu bytes at %p, %zu at a multiple of 16 needed", what, workspace_bytes, workspace,
+                    cresso_expert_product_workspace_bytes(rows, cols, depth, experts, dtype));
+    GroupArgs a{};
+    a.a = x;
+    a.b = w;
+    a.out = out;
+    a.offsets = offsets;
+    a.rows = rows;
+    a.n = cols;
+    a.k = depth;
+    a.a_stride = x_stride;
+    a.b_stride = w_stride;
+    a.b_expert = w_expert_stride;
+    a.experts = experts;
+    const int tile = rows >= 64 * (int64_t)std::max(experts, 1) ? 128 : 64;
+    with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, false, turned != 0, tile, (hipStream_t)stream); });
+    return launched(what);
+}
+
+extern "C" int32_t cresso_expert_product_weight(const void* p, int64_t p_stride, int64_t p_width, const void* q, int64_t q_stride,
+                                                int64_t q_width, int32_t dtype, int64_t rows, int32_t experts, const int32_t* offsets,
+                                                void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* what = "expert product gradient";
+    const int32_t rc = check_group(what, dtype, rows, p_width, q_width, experts);
+    if (rc != CRESSO_OK) return rc;
+    if (experts == 0 || p_width == 0 || q_width == 0) return CRESSO_OK;
+    if (!out || !offsets || (rows > 0 && (!p || !q))) return fail(CRESSO_E_INVALID, "%s: null argument", what);
+    if (!row_stride_ok(p, rows, p_width, p_stride) || !row_stride_ok(q, rows, q_width, q_stride))
+        return fail(CRESSO_E_INVALID, "%s: row strides %lld and %lld below the widths", what, (long long)p_stride, (long long)q_stride);
+    if (!workspace || workspace_bytes < cresso_expert_product_weight_workspace_bytes(rows, p_width, q_width, experts, dtype) ||
+        ((uintptr_t)workspace & 15))
+        return fail(CRESSO_E_INVALID, "%s: workspace of %zu bytes at %p, %zu at a multiple of 16 needed", what, workspace_bytes, workspace,
+                    cresso_expert_product_weight_workspace_bytes(rows, p_width, q_width, experts, dtype));
+    GroupArgs a{};
+    a.a = p;
+    a.b = q;
+    a.out = out;
+    a.offsets = offsets;
+    a.rows = rows;
+    a.m = p_width;
+    a.n = q_width;
+    a.a_stride = p_stride;
+    a.b_stride = q_stride;
+    a.experts = experts;
+    const int tile = p_width > 64 && q_width > 64 ? 128 : 64;
+    with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, true, true, tile, (hipStream_t)stream); });
+    return launched(what);
+}

@@ -1,0 +1,384 @@
+// Products of rows with the matrix of the expert that they belong to.
+//
+//   product         out[i][c] = sum over d of x[i][d] * w[e(i)][c][d]        (or w[e(i)][d][c])
+//   weight gradient out[e][a][b] = sum over expert e's rows i of p[i][a] * q[i][b]
+//
+// Both are out(m, n) = sum over k of A(m, k) * B(n, k) in tiles; an operand is
+// held along k (its rows are m or n, their elements k) or across it (its rows
+// are k, their elements m or n):
+//   product          A = x along k, B = w along k or, for the gradient of x and for a weight that is held the
+//                    other way round, across k;  one expert's rows are cut into tiles of m
+//   weight gradient  A = p, B = q, both across k, which are one expert's rows
+//
+// A stage of a tile is 128 bytes of k: 64 numbers of 16 bits or 32 of fp32.
+// The matrix instructions take 16 x 16 x 32 of 16 bits, or 16 x 16 x 4 of fp32
+// four times; a lane's operand is always 16 bytes of k, and which k the four
+// quarters of a wave take is the same for both operands, so the order of k
+// within a stage is free.  Operands across k are read from LDS transposed.
+#pragma once
+
+#include "row_ops.hpp"
+
+namespace cresso {
+
+struct GroupArgs {
+    const void *a, *b;
+    void* out;
+    const int32_t* offsets;
+    int64_t rows;                          // of all experts
+    int64_t m, n, k;                       // product: n columns, k depth; weight gradient: m and n
+    int64_t a_stride, b_stride, b_expert;  // elements
+    int32_t experts;
+    uint32_t tiles_m, tiles_n;             // product: tiles_m is the most there can be
+    uint32_t tiles;                        // workgroups of tiles; those behind them fill rows without an expert
+};
+
+constexpr int kFillBlocks = 64;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct Group {
+    static constexpr int E = 16 / (int)sizeof(T);    // elements of a piece
+    static constexpr int KS = 128 / (int)sizeof(T);  // k of a stage
+};
+
+// ---------------------------------------------------------------------------
+// LDS.  Pieces of 16 bytes change places by their row's number, so that the
+// lanes that read in one cycle find theirs in different banks: 16 lanes at 16
+// bytes (0-3, 12-15, 20-23, 24-27 and likewise on), 32 at 8, 64 at 4.
+// ---------------------------------------------------------------------------
+// Along k, rows of 8 pieces: A's fragment has rows l16 of its 16.
+__device__ __forceinline__ int turn_a(int row) { return ((row >> 1) & 7) ^ (row & 4); }
+// B's fragment i has rows 4 FN (l16 / 4) + 4 i + l16 % 4, so that a lane ends with 4 FN consecutive columns.
+template <int FN> __device__ __forceinline__ int turn_b(int row) {
+    const int c = row / (4 * FN);
+    return ((row >> 1) & 1) | (c & 1) << 1 | ((c ^ (c >> 1)) & 1) << 2;
+}
+// Across k, rows of TILE elements: the blocks of 16 elements change places.
+template <typename T, int TILE> __device__ __forceinline__ int turn_across(int k) {
+    if constexpr (sizeof(T) == 4) return TILE >= 64 ? (k >> 3) & 3 : (k >> 3) & 1;
+    else if constexpr (TILE >= 128) return (k & 3) | ((k >> 4) & 1) << 2;
+    else if constexpr (TILE == 64) return ((k >> 1) & 1) | ((k >> 4) & 1) << 1;
+    else return (k >> 4) & 1;
+}
+
+// A tile's operand on its way from memory, through registers, to LDS.  It has
+// `size` rows along k, or `size` elements a row across it; what is beyond
+// those, and beyond k, is 0.
+template <typename T, bool ACROSS, int TILE, int NT, int FN /* 0: A */> struct Operand {
+    static constexpr int E = Group<T>::E, KS = Group<T>::KS, P = TILE * 8 / NT;
+    static_assert(P * NT == TILE * 8, "tile");
+    const T* base;
+    int64_t stride, size, depth;
+    u32x4 held[P];
+
+    // Row (or k) and piece that lie at a place of the tile's stage.
+    static __device__ __forceinline__ void at_place(int place, int& row, int& piece) {
+        if constexpr (ACROSS) {
+            constexpr int per = TILE / E, block = 16 / E;   // pieces of a row, of a block
+            row = place / per;
+            const int pos = place % per;
+            piece = ((pos / block) ^ turn_across<T, TILE>(row)) * block + pos % block;
+        } else {
+            row = place >> 3;
+            if constexpr (FN > 0) piece = (place & 7) ^ turn_b<FN>(row);
+            else piece = (place & 7) ^ turn_a(row);
+        }
+    }
+    __device__ __forceinline__ void load(int64_t k0) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            int row, piece;
+            at_place((int)threadIdx.x + i * NT, row, piece);
+            held[i] = u32x4{0, 0, 0, 0};
+            if constexpr (ACROSS) {
+                if (k0 + row < depth) held[i] = load_unit(base + (k0 + row) * stride, piece, size);
+            } else {
+                if (row < size) held[i] = load_unit(base + row * stride, k0 / E + piece, depth);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t* lds) const {
+#pragma unroll
+        for (int i = 0; i < P; ++i) *(u32x4*)(lds + ((int)threadIdx.x + i * NT) * 16) = held[i];
+    }
+};
+
+// Fragments of a wave: 16 m (or n) from `first` on, for step s (0 or 1) of a stage.
+template <typename T, bool ACROSS, int TILE, int FN /* 0: A */> struct Fragments {
+    int at[2];   // along: the byte of fragment 0 for each step; across: of the lane's row, and its turn
+    __device__ __forceinline__ void begin(int first) {
+        const int lane = threadIdx.x & (kWave - 1), l16 = lane & 15, quad = lane >> 4;
+        if constexpr (ACROSS) {
+            const int k = sizeof(T) == 2 ? quad * 16 + (l16 >> 2) : quad * 8;
+            at[0] = k * (TILE * (int)sizeof(T)) + (sizeof(T) == 2 ? (l16 & 3) * 8 : l16 * 4);
+            at[1] = turn_across<T, TILE>(k) ^ (first / 16);
+        } else {
+            const int row = first + (FN > 0 ? (l16 >> 2) * (4 * FN) + (l16 & 3) : l16);
+            const int turn = FN > 0 ? turn_b<(FN > 0 ? FN : 1)>(row) : turn_a(row);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) at[s] = row * 128 + ((quad * 2 + s) ^ turn) * 16;
+        }
+    }
+    __device__ __forceinline__ u32x4 read(const uint8_t* lds, int s, int i) const {
+        if constexpr (!ACROSS) {
+            return *(const u32x4*)(lds + at[s] + i * (FN > 0 ? 4 * 128 : 16 * 128));
+        } else {
+            constexpr int R = TILE * (int)sizeof(T);   // bytes of a row
+            const uint8_t* from = lds + at[0] + ((at[1] ^ i) * (16 * (int)sizeof(T)));
+            if constexpr (sizeof(T) == 2) {
+                // 16 lanes give four rows of 16 numbers and get a column of four each
+                typedef __attribute__((address_space(3))) i16x4* Lds;
+                const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + s * 8 * R));
+                const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(from + (s * 8 + 4) * R));
+                const u32x2 l = __builtin_bit_cast(u32x2, lo), h = __builtin_bit_cast(u32x2, hi);
+                return u32x4{l[0], l[1], h[0], h[1]};
+            } else {
+                u32x4 r;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) r[j] = *(const uint32_t*)(from + (s * 4 + j) * R);
+                return r;
+            }
+        }
+    }
+};
+
+template <typename T> __device__ __forceinline__ f32x4 group_mfma(u32x4 a, u32x4 b, f32x4 c);
+template <> __device__ __forceinline__ f32x4 group_mfma<__hip_bfloat16>(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 group_mfma<__half>(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 group_mfma<float>(u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t x = a[j], y = b[j];
+        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y), c, 0, 0, 0);
+    }
+    return c;
+}
+
+// ---------------------------------------------------------------------------
+// the tiles of ragged groups
+// ---------------------------------------------------------------------------
+// Rows [first, end) of expert e.  Offsets that point outside the rows, or fall, are held within them.
+__device__ __forceinline__ void group_rows(const GroupArgs& a, int e, int64_t& first, int64_t& end) {
+    first = min(max((int64_t)a.offsets[e], (int64_t)0), a.rows);
+    end = min(max((int64_t)a.offsets[e + 1], first), a.rows);
+}
+struct GroupTile {
+    int expert;
+    int64_t first, rows;   // the tile's rows among all
+};
+// Tiles of m rows there are, over all experts.  By each wave.
+__device__ __forceinline__ uint32_t group_tiles(const GroupArgs& a, int tile) {
+    const int lane = threadIdx.x & (kWave - 1);
+    uint32_t n = 0;
+    for (int e = lane; e < a.experts; e += kWave) {
+        int64_t first, end;
+        group_rows(a, e, first, end);
+        n += (uint32_t)((end - first + tile - 1) / tile);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) n += __shfl_xor(n, d, kWave);
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)n);
+}
+// Tile t of m, of those.  By each wave.
+__device__ __forceinline__ GroupTile group_tile(const GroupArgs& a, int tile, uint32_t t) {
+    const int lane = threadIdx.x & (kWave - 1);
+    uint32_t before = 0;
+    GroupTile g{0, 0, 0};
+    for (int e0 = 0; e0 < a.experts; e0 += kWave) {
+        int64_t first = 0, end = 0;
+        if (e0 + lane < a.experts) group_rows(a, e0 + lane, first, end);
+        const uint32_t n = (uint32_t)((end - first + tile - 1) / tile);
+        uint32_t upto = n;
+#pragma unroll
+        for (int d = 1; d < kWave; d <<= 1) {
+            const uint32_t o = __shfl_up(upto, d, kWave);
+            if (lane >= d) upto += o;
+        }
+        const uint64_t past = __ballot(before + upto > t);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const uint32_t ahead = before + (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), l);
+            const int64_t f = __builtin_amdgcn_readlane((int)first, l), z = __builtin_amdgcn_readlane((int)end, l);   // below 2^31
+            g.expert = e0 + l;
+            g.first = f + (int64_t)(t - ahead) * tile;
+            g.rows = min((int64_t)tile, z - g.first);
+            return g;
+        }
+        before += (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1);
+    }
+    return g;
+}
+
+// Tile of a workgroup among `high` x `wide`; false: there is none.  Workgroups
+// go to the 8 XCDs in turn; each XCD takes a run of tiles, in columns of 8
+// tiles of m, so that the tiles that run together on one XCD share rows of both
+// operands in its L2.
+__device__ __forceinline__ bool group_place(uint32_t high, uint32_t wide, uint32_t& tm, uint32_t& tn) {
+    const uint32_t total = high * wide, per = total / 8, rest = total % 8;
+    const uint32_t xcd = blockIdx.x % 8, i = blockIdx.x / 8;
+    if (i >= per + (xcd < rest ? 1u : 0u)) return false;
+    const uint32_t t = xcd * per + min(xcd, rest) + i;
+    const uint32_t group = 8 * wide, g = t / group, in = t - g * group;
+    const uint32_t height = min(8u, high - g * 8);
+    tm = g * 8 + in % height;
+    tn = in / height;
+    return true;
+}
+
+// Zeros into the rows that are no expert's.
+template <typename T> __device__ __forceinline__ void group_fill(const GroupArgs& a, int64_t part, int64_t parts) {
+    const int64_t begin = min(max((int64_t)a.offsets[0], (int64_t)0), a.rows);
+    const int64_t end = min(max((int64_t)a.offsets[a.experts], begin), a.rows);
+    const int64_t units = (a.n + Group<T>::E - 1) / Group<T>::E;
+    for (int64_t r = part; r < begin + a.rows - end; r += parts) {
+        const int64_t row = r < begin ? r : r - begin + end;
+        for (int64_t u = threadIdx.x; u < units; u += blockDim.x) store_unit((T*)a.out + row * a.n, u, a.n, u32x4{0, 0, 0, 0});
+    }
+}
+
+// WM x WN waves of FM x FN fragments of 16 x 16 each.
+template <typename T, bool WEIGHT, bool B_ACROSS, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
+    constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16;
+    constexpr int KS = Group<T>::KS, E = Group<T>::E, STAGE = (TM + TN) * 128;
+    constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
+    __shared__ __align__(16) uint8_t lds[2 * STAGE];
+    if (blockIdx.x >= a.tiles) {
+        group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
+        return;
+    }
+    Operand<T, WEIGHT, TM, NT, 0> oa;
+    Operand<T, ACROSS, TN, NT, FN> ob;
+    uint32_t tm, tn;
+    T* out;
+    int64_t rows, m0;   // rows of the result from `out` on, the tile's first
+    if constexpr (WEIGHT) {
+        const uint32_t per = a.tiles_m * a.tiles_n;
+        if (!group_place(per * a.experts / a.tiles_n, a.tiles_n, tm, tn)) return;
+        const int e = (int)(tm / a.tiles_m);
+        m0 = (int64_t)(tm % a.tiles_m) * TM;
+        const int64_t n0 = (int64_t)tn * TN;
+        int64_t first, end;
+        group_rows(a, e, first, end);
+        oa.base = (const T*)a.a + first * a.a_stride + m0;
+        ob.base = (const T*)a.b + first * a.b_stride + n0;
+        oa.size = a.m - m0;
+        ob.size = a.n - n0;
+        oa.depth = ob.depth = end - first;
+        out = (T*)a.out + (int64_t)e * a.m * a.n;
+        rows = a.m;
+    } else {
+        if (!group_place(group_tiles(a, TM), a.tiles_n, tm, tn)) return;
+        const GroupTile g = group_tile(a, TM, tm);
+        const int64_t n0 = (int64_t)tn * TN;
+        oa.base = (const T*)a.a + g.first * a.a_stride;
+        ob.base = (const T*)a.b + g.expert * a.b_expert + (ACROSS ? n0 : n0 * a.b_stride);
+        oa.size = g.rows;
+        ob.size = a.n - n0;
+        oa.depth = ob.depth = a.k;
+        out = (T*)a.out + g.first * a.n;
+        rows = g.rows;
+        m0 = 0;
+    }
+    oa.stride = a.a_stride;
+    ob.stride = a.b_stride;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int wm = (wave % WM) * (FM * 16), wn = (wave / WM) * (FN * 16), l16 = lane & 15, quad = lane >> 4;
+    Fragments<T, WEIGHT, TM, 0> fa;
+    Fragments<T, ACROSS, TN, FN> fb;
+    fa.begin(wm);
+    fb.begin(wn);
+    f32x4 acc[FN][FM] = {};
+    const int64_t stages = (oa.depth + KS - 1) / KS;
+    if (stages) {
+        oa.load(0);
+        ob.load(0);
+        oa.store(lds);
+        ob.store(lds + TM * 128);
+    }
+    for (int64_t s = 0; s < stages; ++s) {
+        uint8_t* const now = lds + (s & 1) * STAGE;
+        uint8_t* const next = lds + (~s & 1) * STAGE;
+        __syncthreads();   // this stage is there, and the one before it has been read
+        if (s + 1 < stages) {
+            oa.load((s + 1) * KS);
+            ob.load((s + 1) * KS);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 b[FN];
+#pragma unroll
+            for (int i = 0; i < FN; ++i) b[i] = fb.read(now + TM * 128, h, i);
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+                const u32x4 v = fa.read(now, h, j);
+#pragma unroll
+                for (int i = 0; i < FN; ++i) acc[i][j] = group_mfma<T>(b[i], v, acc[i][j]);
+            }
+        }
+        if (s + 1 < stages) {
+            oa.store(next);
+            ob.store(next + TM * 128);
+        }
+    }
+    // a lane holds columns 4 quad to 4 quad + 3 of each fragment's 16, or with B along k 4 FN columns in one piece
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int64_t m = m0 + wm + j * 16 + l16;
+        if (m >= rows) continue;
+        T* to = out + m * a.n;
+        const int64_t n0 = (int64_t)tn * TN + wn;
+        if constexpr (ACROSS || 4 * FN < E) {
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                const int64_t n = n0 + (ACROSS ? i * 16 + quad * 4 : quad * (4 * FN) + i * 4);
+                const f32x4 v = acc[i][j];
+                if constexpr (sizeof(T) == 4) {
+                    store_unit(to + n, 0, a.n - n, __builtin_bit_cast(u32x4, v));
+                } else {
+                    const uint32_t lo = narrow2<T>(v[0], v[1]), hi = narrow2<T>(v[2], v[3]);
+                    if (n + 4 <= a.n) store8(to + n, u32x2{lo, hi});
+                    else if (n < a.n) store_part(to + n, u32x4{lo, hi, 0, 0}, (int)(a.n - n));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4 * FN / E; ++u) {
+                float v[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = acc[(u * E + e) / 4][j][(u * E + e) % 4];
+                store_unit(to, (n0 + quad * (4 * FN)) / E + u, a.n, narrow<T>(v));
+            }
+        }
+    }
+}
+
+// One dtype's kernels, each in a source file of its own.
+template <typename T> void group_launch(GroupArgs a, bool weight, bool across, int tile, hipStream_t st);
+
+#define CRESSO_GROUP_LAUNCH(T)                                                                                          \
+    template <> void group_launch<T>(GroupArgs a, bool weight, bool across, int tile, hipStream_t st) {                 \
+        const auto run = [&](auto kernel, int tm, int tn, int threads) {                                                \
+            a.tiles_n = (uint32_t)((a.n + tn - 1) / tn);                                                                \
+            a.tiles_m = (uint32_t)(weight ? (a.m + tm - 1) / tm : a.rows / tm + a.experts);                             \
+            a.tiles = a.tiles_m * a.tiles_n * (weight ? (uint32_t)a.experts : 1u);                                      \
+            hipLaunchKernelGGL(kernel, dim3(a.tiles + (weight ? 0 : kFillBlocks)), dim3(threads), 0, st, a);            \
+        };                                                                                                              \
+        const auto size = [&](auto w, auto x) {                                                                         \
+            constexpr bool W = decltype(w)::value, X = decltype(x)::value;                                              \
+            if (tile == 128) run(group_kernel<T, W, X, 1, 4, 8, 2>, 128, 128, 256);                                     \
+            else run(group_kernel<T, W, X, 1, 4, 4, 1>, 64, 64, 256);                                                   \
+        };                                                                                                              \
+        if (weight) size(std::true_type{}, std::true_type{});                                                           \
+        else if (across) size(std::false_type{}, std::true_type{});                                                     \
+        else size(std::false_type{}, std::false_type{});                                                                \
+    }
+
+}  // namespace cresso

@@ -11,8 +11,10 @@
 // CRESSO_HIP_LIBRARY chooses it here as it does for ctypes.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -39,6 +41,18 @@ struct Api {
     decltype(&cresso_block_product_workspace_bytes) block_product_workspace_bytes;
     decltype(&cresso_block_product) block_product;
     decltype(&cresso_block_quantize) block_quantize;
+    decltype(&cresso_clip_workspace_bytes) clip_workspace_bytes;
+    decltype(&cresso_clip_gradients) clip_gradients;
+    decltype(&cresso_route_workspace_bytes) route_workspace_bytes;
+    decltype(&cresso_route_forward) route_forward;
+    decltype(&cresso_route_backward) route_backward;
+    decltype(&cresso_dispatch_rows) dispatch_rows;
+    decltype(&cresso_combine_rows) combine_rows;
+    decltype(&cresso_combine_backward) combine_backward;
+    decltype(&cresso_expert_product_workspace_bytes) expert_product_workspace_bytes;
+    decltype(&cresso_expert_product) expert_product;
+    decltype(&cresso_expert_product_weight_workspace_bytes) expert_product_weight_workspace_bytes;
+    decltype(&cresso_expert_product_weight) expert_product_weight;
 } g_api{};
 
 void bind(const std::unordered_map<std::string, uintptr_t>& at) {
@@ -60,6 +74,18 @@ void bind(const std::unordered_map<std::string, uintptr_t>& at) {
     take(a.block_product_workspace_bytes, "cresso_block_product_workspace_bytes");
     take(a.block_product, "cresso_block_product");
     take(a.block_quantize, "cresso_block_quantize");
+    take(a.clip_workspace_bytes, "cresso_clip_workspace_bytes");
+    take(a.clip_gradients, "cresso_clip_gradients");
+    take(a.route_workspace_bytes, "cresso_route_workspace_bytes");
+    take(a.route_forward, "cresso_route_forward");
+    take(a.route_backward, "cresso_route_backward");
+    take(a.dispatch_rows, "cresso_dispatch_rows");
+    take(a.combine_rows, "cresso_combine_rows");
+    take(a.combine_backward, "cresso_combine_backward");
+    take(a.expert_product_workspace_bytes, "cresso_expert_product_workspace_bytes");
+    take(a.expert_product, "cresso_expert_product");
+    take(a.expert_product_weight_workspace_bytes, "cresso_expert_product_weight_workspace_bytes");
+    take(a.expert_product_weight, "cresso_expert_product_weight");
     g_api = a;
 }
 
@@ -625,6 +651,419 @@ std::tuple<Tensor, Tensor> quantize_blocks(const Tensor& weight) {
     return {values, scales};
 }
 
+// ---------------------------------------------------------------------------
+// gradient norm and clipping
+// ---------------------------------------------------------------------------
+struct Written {
+    uintptr_t at, end;
+    bool out;
+};
+// Whether memory that is written belongs to anything else of the call.
+bool shares(std::vector<Written>& spans) {
+    const auto before = [](const Written& a, const Written& b) { return a.at < b.at; };
+    if (!std::is_sorted(spans.begin(), spans.end(), before)) std::sort(spans.begin(), spans.end(), before);
+    uintptr_t any = 0, out = 0;
+    for (const Written& s : spans) {
+        if (s.at < out || (s.out && s.at < any)) return true;
+        any = std::max(any, s.end);
+        if (s.out) out = std::max(out, s.end);
+    }
+    return false;
+}
+Tensor clip(const char* what, const std::vector<optional<Tensor>>& grads, double max_norm, int64_t kind, double grad_scale,
+            const std::vector<optional<Tensor>>* out, bool in_place) {
+    const at::NoGradGuard no_grad;
+    TORCH_CHECK_VALUE(max_norm >= 0.0, what, ": max_norm must not be negative");
+    TORCH_CHECK_VALUE(std::isfinite(grad_scale), what, ": grad_scale must be finite");
+    if (out) TORCH_CHECK_VALUE(out->size() == grads.size(), what, ": ", out->size(), " outputs for ", grads.size(), " gradients");
+    OneGpu gpu{what};
+    std::vector<cresso_grad_desc> descs;
+    std::vector<Written> spans;
+    std::vector<Tensor> keep;                             // copies
+    std::vector<std::pair<Tensor, Tensor>> back;          // written in a copy: where it goes
+    descs.reserve(grads.size());
+    spans.reserve(out ? 2 * grads.size() : grads.size());
+    const Tensor* first = nullptr;
+    const auto span = [&](const Tensor& t, bool written) {
+        const uintptr_t at = (uintptr_t)t.const_data_ptr();
+        int64_t reach = 1;   // elements from the first to the last
+        for (int64_t d = 0; d < t.dim(); ++d) reach += (t.size(d) - 1) * t.stride(d);
+        spans.push_back({at, at + (uintptr_t)(reach * (int64_t)t.element_size()), written});
+    };
+    for (size_t i = 0; i < grads.size(); ++i) {
+        if (!grads[i].has_value()) continue;
+        const Tensor& g = *grads[i];
+        TORCH_CHECK_VALUE(g.layout() == at::kStrided, what, ": gradient ", i, " is sparse");
+        gpu.add("a gradient", g);
+        const int32_t code = code_of(g.scalar_type());
+        TORCH_CHECK_VALUE(code >= 0, what, ": gradient ", i, " must be fp32, fp64, bf16 or fp16, not ", name_of(g.scalar_type()));
+        if (!first) first = &g;
+        Tensor to;
+        if (out) {
+            TORCH_CHECK_VALUE((*out)[i].has_value(), what, ": no output for gradient ", i);
+            to = *(*out)[i];
+            gpu.add("an output", to);
+            TORCH_CHECK_VALUE(to.layout() == at::kStrided && to.sizes() == g.sizes() &&
+                                  (to.scalar_type() == g.scalar_type() || (to.scalar_type() == at::kFloat && g.element_size() == 2)),
+                              what, ": output ", i, " is ", name_of(to.scalar_type()), " ", to.sizes(), " for a gradient of ",
+                              name_of(g.scalar_type()), " ", g.sizes(), " (its own type or, of 16 bits, fp32)");
+        } else if (in_place) {
+            to = g;
+        }
+        if (!g.numel()) continue;
+        cresso_grad_desc d{};
+        d.numel = g.numel();
+        d.dtype = code;
+        const bool same = to.defined() && to.const_data_ptr() == g.const_data_ptr() && to.scalar_type() == g.scalar_type() &&
+                          to.strides() == g.strides();
+        if (to.defined()) {
+            TORCH_CHECK_VALUE(to.is_non_overlapping_and_dense() || at::has_internal_overlap(to) != at::MemOverlap::Yes, what,
+                              ": output ", i, " holds several elements in one place");
+            span(to, true);
+        }
+        if (!same) span(g, false);
+        Tensor from = g;
+        if (!g.is_non_overlapping_and_dense()) {   // any order of the elements serves a norm, gaps do not
+            from = g.contiguous();
+            keep.push_back(from);
+        }
+        d.grad = from.const_data_ptr();
+        if (to.defined()) {
+            d.out_dtype = code_of(to.scalar_type());
+            if (same) {
+                d.out = const_cast<void*>(d.grad);
+                if (!from.is_same(g)) back.emplace_back(to, from);
+            } else if (to.is_non_overlapping_and_dense() && to.strides() == from.strides()) {
+                d.out = to.mutable_data_ptr();
+            } else {
+                const Tensor t = at::empty_strided(from.sizes(), from.strides(), to.options());
+                d.out = t.mutable_data_ptr();
+                back.emplace_back(to, t);
+            }
+        }
+        descs.push_back(d);
+    }
+    TORCH_CHECK_VALUE(!(out || in_place) || !shares(spans), what,
+                      ": memory that is written belongs to two gradients (a parameter that is given twice?), or to an input and another's output");
+    if (!first) return at::zeros({}, at::device(at::kCUDA).dtype(at::kFloat));
+    const c10::DeviceGuard guard(first->device());
+    Tensor norm = at::empty({}, first->options().dtype(at::kFloat).requires_grad(false));
+    const size_t bytes = g_api.clip_workspace_bytes(descs.data(), (int32_t)descs.size());
+    const Tensor ws = workspace(bytes, norm);
+    done(g_api.clip_gradients(descs.data(), (int32_t)descs.size(), (int32_t)kind, max_norm, grad_scale, (float*)norm.mutable_data_ptr(),
+                              ws.mutable_data_ptr(), bytes, stream_of(*first)),
+         what);
+    for (auto& [to, from] : back) to.copy_(from);
+    // written behind torch's back: what has saved them for its own gradient has to notice
+    const std::vector<optional<Tensor>>* written = out ? out : in_place ? &grads : nullptr;
+    if (written)
+        for (const auto& t : *written)
+            if (t.has_value() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    return norm;
+}
+Tensor gradient_norm(const std::vector<optional<Tensor>>& grads, int64_t kind) {
+    return clip("gradient_norm", grads, INFINITY, kind, 1.0, nullptr, false);
+}
+Tensor clip_gradients(const std::vector<optional<Tensor>>& grads, double max_norm, int64_t kind, double grad_scale,
+                      const optional<std::vector<optional<Tensor>>>& out) {
+    return clip("clip_gradients", grads, max_norm, kind, grad_scale, out.has_value() ? &*out : nullptr, !out.has_value());
+}
+
+// ---------------------------------------------------------------------------
+// layers of experts
+// ---------------------------------------------------------------------------
+constexpr int64_t kMaxExperts = 1024, kMaxExpertsOfToken = 32;
+
+struct Route {
+    Tensor logits, bias;
+    int64_t top, score;
+    bool normalize;
+    double scale;
+};
+cresso_route_desc route_desc(const Route& r, std::vector<Tensor>& keep) {
+    cresso_route_desc d{};
+    keep.push_back(rows_of(r.logits, d.logits_stride));
+    d.logits = keep.back().const_data_ptr();
+    if (r.bias.defined()) {
+        keep.push_back(r.bias.contiguous());
+        d.bias = (const float*)keep.back().const_data_ptr();
+    }
+    d.tokens = r.logits.size(0);
+    d.num_experts = (int32_t)r.logits.size(1);
+    d.top = (int32_t)r.top;
+    d.dtype = code_of(r.logits.scalar_type());
+    d.score = (int32_t)r.score;
+    d.normalize = r.normalize;
+    d.scale = (float)r.scale;
+    return d;
+}
+// -> weights, experts, order, places, offsets
+variable_list route_forward(const Route& r) {
+    const int64_t tokens = r.logits.size(0);
+    const auto f32 = r.logits.options().dtype(at::kFloat).requires_grad(false), i32 = f32.dtype(at::kInt);
+    Tensor weights = at::empty({tokens, r.top}, f32), experts = at::empty({tokens, r.top}, i32);
+    Tensor order = at::empty({tokens * r.top}, i32), places = at::empty({tokens, r.top}, i32), offsets = at::empty({r.logits.size(1) + 1}, i32);
+    std::vector<Tensor> keep;
+    keep.reserve(2);
+    cresso_route_desc d = route_desc(r, keep);
+    d.weights = (float*)weights.mutable_data_ptr();
+    d.experts = (int32_t*)experts.mutable_data_ptr();
+    d.order = (int32_t*)order.mutable_data_ptr();
+    d.places = (int32_t*)places.mutable_data_ptr();
+    d.offsets = (int32_t*)offsets.mutable_data_ptr();
+    const c10::DeviceGuard guard(r.logits.device());
+    const size_t bytes = g_api.route_workspace_bytes(&d);
+    const Tensor ws = workspace(bytes, weights);
+    done(g_api.route_forward(&d, ws.mutable_data_ptr(), bytes, stream_of(r.logits)), "route_experts");
+    return {weights, experts, order, places, offsets};
+}
+struct RouteFunction : torch::autograd::Function<RouteFunction> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const optional<Tensor>& bias, int64_t top, int64_t score,
+                                 bool normalize, double scale) {
+        variable_list got = route_forward({logits, or_none(bias), top, score, normalize, scale});
+        ctx->save_for_backward({logits, got[0], got[1]});
+        ctx->saved_data["top"] = top;
+        ctx->saved_data["score"] = score;
+        ctx->saved_data["normalize"] = normalize;
+        ctx->saved_data["scale"] = scale;
+        ctx->mark_non_differentiable({got[1], got[2], got[3], got[4]});
+        ctx->set_materialize_grads(false);
+        return got;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list arrive) {
+        variable_list grads(6);
+        if (!arrive[0].defined()) return grads;
+        const variable_list v = ctx->get_saved_variables();
+        const Route r{v[0], Tensor(), ctx->saved_data["top"].toInt(), ctx->saved_data["score"].toInt(), ctx->saved_data["normalize"].toBool(),
+                      ctx->saved_data["scale"].toDouble()};
+        grads[0] = at::empty(r.logits.sizes(), r.logits.options().requires_grad(false));
+        if (grads[0].numel()) {
+            std::vector<Tensor> keep;
+            keep.reserve(2);
+            cresso_route_desc d = route_desc(r, keep);
+            d.weights = (float*)v[1].const_data_ptr();
+            d.experts = (int32_t*)v[2].const_data_ptr();
+            const Tensor by = arrive[0].detach().contiguous();
+            const c10::DeviceGuard guard(r.logits.device());
+            done(g_api.route_backward(&d, (const float*)by.const_data_ptr(), grads[0].mutable_data_ptr(), stream_of(r.logits)),
+                 "route_experts gradient");
+        }
+        return once(std::move(grads), {arrive[0], v[0]});
+    }
+};
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_experts(const Tensor& logits, int64_t top, int64_t score, bool normalize, double scale,
+                                                                 const optional<Tensor>& bias_) {
+    const char* what = "route_experts";
+    const Tensor bias = or_none(bias_);
+    OneGpu gpu{what};
+    gpu.add("logits", logits);
+    gpu.add("bias", bias);
+    TORCH_CHECK_VALUE(logits.dim() == 2, what, ": logits must be [tokens, experts], not ", logits.sizes());
+    check_row_type(what, "logits", logits);
+    const int64_t experts = logits.size(1);
+    TORCH_CHECK_VALUE(experts >= 1 && experts <= kMaxExperts, what, ": ", experts, " experts, 1 to ", kMaxExperts, " are taken");
+    TORCH_CHECK_VALUE(top >= 1 && top <= std::min(experts, kMaxExpertsOfToken), what, ": top ", top, " of ", experts, " experts, 1 to ",
+                      std::min(experts, kMaxExpertsOfToken), " are taken");
+    TORCH_CHECK_VALUE(logits.size(0) * top < (int64_t)1 << 31, what, ": ", logits.size(0), " tokens are more than one call takes");
+    TORCH_CHECK_VALUE(std::isfinite(scale), what, ": scale must be finite");
+    if (bias.defined())
+        TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == experts && bias.scalar_type() == at::kFloat, what, ": bias must be fp32 [",
+                          experts, "], not ", name_of(bias.scalar_type()), " ", bias.sizes());
+    const variable_list got = wants_grad({logits}) ? RouteFunction::apply(logits, or_null(bias), top, score, normalize, scale)
+                                                   : route_forward({logits, bias, top, score, normalize, scale});
+    return {got[0], got[1], got[2], got[3], got[4]};
+}
+
+// experts and places [tokens, top] of a routing
+void check_slots(const char* what, OneGpu& gpu, const Tensor& experts, const Tensor& places) {
+    gpu.add("experts", experts);
+    gpu.add("places", places);
+    TORCH_CHECK_VALUE(experts.scalar_type() == at::kInt && places.scalar_type() == at::kInt && experts.dim() == 2 &&
+                          places.sizes() == experts.sizes(),
+                      what, ": the routing's experts and places must be int32 [tokens, top], not ", name_of(experts.scalar_type()), " ",
+                      experts.sizes(), " and ", name_of(places.scalar_type()), " ", places.sizes());
+    TORCH_CHECK_VALUE(experts.size(1) >= 1 && experts.size(1) <= kMaxExpertsOfToken, what, ": ", experts.size(1), " experts a token, 1 to ",
+                      kMaxExpertsOfToken, " are taken");
+    TORCH_CHECK_VALUE(experts.numel() < (int64_t)1 << 31, what, ": more rows than one call takes");
+}
+const int32_t* ints(const Tensor& t) { return (const int32_t*)t.const_data_ptr(); }
+
+Tensor dispatch(const Tensor& x, const Tensor& experts_, const Tensor& places_) {
+    Tensor rows = at::empty({experts_.numel(), x.size(1)}, x.options().requires_grad(false));
+    if (rows.numel()) {
+        int64_t stride;
+        const Tensor from = rows_of(x, stride), experts = experts_.contiguous(), places = places_.contiguous();
+        const c10::DeviceGuard guard(x.device());
+        done(g_api.dispatch_rows(from.const_data_ptr(), stride, code_of(x.scalar_type()), x.size(0), (int32_t)experts.size(1), x.size(1),
+                                 ints(experts), ints(places), rows.mutable_data_ptr(), stream_of(x)),
+             "dispatch_rows");
+    }
+    return rows;
+}
+Tensor combine(const char* what, const Tensor& rows, const Tensor& experts_, const Tensor& places_, const Tensor& weights_) {
+    Tensor out = at::empty({experts_.size(0), rows.size(1)}, rows.options().requires_grad(false));
+    if (out.numel()) {
+        int64_t stride;
+        const Tensor from = rows_of(rows, stride), experts = experts_.contiguous(), places = places_.contiguous();
+        const Tensor weights = weights_.defined() ? weights_.contiguous() : Tensor();
+        const c10::DeviceGuard guard(rows.device());
+        done(g_api.combine_rows(from.const_data_ptr(), stride, code_of(rows.scalar_type()), out.size(0), (int32_t)experts.size(1), rows.size(1),
+                                ints(experts), ints(places), weights.defined() ? (const float*)weights.const_data_ptr() : nullptr,
+                                out.mutable_data_ptr(), stream_of(rows)),
+             what);
+    }
+    return out;
+}
+struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& experts, const Tensor& places) {
+        ctx->save_for_backward({experts, places});
+        return dispatch(x, experts, places);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list arrive) {
+        const variable_list v = ctx->get_saved_variables();
+        return once({combine("dispatch_rows gradient", arrive[0].detach(), v[0], v[1], Tensor()), Tensor(), Tensor()}, arrive);
+    }
+};
+struct CombineFunction : torch::autograd::Function<CombineFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& experts, const Tensor& places, const optional<Tensor>& weights) {
+        ctx->save_for_backward({rows, experts, places, or_none(weights)});
+        return combine("combine_rows", rows, experts, places, or_none(weights));
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list arrive) {
+        const variable_list v = ctx->get_saved_variables();
+        const Tensor& rows = v[0];
+        const bool to_rows = ctx->needs_input_grad(0), to_weights = v[3].defined() && ctx->needs_input_grad(3);
+        variable_list grads(4);
+        // places that are none of the rows' are not written
+        if (to_rows) grads[0] = at::empty(rows.sizes(), rows.options().requires_grad(false));
+        if (to_weights) grads[3] = at::empty(v[3].sizes(), v[3].options().requires_grad(false));
+        if (v[1].numel() && (to_rows || to_weights)) {
+            int64_t stride, by_stride;
+            const Tensor from = rows_of(rows, stride), by = rows_of(arrive[0].detach(), by_stride);
+            const Tensor experts = v[1].contiguous(), places = v[2].contiguous(), weights = v[3].defined() ? v[3].contiguous() : Tensor();
+            const c10::DeviceGuard guard(rows.device());
+            done(g_api.combine_backward(from.const_data_ptr(), stride, by.const_data_ptr(), by_stride, code_of(rows.scalar_type()), by.size(0),
+                                        (int32_t)experts.size(1), rows.size(1), ints(experts), ints(places),
+                                        weights.defined() ? (const float*)weights.const_data_ptr() : nullptr,
+                                        to_rows ? grads[0].mutable_data_ptr() : nullptr, to_weights ? (float*)grads[3].mutable_data_ptr() : nullptr,
+                                        stream_of(rows)),
+                 "combine_rows gradient");
+        }
+        return once(std::move(grads), {arrive[0], rows, v[3]});
+    }
+};
+Tensor dispatch_rows(const Tensor& x, const Tensor& experts, const Tensor& places) {
+    const char* what = "dispatch_rows";
+    OneGpu gpu{what};
+    gpu.add("x", x);
+    check_slots(what, gpu, experts, places);
+    check_row_type(what, "x", x);
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == experts.size(0), what, ": x must be [", experts.size(0), ", width], not ", x.sizes());
+    if (wants_grad({x})) return DispatchFunction::apply(x, experts, places);
+    return dispatch(x, experts, places);
+}
+Tensor combine_rows(const Tensor& rows, const Tensor& experts, const Tensor& places, const optional<Tensor>& weights_) {
+    const char* what = "combine_rows";
+    const Tensor weights = or_none(weights_);
+    OneGpu gpu{what};
+    gpu.add("rows", rows);
+    check_slots(what, gpu, experts, places);
+    gpu.add("weights", weights);
+    check_row_type(what, "rows", rows);
+    TORCH_CHECK_VALUE(rows.dim() == 2 && rows.size(0) == experts.numel(), what, ": rows must be [", experts.numel(), ", width], not ", rows.sizes());
+    if (weights.defined())
+        TORCH_CHECK_VALUE(weights.scalar_type() == at::kFloat && weights.sizes() == experts.sizes(), what, ": weights must be fp32 ",
+                          experts.sizes(), ", not ", name_of(weights.scalar_type()), " ", weights.sizes());
+    if (wants_grad({rows, weights})) return CombineFunction::apply(rows, experts, places, or_null(weights));
+    return combine(what, rows, experts, places, weights);
+}
+
+// A stacked weight [experts, outputs, inputs] where it lies: rows along the
+// inputs, or (turned) along the outputs, as a transposed view has them; any
+// other layout is copied.
+struct Stacked {
+    Tensor t;
+    int64_t expert, stride;
+    bool turned;
+};
+Stacked stacked_of(const Tensor& w) {
+    const int64_t n = w.size(1), k = w.size(2);
+    if ((k < 2 || w.stride(2) == 1) && (n < 2 || w.stride(1) >= k) && (w.size(0) < 2 || w.stride(0) >= 0))
+        return {w, w.size(0) < 2 ? 0 : w.stride(0), n < 2 ? k : w.stride(1), false};
+    if ((n < 2 || w.stride(1) == 1) && (k < 2 || w.stride(2) >= n) && (w.size(0) < 2 || w.stride(0) >= 0))
+        return {w, w.size(0) < 2 ? 0 : w.stride(0), k < 2 ? n : w.stride(2), true};
+    return {w.contiguous(), n * k, k, false};
+}
+// x times the transposes of the matrices (forward), or times the matrices (the gradient of x)
+Tensor group_product(const char* what, const Tensor& x, const Tensor& weight, const Tensor& offsets_, bool back) {
+    const int64_t rows = x.size(0), cols = weight.size(back ? 2 : 1), depth = weight.size(back ? 1 : 2);
+    const int32_t experts = (int32_t)weight.size(0), code = code_of(x.scalar_type());
+    Tensor out = at::empty({rows, cols}, x.options().requires_grad(false));
+    if (out.numel()) {
+        int64_t stride;
+        const Tensor from = rows_of(x, stride), offsets = offsets_.contiguous();
+        const Stacked w = stacked_of(weight);
+        const c10::DeviceGuard guard(x.device());
+        const size_t bytes = g_api.expert_product_workspace_bytes(rows, cols, depth, experts, code);
+        const Tensor ws = workspace(bytes, x);
+        done(g_api.expert_product(from.const_data_ptr(), stride, code, rows, cols, depth, w.t.const_data_ptr(), w.expert, w.stride,
+                                  w.turned != back, experts, ints(offsets), out.mutable_data_ptr(), ws.mutable_data_ptr(), bytes,
+                                  stream_of(x)),
+             what);
+    }
+    return out;
+}
+// [experts, outputs, inputs], held as the weight is
+Tensor group_weight(const Tensor& x_, const Tensor& by_, const Tensor& weight, const Tensor& offsets_) {
+    const bool turned = stacked_of(weight).turned;
+    const Tensor &p_ = turned ? x_ : by_, &q_ = turned ? by_ : x_;
+    const int64_t experts = weight.size(0), pw = p_.size(1), qw = q_.size(1);
+    Tensor out = at::empty({experts, pw, qw}, weight.options().requires_grad(false));
+    if (out.numel()) {
+        int64_t ps, qs;
+        const Tensor p = rows_of(p_, ps), q = rows_of(q_, qs), offsets = offsets_.contiguous();
+        const int32_t code = code_of(weight.scalar_type());
+        const c10::DeviceGuard guard(weight.device());
+        const size_t bytes = g_api.expert_product_weight_workspace_bytes(p.size(0), pw, qw, (int32_t)experts, code);
+        const Tensor ws = workspace(bytes, weight);
+        done(g_api.expert_product_weight(p.const_data_ptr(), ps, pw, q.const_data_ptr(), qs, qw, code, p.size(0), (int32_t)experts,
+                                         ints(offsets), out.mutable_data_ptr(), ws.mutable_data_ptr(), bytes, stream_of(weight)),
+             "expert_product gradient of the weight");
+    }
+    return turned ? out.transpose(1, 2) : out;
+}
+struct ExpertFunction : torch::autograd::Function<ExpertFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& offsets) {
+        ctx->save_for_backward({x, weight, offsets});
+        return group_product("expert_product", x, weight, offsets, false);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list arrive) {
+        const variable_list v = ctx->get_saved_variables();
+        const Tensor by = arrive[0].detach();
+        variable_list grads(3);
+        if (ctx->needs_input_grad(0)) grads[0] = group_product("expert_product gradient", by, v[1], v[2], true);
+        if (ctx->needs_input_grad(1)) grads[1] = group_weight(v[0], by, v[1], v[2]);
+        return once(std::move(grads), {arrive[0], v[0], v[1]});
+    }
+};
+Tensor expert_product(const Tensor& x, const Tensor& weight, const Tensor& offsets) {
+    const char* what = "expert_product";
+    OneGpu gpu{what};
+    gpu.add("x", x);
+    gpu.add("weight", weight);
+    gpu.add("offsets", offsets);
+    TORCH_CHECK_VALUE(weight.dim() == 3, what, ": weight must be [experts, outputs, inputs], not ", weight.sizes());
+    check_row_type(what, "x", x);
+    TORCH_CHECK_VALUE(weight.scalar_type() == x.scalar_type(), what, ": weight is ", name_of(weight.scalar_type()), ", x ",
+                      name_of(x.scalar_type()));
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == weight.size(2), what, ": x must be [rows, ", weight.size(2), "], not ", x.sizes());
+    TORCH_CHECK_VALUE(offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.size(0) == weight.size(0) + 1, what,
+                      ": offsets must be int32 [", weight.size(0) + 1, "], not ", name_of(offsets.scalar_type()), " ", offsets.sizes());
+    TORCH_CHECK_VALUE(x.size(0) < (int64_t)1 << 31 && weight.size(0) <= 65536, what, ": more rows or experts than one call takes");
+    if (wants_grad({x, weight})) return ExpertFunction::apply(x, weight, offsets);
+    return group_product(what, x, weight, offsets, false);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_operators, m) {
@@ -638,4 +1077,10 @@ PYBIND11_MODULE(_operators, m) {
     m.def("distill_loss_and_grad", &distill_loss_and_grad, free);
     m.def("block_product", &block_product, free);
     m.def("quantize_blocks", &quantize_blocks, free);
+    m.def("gradient_norm", &gradient_norm, free);
+    m.def("clip_gradients", &clip_gradients, free);
+    m.def("route_experts", &route_experts, free);
+    m.def("dispatch_rows", &dispatch_rows, free);
+    m.def("combine_rows", &combine_rows, free);
+    m.def("expert_product", &expert_product, free);
 }

@@ -20,6 +20,7 @@ from torch import Tensor
 from torch.optim import Optimizer
 
 from . import _native
+from .clip import clip_gradients
 from .modes import freqs_tensor, omega_tensor
 from .spectral import SteadyStep
 
@@ -417,6 +418,13 @@ class CRESSO5(Optimizer):
         for gi, group in enumerate(self.param_groups):
             self._step_group(gi, group)
         return loss
+
+    def clip_gradients(self, max_norm: float, *, norm_type: float = 2.0, grad_scale: float = 1.0) -> Tensor:
+        """Clips the gradients of all parameter groups in place by their common
+        norm, before :meth:`step`; -> the norm before (see
+        :func:`cresso_amd.clip_gradients`)."""
+        return clip_gradients([p.grad for group in self.param_groups for p in group["params"]], max_norm,
+                              norm_type=norm_type, grad_scale=grad_scale)
 
     def _fast_scalar(self, gi: int, group: dict) -> bool:
         """Steady-state path: the group is exactly the cached scalar batch and

@@ -510,6 +510,100 @@ int32_t cresso_block_product(const void* x, int64_t x_stride, int32_t dtype, int
 int32_t cresso_block_quantize(const void* w, int64_t w_stride, int32_t dtype, int64_t rows, int64_t cols, void* values,
                               float* scales, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Layers of experts, and the gradients before the step (no reference
+ * counterpart).  As above: rows of `width` consecutive elements at a row
+ * stride in elements, workspaces of 16-byte alignment that hold nothing between
+ * calls, outputs that share no memory with what a call reads.
+ * ------------------------------------------------------------------------- */
+
+/* The norm over a set of gradients, and the set clipped by it:
+ *   norm = |grad_scale| * (sum g^2)^(1/2)  (CRESSO_NORM_2)  or  |grad_scale| * max |g|  (CRESSO_NORM_MAX)
+ *   out  = g * grad_scale * (norm finite and above max_norm ? max_norm / norm : 1).
+ * out: NULL (the tensor counts for the norm alone), the gradient itself, or
+ * memory that no tensor of the call shares, of the gradient's dtype or, for
+ * f16 and bf16, f32.  Gradients that are written in place share no memory with
+ * one another.  Each is `numel` consecutive elements.  Sums are fp64 in a
+ * fixed order, norm [1] is fp32 (inf above its range) and written for no
+ * tensors at all too (0).  grad_scale is finite; max_norm may be infinite. */
+#define CRESSO_NORM_2 2
+#define CRESSO_NORM_MAX 0
+typedef struct cresso_grad_desc {
+    const void* grad;
+    void* out;
+    int64_t numel;
+    int32_t dtype, out_dtype;
+} cresso_grad_desc;
+size_t cresso_clip_workspace_bytes(const cresso_grad_desc* grads, int32_t count);
+int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t count, int32_t norm_kind, double max_norm,
+                              double grad_scale, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+
+#define CRESSO_SCORE_SOFTMAX 0
+#define CRESSO_SCORE_SIGMOID 1
+
+/* The router of a layer of experts.  A token's key is its logit plus the bias
+ * (fp32; bias may be NULL); the `top` experts of the largest keys are taken,
+ * ties to the lowest expert, NaN above all.  A key of -inf is never taken:
+ * where fewer are left, the last entries are absent (expert -1, weight 0).
+ * Weights [tokens][top] (fp32), of the logits without the bias:
+ *   softmax  scale * exp(z) / sum of exp over all experts, or with `normalize` over the chosen ones
+ *   sigmoid  scale * sigmoid(z), with `normalize` divided by the chosen ones' sum
+ * A slot is token * top + entry.  order [slots]: the slots sorted by expert,
+ * those of one expert in their own order, absent ones last; places [slots]: the
+ * place of each slot in that order; offsets [experts + 1]: where each expert's
+ * slots begin, and the last's end.  2 <= experts + 1 <= 1025, top <= 32 and
+ * at most experts, slots below 2^31. */
+typedef struct cresso_route_desc {
+    const void* logits;
+    const float* bias;
+    float* weights;
+    int32_t *experts, *order, *places, *offsets;
+    int64_t logits_stride, tokens;
+    int32_t num_experts, top, dtype, score, normalize;
+    float scale;
+} cresso_route_desc;
+size_t cresso_route_workspace_bytes(const cresso_route_desc* desc);
+int32_t cresso_route_forward(const cresso_route_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+/* d_logits [tokens][num_experts] (contiguous, of the logits' dtype, written
+ * whole) from d_weights [tokens][top] (contiguous fp32), the call's weights
+ * and experts.  No workspace; order, places and offsets are not read. */
+int32_t cresso_route_backward(const cresso_route_desc* desc, const float* d_weights, void* d_logits, void* stream);
+
+/* Rows between tokens and their slots.  experts [tokens][top]: an entry below 0
+ * is absent; places [tokens][top]: a slot's row; a place outside [0, tokens *
+ * top) is not read or written.
+ *   dispatch: rows[places[t][k]] = x[t], zeros for absent slots
+ *   combine:  out[t] = sum over present k, in their order, of weights[t][k] * rows[places[t][k]]  (weights NULL: 1)
+ *   combine_backward: d_rows[places[t][k]] = weights[t][k] * d_out[t], zeros for absent slots;
+ *                     d_weights[t][k] = sum of d_out[t] * rows[places[t][k]], 0 for absent slots  (NULL: not wanted)
+ * The gradient of dispatch is combine without weights.  rows, out, d_rows that
+ * are written are contiguous.  Sums are fp32. */
+int32_t cresso_dispatch_rows(const void* x, int64_t x_stride, int32_t dtype, int64_t tokens, int32_t top, int64_t width,
+                             const int32_t* experts, const int32_t* places, void* rows, void* stream);
+int32_t cresso_combine_rows(const void* rows, int64_t rows_stride, int32_t dtype, int64_t tokens, int32_t top, int64_t width,
+                            const int32_t* experts, const int32_t* places, const float* weights, void* out, void* stream);
+int32_t cresso_combine_backward(const void* rows, int64_t rows_stride, const void* d_out, int64_t d_out_stride, int32_t dtype,
+                                int64_t tokens, int32_t top, int64_t width, const int32_t* experts, const int32_t* places,
+                                const float* weights, void* d_rows, float* d_weights, void* stream);
+
+/* Products of rows with the matrix of the expert that they belong to: rows
+ * offsets[e] to offsets[e + 1] (device int32 [experts + 1], within 0..rows and
+ * not falling) are expert e's; rows outside offsets[0]..offsets[experts] get zeros.
+ *   product:        out[i][c] = sum over d of x[i][d] * w[e][c][d]     (turned 0: w is [experts][cols][depth])
+ *                                           x[i][d] * w[e][d][c]     (turned 1: w is [experts][depth][cols])
+ *   product_weight: out[e][a][b] = sum over expert e's rows i of p[i][a] * q[i][b]   (zeros without a row)
+ * All of one dtype (f32, bf16, f16); out contiguous; sums are fp32, rounded
+ * once.  w_expert_stride and w_stride: elements between experts and rows. */
+size_t cresso_expert_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype);
+int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int64_t depth,
+                              const void* w, int64_t w_expert_stride, int64_t w_stride, int32_t turned, int32_t experts,
+                              const int32_t* offsets, void* out, void* workspace, size_t workspace_bytes, void* stream);
+size_t cresso_expert_product_weight_workspace_bytes(int64_t rows, int64_t p_width, int64_t q_width, int32_t experts,
+                                                    int32_t dtype);
+int32_t cresso_expert_product_weight(const void* p, int64_t p_stride, int64_t p_width, const void* q, int64_t q_stride,
+                                     int64_t q_width, int32_t dtype, int64_t rows, int32_t experts, const int32_t* offsets,
+                                     void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
