@@ -5,9 +5,9 @@
 #include <algorithm>
 
 namespace cresso {
-template <> void group_launch<float>(GroupArgs, bool, bool, int, hipStream_t);
-template <> void group_launch<__half>(GroupArgs, bool, bool, int, hipStream_t);
-template <> void group_launch<__hip_bfloat16>(GroupArgs, bool, bool, int, hipStream_t);
+template <> void group_launch<float>(GroupArgs, bool, bool, bool, int, hipStream_t);
+template <> void group_launch<__half>(GroupArgs, bool, bool, bool, int, hipStream_t);
+template <> void group_launch<__hip_bfloat16>(GroupArgs, bool, bool, bool, int, hipStream_t);
 
 namespace {
 int32_t check_group(const char* what, int32_t dtype, int64_t rows, int64_t a, int64_t b, int32_t experts) {
@@ -20,6 +20,12 @@ int32_t check_group(const char* what, int32_t dtype, int64_t rows, int64_t a, in
         return fail(CRESSO_E_UNSUPPORTED, "%s: %lld rows, %d matrices of %lld x %lld are more than one call takes", what, (long long)rows,
                     experts, (long long)a, (long long)b);
     return CRESSO_OK;
+}
+// Whether rows at p go to LDS in whole pieces of 16 bytes: so do their width and stride, and a
+// stage's rows lie within 2^31 bytes.
+bool whole_rows(const void* p, int64_t width, int64_t stride, int32_t dtype) {
+    const int64_t e = dtype == CRESSO_F32 ? 4 : 8;
+    return ((uintptr_t)p & 15) == 0 && width % e == 0 && stride % e == 0 && stride >= width && stride < (int64_t)1 << 21 && width < (int64_t)1 << 21;
 }
 }  // namespace
 }  // namespace cresso
@@ -62,8 +68,10 @@ extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_
     a.b_stride = w_stride;
     a.b_expert = w_expert_stride;
     a.experts = experts;
-    const int tile = rows >= 64 * (int64_t)std::max(experts, 1) ? 128 : 64;
-    with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, false, turned != 0, tile, (hipStream_t)stream); });
+    const int64_t mean = rows / std::max(experts, 1);
+    const int tile = mean >= 512 && cols >= 256 ? 256 : mean >= 64 ? 128 : 64;
+    const bool whole = whole_rows(x, depth, x_stride, dtype) && whole_rows(w, w_cols, w_stride, dtype) && w_expert_stride % (dtype == CRESSO_F32 ? 4 : 8) == 0;
+    with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, false, turned != 0, whole, tile, (hipStream_t)stream); });
     return launched(what);
 }
 
@@ -92,7 +100,8 @@ extern "C" int32_t cresso_expert_product_weight(const void* p, int64_t p_stride,
     a.a_stride = p_stride;
     a.b_stride = q_stride;
     a.experts = experts;
-    const int tile = p_width > 64 && q_width > 64 ? 128 : 64;
-    with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, true, true, tile, (hipStream_t)stream); });
+    const int tile = p_width >= 512 && q_width >= 512 ? 256 : p_width > 64 && q_width > 64 ? 128 : 64;
+    const bool whole = whole_rows(p, p_width, p_stride, dtype) && whole_rows(q, q_width, q_stride, dtype);
+    with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, true, true, whole, tile, (hipStream_t)stream); });
     return launched(what);
 }

@@ -10,10 +10,10 @@
 //                    other way round, across k;  one expert's rows are cut into tiles of m
 //   weight gradient  A = p, B = q, both across k, which are one expert's rows
 //
-// A stage of a tile is 128 bytes of k: 64 numbers of 16 bits or 32 of fp32.
-// The matrix instructions take 16 x 16 x 32 of 16 bits, or 16 x 16 x 4 of fp32
-// four times; a lane's operand is always 16 bytes of k, and which k the four
-// quarters of a wave take is the same for both operands, so the order of k
+// A stage of a tile is ROW bytes of k: at 128, 64 numbers of 16 bits or 32 of
+// fp32.  The matrix instructions take 16 x 16 x 32 of 16 bits, or 16 x 16 x 4 of
+// fp32 four times; a lane's operand is always 16 bytes of k, and which k the
+// four quarters of a wave take is the same for both operands, so the order of k
 // within a stage is free.  Operands across k are read from LDS transposed.
 #pragma once
 
@@ -41,7 +41,6 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Group {
     static constexpr int E = 16 / (int)sizeof(T);    // elements of a piece
-    static constexpr int KS = 128 / (int)sizeof(T);  // k of a stage
 };
 
 // ---------------------------------------------------------------------------
@@ -49,49 +48,55 @@ template <typename T> struct Group {
 // lanes that read in one cycle find theirs in different banks: 16 lanes at 16
 // bytes (0-3, 12-15, 20-23, 24-27 and likewise on), 32 at 8, 64 at 4.
 // ---------------------------------------------------------------------------
-// Along k, rows of 8 pieces: A's fragment has rows l16 of its 16.
-__device__ __forceinline__ int turn_a(int row) { return ((row >> 1) & 7) ^ (row & 4); }
-// B's fragment i has rows 4 FN (l16 / 4) + 4 i + l16 % 4, so that a lane ends with 4 FN consecutive columns.
-template <int FN> __device__ __forceinline__ int turn_b(int row) {
-    const int c = row / (4 * FN);
-    return ((row >> 1) & 1) | (c & 1) << 1 | ((c ^ (c >> 1)) & 1) << 2;
+// Along k, rows of 8 or 4 pieces.  A's fragment (FN 0) has rows l16 of its 16, B's fragment i rows
+// 4 FN (l16 / 4) + 4 i + l16 % 4, so that a lane ends with 4 FN consecutive columns.
+template <int ROW, int FN> __device__ __forceinline__ int turn_along(int row) {
+    constexpr int run = FN > 0 ? 4 * FN : 4;
+    const int c = row / run;
+    if constexpr (ROW == 128) {
+        if constexpr (FN == 0) return ((row >> 1) & 7) ^ (row & 4);
+        else return ((row >> 1) & 1) | (c & 1) << 1 | ((c ^ (c >> 1)) & 1) << 2;
+    } else {
+        if constexpr (FN == 4) return ((row >> 4) & 1) * 2 + ((row >> 1) & 1);
+        else return ((c ^ (c >> 1)) & 1) * 2 + ((c >> 1) & 1);
+    }
 }
 // Across k, rows of TILE elements: the blocks of 16 elements change places.
-template <typename T, int TILE> __device__ __forceinline__ int turn_across(int k) {
-    if constexpr (sizeof(T) == 4) return TILE >= 64 ? (k >> 3) & 3 : (k >> 3) & 1;
-    else if constexpr (TILE >= 128) return (k & 3) | ((k >> 4) & 1) << 2;
-    else if constexpr (TILE == 64) return ((k >> 1) & 1) | ((k >> 4) & 1) << 1;
-    else return (k >> 4) & 1;
+template <typename T, int ROW, int TILE> __device__ __forceinline__ int turn_across(int k) {
+    const int far = k >> (ROW == 128 ? 4 : 3);   // what lies in a wave's other quarters
+    if constexpr (sizeof(T) == 4) return ROW == 128 ? (TILE >= 64 ? (k >> 3) & 3 : (k >> 3) & 1) : (k >> 2) & 3;
+    else if constexpr (TILE >= 128) return (k & 3) | (far & 1) << 2;
+    else if constexpr (TILE == 64) return ((k >> 1) & 1) | (far & 1) << 1;
+    else return far & 1;
+}
+// Row (or, across k, k) and piece that lie at a place of a tile's stage.
+template <typename T, bool ACROSS, int ROW, int TILE, int FN> __device__ __forceinline__ void at_place(int place, int& row, int& piece) {
+    if constexpr (ACROSS) {
+        constexpr int E = Group<T>::E, per = TILE / E, block = 16 / E;   // pieces of a row, of a block
+        row = place / per;
+        const int pos = place % per;
+        piece = ((pos / block) ^ turn_across<T, ROW, TILE>(row)) * block + pos % block;
+    } else {
+        row = place / (ROW / 16);
+        piece = (place % (ROW / 16)) ^ turn_along<ROW, FN>(row);
+    }
 }
 
 // A tile's operand on its way from memory, through registers, to LDS.  It has
 // `size` rows along k, or `size` elements a row across it; what is beyond
 // those, and beyond k, is 0.
-template <typename T, bool ACROSS, int TILE, int NT, int FN /* 0: A */> struct Operand {
-    static constexpr int E = Group<T>::E, KS = Group<T>::KS, P = TILE * 8 / NT;
-    static_assert(P * NT == TILE * 8, "tile");
+template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */> struct Operand {
+    static constexpr int E = Group<T>::E, P = TILE * (ROW / 16) / NT;
+    static_assert(P * NT == TILE * (ROW / 16), "tile");
     const T* base;
     int64_t stride, size, depth;
     u32x4 held[P];
 
-    // Row (or k) and piece that lie at a place of the tile's stage.
-    static __device__ __forceinline__ void at_place(int place, int& row, int& piece) {
-        if constexpr (ACROSS) {
-            constexpr int per = TILE / E, block = 16 / E;   // pieces of a row, of a block
-            row = place / per;
-            const int pos = place % per;
-            piece = ((pos / block) ^ turn_across<T, TILE>(row)) * block + pos % block;
-        } else {
-            row = place >> 3;
-            if constexpr (FN > 0) piece = (place & 7) ^ turn_b<FN>(row);
-            else piece = (place & 7) ^ turn_a(row);
-        }
-    }
     __device__ __forceinline__ void load(int64_t k0) {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             int row, piece;
-            at_place((int)threadIdx.x + i * NT, row, piece);
+            at_place<T, ACROSS, ROW, TILE, FN>((int)threadIdx.x + i * NT, row, piece);
             held[i] = u32x4{0, 0, 0, 0};
             if constexpr (ACROSS) {
                 if (k0 + row < depth) held[i] = load_unit(base + (k0 + row) * stride, piece, size);
@@ -106,25 +111,82 @@ template <typename T, bool ACROSS, int TILE, int NT, int FN /* 0: A */> struct O
     }
 };
 
-// Fragments of a wave: 16 m (or n) from `first` on, for step s (0 or 1) of a stage.
-template <typename T, bool ACROSS, int TILE, int FN /* 0: A */> struct Fragments {
+// 16 bytes a lane from a buffer to LDS: lane i's go to lds + 16 * i.  Written
+// out, since with the builtin the compiler waits for all of them before each
+// transposed read of LDS, whichever part that reads (1340 us instead of XXX for
+// the gradient of 32768 x 2048 -> 5632).  It writes no register but m0, which the
+// compiler keeps nothing in (it sets it right before what reads it); group_ready waits for it.
+__device__ __forceinline__ void group_to_lds(u32x4 from, uint32_t lane_at, uint32_t at, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds), "v"(lane_at), "s"(from), "s"(at));
+}
+
+// The same with the pieces going to LDS by themselves, for rows, strides and
+// sizes of whole pieces.  What lies beyond the buffer is 0 in LDS.
+template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */> struct Stream {
+    static constexpr int E = Group<T>::E, P = TILE * (ROW / 16) / NT, KS = ROW / (int)sizeof(T);
+    static_assert(P * NT == TILE * (ROW / 16), "tile");
+    const T* base;
+    int64_t stride, size, depth;
+    uint32_t at[P];   // byte of a thread's piece in the first stage
+    __device__ __forceinline__ void begin() {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            int row, piece;
+            at_place<T, ACROSS, ROW, TILE, FN>((int)threadIdx.x + i * NT, row, piece);
+            at[i] = (uint32_t)row * (uint32_t)(stride * (int)sizeof(T)) + (uint32_t)piece * 16;
+        }
+    }
+    // Stage s to LDS at `to`, which is the wave's part of the buffer; s of `stages` and beyond: zeros.
+    __device__ __forceinline__ void fetch(int s, int stages, uint32_t to) const {
+        const int64_t k0 = (int64_t)s * KS, left = depth - k0;   // k of this stage and behind it
+        const T* from = base;
+        int64_t bytes = 0;
+        if (s < stages) {
+            if constexpr (ACROSS) {
+                from = base + k0 * stride;
+                bytes = ((min(left, (int64_t)KS) - 1) * stride + size) * (int64_t)sizeof(T);
+            } else {
+                bytes = ((min((int64_t)TILE, size) - 1) * stride + depth) * (int64_t)sizeof(T);
+            }
+        }
+        // the descriptor of make_rsrc, in words
+        const u32x4 buffer = {(uint32_t)(uintptr_t)from, (uint32_t)((uintptr_t)from >> 32) & 0xffffu, (uint32_t)bytes, 0x00020000u};
+        const uint32_t step = ACROSS ? 0u : (uint32_t)(k0 * (int)sizeof(T));
+        const bool cut = !ACROSS && left < KS;   // a row's next numbers are another row's
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            uint32_t lane_at = at[i];
+            if (cut) {
+                int row, piece;
+                at_place<T, ACROSS, ROW, TILE, FN>((int)threadIdx.x + i * NT, row, piece);
+                if (piece * E >= left) lane_at = 0x80000000u;   // beyond every buffer
+            }
+            group_to_lds(buffer, lane_at, step, to + i * (NT * 16));
+        }
+    }
+};
+
+// Fragments of a wave: 16 m (or n) from `first` on, for step s of a stage (64 bytes of k each).
+template <typename T, bool ACROSS, int ROW, int TILE, int FN /* 0: A */> struct Fragments {
+    static constexpr int STEPS = ROW / 64;
     int at[2];   // along: the byte of fragment 0 for each step; across: of the lane's row, and its turn
     __device__ __forceinline__ void begin(int first) {
         const int lane = threadIdx.x & (kWave - 1), l16 = lane & 15, quad = lane >> 4;
         if constexpr (ACROSS) {
-            const int k = sizeof(T) == 2 ? quad * 16 + (l16 >> 2) : quad * 8;
+            const int k = sizeof(T) == 2 ? quad * (8 * STEPS) + (l16 >> 2) : quad * (4 * STEPS);
             at[0] = k * (TILE * (int)sizeof(T)) + (sizeof(T) == 2 ? (l16 & 3) * 8 : l16 * 4);
-            at[1] = turn_across<T, TILE>(k) ^ (first / 16);
+            at[1] = turn_across<T, ROW, TILE>(k) ^ (first / 16);
         } else {
             const int row = first + (FN > 0 ? (l16 >> 2) * (4 * FN) + (l16 & 3) : l16);
-            const int turn = FN > 0 ? turn_b<(FN > 0 ? FN : 1)>(row) : turn_a(row);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) at[s] = row * 128 + ((quad * 2 + s) ^ turn) * 16;
+            for (int s = 0; s < STEPS; ++s) at[s] = row * ROW + ((quad * STEPS + s) ^ turn_along<ROW, FN>(row)) * 16;
         }
     }
     __device__ __forceinline__ u32x4 read(const uint8_t* lds, int s, int i) const {
         if constexpr (!ACROSS) {
-            return *(const u32x4*)(lds + at[s] + i * (FN > 0 ? 4 * 128 : 16 * 128));
+            return *(const u32x4*)(lds + at[s] + i * (FN > 0 ? 4 * ROW : 16 * ROW));
         } else {
             constexpr int R = TILE * (int)sizeof(T);   // bytes of a row
             const uint8_t* from = lds + at[0] + ((at[1] ^ i) * (16 * (int)sizeof(T)));
@@ -243,25 +305,13 @@ template <typename T> __device__ __forceinline__ void group_fill(const GroupArgs
     }
 }
 
-// WM x WN waves of FM x FN fragments of 16 x 16 each.
-template <typename T, bool WEIGHT, bool B_ACROSS, int WM, int WN, int FM, int FN>
-__global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
-    constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16;
-    constexpr int KS = Group<T>::KS, E = Group<T>::E, STAGE = (TM + TN) * 128;
-    constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
-    __shared__ __align__(16) uint8_t lds[2 * STAGE];
-    if (blockIdx.x >= a.tiles) {
-        group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
-        return;
-    }
-    Operand<T, WEIGHT, TM, NT, 0> oa;
-    Operand<T, ACROSS, TN, NT, FN> ob;
-    uint32_t tm, tn;
-    T* out;
-    int64_t rows, m0;   // rows of the result from `out` on, the tile's first
+// A workgroup's tile: its operands, its result's rows from `out` on (m0: the tile's first) and its column of tiles.
+// false: there is none.
+template <typename T, bool WEIGHT, bool ACROSS, int TM, int TN, typename A, typename B>
+__device__ __forceinline__ bool group_begin(const GroupArgs& a, A& oa, B& ob, T*& out, int64_t& rows, int64_t& m0, uint32_t& tn) {
+    uint32_t tm;
     if constexpr (WEIGHT) {
-        const uint32_t per = a.tiles_m * a.tiles_n;
-        if (!group_place(per * a.experts / a.tiles_n, a.tiles_n, tm, tn)) return;
+        if (!group_place(a.tiles_m * a.experts, a.tiles_n, tm, tn)) return false;
         const int e = (int)(tm / a.tiles_m);
         m0 = (int64_t)(tm % a.tiles_m) * TM;
         const int64_t n0 = (int64_t)tn * TN;
@@ -275,7 +325,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
         out = (T*)a.out + (int64_t)e * a.m * a.n;
         rows = a.m;
     } else {
-        if (!group_place(group_tiles(a, TM), a.tiles_n, tm, tn)) return;
+        if (!group_place(group_tiles(a, TM), a.tiles_n, tm, tn)) return false;
         const GroupTile g = group_tile(a, TM, tm);
         const int64_t n0 = (int64_t)tn * TN;
         oa.base = (const T*)a.a + g.first * a.a_stride;
@@ -289,52 +339,19 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
     }
     oa.stride = a.a_stride;
     ob.stride = a.b_stride;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-    const int wm = (wave % WM) * (FM * 16), wn = (wave / WM) * (FN * 16), l16 = lane & 15, quad = lane >> 4;
-    Fragments<T, WEIGHT, TM, 0> fa;
-    Fragments<T, ACROSS, TN, FN> fb;
-    fa.begin(wm);
-    fb.begin(wn);
-    f32x4 acc[FN][FM] = {};
-    const int64_t stages = (oa.depth + KS - 1) / KS;
-    if (stages) {
-        oa.load(0);
-        ob.load(0);
-        oa.store(lds);
-        ob.store(lds + TM * 128);
-    }
-    for (int64_t s = 0; s < stages; ++s) {
-        uint8_t* const now = lds + (s & 1) * STAGE;
-        uint8_t* const next = lds + (~s & 1) * STAGE;
-        __syncthreads();   // this stage is there, and the one before it has been read
-        if (s + 1 < stages) {
-            oa.load((s + 1) * KS);
-            ob.load((s + 1) * KS);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            u32x4 b[FN];
-#pragma unroll
-            for (int i = 0; i < FN; ++i) b[i] = fb.read(now + TM * 128, h, i);
-#pragma unroll
-            for (int j = 0; j < FM; ++j) {
-                const u32x4 v = fa.read(now, h, j);
-#pragma unroll
-                for (int i = 0; i < FN; ++i) acc[i][j] = group_mfma<T>(b[i], v, acc[i][j]);
-            }
-        }
-        if (s + 1 < stages) {
-            oa.store(next);
-            ob.store(next + TM * 128);
-        }
-    }
-    // a lane holds columns 4 quad to 4 quad + 3 of each fragment's 16, or with B along k 4 FN columns in one piece
+    return true;
+}
+// A lane holds columns 4 quad to 4 quad + 3 of each fragment's 16, or with B
+// along k 4 FN columns in one piece, of rows l16 of each of FM fragments from m on.
+template <typename T, bool ACROSS, int FM, int FN>
+__device__ __forceinline__ void group_store(const GroupArgs& a, T* out, int64_t rows, int64_t m0, int64_t n0, const f32x4 (&acc)[FN][FM]) {
+    constexpr int E = Group<T>::E;
+    const int lane = threadIdx.x & (kWave - 1), l16 = lane & 15, quad = lane >> 4;
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
-        const int64_t m = m0 + wm + j * 16 + l16;
+        const int64_t m = m0 + j * 16 + l16;
         if (m >= rows) continue;
         T* to = out + m * a.n;
-        const int64_t n0 = (int64_t)tn * TN + wn;
         if constexpr (ACROSS || 4 * FN < E) {
 #pragma unroll
             for (int i = 0; i < FN; ++i) {
@@ -360,11 +377,145 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
     }
 }
 
-// One dtype's kernels, each in a source file of its own.
-template <typename T> void group_launch(GroupArgs a, bool weight, bool across, int tile, hipStream_t st);
+// WM x WN waves of FM x FN fragments of 16 x 16 each; operands of any alignment, through registers.
+template <typename T, bool WEIGHT, bool B_ACROSS, int WM, int WN, int FM, int FN>
+__global__ __launch_bounds__(WM* WN * 64, 2) void group_any_kernel(GroupArgs a) {
+    constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16, ROW = 128;
+    constexpr int KS = ROW / (int)sizeof(T), STAGE = (TM + TN) * ROW;
+    constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
+    __shared__ __align__(16) uint8_t lds[2 * STAGE];
+    if (blockIdx.x >= a.tiles) {
+        group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
+        return;
+    }
+    Operand<T, WEIGHT, ROW, TM, NT, 0> oa;
+    Operand<T, ACROSS, ROW, TN, NT, FN> ob;
+    uint32_t tn;
+    T* out;
+    int64_t rows, m0;
+    if (!group_begin<T, WEIGHT, ACROSS, TM, TN>(a, oa, ob, out, rows, m0, tn)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wm = (wave % WM) * (FM * 16), wn = (wave / WM) * (FN * 16);
+    Fragments<T, WEIGHT, ROW, TM, 0> fa;
+    Fragments<T, ACROSS, ROW, TN, FN> fb;
+    fa.begin(wm);
+    fb.begin(wn);
+    f32x4 acc[FN][FM] = {};
+    const int64_t stages = (oa.depth + KS - 1) / KS;
+    if (stages) {
+        oa.load(0);
+        ob.load(0);
+        oa.store(lds);
+        ob.store(lds + TM * ROW);
+    }
+    for (int64_t s = 0; s < stages; ++s) {
+        uint8_t* const now = lds + (s & 1) * STAGE;
+        uint8_t* const next = lds + (~s & 1) * STAGE;
+        __syncthreads();   // this stage is there, and the one before it has been read
+        if (s + 1 < stages) {
+            oa.load((s + 1) * KS);
+            ob.load((s + 1) * KS);
+        }
+#pragma unroll
+        for (int h = 0; h < ROW / 64; ++h) {
+            u32x4 b[FN];
+#pragma unroll
+            for (int i = 0; i < FN; ++i) b[i] = fb.read(now + TM * ROW, h, i);
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+                const u32x4 v = fa.read(now, h, j);
+#pragma unroll
+                for (int i = 0; i < FN; ++i) acc[i][j] = group_mfma<T>(b[i], v, acc[i][j]);
+            }
+        }
+        if (s + 1 < stages) {
+            oa.store(next);
+            ob.store(next + TM * ROW);
+        }
+    }
+    group_store<T, ACROSS, FM, FN>(a, out, rows, m0 + wm, (int64_t)tn * TN + wn, acc);
+}
+
+// Waits until at most N of the wave's loads are on their way and all its LDS
+// reads have ended (the stage they read is filled anew), then for the other waves.
+template <int N> __device__ __forceinline__ void group_ready() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The same for operands of whole aligned pieces, which go to LDS by themselves,
+// STAGES - 1 stages ahead of the one that is multiplied.
+template <typename T, bool WEIGHT, bool B_ACROSS, int WM, int WN, int FM, int FN, int ROW, int STAGES>
+__global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
+    constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16;
+    constexpr int KS = ROW / (int)sizeof(T), STAGE = (TM + TN) * ROW;
+    constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
+    __shared__ __align__(16) uint8_t lds[STAGES * STAGE];
+    if (blockIdx.x >= a.tiles) {
+        group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
+        return;
+    }
+    typedef Stream<T, WEIGHT, ROW, TM, NT, 0> StreamA;
+    typedef Stream<T, ACROSS, ROW, TN, NT, FN> StreamB;
+    constexpr int LOADS = StreamA::P + StreamB::P;
+    StreamA oa;
+    StreamB ob;
+    uint32_t tn;
+    T* out;
+    int64_t rows, m0;
+    if (!group_begin<T, WEIGHT, ACROSS, TM, TN>(a, oa, ob, out, rows, m0, tn)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wm = (wave % WM) * (FM * 16), wn = (wave / WM) * (FN * 16);
+    Fragments<T, WEIGHT, ROW, TM, 0> fa;
+    Fragments<T, ACROSS, ROW, TN, FN> fb;
+    fa.begin(wm);
+    fb.begin(wn);
+    oa.begin();
+    ob.begin();
+    f32x4 acc[FN][FM] = {};
+    const int stages = (int)((oa.depth + KS - 1) / KS);
+    const uint32_t mine = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)wave * 1024;
+    uint32_t to = 0;
+    int next = 0;
+    const auto fetch = [&] {
+        oa.fetch(next, stages, mine + to);
+        ob.fetch(next, stages, mine + to + TM * ROW);
+        ++next;
+        to = to == (STAGES - 1) * STAGE ? 0 : to + STAGE;
+    };
+    if (stages) {
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) fetch();
+    }
+    int from = 0;
+    for (int s = 0; s < stages; ++s) {
+        group_ready<(STAGES - 2) * LOADS>();
+        fetch();
+        const uint8_t* const now = lds + from;
+#pragma unroll
+        for (int h = 0; h < ROW / 64; ++h) {
+            u32x4 b[FN];
+#pragma unroll
+            for (int i = 0; i < FN; ++i) b[i] = fb.read(now + TM * ROW, h, i);
+#pragma unroll
+            for (int j = 0; j < FM; ++j) {
+                const u32x4 v = fa.read(now, h, j);
+#pragma unroll
+                for (int i = 0; i < FN; ++i) acc[i][j] = group_mfma<T>(b[i], v, acc[i][j]);
+            }
+        }
+        from = from == (STAGES - 1) * STAGE ? 0 : from + STAGE;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way to LDS when the workgroup ends
+    group_store<T, ACROSS, FM, FN>(a, out, rows, m0 + wm, (int64_t)tn * TN + wn, acc);
+}
+
+// One dtype's kernels, each in a source file of its own.  whole: aligned, whole pieces.
+template <typename T> void group_launch(GroupArgs a, bool weight, bool across, bool whole, int tile, hipStream_t st);
 
 #define CRESSO_GROUP_LAUNCH(T)                                                                                          \
-    template <> void group_launch<T>(GroupArgs a, bool weight, bool across, int tile, hipStream_t st) {                 \
+    template <> void group_launch<T>(GroupArgs a, bool weight, bool across, bool whole, int tile, hipStream_t st) {     \
         const auto run = [&](auto kernel, int tm, int tn, int threads) {                                                \
             a.tiles_n = (uint32_t)((a.n + tn - 1) / tn);                                                                \
             a.tiles_m = (uint32_t)(weight ? (a.m + tm - 1) / tm : a.rows / tm + a.experts);                             \
@@ -373,8 +524,13 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, i
         };                                                                                                              \
         const auto size = [&](auto w, auto x) {                                                                         \
             constexpr bool W = decltype(w)::value, X = decltype(x)::value;                                              \
-            if (tile == 128) run(group_kernel<T, W, X, 1, 4, 8, 2>, 128, 128, 256);                                     \
-            else run(group_kernel<T, W, X, 1, 4, 4, 1>, 64, 64, 256);                                                   \
+            if constexpr (sizeof(T) == 2) {                                                                             \
+                if (whole && tile == 256) return run(group_kernel<T, W, X, 2, 4, 8, 4, 64, 4>, 256, 256, 512);          \
+            }                                                                                                           \
+            if (whole && tile >= 128) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128, 128, 256);                    \
+            else if (whole) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3>, 64, 64, 256);                                \
+            else if (tile >= 128) run(group_any_kernel<T, W, X, 1, 4, 8, 2>, 128, 128, 256);                            \
+            else run(group_any_kernel<T, W, X, 1, 4, 4, 1>, 64, 64, 256);                                               \
         };                                                                                                              \
         if (weight) size(std::true_type{}, std::true_type{});                                                           \
         else if (across) size(std::false_type{}, std::true_type{});                                                     \
