@@ -19,6 +19,8 @@
 
 #include "row_ops.hpp"
 
+#include <type_traits>
+
 namespace cresso {
 
 struct GroupArgs {
@@ -57,8 +59,7 @@ template <int ROW, int FN> __device__ __forceinline__ int turn_along(int row) {
         if constexpr (FN == 0) return ((row >> 1) & 7) ^ (row & 4);
         else return ((row >> 1) & 1) | (c & 1) << 1 | ((c ^ (c >> 1)) & 1) << 2;
     } else {
-        if constexpr (FN == 4) return ((row >> 4) & 1) * 2 + ((row >> 1) & 1);
-        else return ((c ^ (c >> 1)) & 1) * 2 + ((c >> 1) & 1);
+        return ((c ^ (c >> 1)) & 1) * 2 + ((c >> 1) & 1);
     }
 }
 // Across k, rows of TILE elements: the blocks of 16 elements change places.
@@ -129,7 +130,10 @@ template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */>
     static_assert(P * NT == TILE * (ROW / 16), "tile");
     const T* base;
     int64_t stride, size, depth;
-    uint32_t at[P];   // byte of a thread's piece in the first stage
+    uint32_t at[P];   // byte of a thread's piece in a stage's part of the buffer
+    u32x4 buffer;     // the descriptor of make_rsrc of the next stage, in words
+    uint32_t step, stage_bytes;
+    int left;         // k of the next stage and behind it
     __device__ __forceinline__ void begin() {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
@@ -137,34 +141,50 @@ template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */>
             at_place<T, ACROSS, ROW, TILE, FN>((int)threadIdx.x + i * NT, row, piece);
             at[i] = (uint32_t)row * (uint32_t)(stride * (int)sizeof(T)) + (uint32_t)piece * 16;
         }
+        const auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+        const uint64_t from = (uint64_t)(uintptr_t)base;
+        const uint32_t row_bytes = scalar((uint32_t)(stride * (int)sizeof(T)));
+        const uint32_t last = scalar((uint32_t)((ACROSS ? size : depth) * (int64_t)sizeof(T)));
+        const uint32_t rows = ACROSS ? (uint32_t)KS : min((uint32_t)TILE, scalar((uint32_t)size));
+        buffer = u32x4{scalar((uint32_t)from), scalar((uint32_t)(from >> 32)) & 0xffffu, (rows - 1) * row_bytes + last, 0x00020000u};
+        stage_bytes = row_bytes * KS;
+        left = (int)scalar((uint32_t)depth);
+        step = 0;
+        ending();
     }
-    // Stage s to LDS at `to`, which is the wave's part of the buffer; s of `stages` and beyond: zeros.
-    __device__ __forceinline__ void fetch(int s, int stages, uint32_t to) const {
-        const int64_t k0 = (int64_t)s * KS, left = depth - k0;   // k of this stage and behind it
-        const T* from = base;
-        int64_t bytes = 0;
-        if (s < stages) {
-            if constexpr (ACROSS) {
-                from = base + k0 * stride;
-                bytes = ((min(left, (int64_t)KS) - 1) * stride + size) * (int64_t)sizeof(T);
-            } else {
-                bytes = ((min((int64_t)TILE, size) - 1) * stride + depth) * (int64_t)sizeof(T);
-            }
-        }
-        // the descriptor of make_rsrc, in words
-        const u32x4 buffer = {(uint32_t)(uintptr_t)from, (uint32_t)((uintptr_t)from >> 32) & 0xffffu, (uint32_t)bytes, 0x00020000u};
-        const uint32_t step = ACROSS ? 0u : (uint32_t)(k0 * (int)sizeof(T));
-        const bool cut = !ACROSS && left < KS;   // a row's next numbers are another row's
+    // Before a stage that is not whole, and before those behind the last: what is behind k is 0.
+    __device__ __forceinline__ void ending() {
+        if (left >= KS) return;
+        if (left <= 0) {
+            buffer[2] = 0;
+        } else if constexpr (ACROSS) {
+            buffer[2] -= (uint32_t)(KS - left) * (stage_bytes / KS);
+        } else {   // a row's next numbers are another row's
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            uint32_t lane_at = at[i];
-            if (cut) {
+            for (int i = 0; i < P; ++i) {
                 int row, piece;
                 at_place<T, ACROSS, ROW, TILE, FN>((int)threadIdx.x + i * NT, row, piece);
-                if (piece * E >= left) lane_at = 0x80000000u;   // beyond every buffer
+                if (piece * E >= left) at[i] = 0x80000000u;   // beyond every buffer
             }
-            group_to_lds(buffer, lane_at, step, to + i * (NT * 16));
         }
+    }
+    __device__ __forceinline__ void next() {
+        left -= KS;
+        if constexpr (ACROSS) {
+            const uint64_t from = ((uint64_t)buffer[1] << 32 | buffer[0]) + stage_bytes;
+            buffer[0] = (uint32_t)from;
+            buffer[1] = (uint32_t)(from >> 32);
+        } else {
+            step += ROW;
+        }
+        ending();
+    }
+    // Piece i of the thread's to the buffer at `to`, which is the wave's part of it.
+    __device__ __forceinline__ void piece(int i, uint32_t to) const { group_to_lds(buffer, at[i], step, to + i * (NT * 16)); }
+    __device__ __forceinline__ void fetch(uint32_t to) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) piece(i, to);
+        next();
     }
 };
 
@@ -221,6 +241,22 @@ template <> __device__ __forceinline__ f32x4 group_mfma<float>(u32x4 a, u32x4 b,
         c = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y), c, 0, 0, 0);
     }
     return c;
+}
+
+// The same with the sum held in one place: with the builtin the compiler moves
+// 256 registers of sums about, since a result may lie elsewhere than what it is
+// added to.  Who reads a sum by anything but these waits with group_mfma_done;
+// the matrix instructions wait for one another where they name the same registers.
+template <typename T> __device__ __forceinline__ void group_mfma_into(u32x4 a, u32x4 b, f32x4& c) {
+    static_assert(sizeof(T) == 2, "16 bits");
+    if constexpr (std::is_same<T, __half>::value) asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+// After the last of them: more than the 18 cycles that a result of four passes takes to be there for others.
+template <int N> __device__ __forceinline__ void group_mfma_done(f32x4 (&c)[N]) {
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+a"(c[i]));   // read behind the wait
 }
 
 // ---------------------------------------------------------------------------
@@ -317,6 +353,8 @@ __device__ __forceinline__ bool group_begin(const GroupArgs& a, A& oa, B& ob, T*
         const int64_t n0 = (int64_t)tn * TN;
         int64_t first, end;
         group_rows(a, e, first, end);
+        first = __builtin_amdgcn_readfirstlane((int)first);   // below 2^31, and the same for all lanes
+        end = __builtin_amdgcn_readfirstlane((int)end);
         oa.base = (const T*)a.a + first * a.a_stride + m0;
         ob.base = (const T*)a.b + first * a.b_stride + n0;
         oa.size = a.m - m0;
@@ -477,11 +515,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
     const int stages = (int)((oa.depth + KS - 1) / KS);
     const uint32_t mine = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)wave * 1024;
     uint32_t to = 0;
-    int next = 0;
     const auto fetch = [&] {
-        oa.fetch(next, stages, mine + to);
-        ob.fetch(next, stages, mine + to + TM * ROW);
-        ++next;
+        oa.fetch(mine + to);
+        ob.fetch(mine + to + TM * ROW);
         to = to == (STAGES - 1) * STAGE ? 0 : to + STAGE;
     };
     if (stages) {
@@ -511,6 +547,94 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
     group_store<T, ACROSS, FM, FN>(a, out, rows, m0 + wm, (int64_t)tn * TN + wn, acc);
 }
 
+// 256 x 256 of 16 bits: four waves of 128 x 128, one to a SIMD, with all of its
+// registers.  Eight waves of 128 x 64 read 96 KB of LDS a stage, as long as
+// their matrix instructions take; these read 64.  A stage's fragments are read
+// while the one before is multiplied, and the pieces of the stage four further
+// on are asked for in between, so that nothing stands before a matrix
+// instruction but the barrier.
+template <typename T, bool WEIGHT, bool B_ACROSS>
+__global__ __launch_bounds__(256, 1) void group_wide_kernel(GroupArgs a) {
+    constexpr int NT = 256, TILE = 256, F = 8, ROW = 64, STAGES = 4;
+    constexpr int KS = ROW / (int)sizeof(T), STAGE = 2 * TILE * ROW;
+    constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
+    __shared__ __align__(16) uint8_t lds[STAGES * STAGE];
+    if (blockIdx.x >= a.tiles) {
+        group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
+        return;
+    }
+    typedef Stream<T, WEIGHT, ROW, TILE, NT, 0> StreamA;
+    typedef Stream<T, ACROSS, ROW, TILE, NT, F> StreamB;
+    constexpr int LOADS = StreamA::P + StreamB::P;
+    static_assert(StreamA::P == 4 && StreamB::P == 4, "a piece for each group of matrix instructions");
+    StreamA oa;
+    StreamB ob;
+    uint32_t tn;
+    T* out;
+    int64_t rows, m0;
+    if (!group_begin<T, WEIGHT, ACROSS, TILE, TILE>(a, oa, ob, out, rows, m0, tn)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wm = (wave & 1) * 128, wn = (wave >> 1) * 128;
+    Fragments<T, WEIGHT, ROW, TILE, 0> fa;
+    Fragments<T, ACROSS, ROW, TILE, F> fb;
+    fa.begin(wm);
+    fb.begin(wn);
+    oa.begin();
+    ob.begin();
+    f32x4 acc[F][F] = {};
+    const int stages = (int)((oa.depth + KS - 1) / KS);
+    const uint32_t mine = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)wave * 1024;
+    u32x4 ra[2][F], rb[2][F];
+    // Multiplies the stage in buffer `now`, whose fragments are in set now % 2;
+    // reads the next one's into the other and fills `now` anew.  A wave issues one
+    // instruction in 4 cycles and a matrix instruction takes 16, so each of them
+    // is followed by at most three others.
+    const auto stage = [&](int now) {
+        group_ready<(STAGES - 2) * LOADS>();
+        const int set = now & 1;
+        const uint8_t* const then = lds + (now + 1) % STAGES * STAGE;
+#pragma unroll
+        for (int j = 0; j < F; ++j) {
+#pragma unroll
+            for (int i = 0; i < F; ++i) {
+                group_mfma_into<T>(rb[set][i], ra[set][j], acc[i][j]);
+                if (i == 0) rb[set ^ 1][j] = fb.read(then + TILE * ROW, 0, j);
+                if (i == 2) ra[set ^ 1][j] = fa.read(then, 0, j);
+                if (i == 5) {
+                    if (j < 4) oa.piece(j, mine + now * STAGE);
+                    else ob.piece(j - 4, mine + now * STAGE + TILE * ROW);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        oa.next();
+        ob.next();
+    };
+    if (stages) {
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) {
+            oa.fetch(mine + i * STAGE);
+            ob.fetch(mine + i * STAGE + TILE * ROW);
+        }
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < F; ++j) {
+            rb[0][j] = fb.read(lds + TILE * ROW, 0, j);
+            ra[0][j] = fa.read(lds, 0, j);
+        }
+        for (int s = 0; s < stages; s += STAGES) {   // stages behind the last are zeros
+#pragma unroll
+            for (int now = 0; now < STAGES; ++now) stage(now);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way to LDS when the workgroup ends
+#pragma unroll
+    for (int i = 0; i < F; ++i) group_mfma_done(acc[i]);
+    group_store<T, ACROSS, F, F>(a, out, rows, m0 + wm, (int64_t)tn * TILE + wn, acc);
+}
+
 // One dtype's kernels, each in a source file of its own.  whole: aligned, whole pieces.
 template <typename T> void group_launch(GroupArgs a, bool weight, bool across, bool whole, int tile, hipStream_t st);
 
@@ -525,7 +649,7 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, b
         const auto size = [&](auto w, auto x) {                                                                         \
             constexpr bool W = decltype(w)::value, X = decltype(x)::value;                                              \
             if constexpr (sizeof(T) == 2) {                                                                             \
-                if (whole && tile == 256) return run(group_kernel<T, W, X, 2, 4, 8, 4, 64, 4>, 256, 256, 512);          \
+                if (whole && tile == 256) return run(group_wide_kernel<T, W, X>, 256, 256, 256);                        \
             }                                                                                                           \
             if (whole && tile >= 128) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128, 128, 256);                    \
             else if (whole) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3>, 64, 64, 256);                                \
