@@ -314,20 +314,35 @@ __device__ __forceinline__ GroupTile group_tile(const GroupArgs& a, int tile, ui
     return g;
 }
 
-// Tile of a workgroup among `high` x `wide`; false: there is none.  Workgroups
-// go to the 8 XCDs in turn; each XCD takes a run of tiles, in columns of 8
-// tiles of m, so that the tiles that run together on one XCD share rows of both
-// operands in its L2.
-__device__ __forceinline__ bool group_place(uint32_t high, uint32_t wide, uint32_t& tm, uint32_t& tn) {
-    const uint32_t total = high * wide, per = total / 8, rest = total % 8;
-    const uint32_t xcd = blockIdx.x % 8, i = blockIdx.x / 8;
-    if (i >= per + (xcd < rest ? 1u : 0u)) return false;
-    const uint32_t t = xcd * per + min(xcd, rest) + i;
+// Which of `total` tiles a workgroup takes.  Workgroups go to the 8 XCDs in
+// turn; each XCD takes a run of tiles.  total or more: none.
+__device__ __forceinline__ uint32_t group_run(uint32_t block, uint32_t total) {
+    const uint32_t per = total / 8, rest = total % 8, xcd = block % 8, i = block / 8;
+    return i < per + (xcd < rest ? 1u : 0u) ? xcd * per + min(xcd, rest) + i : total;
+}
+// Tile t among `high` x `wide`, in columns of 8 tiles of m, so that the tiles that run together on one XCD share rows of
+// both operands in its L2.
+__device__ __forceinline__ void group_place(uint32_t t, uint32_t high, uint32_t wide, uint32_t& tm, uint32_t& tn) {
     const uint32_t group = 8 * wide, g = t / group, in = t - g * group;
     const uint32_t height = min(8u, high - g * 8);
     tm = g * 8 + in % height;
     tn = in / height;
-    return true;
+}
+
+// The expert whose rows are the i-th most (of the first 64, in their order behind those): a weight
+// gradient's tiles take as long as their expert's rows are many, so the longest begin.
+__device__ __forceinline__ int group_longest(const GroupArgs& a, uint32_t i) {
+    if (i >= (uint32_t)kWave) return (int)i;
+    const int lane = threadIdx.x & (kWave - 1), n = min(a.experts, kWave);
+    int64_t first = 0, end = -1;
+    if (lane < n) group_rows(a, lane, first, end);
+    const int mine = (int)(end - first);
+    uint32_t before = 0;
+    for (int e = 0; e < n; ++e) {
+        const int other = __builtin_amdgcn_readlane(mine, e);
+        before += other > mine || (other == mine && e < lane) ? 1u : 0u;
+    }
+    return __builtin_ctzll(__ballot(lane < n && before == i));
 }
 
 // Zeros into the rows that are no expert's.
@@ -341,42 +356,64 @@ template <typename T> __device__ __forceinline__ void group_fill(const GroupArgs
     }
 }
 
-// A workgroup's tile: its operands, its result's rows from `out` on (m0: the tile's first) and its column of tiles.
-// false: there is none.
-template <typename T, bool WEIGHT, bool ACROSS, int TM, int TN, typename A, typename B>
-__device__ __forceinline__ bool group_begin(const GroupArgs& a, A& oa, B& ob, T*& out, int64_t& rows, int64_t& m0, uint32_t& tn) {
-    uint32_t tm;
+// A tile of TM x TN or, from row m0 and column n0 of it on, a part of one: one
+// expert's rows of A and of the result (product), or all its rows as k (weight gradient).
+struct GroupWork {
+    int expert;
+    int64_t first, end;   // rows: of the tile, or of the expert
+    int64_t m0, n0;
+};
+// Tile t of all; high and wide: tiles of m, over all experts (product) or one (weight gradient), and of n.
+template <bool WEIGHT> __device__ __forceinline__ GroupWork group_work(const GroupArgs& a, uint32_t t, uint32_t high, uint32_t wide, int TM, int TN) {
+    GroupWork w;
+    uint32_t tm, tn;
+    if constexpr (WEIGHT) {   // each expert's tiles over all XCDs
+        const uint32_t per = high * wide;
+        w.expert = group_longest(a, t / per);
+        group_place(group_run(t % per, per), high, wide, tm, tn);
+        group_rows(a, w.expert, w.first, w.end);
+        w.first = __builtin_amdgcn_readfirstlane((int)w.first);   // below 2^31, and the same for all lanes
+        w.end = __builtin_amdgcn_readfirstlane((int)w.end);
+        w.m0 = (int64_t)tm * TM;
+    } else {
+        group_place(t, high, wide, tm, tn);
+        const GroupTile g = group_tile(a, TM, tm);
+        w.expert = g.expert;
+        w.first = g.first;
+        w.end = g.first + g.rows;
+        w.m0 = 0;
+    }
+    w.n0 = (int64_t)tn * TN;
+    return w;
+}
+// The operands of a tile's part that begins at m0, n0, and its result's rows from `out` on.
+template <typename T, bool WEIGHT, bool ACROSS, typename A, typename B>
+__device__ __forceinline__ void group_operands(const GroupArgs& a, const GroupWork& w, A& oa, B& ob, T*& out, int64_t& rows) {
     if constexpr (WEIGHT) {
-        if (!group_place(a.tiles_m * a.experts, a.tiles_n, tm, tn)) return false;
-        const int e = (int)(tm / a.tiles_m);
-        m0 = (int64_t)(tm % a.tiles_m) * TM;
-        const int64_t n0 = (int64_t)tn * TN;
-        int64_t first, end;
-        group_rows(a, e, first, end);
-        first = __builtin_amdgcn_readfirstlane((int)first);   // below 2^31, and the same for all lanes
-        end = __builtin_amdgcn_readfirstlane((int)end);
-        oa.base = (const T*)a.a + first * a.a_stride + m0;
-        ob.base = (const T*)a.b + first * a.b_stride + n0;
-        oa.size = a.m - m0;
-        ob.size = a.n - n0;
-        oa.depth = ob.depth = end - first;
-        out = (T*)a.out + (int64_t)e * a.m * a.n;
+        oa.base = (const T*)a.a + w.first * a.a_stride + w.m0;
+        ob.base = (const T*)a.b + w.first * a.b_stride + w.n0;
+        oa.size = a.m - w.m0;
+        oa.depth = ob.depth = w.end - w.first;
+        out = (T*)a.out + (int64_t)w.expert * a.m * a.n;
         rows = a.m;
     } else {
-        if (!group_place(group_tiles(a, TM), a.tiles_n, tm, tn)) return false;
-        const GroupTile g = group_tile(a, TM, tm);
-        const int64_t n0 = (int64_t)tn * TN;
-        oa.base = (const T*)a.a + g.first * a.a_stride;
-        ob.base = (const T*)a.b + g.expert * a.b_expert + (ACROSS ? n0 : n0 * a.b_stride);
-        oa.size = g.rows;
-        ob.size = a.n - n0;
+        oa.base = (const T*)a.a + (w.first + w.m0) * a.a_stride;
+        ob.base = (const T*)a.b + w.expert * a.b_expert + (ACROSS ? w.n0 : w.n0 * a.b_stride);
+        oa.size = w.end - w.first - w.m0;
         oa.depth = ob.depth = a.k;
-        out = (T*)a.out + g.first * a.n;
-        rows = g.rows;
-        m0 = 0;
+        out = (T*)a.out + w.first * a.n;
+        rows = w.end - w.first;
     }
+    ob.size = a.n - w.n0;
     oa.stride = a.a_stride;
     ob.stride = a.b_stride;
+}
+// What a workgroup of a kernel with one size of tiles does.  false: nothing.
+template <bool WEIGHT> __device__ __forceinline__ bool group_begin(const GroupArgs& a, int TM, int TN, GroupWork& w) {
+    const uint32_t high = WEIGHT ? a.tiles_m : group_tiles(a, TM), total = high * a.tiles_n;
+    const uint32_t t = WEIGHT ? blockIdx.x : group_run(blockIdx.x, total);
+    if (!WEIGHT && t >= total) return false;
+    w = group_work<WEIGHT>(a, t, high, a.tiles_n, TM, TN);
     return true;
 }
 // A lane holds columns 4 quad to 4 quad + 3 of each fragment's 16, or with B
@@ -428,10 +465,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_any_kernel(GroupArgs a) 
     }
     Operand<T, WEIGHT, ROW, TM, NT, 0> oa;
     Operand<T, ACROSS, ROW, TN, NT, FN> ob;
-    uint32_t tn;
+    GroupWork w;
+    if (!group_begin<WEIGHT>(a, TM, TN, w)) return;
     T* out;
-    int64_t rows, m0;
-    if (!group_begin<T, WEIGHT, ACROSS, TM, TN>(a, oa, ob, out, rows, m0, tn)) return;
+    int64_t rows;
+    group_operands<T, WEIGHT, ACROSS>(a, w, oa, ob, out, rows);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wm = (wave % WM) * (FM * 16), wn = (wave / WM) * (FN * 16);
     Fragments<T, WEIGHT, ROW, TM, 0> fa;
@@ -471,7 +509,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_any_kernel(GroupArgs a) 
             ob.store(next + TM * ROW);
         }
     }
-    group_store<T, ACROSS, FM, FN>(a, out, rows, m0 + wm, (int64_t)tn * TN + wn, acc);
+    group_store<T, ACROSS, FM, FN>(a, out, rows, w.m0 + wm, w.n0 + wn, acc);
 }
 
 // Waits until at most N of the wave's loads are on their way and all its LDS
@@ -499,10 +537,11 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
     constexpr int LOADS = StreamA::P + StreamB::P;
     StreamA oa;
     StreamB ob;
-    uint32_t tn;
+    GroupWork w;
+    if (!group_begin<WEIGHT>(a, TM, TN, w)) return;
     T* out;
-    int64_t rows, m0;
-    if (!group_begin<T, WEIGHT, ACROSS, TM, TN>(a, oa, ob, out, rows, m0, tn)) return;
+    int64_t rows;
+    group_operands<T, WEIGHT, ACROSS>(a, w, oa, ob, out, rows);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wm = (wave % WM) * (FM * 16), wn = (wave / WM) * (FN * 16);
     Fragments<T, WEIGHT, ROW, TM, 0> fa;
@@ -544,68 +583,57 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
         from = from == (STAGES - 1) * STAGE ? 0 : from + STAGE;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way to LDS when the workgroup ends
-    group_store<T, ACROSS, FM, FN>(a, out, rows, m0 + wm, (int64_t)tn * TN + wn, acc);
+    group_store<T, ACROSS, FM, FN>(a, out, rows, w.m0 + wm, w.n0 + wn, acc);
 }
 
-// 256 x 256 of 16 bits: four waves of 128 x 128, one to a SIMD, with all of its
-// registers.  Eight waves of 128 x 64 read 96 KB of LDS a stage, as long as
-// their matrix instructions take; these read 64.  A stage's fragments are read
-// while the one before is multiplied, and the pieces of the stage four further
-// on are asked for in between, so that nothing stands before a matrix
-// instruction but the barrier.
-template <typename T, bool WEIGHT, bool B_ACROSS>
-__global__ __launch_bounds__(256, 1) void group_wide_kernel(GroupArgs a) {
-    constexpr int NT = 256, TILE = 256, F = 8, ROW = 64, STAGES = 4;
-    constexpr int KS = ROW / (int)sizeof(T), STAGE = 2 * TILE * ROW;
-    constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
-    __shared__ __align__(16) uint8_t lds[STAGES * STAGE];
-    if (blockIdx.x >= a.tiles) {
-        group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
-        return;
-    }
-    typedef Stream<T, WEIGHT, ROW, TILE, NT, 0> StreamA;
-    typedef Stream<T, ACROSS, ROW, TILE, NT, F> StreamB;
-    constexpr int LOADS = StreamA::P + StreamB::P;
-    static_assert(StreamA::P == 4 && StreamB::P == 4, "a piece for each group of matrix instructions");
+// A tile of 32 FM x 32 FN of 16 bits by four waves of 16 FM x 16 FN, one to a
+// SIMD.  A stage's fragments are read while the one before is multiplied, and
+// the pieces of the stage STAGES further on are asked for in between.
+template <typename T, bool WEIGHT, bool ACROSS, int FM, int FN, int STAGES>
+__device__ __forceinline__ void group_large_tile(const GroupArgs& a, const GroupWork& w, uint8_t* const lds) {
+    constexpr int NT = 256, TM = 32 * FM, TN = 32 * FN, ROW = 64;
+    constexpr int KS = ROW / (int)sizeof(T), STAGE = (TM + TN) * ROW;
+    static_assert(STAGES * STAGE >= TM * TN * (int)sizeof(T), "the result goes through the stages' memory");
+    typedef Stream<T, WEIGHT, ROW, TM, NT, 0> StreamA;
+    typedef Stream<T, ACROSS, ROW, TN, NT, FN> StreamB;
+    constexpr int PA = StreamA::P, LOADS = PA + StreamB::P, STEPS = FM * FN;
     StreamA oa;
     StreamB ob;
-    uint32_t tn;
     T* out;
-    int64_t rows, m0;
-    if (!group_begin<T, WEIGHT, ACROSS, TILE, TILE>(a, oa, ob, out, rows, m0, tn)) return;
+    int64_t rows;
+    group_operands<T, WEIGHT, ACROSS>(a, w, oa, ob, out, rows);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int wm = (wave & 1) * 128, wn = (wave >> 1) * 128;
-    Fragments<T, WEIGHT, ROW, TILE, 0> fa;
-    Fragments<T, ACROSS, ROW, TILE, F> fb;
+    const int wm = (wave & 1) * (16 * FM), wn = (wave >> 1) * (16 * FN);
+    Fragments<T, WEIGHT, ROW, TM, 0> fa;
+    Fragments<T, ACROSS, ROW, TN, FN> fb;
     fa.begin(wm);
     fb.begin(wn);
     oa.begin();
     ob.begin();
-    f32x4 acc[F][F] = {};
+    f32x4 acc[FM][FN] = {};
     const int stages = (int)((oa.depth + KS - 1) / KS);
     const uint32_t mine = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)wave * 1024;
-    u32x4 ra[2][F], rb[2][F];
-    // Multiplies the stage in buffer `now`, whose fragments are in set now % 2;
-    // reads the next one's into the other and fills `now` anew.  A wave issues one
-    // instruction in 4 cycles and a matrix instruction takes 16, so each of them
-    // is followed by at most three others.
-    const auto stage = [&](int now) {
+    u32x4 ra[2][FM], rb[2][FN];
+    const auto piece = [&](int i, int buffer) {
+        if (i < PA) oa.piece(i, mine + buffer * STAGE);
+        else if (i < LOADS) ob.piece(i - PA, mine + buffer * STAGE + TM * ROW);
+    };
+    // Multiplies the stage in buffer `now`, whose fragments are in set `set`; reads
+    // the next one's into the other, early enough to be there when the stage ends,
+    // and fills `now` anew.  A wave issues one instruction in 4 cycles and a matrix
+    // instruction takes 16, so each of them is followed by at most three others.
+    const auto stage = [&](int now, int set) {
         group_ready<(STAGES - 2) * LOADS>();
-        const int set = now & 1;
         const uint8_t* const then = lds + (now + 1) % STAGES * STAGE;
+        constexpr int EVERY = STEPS * 3 / 4 / (FM + FN), APART = STEPS / LOADS;
 #pragma unroll
-        for (int j = 0; j < F; ++j) {
-#pragma unroll
-            for (int i = 0; i < F; ++i) {
-                group_mfma_into<T>(rb[set][i], ra[set][j], acc[i][j]);
-                if (i == 0) rb[set ^ 1][j] = fb.read(then + TILE * ROW, 0, j);
-                if (i == 2) ra[set ^ 1][j] = fa.read(then, 0, j);
-                if (i == 5) {
-                    if (j < 4) oa.piece(j, mine + now * STAGE);
-                    else ob.piece(j - 4, mine + now * STAGE + TILE * ROW);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int t = 0; t < STEPS; ++t) {
+            group_mfma_into<T>(rb[set][t % FN], ra[set][t / FN], acc[t / FN][t % FN]);
+            const int r = t / EVERY;
+            if (t % EVERY == 0 && r < FN) rb[set ^ 1][r] = fb.read(then + TM * ROW, 0, r);
+            else if (t % EVERY == 0 && r < FM + FN) ra[set ^ 1][r - FN] = fa.read(then, 0, r - FN);
+            if (t % APART == 1) piece(t / APART, now);
+            __builtin_amdgcn_sched_barrier(0);
         }
         oa.next();
         ob.next();
@@ -614,25 +642,78 @@ __global__ __launch_bounds__(256, 1) void group_wide_kernel(GroupArgs a) {
 #pragma unroll
         for (int i = 0; i < STAGES; ++i) {
             oa.fetch(mine + i * STAGE);
-            ob.fetch(mine + i * STAGE + TILE * ROW);
+            ob.fetch(mine + i * STAGE + TM * ROW);
         }
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
 #pragma unroll
-        for (int j = 0; j < F; ++j) {
-            rb[0][j] = fb.read(lds + TILE * ROW, 0, j);
-            ra[0][j] = fa.read(lds, 0, j);
-        }
-        for (int s = 0; s < stages; s += STAGES) {   // stages behind the last are zeros
+        for (int i = 0; i < FN; ++i) rb[0][i] = fb.read(lds + TM * ROW, 0, i);
 #pragma unroll
-            for (int now = 0; now < STAGES; ++now) stage(now);
+        for (int j = 0; j < FM; ++j) ra[0][j] = fa.read(lds, 0, j);
+        constexpr int ROUND = STAGES % 2 ? 2 * STAGES : STAGES;
+        for (int s = 0; s < stages; s += ROUND) {   // stages behind the last are zeros
+#pragma unroll
+            for (int i = 0; i < ROUND; ++i) stage(i % STAGES, i & 1);
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way to LDS when the workgroup ends
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way to LDS when it is used otherwise
 #pragma unroll
-    for (int i = 0; i < F; ++i) group_mfma_done(acc[i]);
-    group_store<T, ACROSS, F, F>(a, out, rows, m0 + wm, (int64_t)tn * TILE + wn, acc);
+    for (int j = 0; j < FM; ++j) group_mfma_done(acc[j]);
+    // The result through LDS, so that a wave stores long pieces of rows: a lane
+    // writes 4 numbers of a fragment, or 4 FN in a row, and reads 16 bytes of a row.
+    // Pieces change places by the row's number.
+    __syncthreads();
+    const int lane = threadIdx.x & (kWave - 1), l16 = lane & 15, quad = lane >> 4;
+    const auto place = [](int row, int piece) { return row * (TN * 2) + ((piece ^ (row & 15)) * 16); };
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int row = wm + j * 16 + l16;
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            const int n = wn + (ACROSS ? i * 16 + quad * 4 : quad * (4 * FN) + i * 4);
+            *(u32x2*)(lds + place(row, n / 8) + (n & 4) * 2) = u32x2{narrow2<T>(acc[j][i][0], acc[j][i][1]), narrow2<T>(acc[j][i][2], acc[j][i][3])};
+        }
+    }
+    __syncthreads();
+    constexpr int PER = TN / 8;   // pieces of a row
+    const int64_t high = min((int64_t)TM, rows - w.m0), at = (int)threadIdx.x % PER, n = w.n0 + at * 8;
+    T* const to = out + w.m0 * a.n + n;
+#pragma unroll 4
+    for (int r = (int)threadIdx.x / PER; r < high; r += NT / PER) {
+        const u32x4 v = *(const u32x4*)(lds + place(r, at));
+        if (n + 8 <= a.n) store16(to + (int64_t)r * a.n, v);
+        else if (n < a.n) store_part(to + (int64_t)r * a.n, v, (int)(a.n - n));
+    }
+}
+
+// 256 x 256 of 16 bits, one workgroup to a CU: eight waves of 128 x 64 would
+// read 96 KB of LDS a stage, as long as their matrix instructions take; four of
+// 128 x 128 read 64.  What is left behind the last full round of 256 tiles goes
+// in quarters of 128 x 128, if those take less than a round.
+constexpr uint32_t kRound = 256;
+template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(256, 1) void group_large_kernel(GroupArgs a) {
+    constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
+    __shared__ __align__(16) uint8_t lds[4 * 512 * 64];
+    if (blockIdx.x >= a.tiles) {
+        group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
+        return;
+    }
+    const uint32_t high = WEIGHT ? a.tiles_m : group_tiles(a, 256), total = high * a.tiles_n * (WEIGHT ? (uint32_t)a.experts : 1u);
+    uint32_t rest = total % kRound;
+    if (rest > kRound / 2) rest = 0;
+    const uint32_t full = total - rest;
+    if (blockIdx.x < full) {
+        const GroupWork w = group_work<WEIGHT>(a, WEIGHT ? blockIdx.x : group_run(blockIdx.x, full), high, a.tiles_n, 256, 256);
+        group_large_tile<T, WEIGHT, ACROSS, 8, 8, 4>(a, w, lds);
+    } else if (blockIdx.x - full < 4 * rest) {
+        const uint32_t i = blockIdx.x - full;
+        GroupWork w = group_work<WEIGHT>(a, full + i / 4, high, a.tiles_n, 256, 256);
+        w.m0 += (i & 1) * 128;
+        w.n0 += (i & 2) * 64;
+        if (w.n0 >= a.n || w.m0 >= (WEIGHT ? a.m : w.end - w.first)) return;
+        group_large_tile<T, WEIGHT, ACROSS, 4, 4, 8>(a, w, lds);
+    }
 }
 
 // One dtype's kernels, each in a source file of its own.  whole: aligned, whole pieces.
@@ -640,16 +721,16 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, b
 
 #define CRESSO_GROUP_LAUNCH(T)                                                                                          \
     template <> void group_launch<T>(GroupArgs a, bool weight, bool across, bool whole, int tile, hipStream_t st) {     \
-        const auto run = [&](auto kernel, int tm, int tn, int threads) {                                                \
+        const auto run = [&](auto kernel, int tm, int tn, int threads, uint32_t more = 0) {                             \
             a.tiles_n = (uint32_t)((a.n + tn - 1) / tn);                                                                \
             a.tiles_m = (uint32_t)(weight ? (a.m + tm - 1) / tm : a.rows / tm + a.experts);                             \
-            a.tiles = a.tiles_m * a.tiles_n * (weight ? (uint32_t)a.experts : 1u);                                      \
+            a.tiles = a.tiles_m * a.tiles_n * (weight ? (uint32_t)a.experts : 1u) + more;                               \
             hipLaunchKernelGGL(kernel, dim3(a.tiles + (weight ? 0 : kFillBlocks)), dim3(threads), 0, st, a);            \
         };                                                                                                              \
         const auto size = [&](auto w, auto x) {                                                                         \
             constexpr bool W = decltype(w)::value, X = decltype(x)::value;                                              \
             if constexpr (sizeof(T) == 2) {                                                                             \
-                if (whole && tile == 256) return run(group_wide_kernel<T, W, X>, 256, 256, 256);                        \
+                if (whole && tile == 256) return run(group_large_kernel<T, W, X>, 256, 256, 256, 3 * kRound / 2);       \
             }                                                                                                           \
             if (whole && tile >= 128) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128, 128, 256);                    \
             else if (whole) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3>, 64, 64, 256);                                \
