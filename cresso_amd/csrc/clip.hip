@@ -24,22 +24,21 @@ constexpr int CL_NT = 256;
 constexpr int CL_UNITS = 8;                           // 16-byte units a thread holds of a chunk
 constexpr int CL_CHUNK = CL_NT * CL_UNITS * 16;       // bytes
 constexpr int CL_MAX_BLOCKS = 1024;                   // partial sums: each workgroup of the second pass adds them all up
-constexpr int CL_FILL = 160;                          // entries of one fill launch: its arguments stay below 4 KB
+constexpr int CL_FILL = 250;                          // 16-byte entries of one fill launch: its arguments stay below 4 KB
 
-// What a tensor is to the kernels: elements of `in` (and `out`) from chunk
-// `first` on, `tail` of them in its last chunk.
+// What a tensor is to the kernels: its elements from chunk `first` on, `tail` of them in its last chunk.
 struct ClipEntry {
     const void* in;
-    void* out;
     uint32_t first;
-    uint32_t tail_types;   // tail << 4 | in << 2 | out, types as CRESSO_*
+    uint32_t tail_types;   // tail << 5 | written << 4 | type << 2 | type of the output, types as CRESSO_*
 };
-static_assert(sizeof(ClipEntry) == 24 && (CL_CHUNK / 2) < (1 << 28), "entry");
+static_assert(sizeof(ClipEntry) == 16 && (CL_CHUNK / 2) < (1 << 27), "entry");
 struct ClipFill {
-    ClipEntry e[CL_FILL];
+    u32x4 e[CL_FILL];      // entries, or two addresses of outputs each
 };
 struct ClipArgs {
     ClipEntry* table;
+    void** outs;           // of the entries; NULL: each is its own output
     double* partials;
     float* norm;
     uint32_t count, chunks, blocks;
@@ -50,14 +49,11 @@ struct ClipArgs {
 
 int64_t element_bytes(int32_t code) { return code == CRESSO_F64 ? 8 : code == CRESSO_F32 ? 4 : 2; }
 
-// The table, from the arguments of the launch to memory: thread i copies entry i.
-__global__ __launch_bounds__(CL_FILL) void clip_fill_kernel(ClipFill f, ClipEntry* to, uint32_t count) {
+// The table, from the arguments of the launch to memory: thread i copies 16 bytes.
+__global__ __launch_bounds__(CL_FILL) void clip_fill_kernel(ClipFill f, u32x4* to, uint32_t count) {
     // the arguments' own memory, so that the lane's index needs no copy of them
-    const auto* from = (const __attribute__((address_space(4))) ClipEntry*)__builtin_amdgcn_kernarg_segment_ptr();
-    if (threadIdx.x < count) {
-        const ClipEntry e = {from[threadIdx.x].in, from[threadIdx.x].out, from[threadIdx.x].first, from[threadIdx.x].tail_types};
-        to[threadIdx.x] = e;
-    }
+    const auto* from = (const __attribute__((address_space(4))) u32x4*)__builtin_amdgcn_kernarg_segment_ptr();
+    if (threadIdx.x < count) to[threadIdx.x] = from[threadIdx.x];
 }
 
 // Index of the entry that holds `chunk`: how many begin at or before it, less one.
@@ -180,7 +176,7 @@ template <bool MAX> __global__ __launch_bounds__(CL_NT) void clip_norm_kernel(Cl
             end = e + 1 < a.count ? a.table[e + 1].first : a.chunks;
         }
         const char* at = (const char*)t.in + (uint64_t)(c - t.first) * CL_CHUNK;
-        const uint32_t tail = t.tail_types >> 4, type = (t.tail_types >> 2) & 3;
+        const uint32_t tail = t.tail_types >> 5, type = (t.tail_types >> 2) & 3;
         const bool last = c + 1 == end;
         if (type == CRESSO_F32) clip_sum<float>((const float*)at, last ? tail : CL_CHUNK / 4, sum);
         else if (type == CRESSO_BF16) clip_sum<__hip_bfloat16>((const __hip_bfloat16*)at, last ? tail : CL_CHUNK / 2, sum);
@@ -192,10 +188,14 @@ template <bool MAX> __global__ __launch_bounds__(CL_NT) void clip_norm_kernel(Cl
     if (threadIdx.x == 0) a.partials[blockIdx.x] = v;
 }
 
-// E elements from `in` times f, rounded once, to `out`.
-template <typename T, typename O> __device__ __forceinline__ void clip_scale_unit(const T* in, O* out, double f) {
+// The E elements of r times f, rounded once, to `out`; PAST: past the caches.
+template <bool PAST, typename O> __device__ __forceinline__ void clip_store(O* out, u32x4 v) {
+    if constexpr (!PAST) store16(out, v);
+    else if constexpr (sizeof(O) == 4) __builtin_nontemporal_store(v, &((CRESSO_GLOBAL Raw16w*)out)->v);
+    else __builtin_nontemporal_store(v, &((CRESSO_GLOBAL Raw16h*)out)->v);
+}
+template <typename T, typename O, bool PAST> __device__ __forceinline__ void clip_scale_unit(u32x4 r, O* out, double f) {
     constexpr int E = 16 / (int)sizeof(T);
-    const u32x4 r = clip_load(in);
     if constexpr (sizeof(O) == 8) {
         u32x4 w;
 #pragma unroll
@@ -204,7 +204,7 @@ template <typename T, typename O> __device__ __forceinline__ void clip_scale_uni
             w[2 * i] = (uint32_t)v;
             w[2 * i + 1] = (uint32_t)(v >> 32);
         }
-        store16((float*)out, w);
+        clip_store<PAST>((float*)out, w);
     } else {
         constexpr int EO = Unit<O>::n;   // a unit of 16 bytes in is one or two of fp32 out
 #pragma unroll
@@ -212,23 +212,23 @@ template <typename T, typename O> __device__ __forceinline__ void clip_scale_uni
             float v[EO];
 #pragma unroll
             for (int i = 0; i < EO; ++i) v[i] = (float)(clip_value<T>(r, h * EO + i) * f);
-            store16(out + h * EO, narrow<O>(v));
+            clip_store<PAST>(out + h * EO, narrow<O>(v));
         }
     }
 }
-template <typename T, typename O> __device__ __forceinline__ void clip_scale(const T* in, O* out, uint32_t left, double f) {
+template <typename T, typename O, bool PAST = false> __device__ __forceinline__ void clip_scale(const T* in, O* out, uint32_t left, double f) {
     constexpr int E = 16 / (int)sizeof(T);
     if (left == CL_CHUNK / sizeof(T)) {
+        u32x4 r[CL_UNITS];
 #pragma unroll
-        for (int u = 0; u < CL_UNITS; ++u) {
-            const uint32_t at = (uint32_t)(u * CL_NT + threadIdx.x) * E;
-            clip_scale_unit(in + at, out + at, f);
-        }
+        for (int u = 0; u < CL_UNITS; ++u) r[u] = clip_load(in + (uint32_t)(u * CL_NT + threadIdx.x) * E);
+#pragma unroll
+        for (int u = 0; u < CL_UNITS; ++u) clip_scale_unit<T, O, PAST>(r[u], out + (uint32_t)(u * CL_NT + threadIdx.x) * E, f);
         return;
     }
     for (uint32_t u = threadIdx.x * E; u < left; u += CL_NT * E) {
         if (u + E <= left) {
-            clip_scale_unit(in + u, out + u, f);
+            clip_scale_unit<T, O, PAST>(clip_load(in + u), out + u, f);
         } else {
             for (uint32_t i = u; i < left; ++i) {
                 if constexpr (sizeof(T) == 8) out[i] = in[i] * f;
@@ -263,12 +263,13 @@ template <bool MAX> __global__ __launch_bounds__(CL_NT) void clip_scale_kernel(C
             end = t.first;
             t = a.table[--e];
         }
-        if (!t.out || (t.out == t.in && f == 1.0)) continue;
-        const uint32_t tail = t.tail_types >> 4, types = t.tail_types & 15, type = types >> 2;
+        void* const to = a.outs ? a.outs[e] : const_cast<void*>(t.in);
+        if (!(t.tail_types & 16) || (to == t.in && f == 1.0)) continue;
+        const uint32_t tail = t.tail_types >> 5, types = t.tail_types & 15, type = types >> 2;
         const uint32_t size = type == CRESSO_F64 ? 8 : type == CRESSO_F32 ? 4 : 2, out_size = (types & 3) == CRESSO_F64 ? 8 : (types & 3) == CRESSO_F32 ? 4 : 2;
         const uint64_t first = (uint64_t)(c - t.first) * (CL_CHUNK / size);
         const char* in = (const char*)t.in + first * size;
-        char* out = (char*)t.out + first * out_size;
+        char* out = (char*)to + first * out_size;
         const uint32_t left = c + 1 == end ? tail : CL_CHUNK / size;
         if (types == (CRESSO_F32 << 2 | CRESSO_F32)) clip_scale((const float*)in, (float*)out, left, f);
         else if (types == (CRESSO_BF16 << 2 | CRESSO_BF16)) clip_scale((const __hip_bfloat16*)in, (__hip_bfloat16*)out, left, f);
@@ -300,7 +301,8 @@ int32_t check_clip(const cresso_grad_desc* g, int32_t count, uint32_t& entries, 
     chunks = (uint32_t)total;
     return CRESSO_OK;
 }
-size_t table_bytes(uint32_t entries) { return ((size_t)entries * sizeof(ClipEntry) + 15) / 16 * 16; }
+// entries, then their outputs
+size_t clip_bytes(uint32_t entries) { return CL_MAX_BLOCKS * sizeof(double) + (size_t)entries * sizeof(ClipEntry) + ((size_t)entries + 1) / 2 * 16; }
 }  // namespace
 }  // namespace cresso
 
@@ -309,7 +311,7 @@ using namespace cresso;
 extern "C" size_t cresso_clip_workspace_bytes(const cresso_grad_desc* grads, int32_t count) {
     uint32_t entries, chunks;
     if (check_clip(grads, count, entries, chunks) != CRESSO_OK) return 0;
-    return CL_MAX_BLOCKS * sizeof(double) + table_bytes(entries);
+    return clip_bytes(entries);
 }
 
 extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t count, int32_t norm_kind, double max_norm,
@@ -322,7 +324,7 @@ extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t 
     if (!(max_norm >= 0.0)) return fail(CRESSO_E_INVALID, "gradient norm: max_norm must not be negative");
     if (!std::isfinite(grad_scale)) return fail(CRESSO_E_INVALID, "gradient norm: grad_scale must be finite");
     if (!norm) return fail(CRESSO_E_INVALID, "gradient norm: null norm");
-    const size_t need = CL_MAX_BLOCKS * sizeof(double) + table_bytes(entries);
+    const size_t need = clip_bytes(entries);
     if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))
         return fail(CRESSO_E_INVALID, "gradient norm: workspace of %zu bytes at %p, %zu at a multiple of 16 needed", workspace_bytes, workspace, need);
     hipStream_t st = (hipStream_t)stream;
@@ -338,24 +340,42 @@ extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t 
     a.scale = grad_scale;
     a.in_place = 1;
     ClipFill f;
-    uint32_t held = 0, sent = 0, first = 0;
+    uint32_t held = 0;
+    u32x4* to = (u32x4*)a.table;
     const auto flush = [&] {
-        if (held) hipLaunchKernelGGL(clip_fill_kernel, dim3(1), dim3(CL_FILL), 0, st, f, a.table + sent, held);
-        sent += held;
+        if (held) hipLaunchKernelGGL(clip_fill_kernel, dim3(1), dim3(CL_FILL), 0, st, f, to, held);
+        to += held;
         held = 0;
     };
+    uint32_t first = 0;
     for (int32_t i = 0; i < count; ++i) {
         const cresso_grad_desc& g = grads[i];
         if (!g.numel) continue;
         const int64_t per = CL_CHUNK / element_bytes(g.dtype);
         const uint32_t n = (uint32_t)((g.numel + per - 1) / per), tail = (uint32_t)(g.numel - (int64_t)(n - 1) * per);
-        f.e[held++] = {g.grad, g.out, first, tail << 4 | (uint32_t)g.dtype << 2 | (uint32_t)(g.out ? g.out_dtype : 0)};
+        const ClipEntry e = {g.grad, first, tail << 5 | (g.out ? 16u : 0u) | (uint32_t)g.dtype << 2 | (uint32_t)(g.out ? g.out_dtype : 0)};
+        f.e[held++] = __builtin_bit_cast(u32x4, e);
         first += n;
         if (g.out) a.write = 1;
         if (g.out && g.out != g.grad) a.in_place = 0;
         if (held == CL_FILL) flush();
     }
     flush();
+    if (!a.in_place) {
+        a.outs = (void**)to;
+        uint64_t pair[2] = {0, 0};
+        uint32_t half = 0;
+        for (int32_t i = 0; i < count; ++i) {
+            if (!grads[i].numel) continue;
+            pair[half++] = (uint64_t)(uintptr_t)grads[i].out;
+            if (half < 2) continue;
+            f.e[held++] = u32x4{(uint32_t)pair[0], (uint32_t)(pair[0] >> 32), (uint32_t)pair[1], (uint32_t)(pair[1] >> 32)};
+            half = 0;
+            if (held == CL_FILL) flush();
+        }
+        if (half) f.e[held++] = u32x4{(uint32_t)pair[0], (uint32_t)(pair[0] >> 32), 0u, 0u};
+        flush();
+    }
     const auto run = [&](auto norm_kernel, auto scale_kernel) {
         if (a.blocks) hipLaunchKernelGGL(norm_kernel, dim3(a.blocks), dim3(CL_NT), 0, st, a);
         hipLaunchKernelGGL(scale_kernel, dim3(a.write ? std::max(1u, a.blocks) : 1), dim3(CL_NT), 0, st, a);

@@ -5,9 +5,9 @@
 #include <algorithm>
 
 namespace cresso {
-template <> void group_launch<float>(GroupArgs, bool, bool, bool, int, hipStream_t);
-template <> void group_launch<__half>(GroupArgs, bool, bool, bool, int, hipStream_t);
-template <> void group_launch<__hip_bfloat16>(GroupArgs, bool, bool, bool, int, hipStream_t);
+template <> void group_launch<float>(GroupArgs, bool, bool, GroupPlan, hipStream_t);
+template <> void group_launch<__half>(GroupArgs, bool, bool, GroupPlan, hipStream_t);
+template <> void group_launch<__hip_bfloat16>(GroupArgs, bool, bool, GroupPlan, hipStream_t);
 
 namespace {
 int32_t check_group(const char* what, int32_t dtype, int64_t rows, int64_t a, int64_t b, int32_t experts) {
@@ -27,17 +27,56 @@ bool whole_rows(const void* p, int64_t width, int64_t stride, int32_t dtype) {
     const int64_t e = dtype == CRESSO_F32 ? 4 : 8;
     return ((uintptr_t)p & 15) == 0 && width % e == 0 && stride % e == 0 && stride >= width && stride < (int64_t)1 << 21 && width < (int64_t)1 << 21;
 }
+// Which tiles, and whether k is split.
+//
+// A product's time is modelled from its tiles of each side, in us at a depth of
+// 2048 and bf16 (measured from 16 to 16384 rows, 4 to 64 experts): 64 on a side
+// 12 + 0.0245 each, 128 13 + 0.066, 256 0.25 each but 45 at least.  The fastest
+// of 512 x 2048 -> 2048 by 8 experts are 64 (16.8 us, 23.5 and 22.1), of 2000
+// by 32 with 1024 columns 128 (31.8, 26.1, 41.9), of 16384 by 8 256 (215, 151,
+// 129).  fp32 takes 64 for products (2048 x 1024 -> 4096 by 8: 167 us, 193).
+// Weight gradients take the largest that their sides fill (16384 rows by 64 of
+// 2048 x 1024: 328, 214, 172 us).
+//
+// Where the tiles leave CUs idle, k is split as far as parts of 4 stages go.
+GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t experts, int32_t dtype, bool weight, bool whole) {
+    const bool wide = dtype == CRESSO_F32;
+    const int64_t e = std::max(experts, 1);
+    const auto tiles = [&](int64_t t) -> double {
+        const double across = (double)((n + t - 1) / t);
+        return across * (weight ? (double)e * (double)((m + t - 1) / t) : (double)rows / t + 0.5 * (double)std::min(e, rows));
+    };
+    GroupPlan p{64, 1, whole};
+    if (weight) {
+        const int64_t side = std::min(m, n);
+        if (whole && !wide && side >= 512) p.tile = 256;
+        else if (whole && side > 64) p.tile = 128;
+    } else if (!wide) {
+        const double t64 = 12.0 + 0.0245 * tiles(64), t128 = 13.0 + 0.066 * tiles(128), t256 = std::max(45.0, 0.25 * tiles(256));
+        if (t128 < t64) p.tile = 128;
+        if (whole && t256 < std::min(t64, t128)) p.tile = 256;
+    }
+    const int64_t stages = (weight ? rows / e : depth) / (wide ? 32 : 64);
+    if (p.tile < 256) p.splits = (uint32_t)std::min<int64_t>({16, (int64_t)(256.0 / std::max(1.0, tiles(p.tile))), stages / 4});
+    p.splits = std::max(p.splits, 1u);
+    return p;
+}
+size_t group_bytes(const GroupPlan& p, int64_t results) { return p.splits > 1 ? (size_t)p.splits * (size_t)results * 4 : 16; }
 }  // namespace
 }  // namespace cresso
 
 using namespace cresso;
 
 extern "C" size_t cresso_expert_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype) {
-    return check_group("expert product", dtype, rows, cols, depth, experts) == CRESSO_OK ? 16 : 0;
+    if (check_group("expert product", dtype, rows, cols, depth, experts) != CRESSO_OK) return 0;
+    return std::max(group_bytes(group_plan(rows, 0, cols, depth, experts, dtype, false, false), rows * cols),
+                    group_bytes(group_plan(rows, 0, cols, depth, experts, dtype, false, true), rows * cols));
 }
 extern "C" size_t cresso_expert_product_weight_workspace_bytes(int64_t rows, int64_t p_width, int64_t q_width, int32_t experts,
                                                                int32_t dtype) {
-    return check_group("expert product gradient", dtype, rows, p_width, q_width, experts) == CRESSO_OK ? 16 : 0;
+    if (check_group("expert product gradient", dtype, rows, p_width, q_width, experts) != CRESSO_OK) return 0;
+    return std::max(group_bytes(group_plan(rows, p_width, q_width, 0, experts, dtype, true, false), experts * p_width * q_width),
+                    group_bytes(group_plan(rows, p_width, q_width, 0, experts, dtype, true, true), experts * p_width * q_width));
 }
 
 extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int64_t depth,
@@ -68,10 +107,10 @@ extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_
     a.b_stride = w_stride;
     a.b_expert = w_expert_stride;
     a.experts = experts;
-    const int64_t mean = rows / std::max(experts, 1);
-    const int tile = mean >= 512 && cols >= 256 ? 256 : mean >= 64 ? 128 : 64;
+    a.sums = (float*)workspace;
     const bool whole = whole_rows(x, depth, x_stride, dtype) && whole_rows(w, w_cols, w_stride, dtype) && w_expert_stride % (dtype == CRESSO_F32 ? 4 : 8) == 0;
-    with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, false, turned != 0, whole, tile, (hipStream_t)stream); });
+    const GroupPlan plan = group_plan(rows, 0, cols, depth, experts, dtype, false, whole);
+    with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, false, turned != 0, plan, (hipStream_t)stream); });
     return launched(what);
 }
 
@@ -100,8 +139,9 @@ extern "C" int32_t cresso_expert_product_weight(const void* p, int64_t p_stride,
     a.a_stride = p_stride;
     a.b_stride = q_stride;
     a.experts = experts;
-    const int tile = p_width >= 512 && q_width >= 512 ? 256 : p_width > 64 && q_width > 64 ? 128 : 64;
+    a.sums = (float*)workspace;
     const bool whole = whole_rows(p, p_width, p_stride, dtype) && whole_rows(q, q_width, q_stride, dtype);
-    with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, true, true, whole, tile, (hipStream_t)stream); });
+    const GroupPlan plan = group_plan(rows, p_width, q_width, 0, experts, dtype, true, whole);
+    with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, true, true, plan, (hipStream_t)stream); });
     return launched(what);
 }

@@ -19,6 +19,7 @@
 
 #include "row_ops.hpp"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace cresso {
@@ -33,6 +34,9 @@ struct GroupArgs {
     int32_t experts;
     uint32_t tiles_m, tiles_n;             // product: tiles_m is the most there can be
     uint32_t tiles;                        // workgroups of tiles; those behind them fill rows without an expert
+    // where k is split: parts of it, each with workgroups for all tiles, and their sums [splits][result] in fp32
+    uint32_t splits;
+    float* sums;
 };
 
 constexpr int kFillBlocks = 64;
@@ -410,11 +414,20 @@ __device__ __forceinline__ void group_operands(const GroupArgs& a, const GroupWo
 }
 // What a workgroup of a kernel with one size of tiles does.  false: nothing.
 template <bool WEIGHT> __device__ __forceinline__ bool group_begin(const GroupArgs& a, int TM, int TN, GroupWork& w) {
-    const uint32_t high = WEIGHT ? a.tiles_m : group_tiles(a, TM), total = high * a.tiles_n;
-    const uint32_t t = WEIGHT ? blockIdx.x : group_run(blockIdx.x, total);
+    const uint32_t high = WEIGHT ? a.tiles_m : group_tiles(a, TM), total = high * a.tiles_n, block = blockIdx.x % a.tiles;
+    const uint32_t t = WEIGHT ? block : group_run(block, total);
     if (!WEIGHT && t >= total) return false;
     w = group_work<WEIGHT>(a, t, high, a.tiles_n, TM, TN);
     return true;
+}
+// The workgroup's part of k, where it is split: whole stages of KS.
+template <bool WEIGHT, bool ACROSS, int KS, typename A, typename B> __device__ __forceinline__ void group_part(const GroupArgs& a, A& oa, B& ob) {
+    if (a.splits < 2) return;
+    const int64_t part = blockIdx.x / a.tiles, stages = (oa.depth + KS - 1) / KS;
+    const int64_t k0 = stages * part / a.splits * KS, k1 = min(stages * (part + 1) / a.splits * KS, oa.depth);
+    oa.base += WEIGHT ? k0 * oa.stride : k0;
+    ob.base += ACROSS ? k0 * ob.stride : k0;
+    oa.depth = ob.depth = max(k1 - k0, (int64_t)0);
 }
 // A lane holds columns 4 quad to 4 quad + 3 of each fragment's 16, or with B
 // along k 4 FN columns in one piece, of rows l16 of each of FM fragments from m on.
@@ -452,6 +465,42 @@ __device__ __forceinline__ void group_store(const GroupArgs& a, T* out, int64_t 
     }
 }
 
+template <typename T, bool WEIGHT, bool ACROSS, int FM, int FN>
+__device__ __forceinline__ void group_result(const GroupArgs& a, T* out, int64_t rows, int64_t m0, int64_t n0, const f32x4 (&acc)[FN][FM]) {
+    if (a.splits < 2) return group_store<T, ACROSS, FM, FN>(a, out, rows, m0, n0, acc);
+    const int64_t all = (WEIGHT ? (int64_t)a.experts * a.m : a.rows) * a.n;
+    group_store<float, ACROSS, FM, FN>(a, a.sums + (blockIdx.x / a.tiles) * all + (out - (T*)a.out), rows, m0, n0, acc);
+}
+// The parts' sums, in their order; rows that are no expert's are zeros.  A unit of the result a thread.
+template <typename T, bool WEIGHT> __global__ __launch_bounds__(256) void group_join_kernel(GroupArgs a) {
+    constexpr int E = Unit<T>::n;
+    const int64_t all = (WEIGHT ? (int64_t)a.experts * a.m : a.rows) * a.n;
+    int64_t begin = 0, end = all;
+    if constexpr (!WEIGHT) {
+        begin = min(max((int64_t)a.offsets[0], (int64_t)0), a.rows) * a.n;
+        end = min(max((int64_t)a.offsets[a.experts], (int64_t)0), a.rows) * a.n;
+    }
+    const int64_t units = (all + E - 1) / E;
+    for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < units; u += (int64_t)gridDim.x * 256) {
+        float sum[E] = {};
+        for (uint32_t p = 0; p < a.splits; ++p) {
+            const float* from = a.sums + p * all;
+#pragma unroll
+            for (int i = 0; i < E / 4; ++i) {
+                const f32x4 v = __builtin_bit_cast(f32x4, load_unit(from, u * (E / 4) + i, all));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[4 * i + e] += v[e];
+            }
+        }
+        if constexpr (!WEIGHT) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (u * E + e < begin || u * E + e >= end) sum[e] = 0.0f;
+        }
+        store_unit((T*)a.out, u, all, narrow<T>(sum));
+    }
+}
+
 // WM x WN waves of FM x FN fragments of 16 x 16 each; operands of any alignment, through registers.
 template <typename T, bool WEIGHT, bool B_ACROSS, int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void group_any_kernel(GroupArgs a) {
@@ -459,7 +508,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_any_kernel(GroupArgs a) 
     constexpr int KS = ROW / (int)sizeof(T), STAGE = (TM + TN) * ROW;
     constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
     __shared__ __align__(16) uint8_t lds[2 * STAGE];
-    if (blockIdx.x >= a.tiles) {
+    if (blockIdx.x >= a.tiles * a.splits) {
         group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
         return;
     }
@@ -470,6 +519,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_any_kernel(GroupArgs a) 
     T* out;
     int64_t rows;
     group_operands<T, WEIGHT, ACROSS>(a, w, oa, ob, out, rows);
+    group_part<WEIGHT, ACROSS, KS>(a, oa, ob);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wm = (wave % WM) * (FM * 16), wn = (wave / WM) * (FN * 16);
     Fragments<T, WEIGHT, ROW, TM, 0> fa;
@@ -509,7 +559,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_any_kernel(GroupArgs a) 
             ob.store(next + TM * ROW);
         }
     }
-    group_store<T, ACROSS, FM, FN>(a, out, rows, w.m0 + wm, w.n0 + wn, acc);
+    group_result<T, WEIGHT, ACROSS, FM, FN>(a, out, rows, w.m0 + wm, w.n0 + wn, acc);
 }
 
 // Waits until at most N of the wave's loads are on their way and all its LDS
@@ -528,7 +578,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
     constexpr int KS = ROW / (int)sizeof(T), STAGE = (TM + TN) * ROW;
     constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
     __shared__ __align__(16) uint8_t lds[STAGES * STAGE];
-    if (blockIdx.x >= a.tiles) {
+    if (blockIdx.x >= a.tiles * a.splits) {
         group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
         return;
     }
@@ -542,6 +592,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
     T* out;
     int64_t rows;
     group_operands<T, WEIGHT, ACROSS>(a, w, oa, ob, out, rows);
+    group_part<WEIGHT, ACROSS, KS>(a, oa, ob);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wm = (wave % WM) * (FM * 16), wn = (wave / WM) * (FN * 16);
     Fragments<T, WEIGHT, ROW, TM, 0> fa;
@@ -583,7 +634,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
         from = from == (STAGES - 1) * STAGE ? 0 : from + STAGE;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way to LDS when the workgroup ends
-    group_store<T, ACROSS, FM, FN>(a, out, rows, w.m0 + wm, w.n0 + wn, acc);
+    group_result<T, WEIGHT, ACROSS, FM, FN>(a, out, rows, w.m0 + wm, w.n0 + wn, acc);
 }
 
 // A tile of 32 FM x 32 FN of 16 bits by four waves of 16 FM x 16 FN, one to a
@@ -716,26 +767,38 @@ template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(2
     }
 }
 
-// One dtype's kernels, each in a source file of its own.  whole: aligned, whole pieces.
-template <typename T> void group_launch(GroupArgs a, bool weight, bool across, bool whole, int tile, hipStream_t st);
+// How a product is computed: the side of its tiles, and into how many parts k is split.
+struct GroupPlan {
+    int tile;
+    uint32_t splits;
+    bool whole;   // aligned, whole pieces
+};
+// One dtype's kernels, each in a source file of its own.
+template <typename T> void group_launch(GroupArgs a, bool weight, bool across, GroupPlan plan, hipStream_t st);
 
 #define CRESSO_GROUP_LAUNCH(T)                                                                                          \
-    template <> void group_launch<T>(GroupArgs a, bool weight, bool across, bool whole, int tile, hipStream_t st) {     \
-        const auto run = [&](auto kernel, int tm, int tn, int threads, uint32_t more = 0) {                             \
-            a.tiles_n = (uint32_t)((a.n + tn - 1) / tn);                                                                \
-            a.tiles_m = (uint32_t)(weight ? (a.m + tm - 1) / tm : a.rows / tm + a.experts);                             \
+    template <> void group_launch<T>(GroupArgs a, bool weight, bool across, GroupPlan plan, hipStream_t st) {           \
+        const auto run = [&](auto kernel, int tile, uint32_t more = 0) {                                                \
+            a.tiles_n = (uint32_t)((a.n + tile - 1) / tile);                                                            \
+            a.tiles_m = (uint32_t)(weight ? (a.m + tile - 1) / tile : a.rows / tile + a.experts);                       \
             a.tiles = a.tiles_m * a.tiles_n * (weight ? (uint32_t)a.experts : 1u) + more;                               \
-            hipLaunchKernelGGL(kernel, dim3(a.tiles + (weight ? 0 : kFillBlocks)), dim3(threads), 0, st, a);            \
+            a.splits = plan.splits;                                                                                     \
+            hipLaunchKernelGGL(kernel, dim3(a.tiles * a.splits + (weight || a.splits > 1 ? 0 : kFillBlocks)),           \
+                               dim3(256), 0, st, a);                                                                    \
         };                                                                                                              \
         const auto size = [&](auto w, auto x) {                                                                         \
             constexpr bool W = decltype(w)::value, X = decltype(x)::value;                                              \
             if constexpr (sizeof(T) == 2) {                                                                             \
-                if (whole && tile == 256) return run(group_large_kernel<T, W, X>, 256, 256, 256, 3 * kRound / 2);       \
+                if (plan.whole && plan.tile == 256) return run(group_large_kernel<T, W, X>, 256, 3 * kRound / 2);       \
             }                                                                                                           \
-            if (whole && tile >= 128) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128, 128, 256);                    \
-            else if (whole) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3>, 64, 64, 256);                                \
-            else if (tile >= 128) run(group_any_kernel<T, W, X, 1, 4, 8, 2>, 128, 128, 256);                            \
-            else run(group_any_kernel<T, W, X, 1, 4, 4, 1>, 64, 64, 256);                                               \
+            if (plan.whole && plan.tile >= 128) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128);                    \
+            else if (plan.whole) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3>, 64);                                    \
+            else if (plan.tile >= 128) run(group_any_kernel<T, W, X, 1, 4, 8, 2>, 128);                                 \
+            else run(group_any_kernel<T, W, X, 1, 4, 4, 1>, 64);                                                        \
+            if (a.splits < 2) return;                                                                                   \
+            const int64_t units = ((W ? (int64_t)a.experts * a.m : a.rows) * a.n + Unit<T>::n - 1) / Unit<T>::n;        \
+            hipLaunchKernelGGL((group_join_kernel<T, W>), dim3((uint32_t)std::min<int64_t>((units + 255) / 256, 4096)), \
+                               dim3(256), 0, st, a);                                                                    \
         };                                                                                                              \
         if (weight) size(std::true_type{}, std::true_type{});                                                           \
         else if (across) size(std::false_type{}, std::true_type{});                                                     \

@@ -670,8 +670,19 @@ bool shares(std::vector<Written>& spans) {
     }
     return false;
 }
-Tensor clip(const char* what, const std::vector<optional<Tensor>>& grads, double max_norm, int64_t kind, double grad_scale,
-            const std::vector<optional<Tensor>>* out, bool in_place) {
+// The tensors of a Python list, None among them, where they are: a program has
+// hundreds, and a vector of counted references takes longer than the kernels.
+struct Listed {
+    PyObject* list;
+    size_t size() const { return (size_t)PyList_GET_SIZE(list); }
+    const Tensor* at(size_t i) const {
+        PyObject* o = PyList_GET_ITEM(list, i);
+        if (o == Py_None) return nullptr;
+        if (!THPVariable_Check(o)) throw pybind11::type_error("not a tensor");
+        return &THPVariable_Unpack(o);
+    }
+};
+Tensor clip(const char* what, const Listed& grads, double max_norm, int64_t kind, double grad_scale, const Listed* out, bool in_place) {
     const at::NoGradGuard no_grad;
     TORCH_CHECK_VALUE(max_norm >= 0.0, what, ": max_norm must not be negative");
     TORCH_CHECK_VALUE(std::isfinite(grad_scale), what, ": grad_scale must be finite");
@@ -680,65 +691,70 @@ Tensor clip(const char* what, const std::vector<optional<Tensor>>& grads, double
     std::vector<cresso_grad_desc> descs;
     std::vector<Written> spans;
     std::vector<Tensor> keep;                             // copies
-    std::vector<std::pair<Tensor, Tensor>> back;          // written in a copy: where it goes
+    std::vector<std::pair<const Tensor*, Tensor>> back;   // written in a copy: where it goes
     descs.reserve(grads.size());
-    spans.reserve(out ? 2 * grads.size() : grads.size());
+    if (out || in_place) spans.reserve(out ? 2 * grads.size() : grads.size());
     const Tensor* first = nullptr;
-    const auto span = [&](const Tensor& t, bool written) {
-        const uintptr_t at = (uintptr_t)t.const_data_ptr();
+    const auto span = [&](const Tensor& t, uintptr_t at, bool dense, bool written) {
         int64_t reach = 1;   // elements from the first to the last
-        for (int64_t d = 0; d < t.dim(); ++d) reach += (t.size(d) - 1) * t.stride(d);
-        spans.push_back({at, at + (uintptr_t)(reach * (int64_t)t.element_size()), written});
+        if (dense) reach = t.numel();
+        else
+            for (int64_t d = 0; d < t.dim(); ++d) reach += (t.size(d) - 1) * t.stride(d);
+        const uintptr_t end = at + (uintptr_t)(reach * (int64_t)t.element_size());
+        if (!spans.empty() && spans.back().end == at && spans.back().out == written) spans.back().end = end;   // buckets hold them so
+        else spans.push_back({at, end, written});
     };
     for (size_t i = 0; i < grads.size(); ++i) {
-        if (!grads[i].has_value()) continue;
-        const Tensor& g = *grads[i];
+        const Tensor* const given = grads.at(i);
+        if (!given) continue;
+        const Tensor& g = *given;
         TORCH_CHECK_VALUE(g.layout() == at::kStrided, what, ": gradient ", i, " is sparse");
         gpu.add("a gradient", g);
         const int32_t code = code_of(g.scalar_type());
         TORCH_CHECK_VALUE(code >= 0, what, ": gradient ", i, " must be fp32, fp64, bf16 or fp16, not ", name_of(g.scalar_type()));
         if (!first) first = &g;
-        Tensor to;
+        const Tensor* to = in_place ? &g : nullptr;
         if (out) {
-            TORCH_CHECK_VALUE((*out)[i].has_value(), what, ": no output for gradient ", i);
-            to = *(*out)[i];
-            gpu.add("an output", to);
-            TORCH_CHECK_VALUE(to.layout() == at::kStrided && to.sizes() == g.sizes() &&
-                                  (to.scalar_type() == g.scalar_type() || (to.scalar_type() == at::kFloat && g.element_size() == 2)),
-                              what, ": output ", i, " is ", name_of(to.scalar_type()), " ", to.sizes(), " for a gradient of ",
+            to = out->at(i);
+            TORCH_CHECK_VALUE(to, what, ": no output for gradient ", i);
+            TORCH_CHECK_VALUE(to->layout() == at::kStrided && to->sizes() == g.sizes() &&
+                                  (to->scalar_type() == g.scalar_type() || (to->scalar_type() == at::kFloat && g.element_size() == 2)),
+                              what, ": output ", i, " is ", name_of(to->scalar_type()), " ", to->sizes(), " for a gradient of ",
                               name_of(g.scalar_type()), " ", g.sizes(), " (its own type or, of 16 bits, fp32)");
-        } else if (in_place) {
-            to = g;
+            gpu.add("an output", *to);
         }
-        if (!g.numel()) continue;
+        const int64_t numel = g.numel();
+        if (!numel) continue;
         cresso_grad_desc d{};
-        d.numel = g.numel();
+        d.numel = numel;
         d.dtype = code;
-        const bool same = to.defined() && to.const_data_ptr() == g.const_data_ptr() && to.scalar_type() == g.scalar_type() &&
-                          to.strides() == g.strides();
-        if (to.defined()) {
-            TORCH_CHECK_VALUE(to.is_non_overlapping_and_dense() || at::has_internal_overlap(to) != at::MemOverlap::Yes, what,
-                              ": output ", i, " holds several elements in one place");
-            span(to, true);
+        d.grad = g.const_data_ptr();
+        const bool dense = g.is_non_overlapping_and_dense();
+        const bool same = to == &g || (to && to->const_data_ptr() == d.grad && to->scalar_type() == g.scalar_type() && to->strides() == g.strides());
+        bool to_dense = dense;
+        if (to) {
+            if (!same) to_dense = to->is_non_overlapping_and_dense();
+            TORCH_CHECK_VALUE(to_dense || at::has_internal_overlap(*to) != at::MemOverlap::Yes, what, ": output ", i,
+                              " holds several elements in one place");
+            span(*to, (uintptr_t)(same ? d.grad : to->const_data_ptr()), to_dense, true);
         }
-        if (!same) span(g, false);
-        Tensor from = g;
-        if (!g.is_non_overlapping_and_dense()) {   // any order of the elements serves a norm, gaps do not
-            from = g.contiguous();
-            keep.push_back(from);
+        if (!same && out) span(g, (uintptr_t)d.grad, dense, false);
+        const Tensor* from = &g;
+        if (!dense) {   // any order of the elements serves a norm, gaps do not
+            keep.push_back(g.contiguous());
+            d.grad = keep.back().const_data_ptr();
         }
-        d.grad = from.const_data_ptr();
-        if (to.defined()) {
-            d.out_dtype = code_of(to.scalar_type());
+        if (to) {
+            d.out_dtype = code_of(to->scalar_type());
             if (same) {
                 d.out = const_cast<void*>(d.grad);
-                if (!from.is_same(g)) back.emplace_back(to, from);
-            } else if (to.is_non_overlapping_and_dense() && to.strides() == from.strides()) {
-                d.out = to.mutable_data_ptr();
+                if (!dense) back.emplace_back(to, keep.back());
+            } else if (dense && to_dense && to->strides() == from->strides()) {
+                d.out = to->mutable_data_ptr();
             } else {
-                const Tensor t = at::empty_strided(from.sizes(), from.strides(), to.options());
-                d.out = t.mutable_data_ptr();
-                back.emplace_back(to, t);
+                const Tensor rows = dense ? at::empty_strided(g.sizes(), g.strides(), to->options()) : at::empty(g.sizes(), to->options());
+                d.out = rows.mutable_data_ptr();
+                back.emplace_back(to, rows);
             }
         }
         descs.push_back(d);
@@ -753,20 +769,21 @@ Tensor clip(const char* what, const std::vector<optional<Tensor>>& grads, double
     done(g_api.clip_gradients(descs.data(), (int32_t)descs.size(), (int32_t)kind, max_norm, grad_scale, (float*)norm.mutable_data_ptr(),
                               ws.mutable_data_ptr(), bytes, stream_of(*first)),
          what);
-    for (auto& [to, from] : back) to.copy_(from);
+    for (auto& [to, from] : back) to->copy_(from);
     // written behind torch's back: what has saved them for its own gradient has to notice
-    const std::vector<optional<Tensor>>* written = out ? out : in_place ? &grads : nullptr;
-    if (written)
-        for (const auto& t : *written)
-            if (t.has_value() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    const Listed* written = out ? out : in_place ? &grads : nullptr;
+    for (size_t i = 0; written && i < written->size(); ++i) {
+        const Tensor* t = written->at(i);
+        if (t && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    }
     return norm;
 }
-Tensor gradient_norm(const std::vector<optional<Tensor>>& grads, int64_t kind) {
-    return clip("gradient_norm", grads, INFINITY, kind, 1.0, nullptr, false);
+Tensor gradient_norm(const pybind11::list& grads, int64_t kind) {
+    return clip("gradient_norm", {grads.ptr()}, INFINITY, kind, 1.0, nullptr, false);
 }
-Tensor clip_gradients(const std::vector<optional<Tensor>>& grads, double max_norm, int64_t kind, double grad_scale,
-                      const optional<std::vector<optional<Tensor>>>& out) {
-    return clip("clip_gradients", grads, max_norm, kind, grad_scale, out.has_value() ? &*out : nullptr, !out.has_value());
+Tensor clip_gradients(const pybind11::list& grads, double max_norm, int64_t kind, double grad_scale, const optional<pybind11::list>& out) {
+    const Listed to{out.has_value() ? out->ptr() : nullptr};
+    return clip("clip_gradients", {grads.ptr()}, max_norm, kind, grad_scale, out.has_value() ? &to : nullptr, !out.has_value());
 }
 
 // ---------------------------------------------------------------------------
@@ -1077,8 +1094,8 @@ PYBIND11_MODULE(_operators, m) {
     m.def("distill_loss_and_grad", &distill_loss_and_grad, free);
     m.def("block_product", &block_product, free);
     m.def("quantize_blocks", &quantize_blocks, free);
-    m.def("gradient_norm", &gradient_norm, free);
-    m.def("clip_gradients", &clip_gradients, free);
+    m.def("gradient_norm", &gradient_norm);   // these two read Python lists
+    m.def("clip_gradients", &clip_gradients);
     m.def("route_experts", &route_experts, free);
     m.def("dispatch_rows", &dispatch_rows, free);
     m.def("combine_rows", &combine_rows, free);
