@@ -360,9 +360,8 @@ extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t 
         if (g.out && g.out != g.grad) a.in_place = 0;
         if (held == CL_FILL) flush();
     }
-    flush();
-    if (!a.in_place) {
-        a.outs = (void**)to;
+    if (!a.in_place) {   // behind the entries
+        a.outs = (void**)(a.table + entries);
         uint64_t pair[2] = {0, 0};
         uint32_t half = 0;
         for (int32_t i = 0; i < count; ++i) {
@@ -374,8 +373,8 @@ extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t 
             if (held == CL_FILL) flush();
         }
         if (half) f.e[held++] = u32x4{(uint32_t)pair[0], (uint32_t)(pair[0] >> 32), 0u, 0u};
-        flush();
     }
+    flush();
     const auto run = [&](auto norm_kernel, auto scale_kernel) {
         if (a.blocks) hipLaunchKernelGGL(norm_kernel, dim3(a.blocks), dim3(CL_NT), 0, st, a);
         hipLaunchKernelGGL(scale_kernel, dim3(a.write ? std::max(1u, a.blocks) : 1), dim3(CL_NT), 0, st, a);

@@ -34,12 +34,14 @@ bool whole_rows(const void* p, int64_t width, int64_t stride, int32_t dtype) {
 // 12 + 0.0245 each, 128 13 + 0.066, 256 0.25 each but 45 at least.  The fastest
 // of 512 x 2048 -> 2048 by 8 experts are 64 (16.8 us, 23.5 and 22.1), of 2000
 // by 32 with 1024 columns 128 (31.8, 26.1, 41.9), of 16384 by 8 256 (215, 151,
-// 129).  fp32 takes 64 for products (2048 x 1024 -> 4096 by 8: 167 us, 193).
-// Weight gradients take the largest that their sides fill (16384 rows by 64 of
-// 2048 x 1024: 328, 214, 172 us).
+// 129).  With w across k, tiles of 128 take 12 + 0.075 and those of 64 are no
+// faster anywhere.  fp32 takes 64 (2048 x 1024 -> 4096 by 8: 167 us, 193).
+// Weight gradients take 256 from three rounds of them on, if they have rows
+// enough to be more than a store (16384 rows by 64 experts of 2048 x 1024: 173 us,
+// 196 with 128; 2000 by 32: 59 and 53; 8192 by 8 of 2048 x 2048: 75 and 72).
 //
 // Where the tiles leave CUs idle, k is split as far as parts of 4 stages go.
-GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t experts, int32_t dtype, bool weight, bool whole) {
+GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t experts, int32_t dtype, bool weight, bool across, bool whole) {
     const bool wide = dtype == CRESSO_F32;
     const int64_t e = std::max(experts, 1);
     const auto tiles = [&](int64_t t) -> double {
@@ -49,10 +51,12 @@ GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t 
     GroupPlan p{64, 1, whole};
     if (weight) {
         const int64_t side = std::min(m, n);
-        if (whole && !wide && side >= 512) p.tile = 256;
+        if (whole && !wide && side >= 256 && tiles(256) >= 768.0 && rows >= 128 * e) p.tile = 256;
         else if (whole && side > 64) p.tile = 128;
     } else if (!wide) {
-        const double t64 = 12.0 + 0.0245 * tiles(64), t128 = 13.0 + 0.066 * tiles(128), t256 = std::max(45.0, 0.25 * tiles(256));
+        const bool turn = across && whole;
+        const double t64 = turn ? 1e30 : 12.0 + 0.0245 * tiles(64), t128 = turn ? 12.0 + 0.075 * tiles(128) : 13.0 + 0.066 * tiles(128);
+        const double t256 = std::max(45.0, 0.25 * tiles(256));
         if (t128 < t64) p.tile = 128;
         if (whole && t256 < std::min(t64, t128)) p.tile = 256;
     }
@@ -69,14 +73,15 @@ using namespace cresso;
 
 extern "C" size_t cresso_expert_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype) {
     if (check_group("expert product", dtype, rows, cols, depth, experts) != CRESSO_OK) return 0;
-    return std::max(group_bytes(group_plan(rows, 0, cols, depth, experts, dtype, false, false), rows * cols),
-                    group_bytes(group_plan(rows, 0, cols, depth, experts, dtype, false, true), rows * cols));
+    size_t most = 0;
+    for (int i = 0; i < 4; ++i) most = std::max(most, group_bytes(group_plan(rows, 0, cols, depth, experts, dtype, false, i & 1, i & 2), rows * cols));
+    return most;
 }
 extern "C" size_t cresso_expert_product_weight_workspace_bytes(int64_t rows, int64_t p_width, int64_t q_width, int32_t experts,
                                                                int32_t dtype) {
     if (check_group("expert product gradient", dtype, rows, p_width, q_width, experts) != CRESSO_OK) return 0;
-    return std::max(group_bytes(group_plan(rows, p_width, q_width, 0, experts, dtype, true, false), experts * p_width * q_width),
-                    group_bytes(group_plan(rows, p_width, q_width, 0, experts, dtype, true, true), experts * p_width * q_width));
+    return std::max(group_bytes(group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, false), experts * p_width * q_width),
+                    group_bytes(group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, true), experts * p_width * q_width));
 }
 
 extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int64_t depth,
@@ -109,7 +114,7 @@ extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_
     a.experts = experts;
     a.sums = (float*)workspace;
     const bool whole = whole_rows(x, depth, x_stride, dtype) && whole_rows(w, w_cols, w_stride, dtype) && w_expert_stride % (dtype == CRESSO_F32 ? 4 : 8) == 0;
-    const GroupPlan plan = group_plan(rows, 0, cols, depth, experts, dtype, false, whole);
+    const GroupPlan plan = group_plan(rows, 0, cols, depth, experts, dtype, false, turned != 0, whole);
     with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, false, turned != 0, plan, (hipStream_t)stream); });
     return launched(what);
 }
@@ -141,7 +146,7 @@ extern "C" int32_t cresso_expert_product_weight(const void* p, int64_t p_stride,
     a.experts = experts;
     a.sums = (float*)workspace;
     const bool whole = whole_rows(p, p_width, p_stride, dtype) && whole_rows(q, q_width, q_stride, dtype);
-    const GroupPlan plan = group_plan(rows, p_width, q_width, 0, experts, dtype, true, whole);
+    const GroupPlan plan = group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, whole);
     with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, true, true, plan, (hipStream_t)stream); });
     return launched(what);
 }

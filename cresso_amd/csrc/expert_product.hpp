@@ -676,7 +676,7 @@ __device__ __forceinline__ void group_large_tile(const GroupArgs& a, const Group
     const auto stage = [&](int now, int set) {
         group_ready<(STAGES - 2) * LOADS>();
         const uint8_t* const then = lds + (now + 1) % STAGES * STAGE;
-        constexpr int EVERY = STEPS * 3 / 4 / (FM + FN), APART = STEPS / LOADS;
+        constexpr int EVERY = STEPS * 3 / 4 / (FM + FN) > 0 ? STEPS * 3 / 4 / (FM + FN) : 1, APART = STEPS / LOADS;
 #pragma unroll
         for (int t = 0; t < STEPS; ++t) {
             group_mfma_into<T>(rb[set][t % FN], ra[set][t / FN], acc[t / FN][t % FN]);
@@ -703,9 +703,13 @@ __device__ __forceinline__ void group_large_tile(const GroupArgs& a, const Group
 #pragma unroll
         for (int j = 0; j < FM; ++j) ra[0][j] = fa.read(lds, 0, j);
         constexpr int ROUND = STAGES % 2 ? 2 * STAGES : STAGES;
-        for (int s = 0; s < stages; s += ROUND) {   // stages behind the last are zeros
+        for (int s = 0; s < stages; s += ROUND) {
 #pragma unroll
-            for (int i = 0; i < ROUND; ++i) stage(i % STAGES, i & 1);
+            for (int i = 0; i < ROUND; ++i) {
+                // 256 sums leave no registers for several ways out: there, stages behind the last are multiplied, as zeros
+                if (FM * FN < 64 && s + i >= stages) break;
+                stage(i % STAGES, i & 1);
+            }
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way to LDS when it is used otherwise
@@ -716,7 +720,7 @@ __device__ __forceinline__ void group_large_tile(const GroupArgs& a, const Group
     // Pieces change places by the row's number.
     __syncthreads();
     const int lane = threadIdx.x & (kWave - 1), l16 = lane & 15, quad = lane >> 4;
-    const auto place = [](int row, int piece) { return row * (TN * 2) + ((piece ^ (row & 15)) * 16); };
+    const auto place = [](int row, int piece) { return row * (TN * 2) + ((piece ^ (row & (TN / 8 < 16 ? TN / 8 - 1 : 15))) * 16); };
 #pragma unroll
     for (int j = 0; j < FM; ++j) {
         const int row = wm + j * 16 + l16;
@@ -767,6 +771,20 @@ template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(2
     }
 }
 
+// Smaller tiles of 16 bits in the same manner, several workgroups to a CU, for a
+// B across k (weight gradients of 16 rows by 16 experts of 2048 x 5632: 104 us, with
+// group_kernel 133; the gradient of x 46 and 68).  Along k group_kernel's
+// rows of 128 bytes are better than these of 64 (16 x 2048 -> 5632 by 16: 46 us, 49).
+template <typename T, bool WEIGHT, bool B_ACROSS, int F, int STAGES, int BLOCKS> __global__ __launch_bounds__(256, BLOCKS) void group_small_kernel(GroupArgs a) {
+    __shared__ __align__(16) uint8_t lds[STAGES * 64 * F * 64];
+    if (blockIdx.x >= a.tiles) {
+        group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
+        return;
+    }
+    GroupWork w;
+    if (group_begin<WEIGHT>(a, 32 * F, 32 * F, w)) group_large_tile<T, WEIGHT, WEIGHT || B_ACROSS, F, F, STAGES>(a, w, lds);
+}
+
 // How a product is computed: the side of its tiles, and into how many parts k is split.
 struct GroupPlan {
     int tile;
@@ -790,6 +808,10 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, G
             constexpr bool W = decltype(w)::value, X = decltype(x)::value;                                              \
             if constexpr (sizeof(T) == 2) {                                                                             \
                 if (plan.whole && plan.tile == 256) return run(group_large_kernel<T, W, X>, 256, 3 * kRound / 2);       \
+                if constexpr (X)                                                                                        \
+                    if (plan.whole && plan.tile == 128 && plan.splits < 2) return run(group_small_kernel<T, W, X, 4, 4, 2>, 128); \
+                if constexpr (W)                                                                                        \
+                    if (plan.whole && plan.tile == 64 && plan.splits < 2) return run(group_small_kernel<T, W, X, 2, 4, 4>, 64); \
             }                                                                                                           \
             if (plan.whole && plan.tile >= 128) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128);                    \
             else if (plan.whole) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3>, 64);                                    \

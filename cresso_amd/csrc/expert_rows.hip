@@ -64,7 +64,7 @@ template <typename T> __global__ __launch_bounds__(ER_NT) void combine_kernel(Ro
     int lane;
     const int64_t token = token_of(a, lane);
     if (token >= a.tokens) return;
-    constexpr int E = Unit<T>::n, U = 2;
+    constexpr int E = Unit<T>::n, U = 4;
     const int64_t units = (a.width + E - 1) / E;
     for (int64_t u0 = lane; u0 < units; u0 += (int64_t)a.lanes * U) {
         float sum[U][E] = {};
