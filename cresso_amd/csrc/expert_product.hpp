@@ -271,52 +271,55 @@ __device__ __forceinline__ void group_rows(const GroupArgs& a, int e, int64_t& f
     first = min(max((int64_t)a.offsets[e], (int64_t)0), a.rows);
     end = min(max((int64_t)a.offsets[e + 1], first), a.rows);
 }
-struct GroupTile {
-    int expert;
-    int64_t first, rows;   // the tile's rows among all
-};
-// Tiles of m rows there are, over all experts.  By each wave.
-__device__ __forceinline__ uint32_t group_tiles(const GroupArgs& a, int tile) {
-    const int lane = threadIdx.x & (kWave - 1);
-    uint32_t n = 0;
-    for (int e = lane; e < a.experts; e += kWave) {
-        int64_t first, end;
-        group_rows(a, e, first, end);
-        n += (uint32_t)((end - first + tile - 1) / tile);
-    }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) n += __shfl_xor(n, d, kWave);
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)n);
+// Sums over the lanes up to each, by row operations of the vector unit.
+template <int CTRL, int ROW_MASK> __device__ __forceinline__ uint32_t group_add(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROW_MASK, 0xF, false);
 }
-// Tile t of m, of those.  By each wave.
-__device__ __forceinline__ GroupTile group_tile(const GroupArgs& a, int tile, uint32_t t) {
-    const int lane = threadIdx.x & (kWave - 1);
-    uint32_t before = 0;
-    GroupTile g{0, 0, 0};
-    for (int e0 = 0; e0 < a.experts; e0 += kWave) {
-        int64_t first = 0, end = 0;
+__device__ __forceinline__ uint32_t group_upto(uint32_t v) {
+    v = group_add<0x111, 0xF>(v);   // row_shr:1
+    v = group_add<0x112, 0xF>(v);   // row_shr:2
+    v = group_add<0x114, 0xF>(v);   // row_shr:4
+    v = group_add<0x118, 0xF>(v);   // row_shr:8
+    v = group_add<0x142, 0xA>(v);   // row_bcast:15 -> rows 1, 3
+    return group_add<0x143, 0xC>(v);   // row_bcast:31 -> rows 2, 3
+}
+// The tiles of m rows of all experts, 64 experts at a time, one a lane.  By each wave.
+struct GroupTiles {
+    int64_t first, end;     // the lane's expert's rows
+    uint32_t count, upto;   // its tiles, and those of the experts up to it from `expert` on
+    int expert;             // of lane 0
+    uint32_t before, all;   // tiles of the experts before that one; of all experts
+    __device__ __forceinline__ void load(const GroupArgs& a, int tile, int e0) {
+        const int lane = threadIdx.x & (kWave - 1);
+        expert = e0;
+        first = end = 0;
         if (e0 + lane < a.experts) group_rows(a, e0 + lane, first, end);
-        const uint32_t n = (uint32_t)((end - first + tile - 1) / tile);
-        uint32_t upto = n;
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) {
-            const uint32_t o = __shfl_up(upto, d, kWave);
-            if (lane >= d) upto += o;
+        count = (uint32_t)((end - first + tile - 1) / tile);
+        upto = group_upto(count);
+    }
+    __device__ __forceinline__ uint32_t here() const { return (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1); }
+    __device__ __forceinline__ void begin(const GroupArgs& a, int tile) {
+        all = 0;
+        for (int e0 = (a.experts - 1) / kWave * kWave; e0 >= 0; e0 -= kWave) {
+            load(a, tile, e0);
+            all += here();
+        }
+        before = 0;
+    }
+    // Tile t of all: its expert and rows.
+    __device__ __forceinline__ void find(const GroupArgs& a, int tile, uint32_t t, int& e, int64_t& from, int64_t& to) {
+        while (before + here() <= t && expert + kWave < a.experts) {
+            before += here();
+            load(a, tile, expert + kWave);
         }
         const uint64_t past = __ballot(before + upto > t);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            const uint32_t ahead = before + (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), l);
-            const int64_t f = __builtin_amdgcn_readlane((int)first, l), z = __builtin_amdgcn_readlane((int)end, l);   // below 2^31
-            g.expert = e0 + l;
-            g.first = f + (int64_t)(t - ahead) * tile;
-            g.rows = min((int64_t)tile, z - g.first);
-            return g;
-        }
-        before += (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1);
+        const int l = past ? __builtin_ctzll(past) : 0;
+        const uint32_t ahead = before + (uint32_t)__builtin_amdgcn_readlane((int)(upto - count), l);
+        e = expert + l;
+        from = __builtin_amdgcn_readlane((int)first, l) + (int64_t)(t - ahead) * tile;   // below 2^31
+        to = min((int64_t)__builtin_amdgcn_readlane((int)end, l), from + tile);
     }
-    return g;
-}
+};
 
 // Which of `total` tiles a workgroup takes.  Workgroups go to the 8 XCDs in
 // turn; each XCD takes a run of tiles.  total or more: none.
@@ -368,7 +371,8 @@ struct GroupWork {
     int64_t m0, n0;
 };
 // Tile t of all; high and wide: tiles of m, over all experts (product) or one (weight gradient), and of n.
-template <bool WEIGHT> __device__ __forceinline__ GroupWork group_work(const GroupArgs& a, uint32_t t, uint32_t high, uint32_t wide, int TM, int TN) {
+template <bool WEIGHT>
+__device__ __forceinline__ GroupWork group_work(const GroupArgs& a, GroupTiles& tiles, uint32_t t, uint32_t high, uint32_t wide, int TM, int TN) {
     GroupWork w;
     uint32_t tm, tn;
     if constexpr (WEIGHT) {   // each expert's tiles over all XCDs
@@ -381,10 +385,7 @@ template <bool WEIGHT> __device__ __forceinline__ GroupWork group_work(const Gro
         w.m0 = (int64_t)tm * TM;
     } else {
         group_place(t, high, wide, tm, tn);
-        const GroupTile g = group_tile(a, TM, tm);
-        w.expert = g.expert;
-        w.first = g.first;
-        w.end = g.first + g.rows;
+        tiles.find(a, TM, tm, w.expert, w.first, w.end);
         w.m0 = 0;
     }
     w.n0 = (int64_t)tn * TN;
@@ -414,10 +415,12 @@ __device__ __forceinline__ void group_operands(const GroupArgs& a, const GroupWo
 }
 // What a workgroup of a kernel with one size of tiles does.  false: nothing.
 template <bool WEIGHT> __device__ __forceinline__ bool group_begin(const GroupArgs& a, int TM, int TN, GroupWork& w) {
-    const uint32_t high = WEIGHT ? a.tiles_m : group_tiles(a, TM), total = high * a.tiles_n, block = blockIdx.x % a.tiles;
+    GroupTiles tiles;
+    if (!WEIGHT) tiles.begin(a, TM);
+    const uint32_t high = WEIGHT ? a.tiles_m : tiles.all, total = high * a.tiles_n, block = blockIdx.x % a.tiles;
     const uint32_t t = WEIGHT ? block : group_run(block, total);
     if (!WEIGHT && t >= total) return false;
-    w = group_work<WEIGHT>(a, t, high, a.tiles_n, TM, TN);
+    w = group_work<WEIGHT>(a, tiles, t, high, a.tiles_n, TM, TN);
     return true;
 }
 // The workgroup's part of k, where it is split: whole stages of KS.
@@ -754,16 +757,18 @@ template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(2
         group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
         return;
     }
-    const uint32_t high = WEIGHT ? a.tiles_m : group_tiles(a, 256), total = high * a.tiles_n * (WEIGHT ? (uint32_t)a.experts : 1u);
+    GroupTiles tiles;
+    if (!WEIGHT) tiles.begin(a, 256);
+    const uint32_t high = WEIGHT ? a.tiles_m : tiles.all, total = high * a.tiles_n * (WEIGHT ? (uint32_t)a.experts : 1u);
     uint32_t rest = total % kRound;
     if (rest > kRound / 2) rest = 0;
     const uint32_t full = total - rest;
     if (blockIdx.x < full) {
-        const GroupWork w = group_work<WEIGHT>(a, WEIGHT ? blockIdx.x : group_run(blockIdx.x, full), high, a.tiles_n, 256, 256);
+        const GroupWork w = group_work<WEIGHT>(a, tiles, WEIGHT ? blockIdx.x : group_run(blockIdx.x, full), high, a.tiles_n, 256, 256);
         group_large_tile<T, WEIGHT, ACROSS, 8, 8, 4>(a, w, lds);
     } else if (blockIdx.x - full < 4 * rest) {
         const uint32_t i = blockIdx.x - full;
-        GroupWork w = group_work<WEIGHT>(a, full + i / 4, high, a.tiles_n, 256, 256);
+        GroupWork w = group_work<WEIGHT>(a, tiles, full + i / 4, high, a.tiles_n, 256, 256);
         w.m0 += (i & 1) * 128;
         w.n0 += (i & 2) * 64;
         if (w.n0 >= a.n || w.m0 >= (WEIGHT ? a.m : w.end - w.first)) return;
