@@ -27,6 +27,9 @@ bool whole_rows(const void* p, int64_t width, int64_t stride, int32_t dtype) {
     const int64_t e = dtype == CRESSO_F32 ? 4 : 8;
     return ((uintptr_t)p & 15) == 0 && width % e == 0 && stride % e == 0 && stride >= width && stride < (int64_t)1 << 21 && width < (int64_t)1 << 21;
 }
+// Whether rows of the result are whole pieces of 16 bytes of 16-bit numbers, as the large tiles store them.
+bool large_result(const void* out, int64_t n) { return ((uintptr_t)out & 15) == 0 && n % 8 == 0 && n < (int64_t)1 << 21; }
+
 // Which tiles, and whether k is split.
 //
 // A product's time is modelled from its tiles of each side, in us at a depth of
@@ -41,7 +44,7 @@ bool whole_rows(const void* p, int64_t width, int64_t stride, int32_t dtype) {
 // 196 with 128; 2000 by 32: 59 and 53; 8192 by 8 of 2048 x 2048: 75 and 72).
 //
 // Where the tiles leave CUs idle, k is split as far as parts of 4 stages go.
-GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t experts, int32_t dtype, bool weight, bool across, bool whole) {
+GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t experts, int32_t dtype, bool weight, bool across, bool whole, bool large) {
     const bool wide = dtype == CRESSO_F32;
     const int64_t e = std::max(experts, 1);
     const auto tiles = [&](int64_t t) -> double {
@@ -51,14 +54,14 @@ GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t 
     GroupPlan p{64, 1, whole};
     if (weight) {
         const int64_t side = std::min(m, n);
-        if (whole && !wide && side >= 256 && tiles(256) >= 768.0 && rows >= 128 * e) p.tile = 256;
+        if (large && !wide && side >= 256 && tiles(256) >= 768.0 && rows >= 128 * e) p.tile = 256;
         else if (whole && side > 64) p.tile = 128;
     } else if (!wide) {
         const bool turn = across && whole;
         const double t64 = turn ? 1e30 : 12.0 + 0.0245 * tiles(64), t128 = turn ? 12.0 + 0.075 * tiles(128) : 13.0 + 0.066 * tiles(128);
         const double t256 = std::max(45.0, 0.25 * tiles(256));
         if (t128 < t64) p.tile = 128;
-        if (whole && t256 < std::min(t64, t128)) p.tile = 256;
+        if (large && t256 < std::min(t64, t128)) p.tile = 256;
     }
     const int64_t stages = (weight ? rows / e : depth) / (wide ? 32 : 64);
     if (p.tile < 256) p.splits = (uint32_t)std::min<int64_t>({16, (int64_t)(256.0 / std::max(1.0, tiles(p.tile))), stages / 4});
@@ -74,14 +77,17 @@ using namespace cresso;
 extern "C" size_t cresso_expert_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype) {
     if (check_group("expert product", dtype, rows, cols, depth, experts) != CRESSO_OK) return 0;
     size_t most = 0;
-    for (int i = 0; i < 4; ++i) most = std::max(most, group_bytes(group_plan(rows, 0, cols, depth, experts, dtype, false, i & 1, i & 2), rows * cols));
+    for (int i = 0; i < 8; ++i)
+        most = std::max(most, group_bytes(group_plan(rows, 0, cols, depth, experts, dtype, false, i & 1, i & 2, (i & 4) && (i & 2)), rows * cols));
     return most;
 }
 extern "C" size_t cresso_expert_product_weight_workspace_bytes(int64_t rows, int64_t p_width, int64_t q_width, int32_t experts,
                                                                int32_t dtype) {
     if (check_group("expert product gradient", dtype, rows, p_width, q_width, experts) != CRESSO_OK) return 0;
-    return std::max(group_bytes(group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, false), experts * p_width * q_width),
-                    group_bytes(group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, true), experts * p_width * q_width));
+    size_t most = 0;
+    for (int i = 0; i < 3; ++i)
+        most = std::max(most, group_bytes(group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, i > 0, i > 1), experts * p_width * q_width));
+    return most;
 }
 
 extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int64_t depth,
@@ -114,7 +120,7 @@ extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_
     a.experts = experts;
     a.sums = (float*)workspace;
     const bool whole = whole_rows(x, depth, x_stride, dtype) && whole_rows(w, w_cols, w_stride, dtype) && w_expert_stride % (dtype == CRESSO_F32 ? 4 : 8) == 0;
-    const GroupPlan plan = group_plan(rows, 0, cols, depth, experts, dtype, false, turned != 0, whole);
+    const GroupPlan plan = group_plan(rows, 0, cols, depth, experts, dtype, false, turned != 0, whole, whole && large_result(out, cols));
     with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, false, turned != 0, plan, (hipStream_t)stream); });
     return launched(what);
 }
@@ -146,7 +152,7 @@ extern "C" int32_t cresso_expert_product_weight(const void* p, int64_t p_stride,
     a.experts = experts;
     a.sums = (float*)workspace;
     const bool whole = whole_rows(p, p_width, p_stride, dtype) && whole_rows(q, q_width, q_stride, dtype);
-    const GroupPlan plan = group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, whole);
+    const GroupPlan plan = group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, whole, whole && large_result(out, q_width));
     with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, true, true, plan, (hipStream_t)stream); });
     return launched(what);
 }

@@ -285,16 +285,18 @@ __device__ __forceinline__ uint32_t group_upto(uint32_t v) {
 }
 // The tiles of m rows of all experts, 64 experts at a time, one a lane.  By each wave.
 struct GroupTiles {
-    int64_t first, end;     // the lane's expert's rows
+    int first, end;         // the lane's expert's rows, below 2^31
     uint32_t count, upto;   // its tiles, and those of the experts up to it from `expert` on
     int expert;             // of lane 0
     uint32_t before, all;   // tiles of the experts before that one; of all experts
     __device__ __forceinline__ void load(const GroupArgs& a, int tile, int e0) {
         const int lane = threadIdx.x & (kWave - 1);
         expert = e0;
-        first = end = 0;
-        if (e0 + lane < a.experts) group_rows(a, e0 + lane, first, end);
-        count = (uint32_t)((end - first + tile - 1) / tile);
+        int64_t from = 0, to = 0;
+        if (e0 + lane < a.experts) group_rows(a, e0 + lane, from, to);
+        first = (int)from;
+        end = (int)to;
+        count = ((uint32_t)(end - first) + (uint32_t)tile - 1) / (uint32_t)tile;
         upto = group_upto(count);
     }
     __device__ __forceinline__ uint32_t here() const { return (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1); }
@@ -307,17 +309,18 @@ struct GroupTiles {
         before = 0;
     }
     // Tile t of all: its expert and rows.
-    __device__ __forceinline__ void find(const GroupArgs& a, int tile, uint32_t t, int& e, int64_t& from, int64_t& to) {
-        while (before + here() <= t && expert + kWave < a.experts) {
-            before += here();
-            load(a, tile, expert + kWave);
+    __device__ __forceinline__ void find(const GroupArgs& a, int tile, uint32_t t, int& e, int64_t& from, int64_t& to) const {
+        GroupTiles g = *this;
+        while (g.before + g.here() <= t && g.expert + kWave < a.experts) {
+            g.before += g.here();
+            g.load(a, tile, g.expert + kWave);
         }
-        const uint64_t past = __ballot(before + upto > t);
+        const uint64_t past = __ballot(g.before + g.upto > t);
         const int l = past ? __builtin_ctzll(past) : 0;
-        const uint32_t ahead = before + (uint32_t)__builtin_amdgcn_readlane((int)(upto - count), l);
-        e = expert + l;
-        from = __builtin_amdgcn_readlane((int)first, l) + (int64_t)(t - ahead) * tile;   // below 2^31
-        to = min((int64_t)__builtin_amdgcn_readlane((int)end, l), from + tile);
+        const uint32_t ahead = g.before + (uint32_t)__builtin_amdgcn_readlane((int)(g.upto - g.count), l);
+        e = g.expert + l;
+        from = __builtin_amdgcn_readlane(g.first, l) + (int64_t)(t - ahead) * tile;
+        to = min((int64_t)__builtin_amdgcn_readlane(g.end, l), from + tile);
     }
 };
 
@@ -372,7 +375,7 @@ struct GroupWork {
 };
 // Tile t of all; high and wide: tiles of m, over all experts (product) or one (weight gradient), and of n.
 template <bool WEIGHT>
-__device__ __forceinline__ GroupWork group_work(const GroupArgs& a, GroupTiles& tiles, uint32_t t, uint32_t high, uint32_t wide, int TM, int TN) {
+__device__ __forceinline__ GroupWork group_work(const GroupArgs& a, const GroupTiles& tiles, uint32_t t, uint32_t high, uint32_t wide, int TM, int TN) {
     GroupWork w;
     uint32_t tm, tn;
     if constexpr (WEIGHT) {   // each expert's tiles over all XCDs
@@ -747,31 +750,154 @@ __device__ __forceinline__ void group_large_tile(const GroupArgs& a, const Group
 
 // 256 x 256 of 16 bits, one workgroup to a CU: eight waves of 128 x 64 would
 // read 96 KB of LDS a stage, as long as their matrix instructions take; four of
-// 128 x 128 read 64.  What is left behind the last full round of 256 tiles goes
-// in quarters of 128 x 128, if those take less than a round.
+// 128 x 128 read 64.  A workgroup goes from tile to tile, and asks for the next
+// one's first stages before it stores the one that it has done.  What is left
+// behind the last full round of 256 tiles goes in quarters of 128 x 128, if
+// those take less than a round.
 constexpr uint32_t kRound = 256;
 template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(256, 1) void group_large_kernel(GroupArgs a) {
     constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
-    __shared__ __align__(16) uint8_t lds[4 * 512 * 64];
-    if (blockIdx.x >= a.tiles) {
-        group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
+    constexpr int NT = 256, F = 8, TILE = 32 * F, ROW = 64, STAGES = 4;
+    constexpr int KS = ROW / (int)sizeof(T), STAGE = 2 * TILE * ROW, OWN = 32 * 16 * F * (int)sizeof(T);   // of a wave: 32 of its rows
+    __shared__ __align__(16) uint8_t lds[STAGES * STAGE + 4 * OWN];
+    if (blockIdx.x >= kRound) {
+        group_fill<T>(a, blockIdx.x - kRound, gridDim.x - kRound);
         return;
     }
     GroupTiles tiles;
-    if (!WEIGHT) tiles.begin(a, 256);
+    if (!WEIGHT) tiles.begin(a, TILE);
     const uint32_t high = WEIGHT ? a.tiles_m : tiles.all, total = high * a.tiles_n * (WEIGHT ? (uint32_t)a.experts : 1u);
     uint32_t rest = total % kRound;
     if (rest > kRound / 2) rest = 0;
     const uint32_t full = total - rest;
-    if (blockIdx.x < full) {
-        const GroupWork w = group_work<WEIGHT>(a, tiles, WEIGHT ? blockIdx.x : group_run(blockIdx.x, full), high, a.tiles_n, 256, 256);
-        group_large_tile<T, WEIGHT, ACROSS, 8, 8, 4>(a, w, lds);
-    } else if (blockIdx.x - full < 4 * rest) {
-        const uint32_t i = blockIdx.x - full;
+    typedef Stream<T, WEIGHT, ROW, TILE, NT, 0> StreamA;
+    typedef Stream<T, ACROSS, ROW, TILE, NT, F> StreamB;
+    constexpr int PA = StreamA::P, LOADS = PA + StreamB::P, STEPS = F * F;
+    const int lane = threadIdx.x & (kWave - 1), l16 = lane & 15, quad = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int wm = (wave & 1) * (16 * F), wn = (wave >> 1) * (16 * F);
+    uint8_t* const own = lds + STAGES * STAGE + wave * OWN;
+    const uint32_t mine = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)wave * 1024;
+    Fragments<T, WEIGHT, ROW, TILE, 0> fa;
+    Fragments<T, ACROSS, ROW, TILE, F> fb;
+    fa.begin(wm);
+    fb.begin(wn);
+    f32x4 acc[F][F] = {};
+    StreamA oa;
+    StreamB ob;
+    T* out = nullptr;
+    int64_t rows = 0, m0 = 0, n0 = 0;
+    int stages = 0;
+    const auto begin = [&](uint32_t u) __attribute__((always_inline)) {   // tile u: where it lies, and its first stages on their way
+        // weight gradients' tiles fall in length: who had an early one in a round takes a late one in the next
+        const uint32_t at = WEIGHT ? (u / kRound % 2 ? u - u % kRound + kRound - 1 - u % kRound : u) : group_run(u, full);
+        const GroupWork w = group_work<WEIGHT>(a, tiles, at, high, a.tiles_n, TILE, TILE);
+        group_operands<T, WEIGHT, ACROSS>(a, w, oa, ob, out, rows);
+        m0 = w.m0;
+        n0 = w.n0;
+        stages = (int)((oa.depth + KS - 1) / KS);
+        oa.begin();
+        ob.begin();
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) {
+            oa.fetch(mine + i * STAGE);
+            ob.fetch(mine + i * STAGE + TILE * ROW);
+        }
+    };
+    u32x4 ra[2][F], rb[2][F];
+    // Multiplies the stage in buffer `now`, whose fragments are in set now % 2; reads
+    // the next one's into the other, early enough to be there when the stage ends,
+    // and fills `now` anew.  A wave issues one instruction in 4 cycles and a matrix
+    // instruction takes 16, so each of them is followed by at most three others.
+    // later: stores that came after the pieces that are waited for.
+    const auto stage = [&](int now, auto later) __attribute__((always_inline)) {
+        group_ready<(STAGES - 2) * LOADS + decltype(later)::value>();
+        const int set = now & 1;
+        const uint8_t* const then = lds + (now + 1) % STAGES * STAGE;
+#pragma unroll
+        for (int t = 0; t < STEPS; ++t) {
+            group_mfma_into<T>(rb[set][t % F], ra[set][t / F], acc[t / F][t % F]);
+            const int r = t / 3;
+            if (t % 3 == 0 && r < F) rb[set ^ 1][r] = fb.read(then + TILE * ROW, 0, r);
+            else if (t % 3 == 0 && r < 2 * F) ra[set ^ 1][r - F] = fa.read(then, 0, r - F);
+            const int i = t / 8;
+            if (t % 8 == 1 && i < PA) oa.piece(i, mine + now * STAGE);
+            else if (t % 8 == 1) ob.piece(i - PA, mine + now * STAGE + TILE * ROW);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        oa.next();
+        ob.next();
+    };
+    constexpr std::integral_constant<int, 4 * F> STORES{};
+    constexpr std::integral_constant<int, 0> NONE{};
+    const auto first = [&](auto later) __attribute__((always_inline)) {   // the first stage's fragments
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS + decltype(later)::value) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < F; ++i) rb[0][i] = fb.read(lds + TILE * ROW, 0, i);
+#pragma unroll
+        for (int j = 0; j < F; ++j) ra[0][j] = fa.read(lds, 0, j);
+        stage(0, later);
+        stage(1, later);
+        stage(2, later);
+        stage(3, NONE);
+    };
+    uint32_t u = blockIdx.x;
+    if (u < full) {
+        begin(u);
+        first(NONE);
+    }
+    while (u < full) {
+        for (int s = STAGES; s < stages; s += STAGES) {   // 256 sums leave no registers for several ways out: stages behind the last are zeros
+#pragma unroll
+            for (int i = 0; i < STAGES; ++i) stage(i, NONE);
+        }
+        group_ready<0>();   // nothing is on its way to LDS, and all waves have read it
+        const int64_t left = rows - (m0 + wm);   // rows from the wave's first on
+        const uint64_t to = (uint64_t)(uintptr_t)(out + (m0 + wm) * a.n + n0 + wn);
+        const u32x4 result = {(uint32_t)to, (uint32_t)(to >> 32) & 0xffffu, left > 0 ? (uint32_t)(((min(left, (int64_t)128) - 1) * a.n + a.n - n0 - wn) * (int64_t)sizeof(T)) : 0u, 0x00020000u};
+        const uint32_t column = n0 + wn + l16 * 8 < a.n ? (uint32_t)l16 * 16 : 0x80000000u;   // beyond the result
+        u += kRound;
+        if (u < full) begin(u);
+#pragma unroll
+        for (int j = 0; j < F; ++j) group_mfma_done(acc[j]);
+        // The result, 32 rows of the wave's at a time, through LDS of its own: a lane
+        // writes 4 numbers of a fragment, or 32 in a row, and reads 16 bytes of a row.
+        // Pieces change places by the row's number.
+#pragma unroll
+        for (int p = 0; p < F / 2; ++p) {
+#pragma unroll
+            for (int j = 2 * p; j < 2 * p + 2; ++j) {
+#pragma unroll
+                for (int i = 0; i < F; ++i) {
+                    const int n = ACROSS ? i * 16 + quad * 4 : quad * (4 * F) + i * 4;
+                    const f32x4 v = acc[j][i];
+                    acc[j][i] = f32x4{0, 0, 0, 0};
+                    *(u32x2*)(own + ((j & 1) * 16 + l16) * 256 + (((n / 8) ^ l16) * 16) + (n & 4) * 2) = u32x2{narrow2<T>(v[0], v[1]), narrow2<T>(v[2], v[3])};
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const int row = r * 4 + quad;
+                const u32x4 v = *(const u32x4*)(own + row * 256 + ((l16 ^ (row & 15)) * 16));
+                const uint32_t at = column + (uint32_t)(p * 32 + row) * (uint32_t)(a.n * (int64_t)sizeof(T));
+                __builtin_amdgcn_raw_buffer_store_b128(v, __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)((uint64_t)result[1] << 32 | result[0]), (short)0, (int)result[2], 0x00020000), at, 0, 0);
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (u < full) first(STORES);
+    }
+    for (; u - full < 4 * rest; u += kRound) {
+        const uint32_t i = u - full;
         GroupWork w = group_work<WEIGHT>(a, tiles, full + i / 4, high, a.tiles_n, 256, 256);
         w.m0 += (i & 1) * 128;
         w.n0 += (i & 2) * 64;
-        if (w.n0 >= a.n || w.m0 >= (WEIGHT ? a.m : w.end - w.first)) return;
+        if (w.n0 >= a.n || w.m0 >= (WEIGHT ? a.m : w.end - w.first)) continue;
+        __syncthreads();
         group_large_tile<T, WEIGHT, ACROSS, 4, 4, 8>(a, w, lds);
     }
 }
@@ -812,7 +938,13 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, G
         const auto size = [&](auto w, auto x) {                                                                         \
             constexpr bool W = decltype(w)::value, X = decltype(x)::value;                                              \
             if constexpr (sizeof(T) == 2) {                                                                             \
-                if (plan.whole && plan.tile == 256) return run(group_large_kernel<T, W, X>, 256, 3 * kRound / 2);       \
+                if (plan.whole && plan.tile == 256) {                                                                   \
+                    a.tiles_n = (uint32_t)((a.n + 255) / 256);                                                          \
+                    a.tiles_m = (uint32_t)((a.m + 255) / 256);                                                          \
+                    a.splits = 1;                                                                                       \
+                    hipLaunchKernelGGL((group_large_kernel<T, W, X>), dim3(kRound + (W ? 0 : kFillBlocks)), dim3(256), 0, st, a); \
+                    return;                                                                                             \
+                }                                                                                                       \
                 if constexpr (X)                                                                                        \
                     if (plan.whole && plan.tile == 128 && plan.splits < 2) return run(group_small_kernel<T, W, X, 4, 4, 2>, 128); \
                 if constexpr (W)                                                                                        \
