@@ -43,7 +43,12 @@ bool large_result(const void* out, int64_t n) { return ((uintptr_t)out & 15) == 
 // enough to be more than a store (16384 rows by 64 experts of 2048 x 1024: 173 us,
 // 196 with 128; 2000 by 32: 59 and 53; 8192 by 8 of 2048 x 2048: 75 and 72).
 //
-// Where the tiles leave CUs idle, k is split as far as parts of 4 stages go.
+// Where the tiles leave CUs idle, k is split into parts of 8 stages or more: for
+// 16 bits below 256 tiles (64 x 4096 -> 256 by 2: 19.6 us in one part, 11.4 in 8;
+// 512 x 2048 -> 2048 by 8, 384 tiles, 15.7 and 21.5 in 2), for fp32, whose tiles
+// take longer, below 768 or, of any alignment, 1024 (777 x 1001 -> 1500 by 9,
+// 396 tiles: 64.5 and 54.9 in 2, its gradient 93.9 and 55.6 in 3; aligned 36.8
+// and 42.9).
 GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t experts, int32_t dtype, bool weight, bool across, bool whole, bool large) {
     const bool wide = dtype == CRESSO_F32;
     const int64_t e = std::max(experts, 1);
@@ -64,7 +69,8 @@ GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t 
         if (large && t256 < std::min(t64, t128)) p.tile = 256;
     }
     const int64_t stages = (weight ? rows / e : depth) / (wide ? 32 : 64);
-    if (p.tile < 256) p.splits = (uint32_t)std::min<int64_t>({16, (int64_t)(256.0 / std::max(1.0, tiles(p.tile))), stages / 4});
+    const double enough = !wide ? 256.0 : whole ? 768.0 : 1024.0;
+    if (p.tile < 256) p.splits = (uint32_t)std::min<int64_t>({16, (int64_t)(enough / std::max(1.0, tiles(p.tile))), stages / 8});
     p.splits = std::max(p.splits, 1u);
     return p;
 }

@@ -256,6 +256,16 @@ template <typename T> __device__ __forceinline__ void group_mfma_into(u32x4 a, u
     if constexpr (std::is_same<T, __half>::value) asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     else asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
+// Sums of zero, in their registers here and now: a zero that the compiler writes
+// right in front of a matrix instruction, as it does with one that is only
+// assigned, is not there yet when that reads it.
+template <int N> __device__ __forceinline__ void group_zero(f32x4 (&c)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        c[i] = f32x4{0, 0, 0, 0};
+        asm volatile("" : "+a"(c[i]));
+    }
+}
 // After the last of them: more than the 18 cycles that a result of four passes takes to be there for others.
 template <int N> __device__ __forceinline__ void group_mfma_done(f32x4 (&c)[N]) {
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
@@ -667,7 +677,9 @@ __device__ __forceinline__ void group_large_tile(const GroupArgs& a, const Group
     fb.begin(wn);
     oa.begin();
     ob.begin();
-    f32x4 acc[FM][FN] = {};
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int j = 0; j < FM; ++j) group_zero(acc[j]);
     const int stages = (int)((oa.depth + KS - 1) / KS);
     const uint32_t mine = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)wave * 1024;
     u32x4 ra[2][FM], rb[2][FN];
@@ -782,7 +794,9 @@ template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(2
     Fragments<T, ACROSS, ROW, TILE, F> fb;
     fa.begin(wm);
     fb.begin(wn);
-    f32x4 acc[F][F] = {};
+    f32x4 acc[F][F];
+#pragma unroll
+    for (int j = 0; j < F; ++j) group_zero(acc[j]);
     StreamA oa;
     StreamB ob;
     T* out = nullptr;
@@ -790,7 +804,8 @@ template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(2
     int stages = 0;
     const auto begin = [&](uint32_t u) __attribute__((always_inline)) {   // tile u: where it lies, and its first stages on their way
         // weight gradients' tiles fall in length: who had an early one in a round takes a late one in the next
-        const uint32_t at = WEIGHT ? (u / kRound % 2 ? u - u % kRound + kRound - 1 - u % kRound : u) : group_run(u, full);
+        const uint32_t in = u % kRound, round = u - in;   // the last round may be short
+        const uint32_t at = !WEIGHT ? group_run(u, full) : u / kRound % 2 && round + kRound <= full ? round + kRound - 1 - in : u;
         const GroupWork w = group_work<WEIGHT>(a, tiles, at, high, a.tiles_n, TILE, TILE);
         group_operands<T, WEIGHT, ACROSS>(a, w, oa, ob, out, rows);
         m0 = w.m0;
@@ -856,7 +871,7 @@ template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(2
         group_ready<0>();   // nothing is on its way to LDS, and all waves have read it
         const int64_t left = rows - (m0 + wm);   // rows from the wave's first on
         const uint64_t to = (uint64_t)(uintptr_t)(out + (m0 + wm) * a.n + n0 + wn);
-        const u32x4 result = {(uint32_t)to, (uint32_t)(to >> 32) & 0xffffu, left > 0 ? (uint32_t)(((min(left, (int64_t)128) - 1) * a.n + a.n - n0 - wn) * (int64_t)sizeof(T)) : 0u, 0x00020000u};
+        const u32x4 result = {(uint32_t)to, (uint32_t)(to >> 32) & 0xffffu, left > 0 && n0 + wn < a.n ? (uint32_t)(((min(left, (int64_t)128) - 1) * a.n + a.n - n0 - wn) * (int64_t)sizeof(T)) : 0u, 0x00020000u};
         const uint32_t column = n0 + wn + l16 * 8 < a.n ? (uint32_t)l16 * 16 : 0x80000000u;   // beyond the result
         u += kRound;
         if (u < full) begin(u);
@@ -873,10 +888,10 @@ template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(2
                 for (int i = 0; i < F; ++i) {
                     const int n = ACROSS ? i * 16 + quad * 4 : quad * (4 * F) + i * 4;
                     const f32x4 v = acc[j][i];
-                    acc[j][i] = f32x4{0, 0, 0, 0};
                     *(u32x2*)(own + ((j & 1) * 16 + l16) * 256 + (((n / 8) ^ l16) * 16) + (n & 4) * 2) = u32x2{narrow2<T>(v[0], v[1]), narrow2<T>(v[2], v[3])};
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                group_zero(acc[j]);
             }
             __builtin_amdgcn_wave_barrier();
 #pragma unroll

@@ -92,6 +92,17 @@ def test_large_tiles(dtype):
     check(4100, [4100], 512, 1280, dtype)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts,inner,outer,turned", [
+    ([16640], 200, 1288, False),             # 330 tiles of 256: more than one to a workgroup, the rest in quarters
+    ([8000, 0, 1, 9000, 3000], 136, 1544, True),
+    ([130 + 3 * (e % 7) for e in range(48)], 1024, 1040, False),   # weight gradients of several tiles to a workgroup
+    ([300, 0, 5, 700, 120, 260] * 9, 1032, 800, True),
+])
+def test_many_large_tiles(counts, inner, outer, turned, dtype):
+    check(sum(counts) + 17, counts, inner, outer, dtype, first=5, turned=turned)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_one_long_group(dtype):
     """A weight gradient whose sum is long and whose matrix is small."""
