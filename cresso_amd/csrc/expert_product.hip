@@ -23,9 +23,10 @@ int32_t check_group(const char* what, int32_t dtype, int64_t rows, int64_t a, in
 }
 // Whether rows at p go to LDS in whole pieces of 16 bytes: so do their width and stride, and a
 // stage's rows lie within 2^31 bytes.
+bool near_rows(int64_t width, int64_t stride) { return stride >= width && stride < (int64_t)1 << 21 && width < (int64_t)1 << 21; }
 bool whole_rows(const void* p, int64_t width, int64_t stride, int32_t dtype) {
     const int64_t e = dtype == CRESSO_F32 ? 4 : 8;
-    return ((uintptr_t)p & 15) == 0 && width % e == 0 && stride % e == 0 && stride >= width && stride < (int64_t)1 << 21 && width < (int64_t)1 << 21;
+    return ((uintptr_t)p & 15) == 0 && width % e == 0 && stride % e == 0 && near_rows(width, stride);
 }
 // Whether rows of the result are whole pieces of 16 bytes of 16-bit numbers, as the large tiles store them.
 bool large_result(const void* out, int64_t n) { return ((uintptr_t)out & 15) == 0 && n % 8 == 0 && n < (int64_t)1 << 21; }
@@ -46,9 +47,8 @@ bool large_result(const void* out, int64_t n) { return ((uintptr_t)out & 15) == 
 // Where the tiles leave CUs idle, k is split into parts of 8 stages or more: for
 // 16 bits below 256 tiles (64 x 4096 -> 256 by 2: 19.6 us in one part, 11.4 in 8;
 // 512 x 2048 -> 2048 by 8, 384 tiles, 15.7 and 21.5 in 2), for fp32, whose tiles
-// take longer, below 768 or, of any alignment, 1024 (777 x 1001 -> 1500 by 9,
-// 396 tiles: 64.5 and 54.9 in 2, its gradient 93.9 and 55.6 in 3; aligned 36.8
-// and 42.9).
+// take longer, below 768 (777 x 1001 -> 1500 by 9, 396 tiles: 41.8 us and 50.1 in
+// 2; its gradient, 264 tiles: 61.4 and 47.9).
 GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t experts, int32_t dtype, bool weight, bool across, bool whole, bool large) {
     const bool wide = dtype == CRESSO_F32;
     const int64_t e = std::max(experts, 1);
@@ -56,7 +56,7 @@ GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t 
         const double across = (double)((n + t - 1) / t);
         return across * (weight ? (double)e * (double)((m + t - 1) / t) : (double)rows / t + 0.5 * (double)std::min(e, rows));
     };
-    GroupPlan p{64, 1, whole};
+    GroupPlan p{64, 1, whole, false};
     if (weight) {
         const int64_t side = std::min(m, n);
         if (large && !wide && side >= 256 && tiles(256) >= 768.0 && rows >= 128 * e) p.tile = 256;
@@ -69,7 +69,7 @@ GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t 
         if (large && t256 < std::min(t64, t128)) p.tile = 256;
     }
     const int64_t stages = (weight ? rows / e : depth) / (wide ? 32 : 64);
-    const double enough = !wide ? 256.0 : whole ? 768.0 : 1024.0;
+    const double enough = wide ? 768.0 : 256.0;
     if (p.tile < 256) p.splits = (uint32_t)std::min<int64_t>({16, (int64_t)(enough / std::max(1.0, tiles(p.tile))), stages / 8});
     p.splits = std::max(p.splits, 1u);
     return p;
@@ -126,7 +126,8 @@ extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_
     a.experts = experts;
     a.sums = (float*)workspace;
     const bool whole = whole_rows(x, depth, x_stride, dtype) && whole_rows(w, w_cols, w_stride, dtype) && w_expert_stride % (dtype == CRESSO_F32 ? 4 : 8) == 0;
-    const GroupPlan plan = group_plan(rows, 0, cols, depth, experts, dtype, false, turned != 0, whole, whole && large_result(out, cols));
+    GroupPlan plan = group_plan(rows, 0, cols, depth, experts, dtype, false, turned != 0, whole, whole && large_result(out, cols));
+    plan.words = dtype == CRESSO_F32 && near_rows(depth, x_stride) && near_rows(w_cols, w_stride);
     with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, false, turned != 0, plan, (hipStream_t)stream); });
     return launched(what);
 }
@@ -158,7 +159,8 @@ extern "C" int32_t cresso_expert_product_weight(const void* p, int64_t p_stride,
     a.experts = experts;
     a.sums = (float*)workspace;
     const bool whole = whole_rows(p, p_width, p_stride, dtype) && whole_rows(q, q_width, q_stride, dtype);
-    const GroupPlan plan = group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, whole, whole && large_result(out, q_width));
+    GroupPlan plan = group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, whole, whole && large_result(out, q_width));
+    plan.words = dtype == CRESSO_F32 && near_rows(p_width, p_stride) && near_rows(q_width, q_stride);
     with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, true, true, plan, (hipStream_t)stream); });
     return launched(what);
 }

@@ -116,34 +116,44 @@ template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */>
     }
 };
 
-// 16 bytes a lane from a buffer to LDS: lane i's go to lds + 16 * i.  Written
-// out, since with the builtin the compiler waits for all of them before each
-// transposed read of LDS, whichever part that reads (1340 us instead of XXX for
-// the gradient of 32768 x 2048 -> 5632).  It writes no register but m0, which the
-// compiler keeps nothing in (it sets it right before what reads it); group_ready waits for it.
-__device__ __forceinline__ void group_to_lds(u32x4 from, uint32_t lane_at, uint32_t at, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                 :
-                 : "s"(lds), "v"(lane_at), "s"(from), "s"(at));
+// V bytes a lane from a buffer to LDS: lane i's go to lds + V * i.  Written out,
+// since with the builtin the compiler waits for all of them before each
+// transposed read of LDS, whichever part that reads (32768 x 5632 -> 2048, the
+// gradient of x: 1341 us, so 841 with the same tiles).  It writes no register but
+// m0, which the compiler keeps nothing in (it sets it right before what reads it);
+// group_ready waits for it.
+template <int V> __device__ __forceinline__ void group_to_lds(u32x4 from, uint32_t lane_at, uint32_t at, uint32_t lds) {
+    static_assert(V == 16 || V == 4, "bytes of a lane");
+    if constexpr (V == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" : : "s"(lds), "v"(lane_at), "s"(from), "s"(at));
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" : : "s"(lds), "v"(lane_at), "s"(from), "s"(at));
 }
 
-// The same with the pieces going to LDS by themselves, for rows, strides and
-// sizes of whole pieces.  What lies beyond the buffer is 0 in LDS.
-template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */> struct Stream {
-    static constexpr int E = Group<T>::E, P = TILE * (ROW / 16) / NT, KS = ROW / (int)sizeof(T);
-    static_assert(P * NT == TILE * (ROW / 16), "tile");
+// The same with the numbers going to LDS by themselves, V bytes a lane: 16 for
+// rows, strides and sizes of whole aligned pieces, 4 for fp32 of any.  What lies
+// beyond the buffer is 0 in LDS.
+template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */, int V = 16> struct Stream {
+    static constexpr int E = Group<T>::E, P = TILE * (ROW / V) / NT, KS = ROW / (int)sizeof(T);
+    static_assert(P * NT == TILE * (ROW / V) && V % (int)sizeof(T) == 0, "tile");
+    // Row (or, across k, k) of a thread's i-th load, and its first element there.
+    static __device__ __forceinline__ void at_load(int i, int& row, int& element) {
+        const int part = (int)threadIdx.x + i * NT;
+        at_place<T, ACROSS, ROW, TILE, FN>(part / (16 / V), row, element);
+        element = element * E + part % (16 / V) * (V / (int)sizeof(T));
+    }
     const T* base;
     int64_t stride, size, depth;
-    uint32_t at[P];   // byte of a thread's piece in a stage's part of the buffer
+    uint32_t at[P];   // byte of a thread's load in a stage's part of the buffer
     u32x4 buffer;     // the descriptor of make_rsrc of the next stage, in words
     uint32_t step, stage_bytes;
     int left;         // k of the next stage and behind it
     __device__ __forceinline__ void begin() {
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-            int row, piece;
-            at_place<T, ACROSS, ROW, TILE, FN>((int)threadIdx.x + i * NT, row, piece);
-            at[i] = (uint32_t)row * (uint32_t)(stride * (int)sizeof(T)) + (uint32_t)piece * 16;
+            int row, element;
+            at_load(i, row, element);
+            at[i] = (uint32_t)row * (uint32_t)(stride * (int)sizeof(T)) + (uint32_t)element * (uint32_t)sizeof(T);
         }
         const auto scalar = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
         const uint64_t from = (uint64_t)(uintptr_t)base;
@@ -166,9 +176,9 @@ template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */>
         } else {   // a row's next numbers are another row's
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-                int row, piece;
-                at_place<T, ACROSS, ROW, TILE, FN>((int)threadIdx.x + i * NT, row, piece);
-                if (piece * E >= left) at[i] = 0x80000000u;   // beyond every buffer
+                int row, element;
+                at_load(i, row, element);
+                if (element >= left) at[i] = 0x80000000u;   // beyond every buffer
             }
         }
     }
@@ -183,8 +193,8 @@ template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */>
         }
         ending();
     }
-    // Piece i of the thread's to the buffer at `to`, which is the wave's part of it.
-    __device__ __forceinline__ void piece(int i, uint32_t to) const { group_to_lds(buffer, at[i], step, to + i * (NT * 16)); }
+    // The thread's i-th load to the buffer at `to`, which is the wave's part of it.
+    __device__ __forceinline__ void piece(int i, uint32_t to) const { group_to_lds<V>(buffer, at[i], step, to + i * (NT * V)); }
     __device__ __forceinline__ void fetch(uint32_t to) {
 #pragma unroll
         for (int i = 0; i < P; ++i) piece(i, to);
@@ -588,7 +598,7 @@ template <int N> __device__ __forceinline__ void group_ready() {
 
 // The same for operands of whole aligned pieces, which go to LDS by themselves,
 // STAGES - 1 stages ahead of the one that is multiplied.
-template <typename T, bool WEIGHT, bool B_ACROSS, int WM, int WN, int FM, int FN, int ROW, int STAGES>
+template <typename T, bool WEIGHT, bool B_ACROSS, int WM, int WN, int FM, int FN, int ROW, int STAGES, int V = 16>
 __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
     constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16;
     constexpr int KS = ROW / (int)sizeof(T), STAGE = (TM + TN) * ROW;
@@ -598,8 +608,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
         group_fill<T>(a, blockIdx.x - a.tiles, gridDim.x - a.tiles);
         return;
     }
-    typedef Stream<T, WEIGHT, ROW, TM, NT, 0> StreamA;
-    typedef Stream<T, ACROSS, ROW, TN, NT, FN> StreamB;
+    typedef Stream<T, WEIGHT, ROW, TM, NT, 0, V> StreamA;
+    typedef Stream<T, ACROSS, ROW, TN, NT, FN, V> StreamB;
     constexpr int LOADS = StreamA::P + StreamB::P;
     StreamA oa;
     StreamB ob;
@@ -619,7 +629,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
     ob.begin();
     f32x4 acc[FN][FM] = {};
     const int stages = (int)((oa.depth + KS - 1) / KS);
-    const uint32_t mine = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)wave * 1024;
+    const uint32_t mine = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)wave * (kWave * V);
     uint32_t to = 0;
     const auto fetch = [&] {
         oa.fetch(mine + to);
@@ -936,6 +946,7 @@ struct GroupPlan {
     int tile;
     uint32_t splits;
     bool whole;   // aligned, whole pieces
+    bool words;   // fp32 of any alignment whose rows lie apart, near enough for a buffer
 };
 // One dtype's kernels, each in a source file of its own.
 template <typename T> void group_launch(GroupArgs a, bool weight, bool across, GroupPlan plan, hipStream_t st);
@@ -967,6 +978,8 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, G
             }                                                                                                           \
             if (plan.whole && plan.tile >= 128) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128);                    \
             else if (plan.whole) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3>, 64);                                    \
+            else if (sizeof(T) == 4 && plan.words)                                                                      \
+                run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3, sizeof(T) == 4 ? 4 : 16>, 64);                            \
             else if (plan.tile >= 128) run(group_any_kernel<T, W, X, 1, 4, 8, 2>, 128);                                 \
             else run(group_any_kernel<T, W, X, 1, 4, 4, 1>, 64);                                                        \
             if (a.splits < 2) return;                                                                                   \
