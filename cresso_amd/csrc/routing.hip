@@ -71,11 +71,19 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {   // of all lanes, to
 __device__ __forceinline__ float lane_of(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
-__device__ __forceinline__ float wave_largest(float v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, kWave));
-    return v;
+template <int CTRL, int ROW_MASK> __device__ __forceinline__ float dpp_largest(float v) {   // lanes without a source: -inf
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp((int)0xff800000u, __builtin_bit_cast(int, v), CTRL, ROW_MASK, 0xF, false)));
 }
+__device__ __forceinline__ float wave_largest(float v) {
+    v = dpp_largest<0xB1, 0xF>(v);
+    v = dpp_largest<0x4E, 0xF>(v);
+    v = dpp_largest<0x124, 0xF>(v);
+    v = dpp_largest<0x128, 0xF>(v);
+    v = dpp_largest<0x142, 0xA>(v);
+    v = dpp_largest<0x143, 0xC>(v);
+    return lane_of(v, kWave - 1);
+}
+__device__ __forceinline__ float route_sum(float v) { return lane_of(wave_total(v), kWave - 1); }
 
 template <typename T, int J> __device__ __forceinline__ void route_load(const RouteArgs& a, int64_t token, float (&z)[J]) {
     const T* row = (const T*)a.logits + token * a.stride;
@@ -136,7 +144,7 @@ template <int J> __device__ __forceinline__ void route_choose(const RouteArgs& a
 #pragma unroll
             for (int j = 0; j < J; ++j) sum += j * kWave + lane < a.n ? expf(z[j] - m) : 0.0f;
         }
-        sum = wave_sum(sum);
+        sum = route_sum(sum);
         weight = there ? a.scale * (e / sum) : 0.0f;
     } else if (!a.normalize) {
         weight = there ? a.scale * (expf(fminf(mine, 0.0f)) / (1.0f + expf(-fabsf(mine)))) : 0.0f;
@@ -144,7 +152,7 @@ template <int J> __device__ __forceinline__ void route_choose(const RouteArgs& a
         // the chosen ones' largest factor is taken out, so that their sum is at least a half whatever they are
         const float m = fminf(wave_largest(there ? mine : -INFINITY), 0.0f);
         const float q = there ? expf(fminf(mine, 0.0f) - m) / (1.0f + expf(-fabsf(mine))) : 0.0f;
-        const float sum = wave_sum(q);   // by all lanes
+        const float sum = route_sum(q);   // by all lanes
         weight = there ? a.scale * (q / sum) : 0.0f;
     }
 }
@@ -176,14 +184,16 @@ __device__ __forceinline__ int32_t place_of(uint32_t* next, uint32_t e, bool on,
     __builtin_amdgcn_wave_barrier();
     return (int32_t)(first + ahead);
 }
+template <int CTRL, int ROW_MASK> __device__ __forceinline__ uint32_t dpp_sum(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROW_MASK, 0xF, false);
+}
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {   // inclusive
-    const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const uint32_t o = __shfl_up(v, d, kWave);
-        if (lane >= d) v += o;
-    }
-    return v;
+    v = dpp_sum<0x111, 0xF>(v);   // row_shr:1
+    v = dpp_sum<0x112, 0xF>(v);   // row_shr:2
+    v = dpp_sum<0x114, 0xF>(v);   // row_shr:4
+    v = dpp_sum<0x118, 0xF>(v);   // row_shr:8
+    v = dpp_sum<0x142, 0xA>(v);   // row_bcast:15 -> rows 1, 3
+    return dpp_sum<0x143, 0xC>(v);   // row_bcast:31 -> rows 2, 3
 }
 
 template <typename T, int J> __global__ __launch_bounds__(RT_NT) void route_kernel(RouteArgs a) {
@@ -331,7 +341,7 @@ template <typename T, int J> __global__ __launch_bounds__(RT_NT) void route_back
     float g[J], z[J];
     const bool all = a.softmax && !a.normalize;
     float mean = 0.0f;
-    if (a.softmax || a.normalize) mean = wave_sum(there ? p * d : 0.0f);
+    if (a.softmax || a.normalize) mean = route_sum(there ? p * d : 0.0f);
     float mine = there ? w * (a.normalize ? d - mean : d) : 0.0f;
     if (!a.softmax) {   // times 1 - sigmoid(z)
         float zk = 0.0f;
@@ -353,7 +363,7 @@ template <typename T, int J> __global__ __launch_bounds__(RT_NT) void route_back
             z[j] = j * kWave + lane < a.n ? expf(z[j] - m) : 0.0f;
             sum += z[j];
         }
-        const float by = -a.scale * mean / wave_sum(sum);
+        const float by = -a.scale * mean / route_sum(sum);
 #pragma unroll
         for (int j = 0; j < J; ++j) g[j] = z[j] * by;
     }
