@@ -13,10 +13,11 @@ namespace {
 int32_t check_group(const char* what, int32_t dtype, int64_t rows, int64_t a, int64_t b, int32_t experts) {
     if (!row_dtype(dtype)) return fail(CRESSO_E_UNSUPPORTED, "%s: dtype %d not supported (f32, bf16, f16)", what, dtype);
     if (rows < 0 || a < 0 || b < 0 || experts < 0) return fail(CRESSO_E_INVALID, "%s: negative size", what);
-    // offsets of 32 bits; grids of up to 2^31 workgroups of the smallest tiles
-    const int64_t tiles = (rows / 32 + experts) * ((std::max(a, b) + 63) / 64);
-    if (rows >= (int64_t)1 << 31 || a >= (int64_t)1 << 22 || b >= (int64_t)1 << 22 || experts > 1 << 16 || tiles >= (int64_t)1 << 30 ||
-        (int64_t)experts * ((a + 31) / 32) * ((b + 63) / 64) >= (int64_t)1 << 30)
+    // offsets of 32 bits; fewer than 2^24 workgroups of 256 threads, the most of a launch, with the smallest tiles
+    const auto tiles = [](int64_t n) { return (n + 63) / 64; };
+    const int64_t most = ((int64_t)1 << 24) - 4096;
+    if (rows >= (int64_t)1 << 31 || a >= (int64_t)1 << 22 || b >= (int64_t)1 << 22 || experts > 1 << 16 ||
+        (rows / 64 + experts) * tiles(std::max(a, b)) >= most || experts * (tiles(a) * tiles(b)) >= most)
         return fail(CRESSO_E_UNSUPPORTED, "%s: %lld rows, %d matrices of %lld x %lld are more than one call takes", what, (long long)rows,
                     experts, (long long)a, (long long)b);
     return CRESSO_OK;

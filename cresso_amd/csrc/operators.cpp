@@ -117,6 +117,7 @@ struct OneGpu {
         if (!t.defined()) return;
         TORCH_CHECK(t.is_cuda(), what, ": ", name, " is on ", t.device(), "; the operators run on the GPU only");
         TORCH_CHECK(!t._fw_grad(0).defined(), what, ": ", name, " has a forward-mode derivative, the operators have reverse mode only");
+        TORCH_CHECK(!t.is_neg(), what, ": ", name, " is a view that stands for the negative of its memory (resolve_neg gives it its own)");
         if (!first) first = &t;
         TORCH_CHECK(t.device() == first->device(), what, ": ", name, " is on ", t.device(), ", others on ", first->device());
     }
@@ -789,7 +790,7 @@ Tensor clip_gradients(const pybind11::list& grads, double max_norm, int64_t kind
 // ---------------------------------------------------------------------------
 // layers of experts
 // ---------------------------------------------------------------------------
-constexpr int64_t kMaxExperts = 1024, kMaxExpertsOfToken = 32;
+constexpr int64_t kMaxExperts = 1024, kMaxExpertsOfToken = 32, kMaxTokens = 1 << 26;
 
 struct Route {
     Tensor logits, bias;
@@ -881,7 +882,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_experts(const Tensor& l
     TORCH_CHECK_VALUE(experts >= 1 && experts <= kMaxExperts, what, ": ", experts, " experts, 1 to ", kMaxExperts, " are taken");
     TORCH_CHECK_VALUE(top >= 1 && top <= std::min(experts, kMaxExpertsOfToken), what, ": top ", top, " of ", experts, " experts, 1 to ",
                       std::min(experts, kMaxExpertsOfToken), " are taken");
-    TORCH_CHECK_VALUE(logits.size(0) * top < (int64_t)1 << 31, what, ": ", logits.size(0), " tokens are more than one call takes");
+    TORCH_CHECK_VALUE(logits.size(0) < kMaxTokens && logits.size(0) * top < (int64_t)1 << 31, what, ": ", logits.size(0), " tokens are more than one call takes");
     TORCH_CHECK_VALUE(std::isfinite(scale), what, ": scale must be finite");
     if (bias.defined())
         TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == experts && bias.scalar_type() == at::kFloat, what, ": bias must be fp32 [",
@@ -901,7 +902,8 @@ void check_slots(const char* what, OneGpu& gpu, const Tensor& experts, const Ten
                       experts.sizes(), " and ", name_of(places.scalar_type()), " ", places.sizes());
     TORCH_CHECK_VALUE(experts.size(1) >= 1 && experts.size(1) <= kMaxExpertsOfToken, what, ": ", experts.size(1), " experts a token, 1 to ",
                       kMaxExpertsOfToken, " are taken");
-    TORCH_CHECK_VALUE(experts.numel() < (int64_t)1 << 31, what, ": more rows than one call takes");
+    TORCH_CHECK_VALUE(experts.size(0) < kMaxTokens && experts.numel() < (int64_t)1 << 31, what, ": ", experts.size(0),
+                      " tokens are more than one call takes");
 }
 const int32_t* ints(const Tensor& t) { return (const int32_t*)t.const_data_ptr(); }
 

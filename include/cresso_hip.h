@@ -552,7 +552,7 @@ int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t count, int3
  * those of one expert in their own order, absent ones last; places [slots]: the
  * place of each slot in that order; offsets [experts + 1]: where each expert's
  * slots begin, and the last's end.  2 <= experts + 1 <= 1025, top <= 32 and
- * at most experts, slots below 2^31. */
+ * at most experts, tokens below 2^26, slots below 2^31. */
 typedef struct cresso_route_desc {
     const void* logits;
     const float* bias;
@@ -571,7 +571,8 @@ int32_t cresso_route_backward(const cresso_route_desc* desc, const float* d_weig
 
 /* Rows between tokens and their slots.  experts [tokens][top]: an entry below 0
  * is absent; places [tokens][top]: a slot's row; a place outside [0, tokens *
- * top) is not read or written.
+ * top) is not read or written, and no place is given twice.  Tokens below
+ * 2^26, at most 32 entries each, slots below 2^31.
  *   dispatch: rows[places[t][k]] = x[t], zeros for absent slots
  *   combine:  out[t] = sum over present k, in their order, of weights[t][k] * rows[places[t][k]]  (weights NULL: 1)
  *   combine_backward: d_rows[places[t][k]] = weights[t][k] * d_out[t], zeros for absent slots;
@@ -593,7 +594,11 @@ int32_t cresso_combine_backward(const void* rows, int64_t rows_stride, const voi
  *                                           x[i][d] * w[e][d][c]     (turned 1: w is [experts][depth][cols])
  *   product_weight: out[e][a][b] = sum over expert e's rows i of p[i][a] * q[i][b]   (zeros without a row)
  * All of one dtype (f32, bf16, f16); out contiguous; sums are fp32, rounded
- * once.  w_expert_stride and w_stride: elements between experts and rows. */
+ * once.  w_expert_stride and w_stride: elements between experts and rows.
+ * Offsets that are not so leave results unspecified, but nothing outside the
+ * operands is read or written.  Rows below 2^31, widths below 2^22, at most
+ * 65536 experts; (rows / 64 + experts) * the wider side / 64, and the matrices'
+ * elements / 4096, below 2^24. */
 size_t cresso_expert_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype);
 int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int64_t depth,
                               const void* w, int64_t w_expert_stride, int64_t w_stride, int32_t turned, int32_t experts,

@@ -111,6 +111,7 @@ def test_route_arguments(lib):
         refused(lib, fn(route(top=9)), -3, "top 9")
         refused(lib, fn(route(num_experts=64, top=33)), -3, "top 33")
         refused(lib, fn(route(tokens=1 << 30)), -3, "more than one call takes")
+        refused(lib, fn(route(tokens=1 << 26, top=1)), -3, "more than one call takes")   # a launch has fewer than 2^32 threads
         refused(lib, fn(route(score=2)), -1, "unknown score")
         refused(lib, fn(route(scale=math.nan)), -1, "scale")
         refused(lib, fn(route(logits=None)), -1, "null")
@@ -147,6 +148,7 @@ def test_rows_arguments(lib):
         refused(lib, fn(top=0), -3, "0 experts")
         refused(lib, fn(top=33), -3, "33 experts")
         refused(lib, fn(tokens=1 << 30), -3, "more than one call takes")
+        refused(lib, fn(tokens=1 << 26, top=1), -3, "more than one call takes")
         refused(lib, fn(experts=NULL), -1, "null")
         refused(lib, fn(places=NULL), -1, "null")
         refused(lib, fn(stride=15), -1, "row stride")
@@ -190,6 +192,9 @@ def test_product_arguments(lib):
     refused(lib, product(turned=1, w_stride=15), -1, "row stride")
     refused(lib, product(expert=-1), -1, "stride between experts")
     refused(lib, product(depth=1 << 23), -3, "more than one call takes")
+    refused(lib, product(rows=1 << 30, cols=64, dtype=F32), -3, "more than one call takes")   # 2^24 tiles of 64 x 64
+    refused(lib, product(rows=1 << 21, cols=1 << 15), -3, "more than one call takes")
+    refused(lib, weight(experts=1 << 16, pw=1024, qw=1024, p_stride=1024, q_stride=1024), -3, "more than one call takes")
     refused(lib, weight(p=NULL), -1, "null")
     refused(lib, weight(q_stride=15), -1, "row strides")
     assert product(rows=0) == 0 and product(cols=0) == 0 and weight(experts=0) == 0 and weight(pw=0) == 0

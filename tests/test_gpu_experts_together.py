@@ -252,6 +252,15 @@ def test_dual_tensors_are_refused(name):
         call(x.detach())
 
 
+@pytest.mark.parametrize("name", ["route", "bias", "dispatch", "combine", "combine weights", "product", "product weight", "norm", "clip"])
+def test_negative_views_are_refused(name):
+    """Their memory holds the negative of what they are."""
+    call, x = dual_calls()[name]
+    with pytest.raises(RuntimeError, match="negative of its memory"):
+        call(torch._neg_view(x.detach()))
+    call(torch._neg_view(x.detach()).resolve_neg())
+
+
 def test_second_derivatives_are_refused():
     """The gradient of dispatch depends on what arrives alone; that of combine is taken to depend on its rows too."""
     x, gate, up, down = make()
