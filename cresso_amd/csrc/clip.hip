@@ -42,7 +42,6 @@ struct ClipArgs {
     double* partials;
     float* norm;
     uint32_t count, chunks, blocks;
-    int32_t kind;
     double max_norm, scale;
     int32_t write, in_place;   // write: there are outputs; in_place: every one is its input
 };
@@ -188,13 +187,8 @@ template <bool MAX> __global__ __launch_bounds__(CL_NT) void clip_norm_kernel(Cl
     if (threadIdx.x == 0) a.partials[blockIdx.x] = v;
 }
 
-// The E elements of r times f, rounded once, to `out`; PAST: past the caches.
-template <bool PAST, typename O> __device__ __forceinline__ void clip_store(O* out, u32x4 v) {
-    if constexpr (!PAST) store16(out, v);
-    else if constexpr (sizeof(O) == 4) __builtin_nontemporal_store(v, &((CRESSO_GLOBAL Raw16w*)out)->v);
-    else __builtin_nontemporal_store(v, &((CRESSO_GLOBAL Raw16h*)out)->v);
-}
-template <typename T, typename O, bool PAST> __device__ __forceinline__ void clip_scale_unit(u32x4 r, O* out, double f) {
+// The E elements of r times f, rounded once, to `out`.
+template <typename T, typename O> __device__ __forceinline__ void clip_scale_unit(u32x4 r, O* out, double f) {
     constexpr int E = 16 / (int)sizeof(T);
     if constexpr (sizeof(O) == 8) {
         u32x4 w;
@@ -204,7 +198,7 @@ template <typename T, typename O, bool PAST> __device__ __forceinline__ void cli
             w[2 * i] = (uint32_t)v;
             w[2 * i + 1] = (uint32_t)(v >> 32);
         }
-        clip_store<PAST>((float*)out, w);
+        store16((float*)out, w);
     } else {
         constexpr int EO = Unit<O>::n;   // a unit of 16 bytes in is one or two of fp32 out
 #pragma unroll
@@ -212,23 +206,23 @@ template <typename T, typename O, bool PAST> __device__ __forceinline__ void cli
             float v[EO];
 #pragma unroll
             for (int i = 0; i < EO; ++i) v[i] = (float)(clip_value<T>(r, h * EO + i) * f);
-            clip_store<PAST>(out + h * EO, narrow<O>(v));
+            store16(out + h * EO, narrow<O>(v));
         }
     }
 }
-template <typename T, typename O, bool PAST = false> __device__ __forceinline__ void clip_scale(const T* in, O* out, uint32_t left, double f) {
+template <typename T, typename O> __device__ __forceinline__ void clip_scale(const T* in, O* out, uint32_t left, double f) {
     constexpr int E = 16 / (int)sizeof(T);
     if (left == CL_CHUNK / sizeof(T)) {
         u32x4 r[CL_UNITS];
 #pragma unroll
         for (int u = 0; u < CL_UNITS; ++u) r[u] = clip_load(in + (uint32_t)(u * CL_NT + threadIdx.x) * E);
 #pragma unroll
-        for (int u = 0; u < CL_UNITS; ++u) clip_scale_unit<T, O, PAST>(r[u], out + (uint32_t)(u * CL_NT + threadIdx.x) * E, f);
+        for (int u = 0; u < CL_UNITS; ++u) clip_scale_unit<T, O>(r[u], out + (uint32_t)(u * CL_NT + threadIdx.x) * E, f);
         return;
     }
     for (uint32_t u = threadIdx.x * E; u < left; u += CL_NT * E) {
         if (u + E <= left) {
-            clip_scale_unit<T, O, PAST>(clip_load(in + u), out + u, f);
+            clip_scale_unit<T, O>(clip_load(in + u), out + u, f);
         } else {
             for (uint32_t i = u; i < left; ++i) {
                 if constexpr (sizeof(T) == 8) out[i] = in[i] * f;
@@ -335,7 +329,6 @@ extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t 
     a.count = entries;
     a.chunks = chunks;
     a.blocks = std::min<uint32_t>(chunks, CL_MAX_BLOCKS);
-    a.kind = norm_kind;
     a.max_norm = max_norm;
     a.scale = grad_scale;
     a.in_place = 1;

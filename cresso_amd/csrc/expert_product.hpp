@@ -321,10 +321,11 @@ struct GroupTiles {
     }
     __device__ __forceinline__ uint32_t here() const { return (uint32_t)__builtin_amdgcn_readlane((int)upto, kWave - 1); }
     __device__ __forceinline__ void begin(const GroupArgs& a, int tile) {
+        const uint32_t most = (uint32_t)(a.rows / tile) + (uint32_t)a.experts;   // more only where offsets fall
         all = 0;
         for (int e0 = (a.experts - 1) / kWave * kWave; e0 >= 0; e0 -= kWave) {
             load(a, tile, e0);
-            all += here();
+            all = min(all + here(), most);   // below 2^26 + 2^31
         }
         before = 0;
     }
@@ -734,8 +735,7 @@ __device__ __forceinline__ void group_large_tile(const GroupArgs& a, const Group
         for (int s = 0; s < stages; s += ROUND) {
 #pragma unroll
             for (int i = 0; i < ROUND; ++i) {
-                // 256 sums leave no registers for several ways out: there, stages behind the last are multiplied, as zeros
-                if (FM * FN < 64 && s + i >= stages) break;
+                if (s + i >= stages) break;
                 stage(i % STAGES, i & 1);
             }
         }
@@ -976,12 +976,17 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, G
                 if constexpr (W)                                                                                        \
                     if (plan.whole && plan.tile == 64 && plan.splits < 2) return run(group_small_kernel<T, W, X, 2, 4, 4>, 64); \
             }                                                                                                           \
-            if (plan.whole && plan.tile >= 128) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128);                    \
-            else if (plan.whole) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3>, 64);                                    \
-            else if (sizeof(T) == 4 && plan.words)                                                                      \
-                run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3, sizeof(T) == 4 ? 4 : 16>, 64);                            \
-            else if (plan.tile >= 128) run(group_any_kernel<T, W, X, 1, 4, 8, 2>, 128);                                 \
-            else run(group_any_kernel<T, W, X, 1, 4, 4, 1>, 64);                                                        \
+            if (plan.whole && plan.tile >= 128) {                                                                       \
+                if constexpr (W || sizeof(T) == 2) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128);                 \
+            } else if (plan.whole) {                                                                                    \
+                if constexpr (W || !X || sizeof(T) == 4) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3>, 64);            \
+            } else if (plan.words) {                                                                                    \
+                if constexpr (sizeof(T) == 4) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3, 4>, 64);                    \
+            } else if (plan.tile >= 128) {                                                                              \
+                if constexpr (!W && sizeof(T) == 2) run(group_any_kernel<T, W, X, 1, 4, 8, 2>, 128);                    \
+            } else {                                                                                                    \
+                run(group_any_kernel<T, W, X, 1, 4, 4, 1>, 64);                                                         \
+            }                                                                                                           \
             if (a.splits < 2) return;                                                                                   \
             const int64_t units = ((W ? (int64_t)a.experts * a.m : a.rows) * a.n + Unit<T>::n - 1) / Unit<T>::n;        \
             hipLaunchKernelGGL((group_join_kernel<T, W>), dim3((uint32_t)std::min<int64_t>((units + 255) / 256, 4096)), \

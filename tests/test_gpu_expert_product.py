@@ -169,6 +169,32 @@ def test_offsets_that_are_wrong_stay_within_the_rows():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("inner,outer", [(64, 2048), (2048, 64)])
+def test_falling_offsets_take_no_more_tiles_than_others(inner, outer):
+    """Groups that overlap would be ten times the work; the tiles are as many as of groups that do not, the largest ones too."""
+    announce(f"expert_product falling offsets {inner} {outer}")
+    x, w = rand((20000, inner), torch.bfloat16, 1).requires_grad_(True), rand((20, outer, inner), torch.bfloat16, 2, 0.1).requires_grad_(True)
+    for bad in ([0, 20000] * 10 + [0], [20000] + [0, 2 ** 31 - 1] * 10, [*range(18000, -2000, -1000), 20000]):
+        y = cresso_amd.expert_product(x, w, torch.tensor(bad, dtype=torch.int32).cuda())
+        got = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+        assert got[0].shape == x.shape and got[1].shape == w.shape
+    torch.cuda.synchronize()
+
+
+def test_one_matrix_for_all_experts():
+    """A view that repeats one matrix takes the sum of the experts' gradients, as any view does."""
+    announce("expert_product shared matrix")
+    offsets = offsets_of([30, 0, 34])
+    x, w, d = rand((64, 72), torch.float32, 1), rand((40, 72), torch.float32, 2), rand((64, 40), torch.float32, 3)
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y = cresso_amd.expert_product(a, b.expand(3, 40, 72), offsets)
+    dx, dw = torch.autograd.grad(y, (a, b), d)
+    x64, w64, d64 = x.double(), w.double(), d.double()
+    close(y, x64 @ w64.t(), x64.abs() @ w64.abs().t(), 72 + 16, "product")
+    close(dx, d64 @ w64, d64.abs() @ w64.abs(), 40 + 16, "gradient")
+    close(dw, d64.t() @ x64, d64.abs().t() @ x64.abs(), 64 + 16 + 3, "weight gradient")
+
+
 def test_nothing():
     announce("expert_product nothing")
     for rows, experts, outer, inner in ((0, 3, 5, 4), (6, 0, 5, 4), (6, 2, 0, 4), (6, 2, 5, 0)):
