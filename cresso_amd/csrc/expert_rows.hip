@@ -8,8 +8,8 @@
 // bytes a lane; sums are fp32, over k in order.  Bound by HBM, or for a few
 // tokens by the launch and the two loads that wait for one another.  16384 x
 // 2048 bf16, two experts a token: dispatch 34.9 us (5.8 TB/s read and written),
-// combine 44.2 (4.6), its gradient 69.9 (4.8); 333 x 1001 fp32, three: 4.6, 5.3 and
-// 11.0.  8 to 64 lanes a token, as its row has units, so that narrow rows leave no lanes idle.
+// combine 44.2 (4.6), its gradient 68.3 (4.9); 333 x 1001 fp32, three: 4.6, 5.3 and
+// 10.1.  8 to 64 lanes a token, as its row has units, so that narrow rows leave no lanes idle.
 #include "row_ops.hpp"
 
 #include <algorithm>
@@ -98,12 +98,13 @@ template <typename T> __global__ __launch_bounds__(ER_NT) void combine_kernel(Ro
     }
 }
 
-// Both gradients in one pass over d_out and rows; a token's lanes join their products in a fixed order.
+// Both gradients in one pass over d_out and rows, four units of each on their way a lane (16384 x
+// 2048 bf16 from memory 66 us, one of each 74); a token's lanes join their products in a fixed order.
 template <typename T> __global__ __launch_bounds__(ER_NT) void combine_backward_kernel(RowsArgs a) {
     int lane;
     const int64_t token = token_of(a, lane);
     if (token >= a.tokens) return;
-    constexpr int E = Unit<T>::n;
+    constexpr int E = Unit<T>::n, U = 4;
     const int64_t units = (a.width + E - 1) / E;
     const T* by = (const T*)a.d_out + token * a.d_out_stride;
     for (int k = 0; k < a.top; ++k) {
@@ -114,17 +115,26 @@ template <typename T> __global__ __launch_bounds__(ER_NT) void combine_backward_
             const float w = a.weights ? a.weights[slot] : 1.0f;
             const T* row = (const T*)a.x + place * a.x_stride;
             T* to = (T*)a.out + place * a.width;
-            for (int64_t u = lane; u < units; u += a.lanes) {
-                float d[E], v[E];
-                widen<T>(load_unit(by, u, a.width), d);
-                if (there && a.d_weights) {
-                    widen<T>(load_unit(row, u, a.width), v);
+            const bool dots = there && a.d_weights;
+            for (int64_t u0 = lane; u0 < units; u0 += (int64_t)a.lanes * U) {
+                u32x4 r[U], g[U];
 #pragma unroll
-                    for (int e = 0; e < E; ++e) dot = fmaf(d[e], v[e], dot);
+                for (int i = 0; i < U; ++i) g[i] = load_unit(by, u0 + i * a.lanes, a.width);
+#pragma unroll
+                for (int i = 0; i < U; ++i) r[i] = dots ? load_unit(row, u0 + i * a.lanes, a.width) : u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    float d[E], v[E];
+                    widen<T>(g[i], d);
+                    if (dots) {
+                        widen<T>(r[i], v);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) dot = fmaf(d[e], v[e], dot);
+                    }
+#pragma unroll
+                    for (int e = 0; e < E; ++e) d[e] = there ? d[e] * w : 0.0f;
+                    if (a.out) store_unit(to, u0 + i * a.lanes, a.width, narrow<T>(d));
                 }
-#pragma unroll
-                for (int e = 0; e < E; ++e) d[e] = there ? d[e] * w : 0.0f;
-                if (a.out) store_unit(to, u, a.width, narrow<T>(d));
             }
         }
         if (a.d_weights) {
