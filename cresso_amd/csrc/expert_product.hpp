@@ -206,8 +206,10 @@ template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */,
         }
         ending();
     }
-    // The thread's i-th load to the buffer at `to`, which is the wave's part of it.
-    __device__ __forceinline__ void piece(int i, uint32_t to) const { group_to_lds<V>(buffer, at[i], step, to + i * (NT * V)); }
+    // The thread's i-th load to the buffer at `to`, which is the wave's part of it; more: bytes further along k.
+    __device__ __forceinline__ void piece(int i, uint32_t to, uint32_t more = 0) const {
+        group_to_lds<V>(buffer, at[i], step + more, to + i * (NT * V));
+    }
     __device__ __forceinline__ void fetch(uint32_t to) {
 #pragma unroll
         for (int i = 0; i < P; ++i) piece(i, to);
@@ -807,12 +809,21 @@ __device__ __forceinline__ void group_large_tile(const GroupArgs& a, const Group
 // one's first stages before it stores the one that it has done.  What is left
 // behind the last full round of 256 tiles goes in quarters of 128 x 128, if
 // those take less than a round.
+//
+// A stage along k is 64 bytes of each row, half a line of the caches, and by the
+// time of the other half the line has left the first of them: the second one
+// is asked twice for each.  With PAIRS, for two operands along k in whole pairs of
+// stages, both halves are asked for together, A's in even stages and B's in odd
+// ones; they wait in five stages' memory, of which one holds the result while
+// the next tile's first four arrive (32768 x 2048 -> 5632 by 8: 697 us, so 663).
+// Where B lies across k it gains nothing (672 and 677), where both do it loses (605 and 633).
 constexpr uint32_t kRound = 256;
-template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(256, 1) void group_large_kernel(GroupArgs a) {
+template <typename T, bool WEIGHT, bool B_ACROSS, bool PAIRS> __global__ __launch_bounds__(256, 1) void group_large_kernel(GroupArgs a) {
     constexpr bool ACROSS = WEIGHT || B_ACROSS;   // B
-    constexpr int NT = 256, F = 8, TILE = 32 * F, ROW = 64, STAGES = 4;
+    constexpr int NT = 256, F = 8, TILE = 32 * F, ROW = 64, STAGES = 4;   // ahead
     constexpr int KS = ROW / (int)sizeof(T), STAGE = 2 * TILE * ROW, OWN = 32 * 16 * F * (int)sizeof(T);   // of a wave: 32 of its rows
-    __shared__ __align__(16) uint8_t lds[STAGES * STAGE + 4 * OWN];
+    static_assert(4 * OWN == STAGE && !(PAIRS && ACROSS), "a stage's memory holds 32 rows of each wave's result");
+    __shared__ __align__(16) uint8_t lds[(STAGES + 1) * STAGE];
     if (blockIdx.x >= kRound) {
         group_fill<T>(a, blockIdx.x - kRound, gridDim.x - kRound);
         return;
@@ -829,7 +840,9 @@ template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(2
     const int lane = threadIdx.x & (kWave - 1), l16 = lane & 15, quad = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int wm = (wave & 1) * (16 * F), wn = (wave >> 1) * (16 * F);
-    uint8_t* const own = lds + STAGES * STAGE + wave * OWN;
+    uint32_t cur = 0;   // PAIRS: where the stage lies that is multiplied, among five
+    const auto before = [](uint32_t at) { return at == 0 ? STAGES * STAGE : at - STAGE; };
+    const auto behind = [](uint32_t at) { return at == STAGES * STAGE ? 0 : at + STAGE; };
     const uint32_t mine = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)wave * 1024;
     Fragments<T, WEIGHT, ROW, TILE, 0> fa;
     Fragments<T, ACROSS, ROW, TILE, F> fb;
@@ -854,50 +867,70 @@ template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(2
         stages = (int)((oa.depth + KS - 1) / KS);
         oa.begin();
         ob.begin();
+        uint32_t to = cur;
 #pragma unroll
         for (int i = 0; i < STAGES; ++i) {
-            oa.fetch(mine + i * STAGE);
-            ob.fetch(mine + i * STAGE + TILE * ROW);
+            oa.fetch(mine + (PAIRS ? to : i * STAGE));
+            ob.fetch(mine + (PAIRS ? to : i * STAGE) + TILE * ROW);
+            to = behind(to);
         }
     };
     u32x4 ra[2][F], rb[2][F];
-    // Multiplies the stage in buffer `now`, whose fragments are in set now % 2; reads
-    // the next one's into the other, early enough to be there when the stage ends,
-    // and fills `now` anew.  A wave issues one instruction in 4 cycles and a matrix
+    // Multiplies stage `now`, counted from one of the first to the last buffer (PAIRS:
+    // even or odd), whose fragments are in set now % 2; reads the next one's into
+    // the other, early enough to be there when the stage ends, and fills `now` anew
+    // (PAIRS: A's parts of the buffers of this stage and the one before, or B's of
+    // the two before).  A wave issues one instruction in 4 cycles and a matrix
     // instruction takes 16, so each of them is followed by at most three others.
-    // later: stores that came after the pieces that are waited for.
-    const auto stage = [&](int now, auto later) __attribute__((always_inline)) {
-        group_ready<(STAGES - 2) * LOADS + decltype(later)::value>();
-        const int set = now & 1;
-        const uint8_t* const then = lds + (now + 1) % STAGES * STAGE;
+    // wait: loads and stores that came after the pieces of the next stage.
+    const auto stage = [&](auto now, auto wait) __attribute__((always_inline)) {
+        constexpr int N = decltype(now)::value, set = N & 1;
+        group_ready<decltype(wait)::value>();
+        const uint32_t next = PAIRS ? behind(cur) : (N + 1) % STAGES * STAGE;
+        const uint32_t one = PAIRS ? (set == 0 ? before(cur) : before(before(cur))) : N * STAGE, other = set == 0 ? cur : before(cur);
+        const uint8_t* const then = lds + next;
 #pragma unroll
         for (int t = 0; t < STEPS; ++t) {
             group_mfma_into<T>(rb[set][t % F], ra[set][t / F], acc[t / F][t % F]);
             const int r = t / 3;
             if (t % 3 == 0 && r < F) rb[set ^ 1][r] = fb.read(then + TILE * ROW, 0, r);
             else if (t % 3 == 0 && r < 2 * F) ra[set ^ 1][r - F] = fa.read(then, 0, r - F);
-            const int i = t / 8;
-            if (t % 8 == 1 && i < PA) oa.piece(i, mine + now * STAGE);
-            else if (t % 8 == 1) ob.piece(i - PA, mine + now * STAGE + TILE * ROW);
+            if (t % 8 == 1) {
+                const int i = t / 8, half = i % 2;
+                if (!PAIRS && i < PA) oa.piece(i, mine + one);
+                else if (!PAIRS) ob.piece(i - PA, mine + one + TILE * ROW);
+                else if (set == 0) oa.piece(i / 2, mine + (half ? other : one), half * ROW);
+                else ob.piece(i / 2, mine + (half ? other : one) + TILE * ROW, half * ROW);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
-        oa.next();
-        ob.next();
+        if (!PAIRS || set == 0) oa.next();
+        if (!PAIRS || set == 1) ob.next();
+        if (PAIRS && set == 0) oa.next();
+        if (PAIRS && set == 1) ob.next();
+        cur = next;
     };
     constexpr std::integral_constant<int, 4 * F> STORES{};
-    constexpr std::integral_constant<int, 0> NONE{};
-    const auto first = [&](auto later) __attribute__((always_inline)) {   // the first stage's fragments
+    constexpr std::integral_constant<int, 0> NONE{}, S0{};
+    constexpr std::integral_constant<int, 1> S1{};
+    constexpr std::integral_constant<int, 2> S2{};
+    constexpr std::integral_constant<int, 3> S3{};
+    constexpr std::integral_constant<int, 2 * LOADS> TWO{};             // two stages' loads, or a pair's of A and of B
+    constexpr std::integral_constant<int, (PAIRS ? 1 : 2) * LOADS> LAST{};   // before odd stages: a pair's of A
+    const auto first = [&](auto later) __attribute__((always_inline)) {   // later: stores that came after the first stages' pieces
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 1) * LOADS + decltype(later)::value) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        const uint8_t* const from = lds + (PAIRS ? cur : 0);
 #pragma unroll
-        for (int i = 0; i < F; ++i) rb[0][i] = fb.read(lds + TILE * ROW, 0, i);
+        for (int i = 0; i < F; ++i) rb[0][i] = fb.read(from + TILE * ROW, 0, i);
 #pragma unroll
-        for (int j = 0; j < F; ++j) ra[0][j] = fa.read(lds, 0, j);
-        stage(0, later);
-        stage(1, later);
-        stage(2, later);
-        stage(3, NONE);
+        for (int j = 0; j < F; ++j) ra[0][j] = fa.read(from, 0, j);
+        constexpr std::integral_constant<int, 2 * LOADS + decltype(later)::value> BOTH{};
+        stage(S0, BOTH);
+        stage(S1, BOTH);
+        stage(S2, BOTH);
+        stage(S3, LAST);
     };
     uint32_t u = blockIdx.x;
     if (u < full) {
@@ -905,15 +938,20 @@ template <typename T, bool WEIGHT, bool B_ACROSS> __global__ __launch_bounds__(2
         first(NONE);
     }
     while (u < full) {
-        for (int s = STAGES; s < stages; s += STAGES) {   // 256 sums leave no registers for several ways out: stages behind the last are zeros
-#pragma unroll
-            for (int i = 0; i < STAGES; ++i) stage(i, NONE);
+        for (int s = STAGES; s < stages; s += PAIRS ? 2 : STAGES) {   // 256 sums leave no registers for several ways out: stages behind the last are zeros
+            stage(S0, TWO);
+            stage(S1, LAST);
+            if constexpr (!PAIRS) {
+                stage(S2, TWO);
+                stage(S3, LAST);
+            }
         }
         group_ready<0>();   // nothing is on its way to LDS, and all waves have read it
         const int64_t left = rows - (m0 + wm);   // rows from the wave's first on
         const uint64_t to = (uint64_t)(uintptr_t)(out + (m0 + wm) * a.n + n0 + wn);
         const u32x4 result = {(uint32_t)to, (uint32_t)(to >> 32) & 0xffffu, left > 0 && n0 + wn < a.n ? (uint32_t)(((min(left, (int64_t)128) - 1) * a.n + a.n - n0 - wn) * (int64_t)sizeof(T)) : 0u, 0x00020000u};
         const uint32_t column = n0 + wn + l16 * 8 < a.n ? (uint32_t)l16 * 16 : 0x80000000u;   // beyond the result
+        uint8_t* const own = lds + (PAIRS ? before(cur) : STAGES * STAGE) + wave * OWN;
         u += kRound;
         if (u < full) begin(u);
 #pragma unroll
@@ -999,7 +1037,14 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, G
                     a.tiles_n = (uint32_t)((a.n + 255) / 256);                                                          \
                     a.tiles_m = (uint32_t)((a.m + 255) / 256);                                                          \
                     a.splits = 1;                                                                                       \
-                    hipLaunchKernelGGL((group_large_kernel<T, W, X>), dim3(kRound + (W ? 0 : kFillBlocks)), dim3(256), 0, st, a); \
+                    const dim3 grid(kRound + (W ? 0 : kFillBlocks));                                                    \
+                    if constexpr (!X) {                                                                                 \
+                        if (a.k % 64 == 0) {                                                                            \
+                            hipLaunchKernelGGL((group_large_kernel<T, W, X, true>), grid, dim3(256), 0, st, a);         \
+                            return;                                                                                     \
+                        }                                                                                               \
+                    }                                                                                                   \
+                    hipLaunchKernelGGL((group_large_kernel<T, W, X, false>), grid, dim3(256), 0, st, a);                \
                     return;                                                                                             \
                 }                                                                                                       \
                 if constexpr (X)                                                                                        \

@@ -103,6 +103,16 @@ def test_many_large_tiles(counts, inner, outer, turned, dtype):
     check(sum(counts) + 17, counts, inner, outer, dtype, first=5, turned=turned)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("inner", [64, 128, 192, 576])
+def test_large_tiles_of_whole_pairs_of_stages(inner, dtype):
+    """Depths of 64, of fewer stages than are on their way, and of an odd number of pairs; rows that begin within a cache line."""
+    counts = [9000, 0, 300, 7300]
+    check(16640, counts, inner, 1288, dtype, first=11)
+    wide = rand((16640, inner + 24), dtype, 1)
+    check(16640, counts, inner, 1288, dtype, first=11, x=wide[:, 8:8 + inner], d=rand((16640, 1288), dtype, 2))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_one_long_group(dtype):
     """A weight gradient whose sum is long and whose matrix is small."""
