@@ -18,8 +18,8 @@
 //
 // Few rows are bound by HBM (16 by 16 experts, 2048 -> 5632 bf16: 44.2 us, 5.3 TB/s
 // of the matrices that are met), many by the matrix instructions and the power
-// that they draw (32768 by 8: 690 to 724 us, 660 to 678 for the gradient of x, 622 to 656
-// for the weights', 1.05 to 1.2 PFLOP/s), odd sizes by tiles that are partly empty.
+// that they draw (32768 by 8: 663 to 678 us, 661 to 677 for the gradient of x, 603 to 618
+// for the weights', 1.1 to 1.26 PFLOP/s), odd sizes by tiles that are partly empty.
 #pragma once
 
 #include "row_ops.hpp"
@@ -802,13 +802,13 @@ __device__ __forceinline__ void group_large_tile(const GroupArgs& a, const Group
     }
 }
 
-// 256 x 256 of 16 bits, one workgroup to a CU, bound by the matrix unit (busy 63
-// to 71 % of the cycles at a clock that falls to 1.8 GHz under it): eight waves of 128 x 64 would
-// read 96 KB of LDS a stage, as long as their matrix instructions take; four of
-// 128 x 128 read 64.  A workgroup goes from tile to tile, and asks for the next
-// one's first stages before it stores the one that it has done.  What is left
-// behind the last full round of 256 tiles goes in quarters of 128 x 128, if
-// those take less than a round.
+// 256 x 256 of 16 bits, one workgroup to a CU, bound by power and the matrix unit
+// (busy 65 to 73 % of the cycles at a clock that falls to 1.8 GHz): eight waves of
+// 128 x 64 would read 96 KB of LDS a stage, as long as their matrix instructions
+// take; four of 128 x 128 read 64.  A workgroup goes from tile to tile, and asks
+// for the next one's first stages before it stores the one that it has done.
+// What is left behind the last full round of 256 tiles goes in quarters of 128 x
+// 128, if those take less than a round.
 //
 // A stage along k is 64 bytes of each row, half a line of the caches, and by the
 // time of the other half the line has left the first of them: the second one
