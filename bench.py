@@ -181,7 +181,8 @@ TRAFFIC_FILES = {"c2": "profiles/spectral_step_c2_hbm_traffic.md", "c3": "profil
 SOURCE_GLOBS = ("cresso_amd/csrc/*.hip", "cresso_amd/csrc/*.hpp", "cresso_amd/csrc/*.cpp")
 # the operators around the optimizer's step: no workload here launches them, none of its sources includes them
 OPERATOR_SOURCES = {"block_product.hip", "distill.hip", "embedding.hip", "residual_norm.hip", "row_ops.hpp", "overlap.hpp",
-                    "operators.cpp"}
+                    "clip.hip", "routing.hip", "expert_rows.hip", "expert_product.hip", "expert_product.hpp",
+                    "expert_product_bf16.hip", "expert_product_f16.hip", "expert_product_f32.hip", "operators.cpp"}
 
 
 def source_digest():
