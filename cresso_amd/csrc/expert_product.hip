@@ -17,7 +17,7 @@ int32_t check_group(const char* what, int32_t dtype, int64_t rows, int64_t a, in
     const auto tiles = [](int64_t n) { return (n + 63) / 64; };
     const int64_t most = ((int64_t)1 << 24) - 4096;
     if (rows >= (int64_t)1 << 31 || a >= (int64_t)1 << 22 || b >= (int64_t)1 << 22 || experts > 1 << 16 ||
-        (rows / 64 + experts) * tiles(std::max(a, b)) >= most || experts * (tiles(a) * tiles(b)) >= most)
+        (rows / 32 + experts) * tiles(std::max(a, b)) >= most || experts * (tiles(a) * tiles(b)) >= most)
         return fail(CRESSO_E_UNSUPPORTED, "%s: %lld rows, %d matrices of %lld x %lld are more than one call takes", what, (long long)rows,
                     experts, (long long)a, (long long)b);
     return CRESSO_OK;
@@ -40,7 +40,7 @@ bool large_result(const void* out, int64_t n) { return ((uintptr_t)out & 15) == 
 // of 512 x 2048 -> 2048 by 8 experts are 64 (16.8 us, 23.5 and 22.1), of 2000
 // by 32 with 1024 columns 128 (31.8, 26.1, 41.9), of 16384 by 8 256 (215, 151,
 // 129).  With w across k, tiles of 128 take 12 + 0.075 and those of 64 are no
-// faster anywhere.  fp32 takes 64 (2048 x 1024 -> 4096 by 8: 167 us, 193).
+// faster anywhere.  fp32 products take 32 x 64 at any size (kGroupHigh says why).
 // Weight gradients take 256 from three rounds of them on, if they have rows
 // enough to be more than a store (16384 rows by 64 experts of 2048 x 1024: 173 us,
 // 196 with 128; 2000 by 32: 59 and 53; 8192 by 8 of 2048 x 2048: 75 and 72).
@@ -48,14 +48,15 @@ bool large_result(const void* out, int64_t n) { return ((uintptr_t)out & 15) == 
 // Where the tiles leave CUs idle, k is split into parts of 8 stages or more: for
 // 16 bits below 256 tiles (64 x 4096 -> 256 by 2: 19.6 us in one part, 11.4 in 8;
 // 512 x 2048 -> 2048 by 8, 384 tiles, 15.7 and 21.5 in 2), for fp32, whose tiles
-// take longer, below 768 (777 x 1001 -> 1500 by 9, 396 tiles: 41.8 us and 50.1 in
-// 2; its gradient, 264 tiles: 61.4 and 47.9).
+// take longer, below 768 (300 x 4097 -> 515 by 4, 102 tiles: 67.6 us in one part, 35.4
+// in 3, 33.3 in 5 or 7).
 GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t experts, int32_t dtype, bool weight, bool across, bool whole, bool large) {
     const bool wide = dtype == CRESSO_F32;
     const int64_t e = std::max(experts, 1);
     const auto tiles = [&](int64_t t) -> double {
         const double across = (double)((n + t - 1) / t);
-        return across * (weight ? (double)e * (double)((m + t - 1) / t) : (double)rows / t + 0.5 * (double)std::min(e, rows));
+        const int64_t high = wide && !weight ? kGroupHigh<float, false> : t;
+        return across * (weight ? (double)e * (double)((m + t - 1) / t) : (double)rows / high + 0.5 * (double)std::min(e, rows));
     };
     GroupPlan p{64, 1, whole, false};
     if (weight) {

@@ -629,7 +629,7 @@ template <int KS, typename A, typename B> __device__ __forceinline__ void group_
 
 // The same for operands that go to LDS by themselves, STAGES - 1 stages ahead of
 // the one that is multiplied: V = 16 for whole aligned pieces, 4 for fp32 of any
-// alignment (777 x 1001 -> 1500 by 9 41.8 us, through registers 54.9).
+// alignment (777 x 1001 -> 1500 by 9 in tiles of 64 x 64 41.8 us, through registers 54.9).
 template <typename T, bool WEIGHT, bool B_ACROSS, int WM, int WN, int FM, int FN, int ROW, int STAGES, int V = 16>
 __global__ __launch_bounds__(WM* WN * 64, 2) void group_kernel(GroupArgs a) {
     constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16;
@@ -1010,9 +1010,14 @@ template <typename T, bool WEIGHT, bool B_ACROSS, int F, int STAGES, int BLOCKS>
     if (group_begin<WEIGHT>(a, 32 * F, 32 * F, w)) group_large_tile<T, WEIGHT, WEIGHT || B_ACROSS, F, F, STAGES>(a, w, lds);
 }
 
+// The rows of a tile that is 64 wide.  fp32 products take 32: experts' last tiles are
+// emptier where they are higher, and 256 CUs share the others more evenly (777 x
+// 1001 -> 1500 by 9: 36.5 us, 43.0 with 64 rows, the gradient of x 39.5 and 52; 777 x
+// 1024 -> 1536 32.7 and 40.2; 2500 rows an expert lose 3 %).
+template <typename T, bool WEIGHT> constexpr int kGroupHigh = sizeof(T) == 4 && !WEIGHT ? 32 : 64;
 // How a product is computed: the side of its tiles, and into how many parts k is split.
 struct GroupPlan {
-    int tile;
+    int tile;     // 64, 128 or 256; 64 stands for kGroupHigh x 64
     uint32_t splits;
     bool whole;   // aligned, whole pieces
     bool words;   // fp32 of any alignment whose rows lie apart, near enough for a buffer
@@ -1022,10 +1027,10 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, G
 
 #define CRESSO_GROUP_LAUNCH(T)                                                                                          \
     template <> void group_launch<T>(GroupArgs a, bool weight, bool across, GroupPlan plan, hipStream_t st) {           \
-        const auto run = [&](auto kernel, int tile, uint32_t more = 0) {                                                \
-            a.tiles_n = (uint32_t)((a.n + tile - 1) / tile);                                                            \
-            a.tiles_m = (uint32_t)(weight ? (a.m + tile - 1) / tile : a.rows / tile + a.experts);                       \
-            a.tiles = a.tiles_m * a.tiles_n * (weight ? (uint32_t)a.experts : 1u) + more;                               \
+        const auto run = [&](auto kernel, int high, int wide) {                                                         \
+            a.tiles_n = (uint32_t)((a.n + wide - 1) / wide);                                                            \
+            a.tiles_m = (uint32_t)(weight ? (a.m + high - 1) / high : a.rows / high + a.experts);                       \
+            a.tiles = a.tiles_m * a.tiles_n * (weight ? (uint32_t)a.experts : 1u);                                      \
             a.splits = plan.splits;                                                                                     \
             hipLaunchKernelGGL(kernel, dim3(a.tiles * a.splits + (weight || a.splits > 1 ? 0 : kFillBlocks)),           \
                                dim3(256), 0, st, a);                                                                    \
@@ -1048,20 +1053,21 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, G
                     return;                                                                                             \
                 }                                                                                                       \
                 if constexpr (X)                                                                                        \
-                    if (plan.whole && plan.tile == 128 && plan.splits < 2) return run(group_small_kernel<T, W, X, 4, 4, 2>, 128); \
+                    if (plan.whole && plan.tile == 128 && plan.splits < 2) return run(group_small_kernel<T, W, X, 4, 4, 2>, 128, 128);\
                 if constexpr (W)                                                                                        \
-                    if (plan.whole && plan.tile == 64 && plan.splits < 2) return run(group_small_kernel<T, W, X, 2, 4, 4>, 64); \
+                    if (plan.whole && plan.tile == 64 && plan.splits < 2) return run(group_small_kernel<T, W, X, 2, 4, 4>, 64, 64);\
             }                                                                                                           \
+            constexpr int FM = kGroupHigh<T, W> / 16, STAGES = FM == 2 ? 2 : 3;                                         \
             if (plan.whole && plan.tile >= 128) {                                                                       \
-                if constexpr (W || sizeof(T) == 2) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128);                 \
+                if constexpr (W || sizeof(T) == 2) run(group_kernel<T, W, X, 1, 4, 8, 2, 128, 2>, 128, 128);            \
             } else if (plan.whole) {                                                                                    \
-                if constexpr (W || !X || sizeof(T) == 4) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3>, 64);            \
+                if constexpr (W || !X || sizeof(T) == 4) run(group_kernel<T, W, X, 1, 4, FM, 1, 128, STAGES>, 16 * FM, 64);\
             } else if (plan.words) {                                                                                    \
-                if constexpr (sizeof(T) == 4) run(group_kernel<T, W, X, 1, 4, 4, 1, 128, 3, 4>, 64);                    \
+                if constexpr (sizeof(T) == 4) run(group_kernel<T, W, X, 1, 4, FM, 1, 128, STAGES, 4>, 16 * FM, 64);     \
             } else if (plan.tile >= 128) {                                                                              \
-                if constexpr (!W && sizeof(T) == 2) run(group_any_kernel<T, W, X, 1, 4, 8, 2>, 128);                    \
+                if constexpr (!W && sizeof(T) == 2) run(group_any_kernel<T, W, X, 1, 4, 8, 2>, 128, 128);               \
             } else {                                                                                                    \
-                run(group_any_kernel<T, W, X, 1, 4, 4, 1>, 64);                                                         \
+                run(group_any_kernel<T, W, X, 1, 4, FM, 1>, 16 * FM, 64);                                               \
             }                                                                                                           \
             if (a.splits < 2) return;                                                                                   \
             const int64_t units = ((W ? (int64_t)a.experts * a.m : a.rows) * a.n + Unit<T>::n - 1) / Unit<T>::n;        \

@@ -597,7 +597,7 @@ int32_t cresso_combine_backward(const void* rows, int64_t rows_stride, const voi
  * once.  w_expert_stride and w_stride: elements between experts and rows.
  * Offsets that are not so leave results unspecified, but nothing outside the
  * operands is read or written.  Rows below 2^31, widths below 2^22, at most
- * 65536 experts; (rows / 64 + experts) * the wider side / 64, and the matrices'
+ * 65536 experts; (rows / 32 + experts) * the wider side / 64, and the matrices'
  * elements / 4096, below 2^24. */
 size_t cresso_expert_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype);
 int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int64_t depth,

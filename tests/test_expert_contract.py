@@ -192,7 +192,7 @@ def test_product_arguments(lib):
     refused(lib, product(turned=1, w_stride=15), -1, "row stride")
     refused(lib, product(expert=-1), -1, "stride between experts")
     refused(lib, product(depth=1 << 23), -3, "more than one call takes")
-    refused(lib, product(rows=1 << 30, cols=64, dtype=F32), -3, "more than one call takes")   # 2^24 tiles of 64 x 64
+    refused(lib, product(rows=1 << 30, cols=64, dtype=F32), -3, "more than one call takes")   # 2^25 tiles of 32 x 64
     refused(lib, product(rows=1 << 21, cols=1 << 15), -3, "more than one call takes")
     refused(lib, weight(experts=1 << 16, pw=1024, qw=1024, p_stride=1024, q_stride=1024), -3, "more than one call takes")
     refused(lib, weight(p=NULL), -1, "null")
