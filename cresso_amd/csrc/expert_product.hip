@@ -29,8 +29,8 @@ bool whole_rows(const void* p, int64_t width, int64_t stride, int32_t dtype) {
     const int64_t e = dtype == CRESSO_F32 ? 4 : 8;
     return ((uintptr_t)p & 15) == 0 && width % e == 0 && stride % e == 0 && near_rows(width, stride);
 }
-// Whether rows of the result are whole pieces of 16 bytes of 16-bit numbers, as the large tiles store them.
-bool large_result(const void* out, int64_t n) { return ((uintptr_t)out & 15) == 0 && n % 8 == 0 && n < (int64_t)1 << 21; }
+// Whether rows of the result are whole pieces of 16 bytes of 16-bit numbers: others take the large tiles longer to store.
+bool piece_rows(const void* out, int64_t n) { return ((uintptr_t)out & 15) == 0 && n % 8 == 0; }
 
 // Which tiles, and whether k is split.
 //
@@ -76,26 +76,89 @@ GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t 
     p.splits = std::max(p.splits, 1u);
     return p;
 }
-size_t group_bytes(const GroupPlan& p, int64_t results) { return p.splits > 1 ? (size_t)p.splits * (size_t)results * 4 : 16; }
+size_t group_bytes(const GroupPlan& p, int64_t results) { return p.splits > 1 ? ((size_t)p.splits * (size_t)results * 4 + 15) / 16 * 16 : 16; }
+
+// ---------------------------------------------------------------------------
+// Rows of 16-bit numbers that are no whole pieces, laid out anew: in a workspace,
+// with zeros behind each row's end.
+// ---------------------------------------------------------------------------
+struct PadArgs {
+    const __half* from;
+    __half* to;
+    int64_t rows, width, stride;        // of all matrices
+    int64_t matrix_rows, matrix_stride;
+    int32_t lanes;                      // of a row: a power of two
+};
+__global__ __launch_bounds__(256) void group_pad_kernel(PadArgs a) {
+    const int lane = threadIdx.x & (a.lanes - 1), per = 256 / a.lanes;
+    const int64_t units = (a.width + 7) / 8;
+    for (int64_t r = (int64_t)blockIdx.x * per + threadIdx.x / a.lanes; r < a.rows; r += (int64_t)gridDim.x * per) {
+        const int64_t e = r / a.matrix_rows;
+        const __half* row = a.from + e * a.matrix_stride + (r - e * a.matrix_rows) * a.stride;
+        for (int64_t u = lane; u < units; u += a.lanes) store16(a.to + (r * units + u) * 8, load_unit(row, u, a.width));
+    }
+}
+int64_t padded(int64_t width) { return (width + 7) / 8 * 8; }
+void group_pad(const void* from, void* to, int64_t matrices, int64_t matrix_rows, int64_t matrix_stride, int64_t width, int64_t stride, hipStream_t st) {
+    PadArgs a{(const __half*)from, (__half*)to, matrices * matrix_rows, width, stride, matrix_rows, matrix_stride, 8};
+    while (a.lanes < kWave && a.lanes * 8 < width) a.lanes *= 2;
+    const int64_t per = 256 / a.lanes;
+    if (a.rows == 0) return;
+    hipLaunchKernelGGL(group_pad_kernel, dim3((uint32_t)std::min<int64_t>((a.rows + per - 1) / per, 1 << 16)), dim3(256), 0, st, a);
+}
+// Whether that is worth it: the copies take 1 us a million numbers (4 TB/s) and 6
+// for two launches, and save, in us a GFLOP measured with and without them, 0.6 to
+// 1 of a product along k, 0.9 to 2.2 of one across, 2.7 to 5 of a weight gradient
+// (16384 x 2047 -> 4095 by 8: 554 us without, 407 with, 721 and 435, 1355 and 330; 8192 x
+// 1001 -> 1501 by 8: 68 and 71, 108 and 70, 128 and 63; 2000 by 32: 35 and 63, 74 and 64, 82 and 61).
+bool group_pads(int64_t rows, int64_t cols, int64_t depth, int64_t numbers, int32_t dtype, double gain) {
+    if (dtype == CRESSO_F32) return false;
+    const double gflop = 2e-9 * (double)rows * (double)cols * (double)depth;
+    return gflop * gain > 6.0 + 1e-6 * (double)numbers;
+}
+constexpr int64_t kPadMost = ((int64_t)1 << 21) - 8;   // near_rows of the copies
+constexpr double kPadAlong = 1.0, kPadAcross = 2.2, kPadWeight = 3.5;   // us a GFLOP: w along k, w across it, the weight gradient
 }  // namespace
 }  // namespace cresso
 
 using namespace cresso;
 
-extern "C" size_t cresso_expert_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype) {
-    if (check_group("expert product", dtype, rows, cols, depth, experts) != CRESSO_OK) return 0;
+// Numbers of the copies of x and w, where rows of `depth` or `w_cols` are no whole pieces.
+static int64_t product_copies(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype, bool turned) {
+    const int64_t w_cols = turned ? cols : depth;
+    if ((depth % 8 == 0 && w_cols % 8 == 0) || std::max(depth, w_cols) >= kPadMost) return 0;
+    const int64_t numbers = rows * padded(depth) + experts * (turned ? depth : cols) * padded(w_cols);
+    return group_pads(rows, cols, depth, numbers, dtype, turned ? kPadAcross : kPadAlong) ? numbers : 0;
+}
+static int64_t weight_copies(int64_t rows, int64_t p_width, int64_t q_width, int32_t dtype) {
+    if ((p_width % 8 == 0 && q_width % 8 == 0) || std::max(p_width, q_width) >= kPadMost) return 0;
+    const int64_t numbers = rows * (padded(p_width) + padded(q_width));
+    return group_pads(rows, p_width, q_width, numbers, dtype, kPadWeight) ? numbers : 0;
+}
+
+// Bytes of the sums, where k is split, whatever the operands' layouts; copies come behind them.
+static size_t product_sums(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype) {
     size_t most = 0;
     for (int i = 0; i < 8; ++i)
         most = std::max(most, group_bytes(group_plan(rows, 0, cols, depth, experts, dtype, false, i & 1, i & 2, (i & 4) && (i & 2)), rows * cols));
     return most;
 }
-extern "C" size_t cresso_expert_product_weight_workspace_bytes(int64_t rows, int64_t p_width, int64_t q_width, int32_t experts,
-                                                               int32_t dtype) {
-    if (check_group("expert product gradient", dtype, rows, p_width, q_width, experts) != CRESSO_OK) return 0;
+static size_t weight_sums(int64_t rows, int64_t p_width, int64_t q_width, int32_t experts, int32_t dtype) {
     size_t most = 0;
     for (int i = 0; i < 3; ++i)
         most = std::max(most, group_bytes(group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, i > 0, i > 1), experts * p_width * q_width));
     return most;
+}
+
+extern "C" size_t cresso_expert_product_workspace_bytes(int64_t rows, int64_t cols, int64_t depth, int32_t experts, int32_t dtype) {
+    if (check_group("expert product", dtype, rows, cols, depth, experts) != CRESSO_OK) return 0;
+    return product_sums(rows, cols, depth, experts, dtype) +
+           2 * (size_t)std::max(product_copies(rows, cols, depth, experts, dtype, false), product_copies(rows, cols, depth, experts, dtype, true));
+}
+extern "C" size_t cresso_expert_product_weight_workspace_bytes(int64_t rows, int64_t p_width, int64_t q_width, int32_t experts,
+                                                               int32_t dtype) {
+    if (check_group("expert product gradient", dtype, rows, p_width, q_width, experts) != CRESSO_OK) return 0;
+    return weight_sums(rows, p_width, q_width, experts, dtype) + 2 * (size_t)weight_copies(rows, p_width, q_width, dtype);
 }
 
 extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int64_t depth,
@@ -127,8 +190,23 @@ extern "C" int32_t cresso_expert_product(const void* x, int64_t x_stride, int32_
     a.b_expert = w_expert_stride;
     a.experts = experts;
     a.sums = (float*)workspace;
-    const bool whole = whole_rows(x, depth, x_stride, dtype) && whole_rows(w, w_cols, w_stride, dtype) && w_expert_stride % (dtype == CRESSO_F32 ? 4 : 8) == 0;
-    GroupPlan plan = group_plan(rows, 0, cols, depth, experts, dtype, false, turned != 0, whole, whole && large_result(out, cols));
+    a.k_along = depth;
+    a.b_across = cols;
+    bool whole = whole_rows(x, depth, x_stride, dtype) && whole_rows(w, w_cols, w_stride, dtype) && w_expert_stride % (dtype == CRESSO_F32 ? 4 : 8) == 0;
+    if (!whole && product_copies(rows, cols, depth, experts, dtype, turned != 0)) {
+        __half* const to = (__half*)((char*)workspace + product_sums(rows, cols, depth, experts, dtype));
+        group_pad(x, to, 1, rows, 0, depth, x_stride, (hipStream_t)stream);
+        a.a = to;
+        a.a_stride = a.k_along = padded(depth);
+        a.b = to + rows * a.a_stride;
+        a.b_stride = padded(w_cols);
+        group_pad(w, (void*)a.b, experts, w_rows, w_expert_stride, w_cols, w_stride, (hipStream_t)stream);
+        a.b_expert = w_rows * a.b_stride;
+        a.b_across = a.b_stride;
+        whole = true;
+    }
+    a.out_pieces = piece_rows(out, cols);
+    GroupPlan plan = group_plan(rows, 0, cols, depth, experts, dtype, false, turned != 0, whole, whole && cols < kPadMost);
     plan.words = dtype == CRESSO_F32 && near_rows(depth, x_stride) && near_rows(w_cols, w_stride);
     with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, false, turned != 0, plan, (hipStream_t)stream); });
     return launched(what);
@@ -160,8 +238,21 @@ extern "C" int32_t cresso_expert_product_weight(const void* p, int64_t p_stride,
     a.b_stride = q_stride;
     a.experts = experts;
     a.sums = (float*)workspace;
-    const bool whole = whole_rows(p, p_width, p_stride, dtype) && whole_rows(q, q_width, q_stride, dtype);
-    GroupPlan plan = group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, whole, whole && large_result(out, q_width));
+    a.a_across = p_width;
+    a.b_across = q_width;
+    bool whole = whole_rows(p, p_width, p_stride, dtype) && whole_rows(q, q_width, q_stride, dtype);
+    if (!whole && weight_copies(rows, p_width, q_width, dtype)) {
+        __half* const to = (__half*)((char*)workspace + weight_sums(rows, p_width, q_width, experts, dtype));
+        a.a_stride = a.a_across = padded(p_width);
+        a.b_stride = a.b_across = padded(q_width);
+        a.a = to;
+        a.b = to + rows * a.a_stride;
+        group_pad(p, to, 1, rows, 0, p_width, p_stride, (hipStream_t)stream);
+        group_pad(q, (void*)a.b, 1, rows, 0, q_width, q_stride, (hipStream_t)stream);
+        whole = true;
+    }
+    a.out_pieces = piece_rows(out, q_width);
+    GroupPlan plan = group_plan(rows, p_width, q_width, 0, experts, dtype, true, true, whole, whole && q_width < kPadMost);
     plan.words = dtype == CRESSO_F32 && near_rows(p_width, p_stride) && near_rows(q_width, q_stride);
     with_row_dtype(dtype, [&](auto t) { group_launch<decltype(t)>(a, true, true, plan, (hipStream_t)stream); });
     return launched(what);

@@ -35,10 +35,12 @@ struct GroupArgs {
     const int32_t* offsets;
     int64_t rows;                          // of all experts
     int64_t m, n, k;                       // product: n columns, k depth; weight gradient: m and n
+    int64_t k_along, a_across, b_across;   // what rows hold of k, m and n where they end in zeros of a copy, else k, m and n
     int64_t a_stride, b_stride, b_expert;  // elements
     int32_t experts;
     uint32_t tiles_m, tiles_n;             // product: tiles_m is the most there can be
     uint32_t tiles;                        // workgroups of tiles; those behind them fill rows without an expert
+    int32_t out_pieces;   // the result's rows are whole aligned pieces
     // where k is split: parts of it, each with workgroups for all tiles, and their sums [splits][result] in fp32
     uint32_t splits;
     float* sums;
@@ -436,7 +438,7 @@ __device__ __forceinline__ void group_operands(const GroupArgs& a, const GroupWo
     if constexpr (WEIGHT) {
         oa.base = (const T*)a.a + w.first * a.a_stride + w.m0;
         ob.base = (const T*)a.b + w.first * a.b_stride + w.n0;
-        oa.size = a.m - w.m0;
+        oa.size = a.a_across - w.m0;
         oa.depth = ob.depth = w.end - w.first;
         out = (T*)a.out + (int64_t)w.expert * a.m * a.n;
         rows = a.m;
@@ -444,11 +446,12 @@ __device__ __forceinline__ void group_operands(const GroupArgs& a, const GroupWo
         oa.base = (const T*)a.a + (w.first + w.m0) * a.a_stride;
         ob.base = (const T*)a.b + w.expert * a.b_expert + (ACROSS ? w.n0 : w.n0 * a.b_stride);
         oa.size = w.end - w.first - w.m0;
-        oa.depth = ob.depth = a.k;
+        oa.depth = a.k_along;
+        ob.depth = ACROSS ? a.k : a.k_along;
         out = (T*)a.out + w.first * a.n;
         rows = w.end - w.first;
     }
-    ob.size = a.n - w.n0;
+    ob.size = (ACROSS ? a.b_across : a.n) - w.n0;
     oa.stride = a.a_stride;
     ob.stride = a.b_stride;
 }
@@ -469,7 +472,8 @@ template <bool WEIGHT, bool ACROSS, int KS, typename A, typename B> __device__ _
     const int64_t k0 = stages * part / a.splits * KS, k1 = min(stages * (part + 1) / a.splits * KS, oa.depth);
     oa.base += WEIGHT ? k0 * oa.stride : k0;
     ob.base += ACROSS ? k0 * ob.stride : k0;
-    oa.depth = ob.depth = max(k1 - k0, (int64_t)0);
+    oa.depth = max(k1 - k0, (int64_t)0);
+    ob.depth = max(min(ob.depth, k1) - k0, (int64_t)0);
 }
 // A lane holds columns 4 quad to 4 quad + 3 of each fragment's 16, or with B
 // along k 4 FN columns in one piece, of rows l16 of each of FM fragments from m on.
@@ -544,7 +548,8 @@ template <typename T, bool WEIGHT> __global__ __launch_bounds__(256) void group_
 }
 
 // WM x WN waves of FM x FN fragments of 16 x 16 each; operands of any alignment, through registers, for
-// rows that do not go to LDS by themselves: 16 bits at odd strides or addresses, fp32 rows far apart.
+// rows that do not go to LDS by themselves: 16 bits at odd strides or addresses that are not laid out anew, fp32
+// rows far apart.
 template <typename T, bool WEIGHT, bool B_ACROSS, int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(WM* WN * 64, 2) void group_any_kernel(GroupArgs a) {
     constexpr int NT = WM * WN * 64, TM = WM * FM * 16, TN = WN * FN * 16, ROW = 128;
@@ -950,6 +955,7 @@ template <typename T, bool WEIGHT, bool B_ACROSS, bool PAIRS> __global__ __launc
         const int64_t left = rows - (m0 + wm);   // rows from the wave's first on
         const uint64_t to = (uint64_t)(uintptr_t)(out + (m0 + wm) * a.n + n0 + wn);
         const u32x4 result = {(uint32_t)to, (uint32_t)(to >> 32) & 0xffffu, left > 0 && n0 + wn < a.n ? (uint32_t)(((min(left, (int64_t)128) - 1) * a.n + a.n - n0 - wn) * (int64_t)sizeof(T)) : 0u, 0x00020000u};
+        const int wide = (int)min(a.n - n0 - wn, (int64_t)128);   // columns from the wave's first on
         const uint32_t column = n0 + wn + l16 * 8 < a.n ? (uint32_t)l16 * 16 : 0x80000000u;   // beyond the result
         uint8_t* const own = lds + (PAIRS ? before(cur) : STAGES * STAGE) + wave * OWN;
         u += kRound;
@@ -973,12 +979,24 @@ template <typename T, bool WEIGHT, bool B_ACROSS, bool PAIRS> __global__ __launc
                 group_zero(acc[j]);
             }
             __builtin_amdgcn_wave_barrier();
+            if (!a.out_pieces) {
+                T* const rest = (T*)(uintptr_t)((uint64_t)result[1] << 32 | result[0]) + l16 * 8;
+                for (int row = quad; row < 32; row += 4) {
+                    if (p * 32 + row >= left) break;
+                    const u32x4 v = *(const u32x4*)(own + row * 256 + ((l16 ^ (row & 15)) * 16));
+                    T* const to = rest + (p * 32 + row) * a.n;
+                    if (l16 * 8 + 8 <= wide) store16(to, v);
+                    else if (l16 * 8 < wide) store_part(to, v, wide - l16 * 8);
+                }
+                if (p == F / 2 - 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // they are no fixed number, which `first` counts on
+            } else {
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const int row = r * 4 + quad;
-                const u32x4 v = *(const u32x4*)(own + row * 256 + ((l16 ^ (row & 15)) * 16));
-                const uint32_t at = column + (uint32_t)(p * 32 + row) * (uint32_t)(a.n * (int64_t)sizeof(T));
-                __builtin_amdgcn_raw_buffer_store_b128(v, __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)((uint64_t)result[1] << 32 | result[0]), (short)0, (int)result[2], 0x00020000), at, 0, 0);
+                for (int r = 0; r < 8; ++r) {
+                    const int row = r * 4 + quad;
+                    const u32x4 v = *(const u32x4*)(own + row * 256 + ((l16 ^ (row & 15)) * 16));
+                    const uint32_t at = column + (uint32_t)(p * 32 + row) * (uint32_t)(a.n * (int64_t)sizeof(T));
+                    __builtin_amdgcn_raw_buffer_store_b128(v, __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)((uint64_t)result[1] << 32 | result[0]), (short)0, (int)result[2], 0x00020000), at, 0, 0);
+                }
             }
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_sched_barrier(0);
@@ -1044,7 +1062,7 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, G
                     a.splits = 1;                                                                                       \
                     const dim3 grid(kRound + (W ? 0 : kFillBlocks));                                                    \
                     if constexpr (!X) {                                                                                 \
-                        if (a.k % 64 == 0) {                                                                            \
+                        if (a.k_along % 64 == 0) {                                                                           \
                             hipLaunchKernelGGL((group_large_kernel<T, W, X, true>), grid, dim3(256), 0, st, a);         \
                             return;                                                                                     \
                         }                                                                                               \

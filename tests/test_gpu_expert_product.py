@@ -113,6 +113,35 @@ def test_large_tiles_of_whole_pairs_of_stages(inner, dtype):
     check(16640, counts, inner, 1288, dtype, first=11, x=wide[:, 8:8 + inner], d=rand((16640, 1288), dtype, 2))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts,inner,outer,turned", [
+    ([9000, 0, 300, 7300], 333, 1283, False),    # operands laid out anew, results in rows of any alignment
+    ([9000, 0, 300, 7300], 1283, 333, False),
+    ([9000, 0, 300, 7300], 1283, 333, True),
+    ([9000, 0, 300, 7300], 336, 1283, True),     # one of the two sides is whole pieces
+    ([130 + 3 * (e % 7) for e in range(48)], 1001, 1037, False),   # weight gradients of several large tiles to a workgroup
+])
+def test_large_products_of_odd_rows(counts, inner, outer, turned, dtype):
+    check(sum(counts) + 17, counts, inner, outer, dtype, first=5, turned=turned)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_odd_rows_at_a_stride(dtype):
+    """Slices of wider rows and of larger matrices: what lies beside them (NaN) is neither read nor written."""
+    counts, inner, outer = [9000, 0, 300, 7300], 333, 1283
+    offsets = offsets_of(counts)
+    x, w, d = rand((16600, inner), dtype, 1), rand((4, outer, inner), dtype, 2, 0.5), rand((16600, outer), dtype, 3)
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y = cresso_amd.expert_product(a, b, offsets)
+    want = [y, *torch.autograd.grad(y, (a, b), d)]
+    wide, big, dwide = (torch.full(n, math.nan, dtype=dtype, device="cuda") for n in ((16600, inner + 9), (4, outer + 3, inner + 5), (16600, outer + 4)))
+    wide[:, 3:3 + inner], big[:, 1:1 + outer, 2:2 + inner], dwide[:, 1:1 + outer] = x, w, d
+    a, b = wide[:, 3:3 + inner].detach().requires_grad_(True), big[:, 1:1 + outer, 2:2 + inner].detach().requires_grad_(True)
+    y = cresso_amd.expert_product(a, b, offsets)
+    for got, exact in zip([y, *torch.autograd.grad(y, (a, b), dwide[:, 1:1 + outer])], want):
+        assert torch.equal(got, exact)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_one_long_group(dtype):
     """A weight gradient whose sum is long and whose matrix is small."""
