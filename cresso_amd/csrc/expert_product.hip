@@ -40,7 +40,8 @@ bool piece_rows(const void* out, int64_t n) { return ((uintptr_t)out & 15) == 0 
 // of 512 x 2048 -> 2048 by 8 experts are 64 (16.8 us, 23.5 and 22.1), of 2000
 // by 32 with 1024 columns 128 (31.8, 26.1, 41.9), of 16384 by 8 256 (215, 151,
 // 129).  With w across k, tiles of 128 take 12 + 0.075 and those of 64 are no
-// faster anywhere.  fp32 products take 32 x 64 at any size (kGroupHigh says why).
+// faster anywhere; of rows that are not whole it is the other way round (2000 x 1501 -> 1001
+// by 32: 47 us with tiles of 64, 70 with 128).  fp32 products take 32 x 64 at any size (kGroupHigh says why).
 // Weight gradients take 256 from three rounds of them on, if they have rows
 // enough to be more than a store (16384 rows by 64 experts of 2048 x 1024: 173 us,
 // 196 with 128; 2000 by 32: 59 and 53; 8192 by 8 of 2048 x 2048: 75 and 72).
@@ -67,7 +68,7 @@ GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t 
         const bool turn = across && whole;
         const double t64 = turn ? 1e30 : 12.0 + 0.0245 * tiles(64), t128 = turn ? 12.0 + 0.075 * tiles(128) : 13.0 + 0.066 * tiles(128);
         const double t256 = std::max(45.0, 0.25 * tiles(256));
-        if (t128 < t64) p.tile = 128;
+        if (t128 < t64 && (whole || !across)) p.tile = 128;
         if (large && t256 < std::min(t64, t128)) p.tile = 256;
     }
     const int64_t stages = (weight ? rows / e : depth) / (wide ? 32 : 64);
@@ -106,18 +107,19 @@ void group_pad(const void* from, void* to, int64_t matrices, int64_t matrix_rows
     if (a.rows == 0) return;
     hipLaunchKernelGGL(group_pad_kernel, dim3((uint32_t)std::min<int64_t>((a.rows + per - 1) / per, 1 << 16)), dim3(256), 0, st, a);
 }
-// Whether that is worth it: the copies take 1 us a million numbers (4 TB/s) and 6
+// Whether that is worth it: the copies take 0.5 to 0.85 us a million numbers and 8
 // for two launches, and save, in us a GFLOP measured with and without them, 0.6 to
-// 1 of a product along k, 0.9 to 2.2 of one across, 2.7 to 5 of a weight gradient
-// (16384 x 2047 -> 4095 by 8: 554 us without, 407 with, 721 and 435, 1355 and 330; 8192 x
-// 1001 -> 1501 by 8: 68 and 71, 108 and 70, 128 and 63; 2000 by 32: 35 and 63, 74 and 64, 82 and 61).
+// 1.1 of a product along k, 1.7 to 2.2 of one across, 2.3 to 4 of a weight gradient.
+// Without and with: 16384 x 2047 -> 4095 by 8 554 us and 407, 721 and 435, 1355 and 330; 8192 x 1001
+// -> 1501 by 8 67 and 63, 101 and 68, 128 and 61; 4000 x 777 -> 1333 by 16 31 and 43, 46 and 53,
+// 49 and 44; 2000 x 1001 -> 1501 by 32 34 and 63, 47 and 60, 80 and 57.
 bool group_pads(int64_t rows, int64_t cols, int64_t depth, int64_t numbers, int32_t dtype, double gain) {
     if (dtype == CRESSO_F32) return false;
     const double gflop = 2e-9 * (double)rows * (double)cols * (double)depth;
-    return gflop * gain > 6.0 + 1e-6 * (double)numbers;
+    return gflop * gain > 8.0 + 0.6e-6 * (double)numbers;
 }
 constexpr int64_t kPadMost = ((int64_t)1 << 21) - 8;   // near_rows of the copies
-constexpr double kPadAlong = 1.0, kPadAcross = 2.2, kPadWeight = 3.5;   // us a GFLOP: w along k, w across it, the weight gradient
+constexpr double kPadAlong = 0.9, kPadAcross = 2.2, kPadWeight = 3.5;   // us a GFLOP: w along k, w across it, the weight gradient
 }  // namespace
 }  // namespace cresso
 

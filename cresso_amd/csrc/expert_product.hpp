@@ -1083,7 +1083,7 @@ template <typename T> void group_launch(GroupArgs a, bool weight, bool across, G
             } else if (plan.words) {                                                                                    \
                 if constexpr (sizeof(T) == 4) run(group_kernel<T, W, X, 1, 4, FM, 1, 128, STAGES, 4>, 16 * FM, 64);     \
             } else if (plan.tile >= 128) {                                                                              \
-                if constexpr (!W && sizeof(T) == 2) run(group_any_kernel<T, W, X, 1, 4, 8, 2>, 128, 128);               \
+                if constexpr (!X && sizeof(T) == 2) run(group_any_kernel<T, W, X, 1, 4, 8, 2>, 128, 128);               \
             } else {                                                                                                    \
                 run(group_any_kernel<T, W, X, 1, 4, FM, 1>, 16 * FM, 64);                                               \
             }                                                                                                           \
