@@ -173,6 +173,36 @@ def test_graph(tokens):
             assert torch.equal(a, b)
 
 
+def test_graph_of_odd_rows():
+    """Operands that are laid out anew, in the graph's own memory, while eager calls of the same go on beside it."""
+    announce("products of odd rows in a graph")
+    offsets = torch.tensor([0, 9000, 9000, 9300, 16600], dtype=torch.int32).cuda()
+    x, w, d = rand((16600, 333), torch.bfloat16, 1), rand((4, 1283, 333), torch.bfloat16, 2, 0.5), rand((16600, 1283), torch.bfloat16, 3)
+
+    def step():
+        a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        y = cresso_amd.expert_product(a, b, offsets)
+        return [y, *torch.autograd.grad(y, (a, b), d)]
+
+    step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(3):
+        for j, t in enumerate((x, w, d)):
+            t.copy_(rand(tuple(t.shape), t.dtype, 40 + 3 * k + j))
+        graph.replay()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
+
+
 def test_two_streams_at_once():
     announce("layers of experts on two streams")
     sets = [[*make(torch.bfloat16, 200, seed=s), rand((200, WIDTH), torch.bfloat16, s + 9)] for s in (0, 20)]
