@@ -73,7 +73,8 @@ GroupPlan group_plan(int64_t rows, int64_t m, int64_t n, int64_t depth, int32_t 
     }
     const int64_t stages = (weight ? rows / e : depth) / (wide ? 32 : 64);
     const double enough = wide ? 768.0 : 256.0;
-    if (p.tile < 256) p.splits = (uint32_t)std::min<int64_t>({16, (int64_t)(enough / std::max(1.0, tiles(p.tile))), stages / 8});
+    // no expert has no tiles to split: the rows are filled with zeros, by workgroups that products in parts do not have
+    if (p.tile < 256 && experts > 0) p.splits = (uint32_t)std::min<int64_t>({16, (int64_t)(enough / std::max(1.0, tiles(p.tile))), stages / 8});
     p.splits = std::max(p.splits, 1u);
     return p;
 }
