@@ -159,8 +159,11 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
 }
 // A gradient that arrives at a backward pass, as the kernels read it: in its own
 // memory where it is a view that stands for the negative of another's (autograd
-// makes those of conjugated complex numbers).
-Tensor arrived(const Tensor& t) {
+// makes those of conjugated complex numbers), and not a dual tensor, whose
+// tangent the result would lack.
+Tensor arrived(const char* what, const Tensor& t) {
+    TORCH_CHECK(!t._fw_grad(0).defined(), "the gradient that arrives at ", what,
+                " has a forward-mode derivative, the operators have reverse mode only");
     return t.detach().resolve_neg();
 }
 // The kernels' gradients cannot be differentiated again: what a backward pass
@@ -226,7 +229,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const Tensor ids = ctx->get_saved_variables()[0];
-        Tensor table = embedding_table(ids, arrived(grads[0]), ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble());
+        Tensor table = embedding_table(ids, arrived("embedding", grads[0]), ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble());
         return once({Tensor(), table, Tensor()}, grads);
     }
 };
@@ -370,7 +373,7 @@ struct SeamFunction : torch::autograd::Function<SeamFunction> {
         d.stats = (float*)saved[6].mutable_data_ptr();
         const auto arrives = [&](const Tensor& t, int64_t& stride) -> const void* {
             if (!t.defined()) return nullptr;
-            keep.push_back(rows_of(arrived(t), stride));
+            keep.push_back(rows_of(arrived("residual_norm", t), stride));
             return keep.back().const_data_ptr();
         };
         d.d_out = arrives(d_out, d.d_out_stride);
@@ -536,7 +539,7 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
             std::vector<Tensor> keep;
             keep.reserve(5);
             cresso_distill_desc d = distill_desc(c, keep);
-            const Tensor by = arrived(arrive[0]);
+            const Tensor by = arrived("distill_loss", arrive[0]);
             d.stats = (float*)v[5].mutable_data_ptr();
             d.d_loss = (const float*)by.const_data_ptr();
             d.d_loss_stride = by.dim() ? by.stride(0) : 0;
@@ -616,7 +619,7 @@ struct ProductFunction : torch::autograd::Function<ProductFunction> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list arrive) {
         const variable_list v = ctx->get_saved_variables();
-        return once({product(arrived(arrive[0]), v[0], v[1], true), Tensor(), Tensor()}, arrive);
+        return once({product(arrived("block_product", arrive[0]), v[0], v[1], true), Tensor(), Tensor()}, arrive);
     }
 };
 Tensor block_product(const Tensor& x, const Tensor& values, const Tensor& scales) {
@@ -867,7 +870,7 @@ struct RouteFunction : torch::autograd::Function<RouteFunction> {
             cresso_route_desc d = route_desc(r, keep);
             d.weights = (float*)v[1].const_data_ptr();
             d.experts = (int32_t*)v[2].const_data_ptr();
-            const Tensor by = arrived(arrive[0]).contiguous();
+            const Tensor by = arrived("route_experts", arrive[0]).contiguous();
             const c10::DeviceGuard guard(r.logits.device());
             done(g_api.route_backward(&d, (const float*)by.const_data_ptr(), grads[0].mutable_data_ptr(), stream_of(r.logits)),
                  "route_experts gradient");
@@ -946,7 +949,7 @@ struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list arrive) {
         const variable_list v = ctx->get_saved_variables();
-        return once({combine("dispatch_rows gradient", arrived(arrive[0]), v[0], v[1], Tensor()), Tensor(), Tensor()}, arrive);
+        return once({combine("dispatch_rows gradient", arrived("dispatch_rows", arrive[0]), v[0], v[1], Tensor()), Tensor(), Tensor()}, arrive);
     }
 };
 struct CombineFunction : torch::autograd::Function<CombineFunction> {
@@ -964,7 +967,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
         if (to_weights) grads[3] = at::empty(v[3].sizes(), v[3].options().requires_grad(false));
         if (v[1].numel() && (to_rows || to_weights)) {
             int64_t stride, by_stride;
-            const Tensor from = rows_of(rows, stride), by = rows_of(arrived(arrive[0]), by_stride);
+            const Tensor from = rows_of(rows, stride), by = rows_of(arrived("combine_rows", arrive[0]), by_stride);
             const Tensor experts = v[1].contiguous(), places = v[2].contiguous(), weights = v[3].defined() ? v[3].contiguous() : Tensor();
             const c10::DeviceGuard guard(rows.device());
             done(g_api.combine_backward(from.const_data_ptr(), stride, by.const_data_ptr(), by_stride, code_of(rows.scalar_type()), by.size(0),
@@ -1064,7 +1067,7 @@ struct ExpertFunction : torch::autograd::Function<ExpertFunction> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list arrive) {
         const variable_list v = ctx->get_saved_variables();
-        const Tensor by = arrived(arrive[0]);
+        const Tensor by = arrived("expert_product", arrive[0]);
         variable_list grads(3);
         if (ctx->needs_input_grad(0)) grads[0] = group_product("expert_product gradient", by, v[1], v[2], true);
         if (ctx->needs_input_grad(1)) grads[1] = group_weight(v[0], by, v[1], v[2]);

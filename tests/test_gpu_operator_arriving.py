@@ -1,9 +1,10 @@
 """The gradient that arrives at an operator's backward pass: views that stand for
 the negative of their memory (autograd makes them where complex numbers are
-conjugated) count as what they are."""
+conjugated) count as what they are, dual tensors are refused."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from gpu_util import announce, needs_gpu
 from operator_util import rand
@@ -55,3 +56,18 @@ def test_negative_views_arrive(name):
     y = call(x)
     (got,) = torch.autograd.grad(torch.complex(torch.zeros_like(y), y).conj(), x, torch.complex(torch.zeros_like(d), -d))
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_dual_tensors_that_arrive_are_refused(name):
+    """An answer without a tangent would say that the gradient does not change with what arrives."""
+    announce(f"dual tensor arrives: {name}")
+    call, x = calls()[name]
+    x = x.detach().requires_grad_(True)
+    y = call(x)
+    d = rand(tuple(y.shape), seed=11)
+    (want,) = torch.autograd.grad(y, x, d, retain_graph=True)
+    with fwad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, x, fwad.make_dual(d, torch.ones_like(d)), retain_graph=True)
+        assert torch.equal(torch.autograd.grad(y, x, d)[0], want)
