@@ -14,7 +14,8 @@ def gradient_norm(grads: Iterable[Optional[torch.Tensor]], norm_type: float = 2.
     """The norm over all elements of `grads` (a tensor, or tensors of fp32, fp64,
     bf16 and fp16, None among them): 2 or infinity.  -> fp32 scalar on their GPU,
     0 for no elements, infinite above fp32's range, NaN with a NaN.  Sums are
-    fp64, in the same order on every run."""
+    fp64, in the same order on every run; squares of fp64 gradients neither
+    overflow nor vanish in them."""
     given = _listed(grads)
     try:
         return _native.operators().gradient_norm(given, _kind("gradient_norm", norm_type))
@@ -31,9 +32,11 @@ def clip_gradients(grads: Iterable[Optional[torch.Tensor]], max_norm: float, *, 
         g   <- g * grad_scale * (max_norm / norm  where norm is finite and above max_norm, else 1)
 
     in fp64, rounded to the gradient's type.  grad_scale undoes a loss scale (1/65536
-    for a loss times 65536).  A norm that is not finite clips nothing: the
-    gradients, times grad_scale, stay as they are, and the returned norm says so.
-    Nothing waits for the GPU, and where nothing changes nothing is written.
+    for a loss times 65536).  A norm that is infinite or NaN clips nothing: the
+    gradients, times grad_scale, stay as they are.  The norm that counts is the
+    fp64 one; what is returned is rounded to fp32, so that a norm above fp32's
+    range clips but returns infinity.  Nothing waits for the GPU, and where
+    nothing changes nothing is written.
 
     out: where the results go instead, a tensor for each gradient of its shape
     and its type, or fp32 for gradients of 16 bits (then nothing is rounded to 16

@@ -10,8 +10,10 @@
 // tensors are clipped in place it reads nothing but the norm.
 //
 // Squares and their sums are fp64: gradients of 1e-30 and of 1e30 count as they
-// are, and no order of the tensors changes more than the last bits.  A thread's
-// sum, the waves' and the workgroups' are joined in a fixed order.
+// are, and no order of the tensors changes more than the last bits.  fp64
+// gradients whose own squares leave that range are scaled by a power of two and
+// have sums of their own.  A thread's sum, the waves' and the workgroups' are
+// joined in a fixed order.
 //
 // Bound by HBM.  840 fp32 adapters of 220 MB, nothing to clip: 35 us for the norm
 // (6.3 TB/s) and 4 for the second kernel; 199 bf16 tensors of 1.2 B elements to
@@ -44,7 +46,7 @@ struct ClipFill {
 struct ClipArgs {
     ClipEntry* table;
     void** outs;           // of the entries; NULL: each is its own output
-    double* partials;
+    double* partials;      // [CL_SUMS][CL_MAX_BLOCKS]
     float* norm;
     uint32_t count, chunks, blocks;
     double max_norm, scale;
@@ -102,25 +104,57 @@ template <> __device__ __forceinline__ double clip_value<__half>(u32x4 r, int i)
     return (double)(float)h[i & 1];
 }
 
-// Sums of squares are doubles; a maximum is the largest pattern of |g| as a
-// double: patterns order as the magnitudes do, NaN above infinity.
-template <bool MAX> struct ClipSum {
-    double v = 0.0;
-    __device__ __forceinline__ void add(double g) {
-        if constexpr (MAX) join(fabs(g));
-        else v = fma(g, g, v);
-    }
-    __device__ __forceinline__ void join(double o) {
-        if constexpr (MAX) {
-            const uint64_t x = (uint64_t)__double_as_longlong(v), y = (uint64_t)__double_as_longlong(o);
-            v = __longlong_as_double((long long)(x > y ? x : y));
+// What a norm is the root of: a sum of squares; for fp64 gradients three, so
+// that no square leaves a double's range; or the largest magnitude.
+enum ClipKind { CLIP_SQUARES, CLIP_WIDE, CLIP_LARGEST };
+constexpr int CL_SUMS = 3;   // doubles of a partial sum, at most
+// Squares of 2^-480 to 2^480 stay above 2^-960 and, 2^44 of them added up, below
+// 2^1004; larger magnitudes are added up as those of g / 2^600, smaller ones of g * 2^600.
+constexpr double CL_HIGH = 0x1p480, CL_LOW = 0x1p-480, CL_DOWN = 0x1p-600, CL_UP = 0x1p600;
+
+// A largest magnitude is the largest pattern of |g| as a double: patterns order
+// as the magnitudes do, NaN above infinity.
+template <ClipKind KIND> struct ClipSum {
+    static constexpr int N = KIND == CLIP_WIDE ? CL_SUMS : 1;
+    double v[N];   // squares, those of large and of small numbers; or the largest
+    template <typename T> __device__ __forceinline__ void add(double g) {
+        if constexpr (KIND == CLIP_LARGEST) {
+            largest(fabs(g));
+        } else if constexpr (KIND == CLIP_WIDE && sizeof(T) == 8) {
+            const double size = fabs(g);
+            const bool high = size > CL_HIGH, low = size < CL_LOW;   // NaN is neither
+            const double mid = high || low ? 0.0 : g, down = high ? g * CL_DOWN : 0.0, up = low ? g * CL_UP : 0.0;
+            v[0] = fma(mid, mid, v[0]);
+            v[1] = fma(down, down, v[1]);
+            v[2] = fma(up, up, v[2]);
         } else {
-            v += o;
+            v[0] = fma(g, g, v[0]);
         }
+    }
+    __device__ __forceinline__ void largest(double o) {
+        const uint64_t x = (uint64_t)__double_as_longlong(v[0]), y = (uint64_t)__double_as_longlong(o);
+        v[0] = __longlong_as_double((long long)(x > y ? x : y));
+    }
+    __device__ __forceinline__ void join(const ClipSum& o) {
+        if constexpr (KIND == CLIP_LARGEST) {
+            largest(o.v[0]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += o.v[i];
+        }
+    }
+    __device__ __forceinline__ double norm() const {
+        if constexpr (KIND == CLIP_LARGEST) return v[0];
+        if constexpr (KIND == CLIP_WIDE) {   // the sums that are far below another add nothing to it
+            if (v[1] > 0.0) return sqrt(v[1] + v[0] * CL_DOWN * CL_DOWN) * CL_UP;
+            if (v[0] == 0.0) return sqrt(v[2]) * CL_DOWN;
+            return sqrt(v[0] + v[2] * CL_DOWN * CL_DOWN);
+        }
+        return sqrt(v[0]);
     }
 };
 
-template <typename T, bool MAX> __device__ __forceinline__ void clip_sum(const T* at, uint32_t left, ClipSum<MAX> (&sum)[2]) {
+template <typename T, ClipKind KIND> __device__ __forceinline__ void clip_sum(const T* at, uint32_t left, ClipSum<KIND> (&sum)[2]) {
     constexpr int E = 16 / (int)sizeof(T);
     constexpr uint32_t whole = CL_CHUNK / sizeof(T);
     if (left == whole) {
@@ -130,36 +164,38 @@ template <typename T, bool MAX> __device__ __forceinline__ void clip_sum(const T
 #pragma unroll
         for (int u = 0; u < CL_UNITS; ++u)
 #pragma unroll
-            for (int i = 0; i < E; ++i) sum[i & 1].add(clip_value<T>(r[u], i));
+            for (int i = 0; i < E; ++i) sum[i & 1].template add<T>(clip_value<T>(r[u], i));
         return;
     }
     for (uint32_t u = threadIdx.x * E; u < left; u += CL_NT * E) {
         if (u + E <= left) {
             const u32x4 r = clip_load(at + u);
 #pragma unroll
-            for (int i = 0; i < E; ++i) sum[i & 1].add(clip_value<T>(r, i));
+            for (int i = 0; i < E; ++i) sum[i & 1].template add<T>(clip_value<T>(r, i));
         } else {
             for (uint32_t i = u; i < left; ++i) {
-                if constexpr (sizeof(T) == 8) sum[0].add(at[i]);
-                else sum[0].add((double)to_f(at[i]));
+                if constexpr (sizeof(T) == 8) sum[0].template add<T>(at[i]);
+                else sum[0].template add<T>((double)to_f(at[i]));
             }
         }
     }
 }
 
 // Everybody's sums joined: lanes, then waves, in their order.
-template <bool MAX> __device__ __forceinline__ double clip_join(double v, double* lds) {
-    ClipSum<MAX> s;
-    s.v = v;
+template <ClipKind KIND> __device__ __forceinline__ void clip_join(ClipSum<KIND>& s, ClipSum<KIND>* lds) {
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) s.join(__shfl_xor(s.v, m, kWave));
+    for (int m = 32; m >= 1; m >>= 1) {
+        ClipSum<KIND> o;
+#pragma unroll
+        for (int i = 0; i < ClipSum<KIND>::N; ++i) o.v[i] = __shfl_xor(s.v[i], m, kWave);
+        s.join(o);
+    }
     __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = s.v;
+    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = s;
     __syncthreads();
-    s.v = lds[0];
+    s = lds[0];
 #pragma unroll
     for (int w = 1; w < CL_NT / kWave; ++w) s.join(lds[w]);
-    return s.v;
 }
 
 __device__ __forceinline__ void clip_run(const ClipArgs& a, uint32_t& lo, uint32_t& hi) {
@@ -167,12 +203,12 @@ __device__ __forceinline__ void clip_run(const ClipArgs& a, uint32_t& lo, uint32
     hi = (uint32_t)((uint64_t)(blockIdx.x + 1) * a.chunks / a.blocks);
 }
 
-template <bool MAX> __global__ __launch_bounds__(CL_NT) void clip_norm_kernel(ClipArgs a) {
-    __shared__ double lds[CL_NT / kWave];
+template <ClipKind KIND> __global__ __launch_bounds__(CL_NT) void clip_norm_kernel(ClipArgs a) {
+    __shared__ ClipSum<KIND> lds[CL_NT / kWave];
     uint32_t lo, hi;
     clip_run(a, lo, hi);
     uint32_t e = entry_of(a, lo);
-    ClipSum<MAX> sum[2];
+    ClipSum<KIND> sum[2] = {};
     ClipEntry t = a.table[e];
     uint32_t end = e + 1 < a.count ? a.table[e + 1].first : a.chunks;
     for (uint32_t c = lo; c < hi; ++c) {
@@ -188,20 +224,23 @@ template <bool MAX> __global__ __launch_bounds__(CL_NT) void clip_norm_kernel(Cl
         else if (type == CRESSO_F16) clip_sum<__half>((const __half*)at, last ? tail : CL_CHUNK / 2, sum);
         else clip_sum<double>((const double*)at, last ? tail : CL_CHUNK / 8, sum);
     }
-    sum[0].join(sum[1].v);
-    const double v = clip_join<MAX>(sum[0].v, lds);
-    if (threadIdx.x == 0) a.partials[blockIdx.x] = v;
+    sum[0].join(sum[1]);
+    clip_join(sum[0], lds);
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 0; i < ClipSum<KIND>::N; ++i) a.partials[i * CL_MAX_BLOCKS + blockIdx.x] = sum[0].v[i];
+    }
 }
 
-// The E elements of r times f, in fp64, rounded to fp32 and where `out` has 16
+// The E elements of r times f (and late), in fp64, rounded to fp32 and where `out` has 16
 // bits from there: off by at most 2^-24 of the result more than half a step.
-template <typename T, typename O> __device__ __forceinline__ void clip_scale_unit(u32x4 r, O* out, double f) {
+template <typename T, typename O> __device__ __forceinline__ void clip_scale_unit(u32x4 r, O* out, double f, double late) {
     constexpr int E = 16 / (int)sizeof(T);
     if constexpr (sizeof(O) == 8) {
         u32x4 w;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint64_t v = (uint64_t)__double_as_longlong(clip_value<T>(r, i) * f);
+            const uint64_t v = (uint64_t)__double_as_longlong(clip_value<T>(r, i) * f * late);
             w[2 * i] = (uint32_t)v;
             w[2 * i + 1] = (uint32_t)(v >> 32);
         }
@@ -217,43 +256,55 @@ template <typename T, typename O> __device__ __forceinline__ void clip_scale_uni
         }
     }
 }
-template <typename T, typename O> __device__ __forceinline__ void clip_scale(const T* in, O* out, uint32_t left, double f) {
+template <typename T, typename O> __device__ __forceinline__ void clip_scale(const T* in, O* out, uint32_t left, double f, double late = 1.0) {
     constexpr int E = 16 / (int)sizeof(T);
     if (left == CL_CHUNK / sizeof(T)) {
         u32x4 r[CL_UNITS];
 #pragma unroll
         for (int u = 0; u < CL_UNITS; ++u) r[u] = clip_load(in + (uint32_t)(u * CL_NT + threadIdx.x) * E);
 #pragma unroll
-        for (int u = 0; u < CL_UNITS; ++u) clip_scale_unit<T, O>(r[u], out + (uint32_t)(u * CL_NT + threadIdx.x) * E, f);
+        for (int u = 0; u < CL_UNITS; ++u) clip_scale_unit<T, O>(r[u], out + (uint32_t)(u * CL_NT + threadIdx.x) * E, f, late);
         return;
     }
     for (uint32_t u = threadIdx.x * E; u < left; u += CL_NT * E) {
         if (u + E <= left) {
-            clip_scale_unit<T, O>(clip_load(in + u), out + u, f);
+            clip_scale_unit<T, O>(clip_load(in + u), out + u, f, late);
         } else {
             for (uint32_t i = u; i < left; ++i) {
-                if constexpr (sizeof(T) == 8) out[i] = in[i] * f;
+                if constexpr (sizeof(T) == 8) out[i] = in[i] * f * late;
                 else out[i] = from_w<O>((float)((double)to_f(in[i]) * f));
             }
         }
     }
 }
 
-template <bool MAX> __global__ __launch_bounds__(CL_NT) void clip_scale_kernel(ClipArgs a) {
-    __shared__ double lds[CL_NT / kWave];
-    ClipSum<MAX> sum;
+template <ClipKind KIND> __global__ __launch_bounds__(CL_NT) void clip_scale_kernel(ClipArgs a) {
+    __shared__ ClipSum<KIND> lds[CL_NT / kWave];
+    ClipSum<KIND> sum = {};
 #pragma unroll
     for (int i = 0; i < CL_MAX_BLOCKS / CL_NT; ++i) {
         const uint32_t at = i * CL_NT + threadIdx.x;
-        if (at < a.blocks) sum.join(a.partials[at]);
+        if (at >= a.blocks) continue;
+        ClipSum<KIND> o;
+#pragma unroll
+        for (int k = 0; k < ClipSum<KIND>::N; ++k) o.v[k] = a.partials[k * CL_MAX_BLOCKS + at];
+        sum.join(o);
     }
-    const double total = clip_join<MAX>(sum.v, lds);
-    const double norm = (MAX ? total : sqrt(total)) * fabs(a.scale);
+    clip_join(sum, lds);
+    const double norm = sum.norm() * fabs(a.scale);
     if (blockIdx.x == 0 && threadIdx.x == 0) *a.norm = (float)norm;
     if (!a.write) return;
-    double f = a.scale;
-    if (norm > a.max_norm && norm < INFINITY) f *= a.max_norm / norm;
-    if (a.in_place && f == 1.0) return;
+    double f = a.scale, late = 1.0;   // late: of fp64 gradients, where max_norm / norm has too few bits by itself
+    if (norm > a.max_norm && norm < INFINITY) {
+        double by = a.max_norm / norm;
+        if (by < 0x1p-960) {
+            by = a.max_norm * CL_UP / norm;
+            late = CL_DOWN;
+        }
+        f *= by;
+    }
+    const double whole = f * late;
+    if (a.in_place && whole == 1.0) return;
     uint32_t lo, hi;
     clip_run(a, lo, hi);
     uint32_t e = entry_of(a, hi - 1);
@@ -265,19 +316,19 @@ template <bool MAX> __global__ __launch_bounds__(CL_NT) void clip_scale_kernel(C
             t = a.table[--e];
         }
         void* const to = a.outs ? a.outs[e] : const_cast<void*>(t.in);
-        if (!(t.tail_types & 16) || (to == t.in && f == 1.0)) continue;
+        if (!(t.tail_types & 16) || (to == t.in && whole == 1.0)) continue;
         const uint32_t tail = t.tail_types >> 5, types = t.tail_types & 15, type = types >> 2;
         const uint32_t size = type == CRESSO_F64 ? 8 : type == CRESSO_F32 ? 4 : 2, out_size = (types & 3) == CRESSO_F64 ? 8 : (types & 3) == CRESSO_F32 ? 4 : 2;
         const uint64_t first = (uint64_t)(c - t.first) * (CL_CHUNK / size);
         const char* in = (const char*)t.in + first * size;
         char* out = (char*)to + first * out_size;
         const uint32_t left = c + 1 == end ? tail : CL_CHUNK / size;
-        if (types == (CRESSO_F32 << 2 | CRESSO_F32)) clip_scale((const float*)in, (float*)out, left, f);
-        else if (types == (CRESSO_BF16 << 2 | CRESSO_BF16)) clip_scale((const __hip_bfloat16*)in, (__hip_bfloat16*)out, left, f);
-        else if (types == (CRESSO_BF16 << 2 | CRESSO_F32)) clip_scale((const __hip_bfloat16*)in, (float*)out, left, f);
-        else if (types == (CRESSO_F16 << 2 | CRESSO_F16)) clip_scale((const __half*)in, (__half*)out, left, f);
-        else if (types == (CRESSO_F16 << 2 | CRESSO_F32)) clip_scale((const __half*)in, (float*)out, left, f);
-        else clip_scale((const double*)in, (double*)out, left, f);
+        if (types == (CRESSO_F32 << 2 | CRESSO_F32)) clip_scale((const float*)in, (float*)out, left, whole);
+        else if (types == (CRESSO_BF16 << 2 | CRESSO_BF16)) clip_scale((const __hip_bfloat16*)in, (__hip_bfloat16*)out, left, whole);
+        else if (types == (CRESSO_BF16 << 2 | CRESSO_F32)) clip_scale((const __hip_bfloat16*)in, (float*)out, left, whole);
+        else if (types == (CRESSO_F16 << 2 | CRESSO_F16)) clip_scale((const __half*)in, (__half*)out, left, whole);
+        else if (types == (CRESSO_F16 << 2 | CRESSO_F32)) clip_scale((const __half*)in, (float*)out, left, whole);
+        else clip_scale((const double*)in, (double*)out, left, f, late);
     }
 }
 
@@ -303,7 +354,7 @@ int32_t check_clip(const cresso_grad_desc* g, int32_t count, uint32_t& entries, 
     return CRESSO_OK;
 }
 // entries, then their outputs
-size_t clip_bytes(uint32_t entries) { return CL_MAX_BLOCKS * sizeof(double) + (size_t)entries * sizeof(ClipEntry) + ((size_t)entries + 1) / 2 * 16; }
+size_t clip_bytes(uint32_t entries) { return CL_SUMS * CL_MAX_BLOCKS * sizeof(double) + (size_t)entries * sizeof(ClipEntry) + ((size_t)entries + 1) / 2 * 16; }
 }  // namespace
 }  // namespace cresso
 
@@ -331,7 +382,7 @@ extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t 
     hipStream_t st = (hipStream_t)stream;
     ClipArgs a{};
     a.partials = (double*)workspace;
-    a.table = (ClipEntry*)((char*)workspace + CL_MAX_BLOCKS * sizeof(double));
+    a.table = (ClipEntry*)((char*)workspace + CL_SUMS * CL_MAX_BLOCKS * sizeof(double));
     a.norm = norm;
     a.count = entries;
     a.chunks = chunks;
@@ -348,6 +399,7 @@ extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t 
         held = 0;
     };
     uint32_t first = 0;
+    bool wide = false;
     for (int32_t i = 0; i < count; ++i) {
         const cresso_grad_desc& g = grads[i];
         if (!g.numel) continue;
@@ -356,6 +408,7 @@ extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t 
         const ClipEntry e = {g.grad, first, tail << 5 | (g.out ? 16u : 0u) | (uint32_t)g.dtype << 2 | (uint32_t)(g.out ? g.out_dtype : 0)};
         f.e[held++] = __builtin_bit_cast(u32x4, e);
         first += n;
+        wide |= g.dtype == CRESSO_F64;
         if (g.out) a.write = 1;
         if (g.out && g.out != g.grad) a.in_place = 0;
         if (held == CL_FILL) flush();
@@ -379,7 +432,8 @@ extern "C" int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t 
         if (a.blocks) hipLaunchKernelGGL(norm_kernel, dim3(a.blocks), dim3(CL_NT), 0, st, a);
         hipLaunchKernelGGL(scale_kernel, dim3(a.write ? std::max(1u, a.blocks) : 1), dim3(CL_NT), 0, st, a);
     };
-    if (norm_kind == CRESSO_NORM_2) run(clip_norm_kernel<false>, clip_scale_kernel<false>);
-    else run(clip_norm_kernel<true>, clip_scale_kernel<true>);
+    if (norm_kind == CRESSO_NORM_MAX) run(clip_norm_kernel<CLIP_LARGEST>, clip_scale_kernel<CLIP_LARGEST>);
+    else if (wide) run(clip_norm_kernel<CLIP_WIDE>, clip_scale_kernel<CLIP_WIDE>);
+    else run(clip_norm_kernel<CLIP_SQUARES>, clip_scale_kernel<CLIP_SQUARES>);
     return launched("gradient norm");
 }

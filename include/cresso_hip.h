@@ -524,8 +524,10 @@ int32_t cresso_block_quantize(const void* w, int64_t w_stride, int32_t dtype, in
  * memory that no tensor of the call shares, of the gradient's dtype or, for
  * f16 and bf16, f32.  Gradients that are written in place share no memory with
  * one another.  Each is `numel` consecutive elements.  Sums are fp64 in a
- * fixed order, norm [1] is fp32 (inf above its range) and written for no
- * tensors at all too (0).  grad_scale is finite; max_norm may be infinite. */
+ * fixed order (squares of f64 gradients are scaled where they leave its range),
+ * and the norm that is compared with max_norm is fp64 too; norm [1] is that in
+ * fp32 (inf above its range) and written for no tensors at all too (0).
+ * grad_scale is finite; max_norm may be infinite. */
 #define CRESSO_NORM_2 2
 #define CRESSO_NORM_MAX 0
 typedef struct cresso_grad_desc {

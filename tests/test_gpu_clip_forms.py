@@ -1,0 +1,101 @@
+"""Gradient norm and clipping in forms that the general tests do not reach: fp64
+gradients whose squares leave fp64's range."""
+
+import math
+
+import pytest
+import torch
+
+from gpu_util import announce, needs_gpu
+from operator_util import EPS32, rand
+
+import cresso_amd
+
+pytestmark = [pytest.mark.gpu, needs_gpu]
+
+
+def times(t, e):
+    """t * 2^e by two factors that are numbers."""
+    return t * 2.0 ** (e // 2) * 2.0 ** (e - e // 2)
+
+
+def norm_of(grads):
+    """m, e: the 2-norm is m * 2^e, m from 1/2 to the root of the number of elements."""
+    flat = torch.cat([g.double().cpu().reshape(-1) for g in grads])
+    e = math.frexp(float(flat.abs().max()))[1]
+    return float(times(flat, -e).norm()), e
+
+
+def wide(n, exponent, seed, spread=0):
+    """Normal numbers times 2^exponent, and each times 2 to up to +-spread more."""
+    more = torch.randint(-spread, spread + 1, (n,), generator=torch.Generator().manual_seed(seed + 50)).double().cuda()
+    return times(rand((n,), seed=seed).double() * 2.0 ** more, exponent)
+
+
+CASES = {
+    "above": [(5000, 700, 0)],                  # squares above fp64's range
+    "below": [(5000, -700, 0)],                 # squares below it
+    "denormal": [(3000, -1062, 0)],
+    "high": [(20000, 1000, 0), (7, 3, 0)],
+    "around the upper border": [(9000, 480, 6), (70000, 478, 0)],
+    "around the lower border": [(9000, -480, 6), (70000, -482, 0)],
+    "all": [(9000, -900, 0), (33, 0, 0), (20000, 900, 0)],
+    "low and middle": [(9000, -900, 0), (20000, 0, 0)],
+    "low and less": [(9000, -600, 300)],
+}
+
+
+@pytest.mark.parametrize("others", [False, True])
+@pytest.mark.parametrize("name", list(CASES))
+def test_fp64_of_any_size(name, others):
+    announce(f"clip fp64 {name} {others}")
+    make = lambda: [wide(n, e, i, s) for i, (n, e, s) in enumerate(CASES[name])] + (   # noqa: E731
+        [rand((10000,), torch.float32, 7), rand((333,), torch.bfloat16, 8)] if others else [])
+    grads = make()
+    m, e = norm_of(grads)
+    try:
+        exact = math.ldexp(m, e)
+    except OverflowError:
+        exact = math.inf
+    got = cresso_amd.gradient_norm(grads)
+    if exact > 3.5e38:
+        assert float(got) == math.inf    # above fp32
+    else:
+        assert abs(float(got.double()) - exact) <= (EPS32 + 2.0 ** -40) * exact + 2.0 ** -150
+    for low in (2, 1000):         # limits of a quarter of the norm and of 2^-1000 of it
+        max_norm = math.ldexp(m, e - low)
+        if not 0.0 < max_norm < math.inf or exact == math.inf or max_norm < 2.0 ** -1022:
+            continue
+        grads = make()
+        cresso_amd.clip_gradients(grads, max_norm)
+        for g, b in zip(grads, make()):
+            if g.dtype != torch.float64:
+                continue
+            want = times(b, -low)
+            # sums and their root as 1e-11 covers any number of terms; numbers below 2^-1022 are rounded to multiples of 2^-1074
+            assert torch.allclose(g, want, rtol=1e-11, atol=2.0 ** -1073), (name, low)
+
+
+def test_fp64_largest_of_any_size():
+    announce("clip fp64 by the largest")
+    for exponent in (-1000, -600, 600, 1000):
+        g = wide(5000, exponent, 1)
+        before, top = g.clone(), float(g.abs().max())
+        cresso_amd.clip_gradients(g, math.ldexp(top, -2), norm_type=math.inf)
+        assert torch.allclose(g, before / 4, rtol=1e-15, atol=0.0)
+    g = torch.full((1000,), 2.0 ** 1000, dtype=torch.float64, device="cuda")
+    cresso_amd.clip_gradients(g, 2.0 ** -60, norm_type=math.inf)
+    assert torch.equal(g, torch.full_like(g, 2.0 ** -60))
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_fp64_norms_that_are_not_finite(bad):
+    announce(f"clip fp64 large numbers with {bad}")
+    for where in (0, 1):
+        grads = [wide(5000, 700, 1), rand((10000,), torch.float32, 2)]
+        grads[where][77] = bad
+        want = [g.clone() for g in grads]
+        norm = cresso_amd.clip_gradients(grads, 0.5)
+        assert math.isnan(norm) if math.isnan(bad) else float(norm) == math.inf
+        for g, w in zip(grads, want):
+            assert torch.equal(torch.nan_to_num(g, nan=3.0), torch.nan_to_num(w, nan=3.0))
