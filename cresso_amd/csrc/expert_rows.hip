@@ -19,7 +19,7 @@ namespace {
 
 constexpr int ER_NT = 256;
 constexpr int ER_MAX_TOP = 32;
-constexpr int64_t ER_MAX_TOKENS = 1 << 26;   // a launch has fewer than 2^32 threads
+constexpr int64_t ER_MAX_TOKENS = (1 << 26) - 16;   // a launch has fewer than 2^32 threads: 64 a token, in workgroups of 4 tokens or more
 
 struct RowsArgs {
     const void *x, *d_out;         // rows that are read
@@ -148,7 +148,7 @@ int32_t check_rows(const char* what, int32_t dtype, int64_t tokens, int32_t top,
     if (!row_dtype(dtype)) return fail(CRESSO_E_UNSUPPORTED, "%s: dtype %d not supported (f32, bf16, f16)", what, dtype);
     if (tokens < 0 || width < 0) return fail(CRESSO_E_INVALID, "%s: negative size", what);
     if (top < 1 || top > ER_MAX_TOP) return fail(CRESSO_E_UNSUPPORTED, "%s: %d experts a token, 1 to %d are taken", what, top, ER_MAX_TOP);
-    if (tokens >= ER_MAX_TOKENS || tokens * top >= (int64_t)1 << 31 || width >= (int64_t)1 << 31)
+    if (tokens > ER_MAX_TOKENS || tokens * top >= (int64_t)1 << 31 || width >= (int64_t)1 << 31)
         return fail(CRESSO_E_UNSUPPORTED, "%s: %lld rows of %lld are more than one call takes", what, (long long)(tokens * top), (long long)width);
     return CRESSO_OK;
 }

@@ -799,7 +799,7 @@ Tensor clip_gradients(const pybind11::list& grads, double max_norm, int64_t kind
 // ---------------------------------------------------------------------------
 // layers of experts
 // ---------------------------------------------------------------------------
-constexpr int64_t kMaxExperts = 1024, kMaxExpertsOfToken = 32, kMaxTokens = 1 << 26;
+constexpr int64_t kMaxExperts = 1024, kMaxExpertsOfToken = 32, kMaxTokens = (1 << 26) - 16;
 
 struct Route {
     Tensor logits, bias;
@@ -891,7 +891,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_experts(const Tensor& l
     TORCH_CHECK_VALUE(experts >= 1 && experts <= kMaxExperts, what, ": ", experts, " experts, 1 to ", kMaxExperts, " are taken");
     TORCH_CHECK_VALUE(top >= 1 && top <= std::min(experts, kMaxExpertsOfToken), what, ": top ", top, " of ", experts, " experts, 1 to ",
                       std::min(experts, kMaxExpertsOfToken), " are taken");
-    TORCH_CHECK_VALUE(logits.size(0) < kMaxTokens && logits.size(0) * top < (int64_t)1 << 31, what, ": ", logits.size(0), " tokens are more than one call takes");
+    TORCH_CHECK_VALUE(logits.size(0) <= kMaxTokens && logits.size(0) * top < (int64_t)1 << 31, what, ": ", logits.size(0), " tokens are more than one call takes");
     TORCH_CHECK_VALUE(std::isfinite(scale), what, ": scale must be finite");
     if (bias.defined())
         TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == experts && bias.scalar_type() == at::kFloat, what, ": bias must be fp32 [",
@@ -911,7 +911,7 @@ void check_slots(const char* what, OneGpu& gpu, const Tensor& experts, const Ten
                       experts.sizes(), " and ", name_of(places.scalar_type()), " ", places.sizes());
     TORCH_CHECK_VALUE(experts.size(1) >= 1 && experts.size(1) <= kMaxExpertsOfToken, what, ": ", experts.size(1), " experts a token, 1 to ",
                       kMaxExpertsOfToken, " are taken");
-    TORCH_CHECK_VALUE(experts.size(0) < kMaxTokens && experts.numel() < (int64_t)1 << 31, what, ": ", experts.size(0),
+    TORCH_CHECK_VALUE(experts.size(0) <= kMaxTokens && experts.numel() < (int64_t)1 << 31, what, ": ", experts.size(0),
                       " tokens are more than one call takes");
 }
 const int32_t* ints(const Tensor& t) { return (const int32_t*)t.const_data_ptr(); }

@@ -35,7 +35,7 @@ namespace {
 
 constexpr int RT_MAX_EXPERTS = 1024;
 constexpr int RT_MAX_TOP = 32;
-constexpr int64_t RT_MAX_TOKENS = 1 << 26;   // a launch has fewer than 2^32 threads
+constexpr int64_t RT_MAX_TOKENS = (1 << 26) - 16;   // a launch has fewer than 2^32 threads: 64 a token, in workgroups of 16 tokens or 4
 constexpr int RT_NT = 256;
 constexpr int RT_TOKENS = 16;          // of a workgroup
 constexpr int RT_SMALL_NT = 512;       // one workgroup for everything
@@ -403,7 +403,7 @@ int32_t check_route(const cresso_route_desc* d) {
         return fail(CRESSO_E_UNSUPPORTED, "router: %d experts, 1 to %d are taken", d->num_experts, RT_MAX_EXPERTS);
     if (d->top < 1 || d->top > RT_MAX_TOP || d->top > d->num_experts)
         return fail(CRESSO_E_UNSUPPORTED, "router: top %d of %d experts, 1 to %d are taken", d->top, d->num_experts, RT_MAX_TOP);
-    if (d->tokens >= RT_MAX_TOKENS || d->tokens * d->top >= (int64_t)1 << 31)
+    if (d->tokens > RT_MAX_TOKENS || d->tokens * d->top >= (int64_t)1 << 31)
         return fail(CRESSO_E_UNSUPPORTED, "router: %lld tokens are more than one call takes", (long long)d->tokens);
     if (d->score != CRESSO_SCORE_SOFTMAX && d->score != CRESSO_SCORE_SIGMOID) return fail(CRESSO_E_INVALID, "router: unknown score %d", d->score);
     if (!std::isfinite(d->scale)) return fail(CRESSO_E_INVALID, "router: scale must be finite");

@@ -554,7 +554,7 @@ int32_t cresso_clip_gradients(const cresso_grad_desc* grads, int32_t count, int3
  * those of one expert in their own order, absent ones last; places [slots]: the
  * place of each slot in that order; offsets [experts + 1]: where each expert's
  * slots begin, and the last's end.  2 <= experts + 1 <= 1025, top <= 32 and
- * at most experts, tokens below 2^26, slots below 2^31. */
+ * at most experts, at most 2^26 - 16 tokens, slots below 2^31. */
 typedef struct cresso_route_desc {
     const void* logits;
     const float* bias;
@@ -573,8 +573,8 @@ int32_t cresso_route_backward(const cresso_route_desc* desc, const float* d_weig
 
 /* Rows between tokens and their slots.  experts [tokens][top]: an entry below 0
  * is absent; places [tokens][top]: a slot's row; a place outside [0, tokens *
- * top) is not read or written, and no place is given twice.  Tokens below
- * 2^26, at most 32 entries each, slots below 2^31.
+ * top) is not read or written, and no place is given twice.  At most
+ * 2^26 - 16 tokens, 32 entries each, slots below 2^31.
  *   dispatch: rows[places[t][k]] = x[t], zeros for absent slots
  *   combine:  out[t] = sum over present k, in their order, of weights[t][k] * rows[places[t][k]]  (weights NULL: 1)
  *   combine_backward: d_rows[places[t][k]] = weights[t][k] * d_out[t], zeros for absent slots;
