@@ -41,8 +41,8 @@ def clip_gradients(grads: Iterable[Optional[torch.Tensor]], max_norm: float, *, 
     out: where the results go instead, a tensor for each gradient of its shape
     and its type, or fp32 for gradients of 16 bits (then nothing is rounded to 16
     bits a second time); it is always written.  Memory that is written may
-    belong to one gradient only (ValueError otherwise), but a gradient may be its
-    own output.  :meth:`CRESSO5.clip_gradients` takes an optimizer's gradients.
+    belong to one gradient only (ValueError otherwise; slices that interleave are
+    taken as columns of the same rows), but a gradient may be its own output.  :meth:`CRESSO5.clip_gradients` takes an optimizer's gradients.
     """
     given, to = _listed(grads), None if out is None else _listed(out)
     try:

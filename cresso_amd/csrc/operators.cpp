@@ -664,19 +664,65 @@ std::tuple<Tensor, Tensor> quantize_blocks(const Tensor& weight) {
 // ---------------------------------------------------------------------------
 // gradient norm and clipping
 // ---------------------------------------------------------------------------
+// Bytes [at, end) of memory; of those, where `row` is not 0, `width` ones at `at`
+// and at whole multiples of `row` behind it.
 struct Written {
     uintptr_t at, end;
     bool out;
+    uintptr_t row = 0, width = 0;
 };
-// Whether memory that is written belongs to anything else of the call.
-bool shares(std::vector<Written>& spans) {
-    const auto before = [](const Written& a, const Written& b) { return a.at < b.at; };
-    if (!std::is_sorted(spans.begin(), spans.end(), before)) std::sort(spans.begin(), spans.end(), before);
+// A tensor's bytes.  Slices that leave gaps are rows of one piece each where their strides say so.
+Written bytes_of(const Tensor& t, uintptr_t at, bool dense, bool out) {
+    const uintptr_t size = (uintptr_t)t.element_size();
+    if (dense) return {at, at + (uintptr_t)t.numel() * size, out};
+    std::vector<std::pair<int64_t, int64_t>> dims;   // stride, size
+    int64_t reach = 1;   // elements from the first to the last
+    for (int64_t d = 0; d < t.dim(); ++d) {
+        reach += (t.size(d) - 1) * t.stride(d);
+        if (t.size(d) > 1) dims.emplace_back(t.stride(d), t.size(d));
+    }
+    std::sort(dims.begin(), dims.end());
+    int64_t width = 1, row = 0;
+    for (const auto& [stride, n] : dims) {
+        if (!row && stride == width) width *= n;
+        else if (!row) row = stride;
+        if (row && (row <= width || stride % row)) return {at, at + (uintptr_t)reach * size, out};
+    }
+    return {at, at + (uintptr_t)reach * size, out, (uintptr_t)row * size, (uintptr_t)width * size};
+}
+// Whether bytes that are written are another's too, rows taken as whole blocks; spans by their begin.
+template <typename It> bool overlaps(It first, It last) {
     uintptr_t any = 0, out = 0;
-    for (const Written& s : spans) {
-        if (s.at < out || (s.out && s.at < any)) return true;
-        any = std::max(any, s.end);
-        if (s.out) out = std::max(out, s.end);
+    for (; first != last; ++first) {
+        if (first->at < out || (first->out && first->at < any)) return true;
+        any = std::max(any, first->end);
+        if (first->out) out = std::max(out, first->end);
+    }
+    return false;
+}
+bool before(const Written& a, const Written& b) { return a.at < b.at; }
+// Whether memory that is written belongs to anything else of the call.  Slices
+// that interleave share nothing where they are columns of the same rows, others
+// count as sharing.
+bool shares(std::vector<Written>& spans) {
+    if (!std::is_sorted(spans.begin(), spans.end(), before)) std::sort(spans.begin(), spans.end(), before);
+    if (!overlaps(spans.begin(), spans.end())) return false;
+    for (auto first = spans.begin(); first != spans.end();) {
+        uintptr_t end = first->end;
+        auto last = first + 1;   // spans that hang together
+        for (; last != spans.end() && last->at < end; ++last) end = std::max(end, last->end);
+        if (overlaps(first, last)) {
+            std::vector<Written> columns;
+            for (auto s = first; s != last; ++s) {
+                if (!s->row || s->row != first->row) return true;
+                const uintptr_t at = (s->at - first->at) % s->row, to = at + s->width;
+                columns.push_back({at, std::min(to, s->row), s->out});
+                if (to > s->row) columns.push_back({0, to - s->row, s->out});
+            }
+            std::sort(columns.begin(), columns.end(), before);
+            if (overlaps(columns.begin(), columns.end())) return true;
+        }
+        first = last;
     }
     return false;
 }
@@ -705,14 +751,10 @@ Tensor clip(const char* what, const Listed& grads, double max_norm, int64_t kind
     descs.reserve(grads.size());
     if (out || in_place) spans.reserve(out ? 2 * grads.size() : grads.size());
     const Tensor* first = nullptr;
-    const auto span = [&](const Tensor& t, uintptr_t at, bool dense, bool written) {
-        int64_t reach = 1;   // elements from the first to the last
-        if (dense) reach = t.numel();
-        else
-            for (int64_t d = 0; d < t.dim(); ++d) reach += (t.size(d) - 1) * t.stride(d);
-        const uintptr_t end = at + (uintptr_t)(reach * (int64_t)t.element_size());
-        if (!spans.empty() && spans.back().end == at && spans.back().out == written) spans.back().end = end;   // buckets hold them so
-        else spans.push_back({at, end, written});
+    const auto span = [&](const Tensor& t, uintptr_t at, bool dense, bool out) {
+        const Written s = bytes_of(t, at, dense, out);
+        if (dense && !spans.empty() && !spans.back().row && spans.back().end == at && spans.back().out == out) spans.back().end = s.end;   // buckets hold them so
+        else spans.push_back(s);
     };
     for (size_t i = 0; i < grads.size(); ++i) {
         const Tensor* const given = grads.at(i);
@@ -770,7 +812,8 @@ Tensor clip(const char* what, const Listed& grads, double max_norm, int64_t kind
         descs.push_back(d);
     }
     TORCH_CHECK_VALUE(!(out || in_place) || !shares(spans), what,
-                      ": memory that is written belongs to two gradients (a parameter that is given twice?), or to an input and another's output");
+                      ": memory that is written belongs to two gradients (a parameter that is given twice? slices that interleave and are no "
+                      "columns of the same rows?), or to an input and another's output");
     if (!first) return at::zeros({}, at::device(at::kCUDA).dtype(at::kFloat));
     const c10::DeviceGuard guard(first->device());
     Tensor norm = at::empty({}, first->options().dtype(at::kFloat).requires_grad(false));

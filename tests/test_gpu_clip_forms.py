@@ -1,5 +1,5 @@
 """Gradient norm and clipping in forms that the general tests do not reach: fp64
-gradients whose squares leave fp64's range."""
+gradients whose squares leave fp64's range, slices that interleave."""
 
 import math
 
@@ -99,3 +99,67 @@ def test_fp64_norms_that_are_not_finite(bad):
         assert math.isnan(norm) if math.isnan(bad) else float(norm) == math.inf
         for g, w in zip(grads, want):
             assert torch.equal(torch.nan_to_num(g, nan=3.0), torch.nan_to_num(w, nan=3.0))
+
+
+def slices(buffer, kind):
+    if kind == "columns":
+        return [buffer[:, :30], buffer[:, 30:31], buffer[:, 31:]]
+    if kind == "columns that begin within":
+        return [buffer.view(-1)[50:50 + 37 * 64].view(37, 64)[:, :20], buffer[:, 6:50]]   # columns 50 to 63 and 0 to 5
+    if kind == "middle":
+        return list(buffer.view(10, 4, 64).split([1, 3], 1))
+    if kind == "every other":
+        return [buffer[:, ::2], buffer[:, 1::2]]
+    raise ValueError(kind)
+
+
+KINDS = ["columns", "columns that begin within", "middle", "every other"]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("kind", KINDS)
+def test_slices_that_interleave(kind, dtype):
+    """They share no memory: clipped in place, and to slices of another buffer, with nothing beside them changed."""
+    announce(f"clip {kind} {dtype}")
+    for elsewhere in (False, True):
+        buffer, other = rand((40, 64), dtype, 1), torch.full((40, 64), 7.0, dtype=dtype, device="cuda")
+        norm = float(torch.cat([t.double().flatten() for t in slices(buffer, kind)]).norm())
+        want, to = buffer.clone(), other if elsewhere else buffer
+        marks = torch.zeros_like(buffer, dtype=torch.bool)
+        for t in slices(marks, kind):
+            assert not t.any()
+            t.fill_(True)
+        got = cresso_amd.clip_gradients(slices(buffer, kind), 0.5, out=slices(other, kind) if elsewhere else None)
+        assert abs(float(got) - norm) <= 2.0 ** -23 * norm
+        assert torch.equal(to[~marks], (torch.full_like(want, 7.0) if elsewhere else want)[~marks])
+        exact = want.double() * (0.5 / norm)
+        # half a step of the type, and what fp32 adds in front of a rounding to 16 bits
+        assert ((to.double() - exact).abs() <= exact.abs() * (torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -10) + 2.0 ** -40))[marks].all()
+
+
+def test_gradients_of_a_concatenation():
+    """Autograd hands out the columns of one tensor."""
+    announce("clip gradients of a concatenation")
+    leaves = [rand((30, n), seed=n).requires_grad_(True) for n in (7, 20, 1)]
+    d = rand((30, 28), seed=4)
+    y = torch.cat(leaves, 1)
+    grads = torch.autograd.grad(y, leaves, d)
+    want, norm = [g.clone() for g in grads], float(d.double().norm())
+    cresso_amd.clip_gradients(grads, 0.5)
+    for g, w in zip(grads, want):
+        assert torch.allclose(g, w * (0.5 / norm), rtol=2.0 ** -22, atol=0.0)
+
+
+def test_slices_that_share_are_refused():
+    announce("clip slices that share")
+    b = rand((40, 64))
+    flat = b.view(-1)
+    for grads in ([b[:, :30], b[:, 29:]], [b[:, :30], b[:, :30]], [b[:, :30], b[:, 40:], b[3, 20:45]],
+                  [flat[50:50 + 37 * 64].view(37, 64)[:, :20], b[:, :10]], [flat[50:50 + 37 * 64].view(37, 64)[:, :20], b[:, 55:]],
+                  [b[:, ::2], b[:, 2:4]], [b.t()[:30], b[:, 29:]], [b[:, :30], flat[:2000].view(40, 50)[:, 45:]]):
+        with pytest.raises(ValueError, match="belongs to two"):
+            cresso_amd.clip_gradients(grads, 0.5)
+        cresso_amd.gradient_norm(grads)
+    with pytest.raises(ValueError, match="belongs to two"):   # an input's columns are another's output
+        cresso_amd.clip_gradients([b[:, :30], b[:, 30:]], 0.5, out=[b[:, 20:50], rand((40, 34))])
+    cresso_amd.clip_gradients([b[:, :30], b[:, :30]], 0.5, out=[b[:, 30:60], rand((40, 30))])   # inputs may share
