@@ -42,7 +42,10 @@ def clip_gradients(grads: Iterable[Optional[torch.Tensor]], max_norm: float, *, 
     and its type, or fp32 for gradients of 16 bits (then nothing is rounded to 16
     bits a second time); it is always written.  Memory that is written may
     belong to one gradient only (ValueError otherwise; slices that interleave are
-    taken as columns of the same rows), but a gradient may be its own output.  :meth:`CRESSO5.clip_gradients` takes an optimizer's gradients.
+    taken as columns of the same rows), but a gradient may be its own output.
+    Outside torch.no_grad() it may be no leaf that requires a gradient
+    (RuntimeError): these are gradients, not the parameters that have them.
+    :meth:`CRESSO5.clip_gradients` takes an optimizer's gradients.
     """
     given, to = _listed(grads), None if out is None else _listed(out)
     try:

@@ -739,6 +739,7 @@ struct Listed {
     }
 };
 Tensor clip(const char* what, const Listed& grads, double max_norm, int64_t kind, double grad_scale, const Listed* out, bool in_place) {
+    const bool recorded = at::GradMode::is_enabled();
     const at::NoGradGuard no_grad;
     TORCH_CHECK_VALUE(max_norm >= 0.0, what, ": max_norm must not be negative");
     TORCH_CHECK_VALUE(std::isfinite(grad_scale), what, ": grad_scale must be finite");
@@ -775,6 +776,9 @@ Tensor clip(const char* what, const Listed& grads, double max_norm, int64_t kind
                               name_of(g.scalar_type()), " ", g.sizes(), " (its own type or, of 16 bits, fp32)");
             gpu.add("an output", *to);
         }
+        // as torch's own operations in place, which refuse a leaf where they are recorded: a parameter in its gradient's stead
+        TORCH_CHECK(!to || !recorded || !to->requires_grad() || !(to->is_leaf() || (to->is_view() && to->_base().is_leaf())), what, ": ",
+                    in_place ? "gradient " : "output ", i, " is a leaf that requires a gradient, and would be scaled itself (a parameter instead of its .grad?)");
         const int64_t numel = g.numel();
         if (!numel) continue;
         cresso_grad_desc d{};

@@ -423,8 +423,9 @@ class CRESSO5(Optimizer):
         """Clips the gradients of all parameter groups in place by their common
         norm, before :meth:`step`; -> the norm before (see
         :func:`cresso_amd.clip_gradients`)."""
-        return clip_gradients([p.grad for group in self.param_groups for p in group["params"]], max_norm,
-                              norm_type=norm_type, grad_scale=grad_scale)
+        with torch.no_grad():
+            return clip_gradients([p.grad for group in self.param_groups for p in group["params"]], max_norm,
+                                  norm_type=norm_type, grad_scale=grad_scale)
 
     def _fast_scalar(self, gi: int, group: dict) -> bool:
         """Steady-state path: the group is exactly the cached scalar batch and

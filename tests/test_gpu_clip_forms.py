@@ -1,5 +1,6 @@
 """Gradient norm and clipping in forms that the general tests do not reach: fp64
-gradients whose squares leave fp64's range, slices that interleave."""
+gradients whose squares leave fp64's range, slices that interleave, parameters
+in their gradients' stead."""
 
 import math
 
@@ -163,3 +164,23 @@ def test_slices_that_share_are_refused():
     with pytest.raises(ValueError, match="belongs to two"):   # an input's columns are another's output
         cresso_amd.clip_gradients([b[:, :30], b[:, 30:]], 0.5, out=[b[:, 20:50], rand((40, 34))])
     cresso_amd.clip_gradients([b[:, :30], b[:, :30]], 0.5, out=[b[:, 30:60], rand((40, 30))])   # inputs may share
+
+
+def test_parameters_are_not_taken_for_gradients():
+    announce("clip parameters")
+    p, q = (torch.nn.Parameter(rand((20, 8), seed=i)) for i in (1, 2))
+    want = p.detach().clone()
+    for call in (lambda: cresso_amd.clip_gradients([p, q], 0.1), lambda: cresso_amd.clip_gradients(p.view(-1), 0.1),
+                 lambda: cresso_amd.clip_gradients([want], 0.1, out=[p])):
+        with pytest.raises(RuntimeError, match="leaf that requires a gradient"):
+            call()
+        assert torch.equal(p, want)
+    assert abs(float(cresso_amd.gradient_norm([p])) / float(want.norm()) - 1.0) < 1e-6   # reading is fine
+    cresso_amd.clip_gradients([p], 0.1, out=[torch.empty_like(want)])
+    (g,) = torch.autograd.grad((p * p).sum(), p, create_graph=True)
+    cresso_amd.clip_gradients([g], 0.1)   # a gradient with a history of its own is no leaf
+    assert abs(float(g.detach().norm()) - 0.1) < 1e-6
+    opt = cresso_amd.CRESSO5([p, q])
+    p.grad = torch.ones_like(p).requires_grad_(True)
+    assert abs(float(opt.clip_gradients(0.5)) / 160 ** 0.5 - 1.0) < 1e-6
+    assert abs(float(p.grad.detach().norm()) - 0.5) < 1e-6
