@@ -127,8 +127,9 @@ template <typename T, bool ACROSS, int ROW, int TILE, int NT, int FN /* 0: A */>
 // since with the builtin the compiler waits for all of them before each
 // transposed read of LDS, whichever part that reads (32768 x 5632 -> 2048, the
 // gradient of x: 1341 us, so 841 with the same tiles).  It writes no register but
-// m0, which the compiler keeps nothing in (it sets it right before what reads it);
-// group_ready waits for it.
+// m0, a reserved one: the compiler keeps nothing in it, sets it right before what
+// reads it, and warns where it is named as clobbered.  group_ready waits for the
+// loads.
 template <int V> __device__ __forceinline__ void group_to_lds(u32x4 from, uint32_t lane_at, uint32_t at, uint32_t lds) {
     static_assert(V == 16 || V == 4, "bytes of a lane");
     if constexpr (V == 16)

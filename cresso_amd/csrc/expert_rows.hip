@@ -5,11 +5,13 @@
 //   gradient: d_rows[place(t,k)] = w[t,k] * d_out[t],  d_w[t,k] = d_out[t] . rows[place(t,k)]
 //
 // Each token's lanes read its row once and write, or read, its slots' rows, 16
-// bytes a lane; sums are fp32, over k in order.  Bound by HBM, or for a few
-// tokens by the launch and the two loads that wait for one another.  16384 x
-// 2048 bf16, two experts a token: dispatch 34.9 us (5.8 TB/s read and written),
-// combine 44.2 (4.6), its gradient 68.3 (4.9); 333 x 1001 fp32, three: 4.6, 5.3 and
-// 10.1.  8 to 64 lanes a token, as its row has units, so that narrow rows leave no lanes idle.
+// bytes a lane; sums are fp32, over k in order.  Many tokens are bound by HBM:
+// 16384 x 2048 bf16, two experts a token: dispatch 34.9 us (5.8 TB/s read and
+// written), combine 44.2 (4.6), its gradient 68.3 (4.9).  Few are bound by the
+// chain of loads of one token, whose lanes take its columns four units at a time
+// and its slots one after another (two at a time in combine): 8 x 2048 with two
+// experts 3.0, 3.4 and 5.5 us, 333 x 1001 fp32 with three 4.6, 5.3 and 10.1, but 8 x 7168
+// with eight 15.0, 20.7 and 41.8.  8 to 64 lanes a token, as its row has units, so that narrow rows leave no lanes idle.
 #include "row_ops.hpp"
 
 #include <algorithm>

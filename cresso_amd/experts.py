@@ -44,8 +44,9 @@ def route_experts(logits: torch.Tensor, top: int, *, score: str = "softmax", nor
     A token takes the `top` experts of the largest logit + bias (fp32), the lowest
     expert where they are equal; NaN counts as the largest, and -inf is never
     taken: where fewer are left the last entries are absent, with weight 0.
-    Their weights come from the logits without the bias (which balances the load
-    and takes no gradient):
+    The bias is added to the logit, not to its softmax or sigmoid: a bias that was
+    trained beside those chooses other experts here.  Their weights come from the
+    logits without the bias (which balances the load and takes no gradient):
 
         softmax   scale * softmax(logits), over all experts or, with `normalize`, over the chosen ones
         sigmoid   scale * sigmoid(logits), with `normalize` divided by the chosen ones' sum
